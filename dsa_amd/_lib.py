@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libdsa_amd.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -116,6 +116,14 @@ _SIGNATURES: dict[str, list] = {
     "dsa_project_weights": [_p, _i64, _i64, _i64, _p, _i64, ctypes.c_float, _p, _p, _i64, _p],
     "dsa_encode_queries_gemm": [_p, _i64, _i64, _i64, _p, _i32, _p, _p, ctypes.c_float, ctypes.c_float, _p, _p, _p,
                                 _i64, _p],
+    "dsa_paged_append": [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _i32, _p, _p, _i64, _i32, ctypes.c_double, _p],
+    "dsa_paged_attention": [
+        _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i32, _i32, ctypes.c_float, _i32, _p, _p, _p, _i64, _p,
+    ],
+    "dsa_paged_selected_attention": [
+        _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i32, _i32, _p, _i64, _i64, ctypes.c_float, _p, _p, _p, _i64,
+        _p,
+    ],
     "dsa_dim_sketch": [_p, _i64, _i32, _i32, _p, _i32, _i32, _i32, ctypes.c_float, _p, _i32, _p],
     "dsa_abs_max": [_p, _i64, _i32, _p, _p],
     "dsa_fake_quantize": [_p, _i64, _i32, _i32, ctypes.c_float, _p, _p, _p],
@@ -130,6 +138,8 @@ _RESTYPES: dict[str, object] = {
     "dsa_project_weights_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "dsa_encode_keys_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "dsa_encode_queries_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "dsa_paged_attention_workspace_bytes": (_i64, [_p, _i64, _i64, _i32, _i64, _i32]),
+    "dsa_paged_selected_workspace_bytes": (_i64, [_p, _i64, _i32, _i64]),
 }
 
 
@@ -164,6 +174,28 @@ class VerifierSpecC(ctypes.Structure):
         ("rescue_fraction", ctypes.c_double),
         ("promotion_threshold", ctypes.c_float),
         ("sketch_scale", ctypes.c_float),
+    ]
+
+
+class PagedCacheC(ctypes.Structure):
+    """``dsa_paged_cache`` of include/dsa_amd.h."""
+
+    _fields_ = [
+        ("keys", _p),
+        ("values", _p),
+        ("key_scales", _p),
+        ("value_scales", _p),
+        ("pages", _i64),
+        ("key_page_stride", _i64),
+        ("key_slot_stride", _i64),
+        ("key_head_stride", _i64),
+        ("value_page_stride", _i64),
+        ("value_slot_stride", _i64),
+        ("value_head_stride", _i64),
+        ("page_size", _i32),
+        ("kv_heads", _i32),
+        ("head_dim", _i32),
+        ("dtype", _i32),
     ]
 
 

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define DSA_ABI_VERSION 5
+#define DSA_ABI_VERSION 6
 
 #define DSA_STATUS_OK 0
 #define DSA_STATUS_INVALID_ARGUMENT 1
@@ -830,6 +830,87 @@ int dsa_encode_queries_gemm(const void* hidden, int64_t hidden_stride, int64_t t
                             int32_t heads, const float* weights_proj, const int64_t* positions, float theta,
                             float weight_scale, void* out_queries, float* out_weights, void* workspace,
                             int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged key/value cache, and attention over it (no counterpart in the
+ * reference, which stops at the selection: sidecar.py:89-107 scores the keys,
+ * metrics.py:9-22 selects, and the selected positions go back to the model's
+ * own attention).
+ *
+ * A cache row is one token's keys (or values) of kv_heads heads; row r is slot
+ * r % page_size of page r / page_size, and position p of sequence s is row
+ * page_table[s][p / page_size] * page_size + p % page_size.  Element (page,
+ * slot, head, d) of the keys lies at page * key_page_stride + slot *
+ * key_slot_stride + head * key_head_stride + d elements, the values' likewise:
+ * any order of pages, slots and heads, head_dim contiguous elements.  dtype is
+ * bf16, fp16 or fp8 e4m3; an fp8 cache stands for code * scale, with one fp32
+ * scale per (page, slot, head) in contiguous [pages][page_size][kv_heads].
+ * page_size a power of two, head_dim 64, 128 or 256, pages * page_size below
+ * 2^31; pointers and strides 16-byte aligned, page and slot strides below 4 GiB.
+ * Offsets are 64-bit.  The descriptor is host memory, read during the call.
+ * ------------------------------------------------------------------------ */
+typedef struct dsa_paged_cache {
+  void* keys;
+  void* values;
+  float* key_scales;   /* fp8 only, else ignored */
+  float* value_scales;
+  int64_t pages;
+  int64_t key_page_stride, key_slot_stride, key_head_stride;
+  int64_t value_page_stride, value_slot_stride, value_head_stride;
+  int32_t page_size, kv_heads, head_dim, dtype;
+} dsa_paged_cache;
+
+/* Writes tokens' keys and values [tokens][kv_heads][head_dim] (token strides in
+ * elements) into cache rows rows[t], the keys' first rope_dim dims turned by the
+ * non-interleaved RoPE of positions[t] (pairs (i, i + rope_dim / 2), angle
+ * position * theta^(-2 i / rope_dim), evaluated to fp32 accuracy at any
+ * position; sidecar.py:10-28 takes the angle's product in fp32).  Products and
+ * sums are fp32, rounded once to the cache's type.  Tokens whose row is outside
+ * the cache are not written; two tokens with one row leave either's values.
+ * fp8: scale = max(max|x| / 448, 2^-126) over a head, code = round-to-nearest
+ * (x / scale); rows must be finite.  queries (nullable, [tokens][heads]
+ * [head_dim]) are turned by the same angles into out_queries (dense, may not
+ * overlap).  dtype is that of keys, values and queries: the cache's, or bf16 for
+ * an fp8 cache.  rope_dim a multiple of 16 up to head_dim (0: no rotation). */
+int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, int64_t key_stride, const void* values,
+                     int64_t value_stride, const void* queries, int64_t query_stride, void* out_queries,
+                     int32_t heads, int32_t dtype, const int64_t* rows, const int64_t* positions, int64_t tokens,
+                     int32_t rope_dim, double theta, void* stream);
+
+/* Attention of each sequence's newest tokens over its whole cache:
+ *   out[t][h] = sum_j softmax_j(scale q[t][h] . k[j][h / group]) v[j][h / group]
+ * queries and out [tokens][heads][head_dim] (queries' token stride in elements,
+ * out dense), heads a multiple of kv_heads, group = heads / kv_heads.  Sequence
+ * s has tokens starts[s] .. starts[s + 1] (starts[0] = 0, ascending,
+ * starts[sequences] = tokens; NULL: tokens / sequences each) and lengths[s]
+ * keys, its new tokens' included, at most columns * page_size.  With causal, the
+ * i-th of n new tokens sees keys j <= lengths[s] - n + i, else every key of the
+ * sequence.  A row that sees no key gets zeros and lse -inf.  lse (nullable,
+ * [tokens][heads] fp32) is the natural log of the softmax's denominator.  Cache
+ * rows past a sequence's length are never used.  Page ids outside the cache read
+ * other rows of it.  Workspace (16-byte aligned, need not be cleared): the bytes
+ * that the query below gives for the same sizes, uniform = (starts == NULL). */
+int64_t dsa_paged_attention_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
+                                            int32_t heads, int64_t columns, int32_t uniform);
+int dsa_paged_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
+                        const int32_t* page_table, int64_t table_stride, int64_t columns, const int32_t* lengths,
+                        const int32_t* starts, int64_t sequences, int64_t tokens, int32_t heads, int32_t dtype,
+                        float scale, int32_t causal, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
+/* The same over the keys that each token's list names: indices int64
+ * [tokens][index_stride], the first k of each row being positions in the
+ * token's sequence, shared by its heads, in any order; entries below 0 or not
+ * below lengths[s] are padding, whatever stands there.  A position named twice
+ * counts twice.  The lists of dsa_score_topk and dsa_score_queries_topk fit as
+ * they are. */
+int64_t dsa_paged_selected_workspace_bytes(const dsa_paged_cache* cache, int64_t tokens, int32_t heads, int64_t k);
+int dsa_paged_selected_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
+                                 const int32_t* page_table, int64_t table_stride, int64_t columns,
+                                 const int32_t* lengths, const int32_t* starts, int64_t sequences, int64_t tokens,
+                                 int32_t heads, int32_t dtype, const int64_t* indices, int64_t index_stride, int64_t k,
+                                 float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
 
 /* ------------------------------------------------------------------------
  * Measurement utility (no counterpart in the reference; it serves the
