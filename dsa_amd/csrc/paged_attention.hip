@@ -24,16 +24,6 @@ namespace {
 constexpr int kSpan = 2048;  // keys whose cache rows are looked up at a time
 constexpr int kStep = 32;    // keys per wave and step
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-// ds_read_b64_tr_b16: lane i of a group of 16 reads 8 bytes at its own address;
-// with rows r = i / 4 and 4-element runs i % 4 of a 4 x 16 block, lane i gets
-// column i: one element of each of the four rows.
-__device__ __forceinline__ uint2 read_transposed(const char* lds) {
-  typedef __attribute__((address_space(3))) s16x4* Ptr;
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(lds)));
-}
-
 // LDS that the lanes of one wave share: a wave's LDS accesses are served in
 // order, so only the compiler has to keep them so.
 __device__ __forceinline__ void wave_order() {
@@ -59,7 +49,7 @@ struct Tile {
 };
 
 template <class Tag, bool kFp8, int D, bool kSelected>
-__global__ __launch_bounds__(256, 2) void paged_stream_kernel(PagedAttentionArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(PagedAttentionArgs a) {
   constexpr int kLoads = Tile<kFp8, D>::kLoads;
   constexpr int kQ = D / 32;  // k-steps of the first product
   constexpr int kO = D / 16;  // dim tiles of the second
@@ -86,43 +76,17 @@ __global__ __launch_bounds__(256, 2) void paged_stream_kernel(PagedAttentionArgs
     token0 = item / tiles;
     row0 = item % tiles * 16u;
     rows = a.group;
-    if (a.starts) {
-      uint32_t before = 0;
-      for (uint32_t b = 0; b < a.sequences; b += kWave)
-        before += (uint32_t)__popcll(__ballot(b + lane < a.sequences && a.starts[b + lane + 1] <= (int32_t)token0));
-      sequence = min(before, a.sequences - 1u);
-    } else {
-      sequence = token0 / (a.tokens / a.sequences);
-    }
+    sequence = sequence_of(a, token0);
     length = keys_of(a, sequence);
     visible = length ? a.k : 0u;
   } else {
     // item: a tile of some sequence's (token, head) rows, counted over the sequences
-    uint32_t left = item;
-    Span span = {0, 0};
-    bool found = false;
-    for (uint32_t b = 0; b < a.sequences && !found; b += kWave) {
-      Span s = {0, 0};
-      if (b + lane < a.sequences) s = tokens_of(a, b + lane);
-      uint32_t n = s.count * a.group;
-      if (n > a.most_rows) n = 0;
-      const uint32_t tiles = (n + 15u) / 16u;
-      const uint32_t upto = wave_incl_scan(tiles);
-      const uint64_t owner = __ballot(left < upto);
-      if (owner) {
-        const int at = __builtin_ctzll(owner);
-        sequence = b + (uint32_t)at;
-        left -= (uint32_t)__builtin_amdgcn_readlane(upto - tiles, at);
-        span.first = (uint32_t)__builtin_amdgcn_readlane(s.first, at);
-        span.count = (uint32_t)__builtin_amdgcn_readlane(s.count, at);
-        found = true;
-      } else {
-        left -= (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
-      }
-    }
-    if (!found) return;
+    RowTile tile;
+    if (!find_row_tile(a, item, 16u, tile)) return;
+    sequence = tile.sequence;
+    const Span span = tile.span;
     token0 = span.first;
-    row0 = left * 16u;
+    row0 = tile.index * 16u;
     rows = span.count * a.group;
     length = keys_of(a, sequence);
     // row r sees keys below seen0 + r / group + 1 of a causal chunk
@@ -356,6 +320,10 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
   __shared__ floatx4 sums[256];
   const uint32_t lane = lane_id();
   const uint64_t row = blockIdx.x;
+  if (a.starts && !a.indices) {  // a mixed batch: another kernel's rows are not in these pieces
+    const uint32_t rows = tokens_of(a, sequence_of(a, blockIdx.x / a.heads)).count * a.group;
+    if (rows < a.least_rows || rows > a.most_rows) return;
+  }
   const float2* part = a.part_sum + row * a.splits;
   float top = kNoKeys;
   for (uint32_t p = lane; p < a.splits; p += kWave) top = fmaxf(top, part[p].x);
@@ -402,6 +370,15 @@ void launch_combine(const PagedAttentionArgs& a, int32_t dim, hipStream_t s) {
     hipLaunchKernelGGL((paged_combine_kernel<Tag, 256>), grid, dim3(256), 0, s, a);
 }
 
+int combine(const PagedAttentionArgs& a, int32_t dim, int32_t dtype, hipStream_t s) {
+  if (a.splits == 1) return 0;
+  if (dtype == kBF16)
+    launch_combine<Bf16Tag>(a, dim, s);
+  else
+    launch_combine<F16Tag>(a, dim, s);
+  return check_launch("paged_combine_kernel");
+}
+
 template <bool kSelected>
 int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dtype, int64_t items, hipStream_t s) {
   const int64_t grid = items * a.splits * a.cache.kv_heads;
@@ -414,21 +391,14 @@ int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dt
   else
     launch_stream<F16Tag, false, kSelected>(a, dim, (uint32_t)grid, s);
   if (int st = check_launch("paged_stream_kernel")) return st;
-  if (a.splits > 1) {
-    if (dtype == kBF16)
-      launch_combine<Bf16Tag>(a, dim, s);
-    else
-      launch_combine<F16Tag>(a, dim, s);
-    return check_launch("paged_combine_kernel");
-  }
-  return 0;
+  return combine(a, dim, dtype, s);
 }
 
-// Pieces of each row's keys: enough workgroups for four per CU, none of fewer
-// than 128 keys.
-uint32_t splits_for(int64_t workgroups, int64_t most_keys) {
-  const int64_t want = (1024 + workgroups - 1) / workgroups;
-  const int64_t most = (most_keys + 127) / 128;
+// Pieces of each row's keys: enough workgroups to fill the GPU `rounds` times,
+// none of fewer than `least` keys.
+uint32_t splits_for(int64_t workgroups, int64_t want_workgroups, int64_t most_keys, int64_t least) {
+  const int64_t want = (want_workgroups + workgroups - 1) / workgroups;
+  const int64_t most = (most_keys + least - 1) / least;
   const int64_t splits = want < most ? want : most;
   return (uint32_t)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
 }
@@ -437,11 +407,11 @@ int64_t part_bytes(int64_t rows, int64_t splits, int64_t dim) {
   return splits > 1 ? rows * splits * (dim + 2) * 4 : 0;
 }
 
-// Tiles of 16 rows over all sequences: each sequence's last one may be partial.
-int64_t dense_items(int64_t sequences, int64_t tokens, int64_t group, bool uniform) {
-  if (uniform) return sequences * ((tokens / sequences * group + 15) / 16);
+// Tiles of `size` rows over all sequences: each sequence's last one may be partial.
+int64_t row_tiles(int64_t sequences, int64_t tokens, int64_t group, bool uniform, int64_t size) {
+  if (uniform) return sequences * ((tokens / sequences * group + size - 1) / size);
   const int64_t most = tokens < sequences ? tokens : sequences;  // sequences that have tokens
-  return (tokens * group + 15 * most) / 16;
+  return (tokens * group + (size - 1) * most) / size;
 }
 
 int check_common(const dsa_paged_cache* cache, const void* queries, int64_t query_stride, const int32_t* page_table,
@@ -474,7 +444,6 @@ int check_common(const dsa_paged_cache* cache, const void* queries, int64_t quer
   a.tokens = (uint32_t)tokens;
   a.heads = (uint32_t)heads;
   a.group = (uint32_t)(heads / cache->kv_heads);
-  a.most_rows = 0xffffffffu;
   a.scale = scale * kLog2E;
   return 0;
 }
@@ -490,19 +459,32 @@ int take_workspace(PagedAttentionArgs& a, int64_t dim, void* workspace, int64_t 
   return 0;
 }
 
+constexpr int64_t kStreamRows = 16;  // most rows of a sequence that the stream kernel takes
+
 struct Plan {
+  int64_t stream_items, chunk_items;  // 0: no sequence of that kind
+  uint32_t stream_splits, chunk_splits;
+};
+
+Plan dense_plan(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t capacity, bool uniform) {
+  const int64_t group = heads / kv_heads;
+  Plan p = {0, 0, 1, 1};
+  const int64_t each = tokens / sequences * group;
+  if (!uniform || each <= kStreamRows) p.stream_items = uniform ? sequences : (tokens < sequences ? tokens : sequences);
+  if (!uniform || each > kStreamRows) p.chunk_items = row_tiles(sequences, tokens, group, uniform, kChunkRows);
+  if (p.stream_items) p.stream_splits = splits_for(p.stream_items * kv_heads, 1024, capacity, 128);
+  if (p.chunk_items) p.chunk_splits = splits_for(p.chunk_items * kv_heads, 512, capacity, 256);
+  return p;
+}
+
+struct SelectedPlan {
   int64_t items;
   uint32_t splits;
 };
 
-Plan dense_plan(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t capacity, bool uniform) {
-  const int64_t items = dense_items(sequences, tokens, heads / kv_heads, uniform);
-  return {items, splits_for(items * kv_heads, capacity)};
-}
-
-Plan selected_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t k) {
+SelectedPlan selected_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t k) {
   const int64_t items = tokens * ((heads / kv_heads + 15) / 16);
-  return {items, splits_for(items * kv_heads, k)};
+  return {items, splits_for(items * kv_heads, 1024, k, 128)};
 }
 
 bool sizes_valid(const dsa_paged_cache* c, int64_t sequences, int64_t tokens, int32_t heads) {
@@ -518,7 +500,7 @@ extern "C" int64_t dsa_paged_attention_workspace_bytes(const dsa_paged_cache* ca
                                                        int32_t heads, int64_t columns, int32_t uniform) {
   if (!sizes_valid(cache, sequences, tokens, heads)) return 0;
   const Plan p = dense_plan(sequences, tokens, heads, cache->kv_heads, columns * cache->page_size, uniform != 0);
-  return part_bytes(tokens * heads, p.splits, cache->head_dim);
+  return part_bytes(tokens * heads, p.stream_splits > p.chunk_splits ? p.stream_splits : p.chunk_splits, cache->head_dim);
 }
 
 extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
@@ -532,18 +514,36 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
     return st;
   if (tokens == 0) return 0;
   const Plan p = dense_plan(sequences, tokens, heads, cache->kv_heads, columns * cache->page_size, !starts);
-  a.splits = p.splits;
   a.causal = causal != 0;
   a.out = static_cast<char*>(out);
   a.lse = lse;
-  if (int st = take_workspace(a, cache->head_dim, workspace, workspace_bytes)) return st;
-  return launch<false>(a, cache, dtype, p.items, static_cast<hipStream_t>(stream));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  // A sequence of few rows (one decoded token, a few drafted ones) is bound by
+  // reading its cache, one of many by the products: a mixed batch has both.
+  if (p.stream_items) {
+    a.splits = p.stream_splits;
+    a.least_rows = 1;
+    a.most_rows = kStreamRows;
+    if (int st = take_workspace(a, cache->head_dim, workspace, workspace_bytes)) return st;
+    if (int st = launch<false>(a, cache, dtype, p.stream_items, s)) return st;
+  }
+  if (p.chunk_items) {
+    a.splits = p.chunk_splits;
+    a.least_rows = kStreamRows + 1;
+    a.most_rows = 0xffffffffu;
+    if (int st = take_workspace(a, cache->head_dim, workspace, workspace_bytes)) return st;
+    const int64_t grid = p.chunk_items * a.splits * a.cache.kv_heads;
+    DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
+    if (int st = launch_paged_chunk(a, cache->head_dim, cache->dtype, (uint32_t)grid, s)) return st;
+    return combine(a, cache->head_dim, dtype, s);
+  }
+  return 0;
 }
 
 extern "C" int64_t dsa_paged_selected_workspace_bytes(const dsa_paged_cache* cache, int64_t tokens, int32_t heads,
                                                       int64_t k) {
   if (!sizes_valid(cache, 1, tokens, heads)) return 0;
-  const Plan p = selected_plan(tokens, heads, cache->kv_heads, k);
+  const SelectedPlan p = selected_plan(tokens, heads, cache->kv_heads, k);
   return part_bytes(tokens * heads, p.splits, cache->head_dim);
 }
 
@@ -560,7 +560,7 @@ extern "C" int dsa_paged_selected_attention(const dsa_paged_cache* cache, const 
   DSA_REQUIRE(k >= 0 && k < (1LL << 31) - 64 && (indices || k == 0) && index_stride >= k, "index lists of %lld out of range",
               (long long)k);
   if (tokens == 0) return 0;
-  const Plan p = selected_plan(tokens, heads, cache->kv_heads, k);
+  const SelectedPlan p = selected_plan(tokens, heads, cache->kv_heads, k);
   a.splits = p.splits;
   a.indices = indices;
   a.index_stride = index_stride;

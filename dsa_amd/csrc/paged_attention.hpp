@@ -72,6 +72,57 @@ __device__ __forceinline__ uint32_t cache_row(const PagedAttentionArgs& a, const
   return (page << a.cache.shift) | (key & ((1u << a.cache.shift) - 1u));
 }
 
+// A tile of `size` consecutive (token, head) rows of one kv head of a sequence.
+struct RowTile {
+  uint32_t sequence;
+  uint32_t index;  // of the tile among its sequence's
+  Span span;
+};
+
+// Tile `item` of the sequences of least_rows .. most_rows rows, counted over them
+// in order; every wave searches for itself.  False past the last.
+__device__ __forceinline__ bool find_row_tile(const PagedAttentionArgs& a, uint32_t item, uint32_t size, RowTile& tile) {
+  const uint32_t lane = lane_id();
+  for (uint32_t b = 0; b < a.sequences; b += kWave) {
+    Span s = {0, 0};
+    if (b + lane < a.sequences) s = tokens_of(a, b + lane);
+    const uint32_t n = s.count * a.group;
+    const uint32_t tiles = n < a.least_rows || n > a.most_rows ? 0u : (n + size - 1u) / size;
+    const uint32_t upto = wave_incl_scan(tiles);
+    const uint64_t owner = __ballot(item < upto);
+    if (owner) {
+      const int at = __builtin_ctzll(owner);
+      tile.sequence = b + (uint32_t)at;
+      tile.index = item - (uint32_t)__builtin_amdgcn_readlane(upto - tiles, at);
+      tile.span.first = (uint32_t)__builtin_amdgcn_readlane(s.first, at);
+      tile.span.count = (uint32_t)__builtin_amdgcn_readlane(s.count, at);
+      return true;
+    }
+    item -= (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return false;
+}
+
+// The sequence of a token.
+__device__ __forceinline__ uint32_t sequence_of(const PagedAttentionArgs& a, uint32_t token) {
+  if (!a.starts) return token / (a.tokens / a.sequences);
+  const uint32_t lane = lane_id();
+  uint32_t before = 0;
+  for (uint32_t b = 0; b < a.sequences; b += kWave)
+    before += (uint32_t)__popcll(__ballot(b + lane < a.sequences && a.starts[b + lane + 1] <= (int32_t)token));
+  return min(before, a.sequences - 1u);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// ds_read_b64_tr_b16: lane i of a group of 16 reads 8 bytes at its own address;
+// with rows r = i / 4 and 4-element runs i % 4 of a 4 x 16 block, lane i gets
+// column i: one element of each of the four rows.
+__device__ __forceinline__ uint2 read_transposed(const char* lds) {
+  typedef __attribute__((address_space(3))) s16x4* Ptr;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(lds)));
+}
+
 // One split's result of one row, or the final one where nothing is split:
 // `o` is four dims' weighted sum under `reference`, `total` the weights' sum.
 template <class Tag, int D>
@@ -89,5 +140,10 @@ __device__ __forceinline__ void store_row(const PagedAttentionArgs& a, uint32_t 
       make_uint2(pack2(Tag{}, o[0] * inv, o[1] * inv), pack2(Tag{}, o[2] * inv, o[3] * inv));
   if (a.lse && dim == 0) a.lse[row] = total > 0.f ? (reference + log2f(total)) * kLn2 : -INFINITY;
 }
+
+constexpr int kChunkRows = 128;  // rows of a workgroup of the chunk kernel
+
+// paged_chunk.hip: the chunk kernel over `grid` workgroups.
+int launch_paged_chunk(const PagedAttentionArgs& a, int32_t dim, int32_t cache_dtype, uint32_t grid, hipStream_t s);
 
 }  // namespace dsa
