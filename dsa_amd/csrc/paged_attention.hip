@@ -23,6 +23,8 @@ namespace {
 
 constexpr int kSpan = 2048;  // keys whose cache rows are looked up at a time
 constexpr int kStep = 32;    // keys per wave and step
+constexpr int kMostSplits = 256;
+constexpr int kMostTiles = 1024;  // row tiles x kv heads that are split (each has a counter)
 
 // LDS that the lanes of one wave share: a wave's LDS accesses are served in
 // order, so only the compiler has to keep them so.
@@ -57,6 +59,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
   __shared__ __attribute__((aligned(16))) int32_t table[kSpan];
   __shared__ __attribute__((aligned(16))) float scales[4][64];
   __shared__ float2 sums[4][16];
+  __shared__ uint32_t last_piece;
   const uint32_t lane = lane_id();
   const uint32_t wave = threadIdx.x / kWave;
   const uint32_t col = lane & 15u;
@@ -304,14 +307,77 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
       sum += *reinterpret_cast<const floatx4*>(values[w] + r * (D * 4) + ((c ^ r) << 4));
       weight += sums[w][r].y * exp2_fast(sums[w][r].x - top);
     }
-    const uint32_t row = row0 + r;
-    const uint32_t token = kSelected ? token0 : token0 + row / a.group;
-    const uint32_t head = g * a.group + (kSelected ? row : row % a.group);
-    store_row<Tag, D>(a, token, head, piece, 4u * c, sum, top, weight);
+    const uint32_t token = kSelected ? token0 : token0 + (row0 + r) / a.group;
+    const uint32_t head = g * a.group + (kSelected ? row0 + r : (row0 + r) % a.group);
+    if (a.splits > 1)
+      store_part<D, true>(a, token, head, piece, 4u * c, sum, top, weight);
+    else
+      store_out<Tag, D>(a, token, head, 4u * c, sum, top, weight);
+  }
+  if (a.splits == 1) return;
+
+  // The tile's last piece to finish joins them all, in the order of the pieces:
+  // the same bits whichever it is.  The pieces are stored and loaded past the
+  // XCDs' own L2s, so no cache is written back or dropped (a release and an
+  // acquire of agent scope here took 140 us of a 385 us step): each wave waits for
+  // its stores, the counter is raised after all four waves have, and what the
+  // last workgroup loads depends on the counter it read.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t* arrived = a.arrived + (item * a.cache.kv_heads + g);
+    const uint32_t before = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last_piece = before + 1u == a.splits;
+    if (before + 1u == a.splits) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last_piece) return;
+  const uint32_t live = min(16u, rows - row0);
+  auto row_of = [&](uint32_t r) {
+    const uint64_t token = kSelected ? token0 : token0 + (row0 + r) / a.group;
+    return token * a.heads + g * a.group + (kSelected ? row0 + r : (row0 + r) % a.group);
+  };
+  float* weights = reinterpret_cast<float*>(values[0]);  // [16][splits]
+  static_assert(sizeof(values) >= 16 * kMostSplits * sizeof(float), "weights of the pieces");
+  {
+    const uint32_t r = threadIdx.x / 16u;
+    float top = kNoKeys;
+    float sum = 0.f;
+    if (r < live) {
+      const float2* part = a.part_sum + row_of(r) * a.splits;
+      for (uint32_t p = threadIdx.x % 16u; p < a.splits; p += 16u) top = fmaxf(top, load_shared(part + p).x);
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+      for (uint32_t p = threadIdx.x % 16u; p < a.splits; p += 16u) {
+        const float2 s = load_shared(part + p);
+        const float w = exp2_fast(s.x - top);
+        weights[r * a.splits + p] = w;
+        sum += s.y * w;
+      }
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+      if (threadIdx.x % 16u == 0) sums[0][r] = make_float2(top, sum);
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < live * (D / 4); i += 256u) {
+    const uint32_t r = i / (D / 4);
+    const uint32_t c = i % (D / 4);
+    const uint64_t row = row_of(r);
+    const float* part = a.part_out + row * a.splits * D + 4u * c;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (uint32_t p = 0; p < a.splits; ++p) {
+      const float2* o2 = reinterpret_cast<const float2*>(part + (uint64_t)p * D);
+      const float2 lo = load_shared(o2);
+      const float2 hi = load_shared(o2 + 1);
+      sum += floatx4{lo.x, lo.y, hi.x, hi.y} * weights[r * a.splits + p];
+    }
+    store_out<Tag, D>(a, (uint32_t)(row / a.heads), (uint32_t)(row % a.heads), 4u * c, sum, sums[0][r].x, sums[0][r].y);
   }
 }
 
-// Joins the pieces of one (token, head) row: references to their maximum, sums
+// The chunk kernel's pieces of one (token, head) row: references to their maximum, sums
 // and outputs scaled to it and added in the order of the pieces.
 template <class Tag, int D>
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a) {
@@ -320,9 +386,9 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
   __shared__ floatx4 sums[256];
   const uint32_t lane = lane_id();
   const uint64_t row = blockIdx.x;
-  if (a.starts && !a.indices) {  // a mixed batch: another kernel's rows are not in these pieces
+  if (a.starts) {  // a mixed batch: the stream kernel's rows are not in these pieces
     const uint32_t rows = tokens_of(a, sequence_of(a, blockIdx.x / a.heads)).count * a.group;
-    if (rows < a.least_rows || rows > a.most_rows) return;
+    if (rows < a.least_rows) return;
   }
   const float2* part = a.part_sum + row * a.splits;
   float top = kNoKeys;
@@ -343,10 +409,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
   __syncthreads();
   if (threadIdx.x >= kLanes) return;
   for (uint32_t i = 1; i < kGroups; ++i) o += sums[i * kLanes + c];
-  const float inv = total > 0.f ? 1.f / total : 0.f;
-  *reinterpret_cast<uint2*>(a.out + (row * D + 4u * c) * 2) =
-      make_uint2(pack2(Tag{}, o[0] * inv, o[1] * inv), pack2(Tag{}, o[2] * inv, o[3] * inv));
-  if (a.lse && c == 0) a.lse[row] = total > 0.f ? (top + log2f(total)) * kLn2 : -INFINITY;
+  store_out<Tag, D>(a, (uint32_t)(row / a.heads), (uint32_t)(row % a.heads), 4u * c, o, top, total);
 }
 
 template <class Tag, bool kFp8, bool kSelected>
@@ -390,8 +453,7 @@ int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dt
     launch_stream<Bf16Tag, false, kSelected>(a, dim, (uint32_t)grid, s);
   else
     launch_stream<F16Tag, false, kSelected>(a, dim, (uint32_t)grid, s);
-  if (int st = check_launch("paged_stream_kernel")) return st;
-  return combine(a, dim, dtype, s);
+  return check_launch("paged_stream_kernel");
 }
 
 // Pieces of each row's keys: enough workgroups to fill the GPU `rounds` times,
@@ -400,11 +462,12 @@ uint32_t splits_for(int64_t workgroups, int64_t want_workgroups, int64_t most_ke
   const int64_t want = (want_workgroups + workgroups - 1) / workgroups;
   const int64_t most = (most_keys + least - 1) / least;
   const int64_t splits = want < most ? want : most;
-  return (uint32_t)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+  return (uint32_t)(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
 }
 
+// Counters first, at one place for every shape, then the pieces.
 int64_t part_bytes(int64_t rows, int64_t splits, int64_t dim) {
-  return splits > 1 ? rows * splits * (dim + 2) * 4 : 0;
+  return splits > 1 ? kMostTiles * 4 + rows * splits * (dim + 2) * 4 : 0;
 }
 
 // Tiles of `size` rows over all sequences: each sequence's last one may be partial.
@@ -454,7 +517,8 @@ int take_workspace(PagedAttentionArgs& a, int64_t dim, void* workspace, int64_t 
   if (!workspace || bytes < part_bytes(rows, a.splits, dim) || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(DSA_STATUS_WORKSPACE_TOO_SMALL, "paged attention needs %lld bytes of 16-byte aligned workspace",
                 (long long)part_bytes(rows, a.splits, dim));
-  a.part_out = static_cast<float*>(workspace);
+  a.arrived = static_cast<uint32_t*>(workspace);
+  a.part_out = reinterpret_cast<float*>(a.arrived + kMostTiles);
   a.part_sum = reinterpret_cast<float2*>(a.part_out + rows * a.splits * dim);
   return 0;
 }
@@ -472,7 +536,7 @@ Plan dense_plan(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_hea
   const int64_t each = tokens / sequences * group;
   if (!uniform || each <= kStreamRows) p.stream_items = uniform ? sequences : (tokens < sequences ? tokens : sequences);
   if (!uniform || each > kStreamRows) p.chunk_items = row_tiles(sequences, tokens, group, uniform, kChunkRows);
-  if (p.stream_items) p.stream_splits = splits_for(p.stream_items * kv_heads, 1024, capacity, 128);
+  if (p.stream_items) p.stream_splits = splits_for(p.stream_items * kv_heads, kMostTiles, capacity, 128);
   if (p.chunk_items) p.chunk_splits = splits_for(p.chunk_items * kv_heads, 512, capacity, 256);
   return p;
 }
@@ -484,7 +548,7 @@ struct SelectedPlan {
 
 SelectedPlan selected_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t k) {
   const int64_t items = tokens * ((heads / kv_heads + 15) / 16);
-  return {items, splits_for(items * kv_heads, 1024, k, 128)};
+  return {items, splits_for(items * kv_heads, kMostTiles, k, 128)};
 }
 
 bool sizes_valid(const dsa_paged_cache* c, int64_t sequences, int64_t tokens, int32_t heads) {

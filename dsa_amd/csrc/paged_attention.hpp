@@ -43,6 +43,7 @@ struct PagedAttentionArgs {
   float* lse;               // nullable: [tokens][heads]
   float* part_out;          // [tokens][heads][splits][dim], splits > 1
   float2* part_sum;         // [tokens][heads][splits] {reference, sum}
+  uint32_t* arrived;        // pieces of each row tile that are done (stream kernel); zero between calls
 };
 
 struct Span {
@@ -123,22 +124,42 @@ __device__ __forceinline__ uint2 read_transposed(const char* lds) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(lds)));
 }
 
-// One split's result of one row, or the final one where nothing is split:
-// `o` is four dims' weighted sum under `reference`, `total` the weights' sum.
-template <class Tag, int D>
-__device__ __forceinline__ void store_row(const PagedAttentionArgs& a, uint32_t token, uint32_t head, uint32_t piece,
-                                          uint32_t dim, floatx4 o, float reference, float total) {
-  const uint64_t row = (uint64_t)token * a.heads + head;
-  if (a.splits > 1) {
-    const uint64_t at = row * a.splits + piece;
-    *reinterpret_cast<floatx4*>(a.part_out + at * D + dim) = o;
+// 8 bytes past the caches that XCDs do not share (agent-scope accesses), for
+// pieces that another workgroup of the same launch joins.
+__device__ __forceinline__ void store_shared(float2* p, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, make_float2(x, y)), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_shared(const float2* p) {
+  return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                      __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Four dims of a row's result: `o` their weighted sum under `reference`, `total`
+// the weights' sum.  Of one piece, for the join (kShared: in this launch):
+template <int D, bool kShared>
+__device__ __forceinline__ void store_part(const PagedAttentionArgs& a, uint32_t token, uint32_t head, uint32_t piece,
+                                           uint32_t dim, floatx4 o, float reference, float total) {
+  const uint64_t at = ((uint64_t)token * a.heads + head) * a.splits + piece;
+  float* to = a.part_out + at * D + dim;
+  if constexpr (kShared) {
+    store_shared(reinterpret_cast<float2*>(to), o[0], o[1]);
+    store_shared(reinterpret_cast<float2*>(to) + 1, o[2], o[3]);
+    if (dim == 0) store_shared(a.part_sum + at, reference, total);
+  } else {
+    *reinterpret_cast<floatx4*>(to) = o;
     if (dim == 0) a.part_sum[at] = make_float2(reference, total);
-    return;
   }
-  const float inv = total > 0.f ? 1.f / total : 0.f;
+}
+// Of all keys:
+template <class Tag, int D>
+__device__ __forceinline__ void store_out(const PagedAttentionArgs& a, uint32_t token, uint32_t head, uint32_t dim,
+                                          floatx4 o, float reference, float total) {
+  const uint64_t row = (uint64_t)token * a.heads + head;
+  const float inv = total > 0.f ? 1.f / total : total;  // NaN stays
   *reinterpret_cast<uint2*>(a.out + (row * D + dim) * 2) =
       make_uint2(pack2(Tag{}, o[0] * inv, o[1] * inv), pack2(Tag{}, o[2] * inv, o[3] * inv));
-  if (a.lse && dim == 0) a.lse[row] = total > 0.f ? (reference + log2f(total)) * kLn2 : -INFINITY;
+  if (a.lse && dim == 0) a.lse[row] = total == 0.f ? -INFINITY : (reference + log2f(total)) * kLn2;
 }
 
 constexpr int kChunkRows = 128;  // rows of a workgroup of the chunk kernel

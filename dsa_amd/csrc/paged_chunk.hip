@@ -255,9 +255,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-      store_row<Tag, D>(a, my_token, my_head, piece, 32u * i + 8u * b + 4u * half,
-                        floatx4{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]}, reference, total);
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t dim = 32u * i + 8u * b + 4u * half;
+      const floatx4 part = {o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
+      if (a.splits > 1)
+        store_part<D, false>(a, my_token, my_head, piece, dim, part, reference, total);
+      else
+        store_out<Tag, D>(a, my_token, my_head, dim, part, reference, total);
+    }
 }
 
 }  // namespace

@@ -129,6 +129,13 @@ def _rows(x: torch.Tensor, dim: int) -> tuple[torch.Tensor, int]:
     return x, stride
 
 
+def _dense_like(x: torch.Tensor, stride: int) -> torch.Tensor:
+    """An uninitialised dense tensor like the rows ``x`` (empty_like is the
+    cheaper call by 0.6 us, a twentieth of a short call's host time)."""
+
+    return torch.empty_like(x) if stride == x.shape[1] * x.shape[2] else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
 def _queries(queries: torch.Tensor, cache: PagedCache) -> tuple[torch.Tensor, int]:
     if queries.ndim != 3 or queries.shape[2] != cache.head_dim:
         raise ValueError("queries must be [tokens,heads,head_dim]")
@@ -184,7 +191,7 @@ def append(
             raise ValueError("queries must be [tokens,heads,head_dim]")
         queries, query_stride = _queries(queries, cache)
         heads = queries.shape[1]
-        out = torch.empty((tokens, heads, dim), device=keys.device, dtype=keys.dtype)
+        out = _dense_like(queries, query_stride)
     if tokens == 0:
         return out
     keys, key_stride = _rows(keys, dim)
@@ -239,7 +246,7 @@ def _batch(queries, cache, page_table, lengths, starts):
 def _workspace(cache: PagedCache, stream: int, need: int) -> torch.Tensor | None:
     if need <= 0:
         return None
-    return _lib.workspace("paged_attention", cache.keys.device, stream, need, zeroed=False)
+    return _lib.workspace("paged_attention", cache.keys.device, stream, need, zeroed=True)
 
 
 def attention(
@@ -271,7 +278,7 @@ def attention(
     page_table, table_stride, lengths, starts = _batch(queries, cache, page_table, lengths, starts)
     tokens, heads, dim = queries.shape
     device = queries.device
-    out = torch.empty((tokens, heads, dim), device=device, dtype=queries.dtype)
+    out = _dense_like(queries, query_stride)
     lse = torch.empty((tokens, heads), device=device, dtype=torch.float32) if return_lse else None
     if tokens:
         sequences, columns = page_table.shape
@@ -317,7 +324,7 @@ def selected_attention(
     if indices.dtype != torch.int64 or indices.device != device or (k > 1 and indices.stride(1) != 1) or index_stride < k:
         indices = indices.to(device=device, dtype=torch.int64).contiguous()
         index_stride = k
-    out = torch.empty((tokens, heads, dim), device=device, dtype=queries.dtype)
+    out = _dense_like(queries, query_stride)
     lse = torch.empty((tokens, heads), device=device, dtype=torch.float32) if return_lse else None
     if tokens:
         sequences, columns = page_table.shape

@@ -888,8 +888,10 @@ int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, int64_t key
  * sequence.  A row that sees no key gets zeros and lse -inf.  lse (nullable,
  * [tokens][heads] fp32) is the natural log of the softmax's denominator.  Cache
  * rows past a sequence's length are never used.  Page ids outside the cache read
- * other rows of it.  Workspace (16-byte aligned, need not be cleared): the bytes
- * that the query below gives for the same sizes, uniform = (starts == NULL). */
+ * other rows of it.  Workspace (16-byte aligned): the bytes that the query below
+ * gives for the same sizes, uniform = (starts == NULL); its first 4 KiB are zero
+ * before the first call, and every call leaves them so.  Calls that share one are
+ * ordered on one stream. */
 int64_t dsa_paged_attention_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
                                             int32_t heads, int64_t columns, int32_t uniform);
 int dsa_paged_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
