@@ -41,6 +41,23 @@ int make_paged_view(const dsa_paged_cache* cache, PagedView& view);
 // 2^x by the hardware instruction (results below the normal range become 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+struct Low {
+  static constexpr bool value = false;
+};
+struct High {
+  static constexpr bool value = true;
+};
+
+// 8 e4m3 codes to 8 bf16, exactly: two codes per instruction at a scale of 1.
+__device__ __forceinline__ uint4 fp8x8_to_bf16x8_paired(uint2 v) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  auto two = [](uint32_t w, auto high) {
+    const pair p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, decltype(high)::value);
+    return __builtin_bit_cast(uint32_t, p);
+  };
+  return make_uint4(two(v.x, Low{}), two(v.x, High{}), two(v.y, Low{}), two(v.y, High{}));
+}
+
 // Two fp32 rounded to nearest-even bf16 or fp16, packed.
 __device__ __forceinline__ uint32_t pack2(Bf16Tag, float lo, float hi) {
   typedef __bf16 pair __attribute__((ext_vector_type(2)));

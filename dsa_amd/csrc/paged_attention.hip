@@ -23,8 +23,12 @@ namespace {
 
 constexpr int kSpan = 2048;  // keys whose cache rows are looked up at a time
 constexpr int kStep = 32;    // keys per wave and step
-constexpr int kMostSplits = 256;
-constexpr int kMostTiles = 1024;  // row tiles x kv heads that are split (each has a counter)
+// Workgroups that run at a time: what the registers of each head_dim allow on 256
+// CUs.  Work is cut to fill them once.
+template <int D>
+constexpr int kPerCu = D == 64 ? 3 : D == 128 ? 2 : 1;
+constexpr int64_t resident_workgroups(int64_t dim) { return 256 * (dim == 64 ? kPerCu<64> : dim == 128 ? kPerCu<128> : kPerCu<256>); }
+constexpr int kCounters = 4096;  // of row tiles that are cut, by kv head
 
 // LDS that the lanes of one wave share: a wave's LDS accesses are served in
 // order, so only the compiler has to keep them so.
@@ -42,6 +46,11 @@ __device__ __forceinline__ uint32_t value_place(uint32_t row, uint32_t chunk) {
   return row * (D * 2) + ((chunk ^ x) << 4);
 }
 
+template <uint32_t N>
+struct Rounds {
+  static constexpr uint32_t value = N;
+};
+
 template <bool kFp8, int D>
 struct Tile {
   static constexpr int kLoads = kFp8 ? D / 64 : D / 32;  // 16-byte loads per lane and 16-key tile
@@ -51,8 +60,9 @@ struct Tile {
 };
 
 template <class Tag, bool kFp8, int D, bool kSelected>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(PagedAttentionArgs a) {
+__global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAttentionArgs a) {
   constexpr int kLoads = Tile<kFp8, D>::kLoads;
+  constexpr uint32_t kAhead = kFp8 ? 2 : 1;  // steps loaded ahead
   constexpr int kQ = D / 32;  // k-steps of the first product
   constexpr int kO = D / 16;  // dim tiles of the second
   __shared__ __attribute__((aligned(16))) char values[4][kStep * D * 2];  // a wave's value tile; its output at the end
@@ -65,49 +75,66 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
   const uint32_t col = lane & 15u;
   const uint32_t quad = lane >> 4;
 
-  // Heads vary fastest: workgroups go round-robin over the XCDs, so a kv head's
-  // rows meet in few L2s.
-  const uint32_t g = blockIdx.x % a.cache.kv_heads;
-  const uint32_t rest = blockIdx.x / a.cache.kv_heads;
-  const uint32_t piece = rest % a.splits;
-  const uint32_t item = rest / a.splits;
+  // Workgroups go round-robin over the XCDs.  Heads vary fastest, so a kv head's
+  // rows meet in few L2s; but the heads of an fp8 piece, whose scales share cache
+  // lines, follow each other on one XCD (16 bit / fp8 decode steps, us: heads
+  // fastest 385 / 209, heads on one XCD 397 / 191).
+  constexpr bool kTogether = kFp8 && !kSelected;
+  const uint32_t turn = kTogether ? blockIdx.x / kXcds : blockIdx.x;
+  const uint32_t g = turn % a.cache.kv_heads;
+  const uint32_t id = kTogether ? turn / a.cache.kv_heads * kXcds + blockIdx.x % kXcds : turn / a.cache.kv_heads;
 
-  uint32_t sequence, token0, row0, rows, length, visible, seen0 = 0;
+  uint32_t sequence, token0, row0, rows, length, begin, end, pieces, index, slot, tile_slot, seen0 = 0;
   if constexpr (kSelected) {
-    // item: a tile of a token's heads
+    // a piece of the list of a tile of a token's heads
     const uint32_t tiles = (a.group + 15u) / 16u;
+    const uint32_t item = id / a.splits;
+    const uint32_t piece = id % a.splits;
     token0 = item / tiles;
     row0 = item % tiles * 16u;
     rows = a.group;
     sequence = sequence_of(a, token0);
     length = keys_of(a, sequence);
-    visible = length ? a.k : 0u;
+    const uint32_t visible = length ? a.k : 0u;
+    const uint32_t chunk = max(128u, ((a.k + a.splits - 1u) / a.splits + 31u) & ~31u);
+    begin = min(piece * chunk, visible);
+    end = min(begin + chunk, visible);
+    pieces = a.splits;
+    index = piece;
+    tile_slot = item;
+    slot = item * a.splits;
   } else {
-    // item: a tile of some sequence's (token, head) rows, counted over the sequences
-    RowTile tile;
-    if (!find_row_tile(a, item, 16u, tile)) return;
-    sequence = tile.sequence;
-    const Span span = tile.span;
-    token0 = span.first;
-    row0 = tile.index * 16u;
-    rows = span.count * a.group;
-    length = keys_of(a, sequence);
-    // row r sees keys below seen0 + r / group + 1 of a causal chunk
-    seen0 = a.causal ? length - span.count : length;  // may wrap below zero: see `sees`
-    const uint32_t last = min(row0 + 15u, rows - 1u) / a.group;
-    visible = a.causal ? (uint32_t)max(0, (int32_t)(length - span.count + last + 1u)) : length;
+    Piece piece;
+    if (!find_piece(a, id, piece)) return;
+    sequence = piece.sequence;
+    token0 = piece.span.first;
+    row0 = 0;
+    rows = piece.span.count * a.group;  // at most 16
+    length = piece.keys;
+    // row r sees keys below seen0 + r / group + 1 of a causal chunk; the last sees all
+    seen0 = length - piece.span.count;  // may wrap below zero: see `sees`
+    begin = min(piece.index * piece.units * kUnit, length);
+    end = min(begin + piece.units * kUnit, length);
+    pieces = piece.count;
+    index = piece.index;
+    tile_slot = slot = piece.slot;
   }
 
   // This lane's row, and the keys it sees.
   const uint32_t my_row = min(row0 + col, rows - 1u);
   const uint32_t my_token = kSelected ? token0 : token0 + my_row / a.group;
   const uint32_t my_head = g * a.group + (kSelected ? my_row : my_row % a.group);
-  const uint32_t sees = kSelected || !a.causal ? visible : (uint32_t)max(0, (int32_t)(seen0 + my_row / a.group + 1u));
-  const uint32_t all_see = kSelected || !a.causal ? visible : (uint32_t)max(0, (int32_t)(seen0 + row0 / a.group + 1u));
+  const bool partly = !kSelected && a.causal;
+  const uint32_t sees = partly ? (uint32_t)max(0, (int32_t)(seen0 + my_row / a.group + 1u)) : end;
+  const uint32_t all_see = partly ? (uint32_t)max(0, (int32_t)(seen0 + row0 / a.group + 1u)) : end;
 
-  const uint32_t chunk = max(128u, ((visible + a.splits - 1u) / a.splits + 31u) & ~31u);
-  const uint32_t begin = min(piece * chunk, visible);
-  const uint32_t end = min(begin + chunk, visible);
+  auto out_row = [&](uint32_t r) {
+    const uint64_t token = kSelected ? token0 : token0 + (row0 + r) / a.group;
+    return token * a.heads + g * a.group + (kSelected ? row0 + r : (row0 + r) % a.group);
+  };
+  auto part_at = [&](uint32_t piece, uint32_t r) {
+    return ((uint64_t)piece * a.cache.kv_heads + g) * a.part_rows + r;
+  };
 
   uint4 q[kQ];
   {
@@ -165,8 +192,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
         if (kSelected && drop) v = make_uint4(0u, 0u, 0u, 0u);
         if constexpr (kFp8) {
           const uint32_t c = 2u * (4u * j + quad);
-          *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, c)) = fp8x8_to_bf16x8(make_uint2(v.x, v.y));
-          *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, c + 1u)) = fp8x8_to_bf16x8(make_uint2(v.z, v.w));
+          *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
+          *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
         } else {
           *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, 4u * j + quad)) = v;
         }
@@ -183,8 +210,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
       for (int j = 0; j < kLoads; ++j) {
         const uint4 k = t.k[h][j];
         if constexpr (kFp8) {
-          s = mfma_16x16x32(Tag{}, fp8x8_to_bf16x8(make_uint2(k.x, k.y)), q[2 * j], s);
-          s = mfma_16x16x32(Tag{}, fp8x8_to_bf16x8(make_uint2(k.z, k.w)), q[2 * j + 1], s);
+          s = mfma_16x16x32(Tag{}, fp8x8_to_bf16x8_paired(make_uint2(k.x, k.y)), q[2 * j], s);
+          s = mfma_16x16x32(Tag{}, fp8x8_to_bf16x8_paired(make_uint2(k.z, k.w)), q[2 * j + 1], s);
         } else {
           s = mfma_16x16x32(Tag{}, k, q[j], s);
         }
@@ -251,31 +278,55 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
     const uint32_t n = min((uint32_t)kSpan, end - base);
     const uint32_t steps = (n + kStep - 1) / kStep;
     if (base != begin) __syncthreads();
-    for (uint32_t i = threadIdx.x; i < steps * kStep; i += 256u) {
+    auto look_up = [&](auto rounds) {  // all under way before the first is waited for
+      constexpr uint32_t kRounds = decltype(rounds)::value;
+      uint32_t row[kRounds];
       if constexpr (kSelected) {
-        const int64_t key = i < n ? list[base + i] : -1;
-        const bool named = key >= 0 && key < (int64_t)length;
-        const uint32_t row = cache_row(a, pages, named ? (uint32_t)key : 0u);
-        table[i] = (int32_t)(row | (named ? 0u : 0x80000000u));
+        int64_t key[kRounds];
+#pragma unroll
+        for (uint32_t j = 0; j < kRounds; ++j) {
+          const uint32_t i = threadIdx.x + 256u * j;
+          key[j] = list[base + min(i, n - 1u)];
+          if (i >= n || key[j] >= (int64_t)length) key[j] = -1;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kRounds; ++j)
+          row[j] = cache_row(a, pages, (uint32_t)max(key[j], (int64_t)0)) | (key[j] < 0 ? 0x80000000u : 0u);
       } else {
-        table[i] = (int32_t)cache_row(a, pages, min(base + i, end - 1u));
+#pragma unroll
+        for (uint32_t j = 0; j < kRounds; ++j) row[j] = cache_row(a, pages, min(base + threadIdx.x + 256u * j, end - 1u));
       }
-    }
+#pragma unroll
+      for (uint32_t j = 0; j < kRounds; ++j) table[threadIdx.x + 256u * j] = (int32_t)row[j];
+    };
+    if (n <= 256u)
+      look_up(Rounds<1>{});
+    else
+      look_up(Rounds<kSpan / 256>{});
     __syncthreads();
-    Tile<kFp8, D> t0, t1;
-    uint32_t step = wave;
-    if (step < steps) {
-      load(t0, step);
-      while (true) {
-        // the next step's loads run under this one's products; past the end they repeat the last
-        load(t1, min(step + 4u, steps - 1u));
-        compute(t0, step, base);
-        step += 4u;
-        if (step >= steps) break;
-        load(t0, min(step + 4u, steps - 1u));
-        compute(t1, step, base);
-        step += 4u;
-        if (step >= steps) break;
+    if (steps <= 4u) {
+      // one step a wave: nothing to load ahead
+      Tile<kFp8, D> tile;
+      if (wave < steps) {
+        load(tile, wave);
+        compute(tile, wave, base);
+      }
+    } else {
+      // kAhead steps' loads run under this one's products; past the end they
+      // repeat the last.
+      Tile<kFp8, D> tile[kAhead + 1];
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; ++i) load(tile[i], min(wave + 4u * i, steps - 1u));
+      // (No way out of the loop but its end: with one after each step the
+      // compiler waits for every load in flight at its head.)
+      for (uint32_t first = wave; first < steps; first += 4u * (kAhead + 1u)) {
+#pragma unroll
+        for (uint32_t i = 0; i <= kAhead; ++i) {
+          const uint32_t step = first + 4u * i;
+          load(tile[(i + kAhead) % (kAhead + 1u)], min(step + 4u * kAhead, steps - 1u));
+          __builtin_amdgcn_sched_barrier(0);
+          if (step < steps) compute(tile[i], step, base);
+        }
       }
     }
   }
@@ -307,14 +358,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
       sum += *reinterpret_cast<const floatx4*>(values[w] + r * (D * 4) + ((c ^ r) << 4));
       weight += sums[w][r].y * exp2_fast(sums[w][r].x - top);
     }
-    const uint32_t token = kSelected ? token0 : token0 + (row0 + r) / a.group;
-    const uint32_t head = g * a.group + (kSelected ? row0 + r : (row0 + r) % a.group);
-    if (a.splits > 1)
-      store_part<D, true>(a, token, head, piece, 4u * c, sum, top, weight);
-    else
-      store_out<Tag, D>(a, token, head, 4u * c, sum, top, weight);
+    if (pieces == 1u) {
+      store_out<Tag, D>(a, out_row(r), 4u * c, sum, top, weight);
+    } else {
+      const uint64_t at = part_at(slot + index, r);
+      float2* to = reinterpret_cast<float2*>(a.part_out + at * D + 4u * c);
+      store_shared(to, sum[0], sum[1]);
+      store_shared(to + 1, sum[2], sum[3]);
+      if (c == 0) store_shared(a.part_sum + at, top, weight);
+    }
   }
-  if (a.splits == 1) return;
+  if (pieces == 1u) return;
 
   // The tile's last piece to finish joins them all, in the order of the pieces:
   // the same bits whichever it is.  The pieces are stored and loaded past the
@@ -325,55 +379,64 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_stream_kernel(Pag
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    uint32_t* arrived = a.arrived + (item * a.cache.kv_heads + g);
+    uint32_t* arrived = a.arrived + (tile_slot * a.cache.kv_heads + g);
     const uint32_t before = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last_piece = before + 1u == a.splits;
-    if (before + 1u == a.splits) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last_piece = before + 1u == pieces;
+    if (before + 1u == pieces) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!last_piece) return;
+
+  // Four dims of a row per thread, the pieces dealt to as many groups of threads as
+  // the rows leave, kPieces pieces' loads under way at a time.  (Kept short: it runs
+  // once, from a cold instruction cache.)
+  constexpr uint32_t kPieces = 8;
   const uint32_t live = min(16u, rows - row0);
-  auto row_of = [&](uint32_t r) {
-    const uint64_t token = kSelected ? token0 : token0 + (row0 + r) / a.group;
-    return token * a.heads + g * a.group + (kSelected ? row0 + r : (row0 + r) % a.group);
-  };
-  float* weights = reinterpret_cast<float*>(values[0]);  // [16][splits]
-  static_assert(sizeof(values) >= 16 * kMostSplits * sizeof(float), "weights of the pieces");
-  {
-    const uint32_t r = threadIdx.x / 16u;
+  const uint32_t cells = live * (D / 4);
+  const uint32_t groups = max(1u, 256u / cells);
+  floatx4* joined = reinterpret_cast<floatx4*>(values[0]);  // [256]
+  floatx2* joined_sum = reinterpret_cast<floatx2*>(table);  // [256]
+  static_assert(sizeof(values) >= 256 * sizeof(floatx4) && sizeof(table) >= 256 * sizeof(floatx2), "join");
+  const uint32_t group = threadIdx.x / cells;
+  for (uint32_t cell = threadIdx.x % cells; cell < cells; cell += 256u) {
+    const uint32_t r = cell / (D / 4);
+    const uint32_t dim = 4u * (cell % (D / 4));
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
     float top = kNoKeys;
-    float sum = 0.f;
-    if (r < live) {
-      const float2* part = a.part_sum + row_of(r) * a.splits;
-      for (uint32_t p = threadIdx.x % 16u; p < a.splits; p += 16u) top = fmaxf(top, load_shared(part + p).x);
+    float weight = 0.f;
+    auto add = [&](float reference, float w, floatx4 v) {
+      const float raised = fmaxf(top, reference);
+      const float keep = exp2_fast(top - raised);
+      const float take = exp2_fast(reference - raised);
+      sum = sum * keep + v * take;
+      weight = weight * keep + w * take;
+      top = raised;
+    };
+    for (uint32_t p = group; p < pieces && group < groups; p += groups * kPieces) {
+      float2 s[kPieces], lo[kPieces], hi[kPieces];
 #pragma unroll
-      for (int off = 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-      for (uint32_t p = threadIdx.x % 16u; p < a.splits; p += 16u) {
-        const float2 s = load_shared(part + p);
-        const float w = exp2_fast(s.x - top);
-        weights[r * a.splits + p] = w;
-        sum += s.y * w;
+      for (uint32_t j = 0; j < kPieces; ++j) {
+        const uint64_t at = part_at(slot + min(p + groups * j, pieces - 1u), r);
+        const float2* from = reinterpret_cast<const float2*>(a.part_out + at * D + dim);
+        s[j] = load_shared(a.part_sum + at);
+        lo[j] = load_shared(from);
+        hi[j] = load_shared(from + 1);
       }
 #pragma unroll
-      for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-      if (threadIdx.x % 16u == 0) sums[0][r] = make_float2(top, sum);
+      for (uint32_t j = 0; j < kPieces; ++j)
+        if (p + groups * j < pieces) add(s[j].x, s[j].y, floatx4{lo[j].x, lo[j].y, hi[j].x, hi[j].y});
     }
-  }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < live * (D / 4); i += 256u) {
-    const uint32_t r = i / (D / 4);
-    const uint32_t c = i % (D / 4);
-    const uint64_t row = row_of(r);
-    const float* part = a.part_out + row * a.splits * D + 4u * c;
-    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (uint32_t p = 0; p < a.splits; ++p) {
-      const float2* o2 = reinterpret_cast<const float2*>(part + (uint64_t)p * D);
-      const float2 lo = load_shared(o2);
-      const float2 hi = load_shared(o2 + 1);
-      sum += floatx4{lo.x, lo.y, hi.x, hi.y} * weights[r * a.splits + p];
+    if (groups > 1u) {  // then one round of cells takes every thread
+      joined[threadIdx.x] = sum;
+      joined_sum[threadIdx.x] = floatx2{top, weight};
+      __syncthreads();
+      if (group > 0) return;
+      for (uint32_t i = 1; i < groups; ++i) {
+        const floatx2 s = joined_sum[i * cells + cell];
+        add(s[0], s[1], joined[i * cells + cell]);
+      }
     }
-    store_out<Tag, D>(a, (uint32_t)(row / a.heads), (uint32_t)(row % a.heads), 4u * c, sum, sums[0][r].x, sums[0][r].y);
+    if (group == 0) store_out<Tag, D>(a, out_row(r), dim, sum, top, weight);
   }
 }
 
@@ -409,7 +472,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
   __syncthreads();
   if (threadIdx.x >= kLanes) return;
   for (uint32_t i = 1; i < kGroups; ++i) o += sums[i * kLanes + c];
-  store_out<Tag, D>(a, (uint32_t)(row / a.heads), (uint32_t)(row % a.heads), 4u * c, o, top, total);
+  store_out<Tag, D>(a, row, 4u * c, o, top, total);
 }
 
 template <class Tag, bool kFp8, bool kSelected>
@@ -443,8 +506,8 @@ int combine(const PagedAttentionArgs& a, int32_t dim, int32_t dtype, hipStream_t
 }
 
 template <bool kSelected>
-int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dtype, int64_t items, hipStream_t s) {
-  const int64_t grid = items * a.splits * a.cache.kv_heads;
+int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dtype, int64_t pieces, hipStream_t s) {
+  const int64_t grid = pieces * a.cache.kv_heads;
   DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
   const int32_t dim = cache->head_dim;
   if (cache->dtype == kFP8E4M3)
@@ -456,18 +519,13 @@ int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dt
   return check_launch("paged_stream_kernel");
 }
 
-// Pieces of each row's keys: enough workgroups to fill the GPU `rounds` times,
-// none of fewer than `least` keys.
-uint32_t splits_for(int64_t workgroups, int64_t want_workgroups, int64_t most_keys, int64_t least) {
-  const int64_t want = (want_workgroups + workgroups - 1) / workgroups;
+// Pieces of each row's keys: enough for `want` workgroups, none of fewer than
+// `least` keys.
+uint32_t splits_for(int64_t workgroups, int64_t want, int64_t most_keys, int64_t least) {
+  const int64_t enough = (want + workgroups - 1) / workgroups;
   const int64_t most = (most_keys + least - 1) / least;
-  const int64_t splits = want < most ? want : most;
+  const int64_t splits = enough < most ? enough : most;
   return (uint32_t)(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
-}
-
-// Counters first, at one place for every shape, then the pieces.
-int64_t part_bytes(int64_t rows, int64_t splits, int64_t dim) {
-  return splits > 1 ? kMostTiles * 4 + rows * splits * (dim + 2) * 4 : 0;
 }
 
 // Tiles of `size` rows over all sequences: each sequence's last one may be partial.
@@ -490,7 +548,7 @@ int check_common(const dsa_paged_cache* cache, const void* queries, int64_t quer
   DSA_REQUIRE(dtype == (cache->dtype == kFP8E4M3 ? kBF16 : cache->dtype),
               "queries must have the cache's type (bf16 for an fp8 cache)");
   DSA_REQUIRE(starts || tokens % sequences == 0, "without starts every sequence has as many tokens");
-  DSA_REQUIRE(columns > 0 && columns < (1LL << 31) && columns * cache->page_size < (1LL << 31) && table_stride >= columns,
+  DSA_REQUIRE(columns > 0 && columns < (1LL << 31) && columns * cache->page_size <= (1LL << 30) && table_stride >= columns,
               "page table of %lld columns out of range", (long long)columns);
   DSA_REQUIRE(query_stride >= (int64_t)heads * cache->head_dim && query_stride % 8 == 0,
               "query_stride must cover the heads and be a multiple of 8");
@@ -511,44 +569,67 @@ int check_common(const dsa_paged_cache* cache, const void* queries, int64_t quer
   return 0;
 }
 
-int take_workspace(PagedAttentionArgs& a, int64_t dim, void* workspace, int64_t bytes) {
-  if (a.splits == 1) return 0;
-  const int64_t rows = (int64_t)a.tokens * a.heads;
-  if (!workspace || bytes < part_bytes(rows, a.splits, dim) || reinterpret_cast<uintptr_t>(workspace) % 16)
+constexpr int64_t kStreamRows = 16;  // most rows of a sequence that the stream kernel takes
+
+// Workspace: the counters, at one place for every shape, then results of
+// `parts` rows and their sums.
+int64_t part_bytes(int64_t parts, int64_t dim) { return parts ? kCounters * 4 + parts * (dim + 2) * 4 : 0; }
+
+int take_workspace(PagedAttentionArgs& a, int64_t parts, int64_t dim, void* workspace, int64_t bytes) {
+  if (parts == 0) return 0;
+  if (!workspace || bytes < part_bytes(parts, dim) || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(DSA_STATUS_WORKSPACE_TOO_SMALL, "paged attention needs %lld bytes of 16-byte aligned workspace",
-                (long long)part_bytes(rows, a.splits, dim));
+                (long long)part_bytes(parts, dim));
   a.arrived = static_cast<uint32_t*>(workspace);
-  a.part_out = reinterpret_cast<float*>(a.arrived + kMostTiles);
-  a.part_sum = reinterpret_cast<float2*>(a.part_out + rows * a.splits * dim);
+  a.part_out = reinterpret_cast<float*>(a.arrived + kCounters);
+  a.part_sum = reinterpret_cast<float2*>(a.part_out + parts * dim);
   return 0;
 }
 
-constexpr int64_t kStreamRows = 16;  // most rows of a sequence that the stream kernel takes
-
 struct Plan {
   int64_t stream_items, chunk_items;  // 0: no sequence of that kind
-  uint32_t stream_splits, chunk_splits;
+  uint32_t cuts, part_rows;           // stream kernel
+  uint32_t chunk_splits;
+  int64_t stream_pieces;  // at most
+  int64_t parts;
 };
 
-Plan dense_plan(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t capacity, bool uniform) {
+Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens, int64_t heads, int64_t capacity,
+                bool uniform) {
+  const int64_t kv_heads = cache->kv_heads;
   const int64_t group = heads / kv_heads;
-  Plan p = {0, 0, 1, 1};
+  Plan p = {};
   const int64_t each = tokens / sequences * group;
   if (!uniform || each <= kStreamRows) p.stream_items = uniform ? sequences : (tokens < sequences ? tokens : sequences);
   if (!uniform || each > kStreamRows) p.chunk_items = row_tiles(sequences, tokens, group, uniform, kChunkRows);
-  if (p.stream_items) p.stream_splits = splits_for(p.stream_items * kv_heads, kMostTiles, capacity, 128);
-  if (p.chunk_items) p.chunk_splits = splits_for(p.chunk_items * kv_heads, 512, capacity, 256);
+  if (p.stream_items) {
+    p.cuts = (uint32_t)((resident_workgroups(cache->head_dim) + kv_heads - 1) / kv_heads);
+    p.part_rows = (uint32_t)(uniform ? each : kStreamRows);
+    const int64_t least = kLeastUnits * kUnit;
+    p.stream_pieces = p.stream_items * ((capacity + least - 1) / least);
+    if (p.stream_pieces > p.stream_items + p.cuts) p.stream_pieces = p.stream_items + p.cuts;
+    p.parts = 2 * kv_heads * p.part_rows * p.cuts;
+  }
+  if (p.chunk_items) {
+    p.chunk_splits = splits_for(p.chunk_items * kv_heads, 512, capacity, 256);
+    if (p.chunk_splits > 1 && p.parts < tokens * heads * p.chunk_splits) p.parts = tokens * heads * p.chunk_splits;
+  }
   return p;
 }
 
 struct SelectedPlan {
   int64_t items;
-  uint32_t splits;
+  uint32_t splits, part_rows;
+  int64_t parts;
 };
 
-SelectedPlan selected_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t k) {
-  const int64_t items = tokens * ((heads / kv_heads + 15) / 16);
-  return {items, splits_for(items * kv_heads, kMostTiles, k, 128)};
+SelectedPlan selected_plan(const dsa_paged_cache* cache, int64_t tokens, int64_t heads, int64_t k) {
+  const int64_t kv_heads = cache->kv_heads;
+  const int64_t group = heads / kv_heads;
+  const int64_t items = tokens * ((group + 15) / 16);
+  SelectedPlan p = {items, splits_for(items * kv_heads, resident_workgroups(cache->head_dim), k, 128), (uint32_t)(group < 16 ? group : 16), 0};
+  if (p.splits > 1) p.parts = items * p.splits * kv_heads * p.part_rows;
+  return p;
 }
 
 bool sizes_valid(const dsa_paged_cache* c, int64_t sequences, int64_t tokens, int32_t heads) {
@@ -563,8 +644,8 @@ using namespace dsa;
 extern "C" int64_t dsa_paged_attention_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
                                                        int32_t heads, int64_t columns, int32_t uniform) {
   if (!sizes_valid(cache, sequences, tokens, heads)) return 0;
-  const Plan p = dense_plan(sequences, tokens, heads, cache->kv_heads, columns * cache->page_size, uniform != 0);
-  return part_bytes(tokens * heads, p.stream_splits > p.chunk_splits ? p.stream_splits : p.chunk_splits, cache->head_dim);
+  const Plan p = dense_plan(cache, sequences, tokens, heads, columns * cache->page_size, uniform != 0);
+  return part_bytes(p.parts, cache->head_dim);
 }
 
 extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
@@ -577,25 +658,25 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
                             tokens, heads, dtype, scale, out, a))
     return st;
   if (tokens == 0) return 0;
-  const Plan p = dense_plan(sequences, tokens, heads, cache->kv_heads, columns * cache->page_size, !starts);
+  const Plan p = dense_plan(cache, sequences, tokens, heads, columns * cache->page_size, !starts);
   a.causal = causal != 0;
   a.out = static_cast<char*>(out);
   a.lse = lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
   // A sequence of few rows (one decoded token, a few drafted ones) is bound by
   // reading its cache, one of many by the products: a mixed batch has both.
+  if (int st = take_workspace(a, p.parts, cache->head_dim, workspace, workspace_bytes)) return st;
   if (p.stream_items) {
-    a.splits = p.stream_splits;
+    a.cuts = p.cuts;
+    a.part_rows = p.part_rows;
     a.least_rows = 1;
     a.most_rows = kStreamRows;
-    if (int st = take_workspace(a, cache->head_dim, workspace, workspace_bytes)) return st;
-    if (int st = launch<false>(a, cache, dtype, p.stream_items, s)) return st;
+    if (int st = launch<false>(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
   }
   if (p.chunk_items) {
     a.splits = p.chunk_splits;
     a.least_rows = kStreamRows + 1;
     a.most_rows = 0xffffffffu;
-    if (int st = take_workspace(a, cache->head_dim, workspace, workspace_bytes)) return st;
     const int64_t grid = p.chunk_items * a.splits * a.cache.kv_heads;
     DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
     if (int st = launch_paged_chunk(a, cache->head_dim, cache->dtype, (uint32_t)grid, s)) return st;
@@ -607,8 +688,8 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
 extern "C" int64_t dsa_paged_selected_workspace_bytes(const dsa_paged_cache* cache, int64_t tokens, int32_t heads,
                                                       int64_t k) {
   if (!sizes_valid(cache, 1, tokens, heads)) return 0;
-  const SelectedPlan p = selected_plan(tokens, heads, cache->kv_heads, k);
-  return part_bytes(tokens * heads, p.splits, cache->head_dim);
+  const SelectedPlan p = selected_plan(cache, tokens, heads, k);
+  return part_bytes(p.parts, cache->head_dim);
 }
 
 extern "C" int dsa_paged_selected_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
@@ -624,13 +705,14 @@ extern "C" int dsa_paged_selected_attention(const dsa_paged_cache* cache, const 
   DSA_REQUIRE(k >= 0 && k < (1LL << 31) - 64 && (indices || k == 0) && index_stride >= k, "index lists of %lld out of range",
               (long long)k);
   if (tokens == 0) return 0;
-  const SelectedPlan p = selected_plan(tokens, heads, cache->kv_heads, k);
+  const SelectedPlan p = selected_plan(cache, tokens, heads, k);
   a.splits = p.splits;
+  a.part_rows = p.part_rows;
   a.indices = indices;
   a.index_stride = index_stride;
   a.k = (uint32_t)k;
   a.out = static_cast<char*>(out);
   a.lse = lse;
-  if (int st = take_workspace(a, cache->head_dim, workspace, workspace_bytes)) return st;
-  return launch<true>(a, cache, dtype, p.items, static_cast<hipStream_t>(stream));
+  if (int st = take_workspace(a, p.parts, cache->head_dim, workspace, workspace_bytes)) return st;
+  return launch<true>(a, cache, dtype, p.items * p.splits, static_cast<hipStream_t>(stream));
 }

@@ -34,16 +34,20 @@ struct PagedAttentionArgs {
   uint32_t k;
   uint32_t sequences, tokens, heads;
   uint32_t group;           // query heads per kv head
-  uint32_t splits;          // pieces that a row's keys are cut into
+  uint32_t splits;          // pieces that a row's keys are cut into (not the dense stream kernel)
+  uint32_t cuts;            // dense stream kernel: pieces that the batch's keys are cut for
   uint32_t causal;
   uint32_t most_rows;       // sequences of more (token, head) rows per kv head are another kernel's
   uint32_t least_rows;
   float scale;              // times log2 e
   char* out;                // [tokens][heads][dim]
   float* lse;               // nullable: [tokens][heads]
-  float* part_out;          // [tokens][heads][splits][dim], splits > 1
-  float2* part_sum;         // [tokens][heads][splits] {reference, sum}
-  uint32_t* arrived;        // pieces of each row tile that are done (stream kernel); zero between calls
+  // Pieces' results: the chunk kernel's by row, [tokens][heads][splits][dim]; the
+  // stream kernel's by piece, [slot][kv_heads][part_rows][dim].
+  float* part_out;
+  float2* part_sum;         // {reference, sum} of each
+  uint32_t part_rows;
+  uint32_t* arrived;        // stream kernel: pieces of each row tile that are done; zero between calls
 };
 
 struct Span {
@@ -104,6 +108,83 @@ __device__ __forceinline__ bool find_row_tile(const PagedAttentionArgs& a, uint3
   return false;
 }
 
+// One piece of the keys of a sequence of few rows (dense stream kernel).
+constexpr uint32_t kUnit = 32;         // keys that the batch is cut in
+constexpr uint32_t kLeastUnits = 4;    // of a piece: a step for each wave
+constexpr uint32_t kMostSplits = 256;  // pieces of a sequence
+
+struct Piece {
+  uint32_t sequence;
+  Span span;
+  uint32_t keys;   // of the sequence
+  uint32_t units;  // of every piece of the batch but a sequence's last
+  uint32_t index, count;
+  uint32_t slot;   // of the sequence's first piece, where there are several
+};
+
+// Piece `id` of the batch.  All pieces are as long, whatever the sequences'
+// lengths, so every wave sums the batch's keys first: one load and a scan for up
+// to 64 sequences.  `cuts` pieces fill the GPU once, and a few more would run
+// alone after them (a batch of 128K to 56K fp8 keys took 194 us in 1040 pieces of
+// 1024 that run at a time); so for up to 64 sequences pieces are lengthened until
+// the sequences' last ones fit too.  At most cuts + sequences pieces, and at most
+// twice `cuts` of sequences that have several.
+__device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, uint32_t id, Piece& p) {
+  const uint32_t lane = lane_id();
+  Span span = {0, 0};
+  uint32_t keys = 0, units = 0;
+  bool mine = false;
+  auto look = [&](uint32_t b) {
+    span = {0, 0};
+    keys = 0;
+    if (b + lane < a.sequences) {
+      span = tokens_of(a, b + lane);
+      keys = keys_of(a, b + lane);
+    }
+    const uint32_t rows = span.count * a.group;
+    mine = rows >= a.least_rows && rows <= a.most_rows;
+    units = mine ? (keys + kUnit - 1u) / kUnit : 0u;
+  };
+  uint64_t all = 0;
+  uint32_t most = 0;
+  for (uint32_t b = 0; b < a.sequences; b += kWave) {
+    look(b);
+    all += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(units), kWave - 1);
+    most = max(most, wave_max_u32(units));
+  }
+  p.units = max(max(kLeastUnits, (most + kMostSplits - 1u) / kMostSplits), (uint32_t)((all + a.cuts - 1u) / a.cuts));
+  if (a.sequences <= kWave) {
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t pieces = mine ? max(1u, (units + p.units - 1u) / p.units) : 0u;
+      if ((uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(pieces), kWave - 1) <= a.cuts) break;
+      p.units += (p.units + 31u) / 32u;
+    }
+  }
+  p.slot = 0;
+  for (uint32_t b = 0; b < a.sequences; b += kWave) {
+    if (a.sequences > kWave) look(b);
+    const uint32_t pieces = mine ? max(1u, (units + p.units - 1u) / p.units) : 0u;
+    const uint32_t upto = wave_incl_scan(pieces);
+    const uint32_t several = pieces > 1u ? pieces : 0u;
+    const uint32_t slots = wave_incl_scan(several);
+    const uint64_t owner = __ballot(id < upto);
+    if (owner) {
+      const int at = __builtin_ctzll(owner);
+      p.sequence = b + (uint32_t)at;
+      p.index = id - (uint32_t)__builtin_amdgcn_readlane(upto - pieces, at);
+      p.count = (uint32_t)__builtin_amdgcn_readlane(pieces, at);
+      p.slot += (uint32_t)__builtin_amdgcn_readlane(slots - several, at);
+      p.keys = (uint32_t)__builtin_amdgcn_readlane(keys, at);
+      p.span.first = (uint32_t)__builtin_amdgcn_readlane(span.first, at);
+      p.span.count = (uint32_t)__builtin_amdgcn_readlane(span.count, at);
+      return true;
+    }
+    id -= (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
+    p.slot += (uint32_t)__builtin_amdgcn_readlane(slots, kWave - 1);
+  }
+  return false;
+}
+
 // The sequence of a token.
 __device__ __forceinline__ uint32_t sequence_of(const PagedAttentionArgs& a, uint32_t token) {
   if (!a.starts) return token / (a.tokens / a.sequences);
@@ -136,26 +217,10 @@ __device__ __forceinline__ float2 load_shared(const float2* p) {
 }
 
 // Four dims of a row's result: `o` their weighted sum under `reference`, `total`
-// the weights' sum.  Of one piece, for the join (kShared: in this launch):
-template <int D, bool kShared>
-__device__ __forceinline__ void store_part(const PagedAttentionArgs& a, uint32_t token, uint32_t head, uint32_t piece,
-                                           uint32_t dim, floatx4 o, float reference, float total) {
-  const uint64_t at = ((uint64_t)token * a.heads + head) * a.splits + piece;
-  float* to = a.part_out + at * D + dim;
-  if constexpr (kShared) {
-    store_shared(reinterpret_cast<float2*>(to), o[0], o[1]);
-    store_shared(reinterpret_cast<float2*>(to) + 1, o[2], o[3]);
-    if (dim == 0) store_shared(a.part_sum + at, reference, total);
-  } else {
-    *reinterpret_cast<floatx4*>(to) = o;
-    if (dim == 0) a.part_sum[at] = make_float2(reference, total);
-  }
-}
-// Of all keys:
+// the weights' sum.
 template <class Tag, int D>
-__device__ __forceinline__ void store_out(const PagedAttentionArgs& a, uint32_t token, uint32_t head, uint32_t dim,
-                                          floatx4 o, float reference, float total) {
-  const uint64_t row = (uint64_t)token * a.heads + head;
+__device__ __forceinline__ void store_out(const PagedAttentionArgs& a, uint64_t row, uint32_t dim, floatx4 o,
+                                          float reference, float total) {
   const float inv = total > 0.f ? 1.f / total : total;  // NaN stays
   *reinterpret_cast<uint2*>(a.out + (row * D + dim) * 2) =
       make_uint2(pack2(Tag{}, o[0] * inv, o[1] * inv), pack2(Tag{}, o[2] * inv, o[3] * inv));

@@ -129,10 +129,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
     for (int i = 0; i < kLoads; ++i) {
       const uint32_t row = load_row + kPass * i;
       if constexpr (kFp8) {
-        *reinterpret_cast<uint4*>(keys + key_place<D>(row, 2u * load_chunk)) = fp8x8_to_bf16x8(make_uint2(kr[i].x, kr[i].y));
-        *reinterpret_cast<uint4*>(keys + key_place<D>(row, 2u * load_chunk + 1u)) = fp8x8_to_bf16x8(make_uint2(kr[i].z, kr[i].w));
-        *reinterpret_cast<uint4*>(values + tile_value_place<D>(row, 2u * load_chunk)) = fp8x8_to_bf16x8(make_uint2(vr[i].x, vr[i].y));
-        *reinterpret_cast<uint4*>(values + tile_value_place<D>(row, 2u * load_chunk + 1u)) = fp8x8_to_bf16x8(make_uint2(vr[i].z, vr[i].w));
+        *reinterpret_cast<uint4*>(keys + key_place<D>(row, 2u * load_chunk)) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].x, kr[i].y));
+        *reinterpret_cast<uint4*>(keys + key_place<D>(row, 2u * load_chunk + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].z, kr[i].w));
+        *reinterpret_cast<uint4*>(values + tile_value_place<D>(row, 2u * load_chunk)) = fp8x8_to_bf16x8_paired(make_uint2(vr[i].x, vr[i].y));
+        *reinterpret_cast<uint4*>(values + tile_value_place<D>(row, 2u * load_chunk + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(vr[i].z, vr[i].w));
       } else {
         *reinterpret_cast<u32x4*>(keys + key_place<D>(row, load_chunk)) = kr[i];
         *reinterpret_cast<u32x4*>(values + tile_value_place<D>(row, load_chunk)) = vr[i];
@@ -252,16 +252,20 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
   total += __shfl_xor(total, 32, kWave);
   if (total == 0.f) reference = kNoKeys;
   if (row0 + 32u * wave + col >= rows) return;
+  const uint64_t my_out = (uint64_t)my_token * a.heads + my_head;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const uint32_t dim = 32u * i + 8u * b + 4u * half;
       const floatx4 part = {o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
-      if (a.splits > 1)
-        store_part<D, false>(a, my_token, my_head, piece, dim, part, reference, total);
-      else
-        store_out<Tag, D>(a, my_token, my_head, dim, part, reference, total);
+      if (a.splits > 1) {
+        const uint64_t at = my_out * a.splits + piece;
+        *reinterpret_cast<floatx4*>(a.part_out + at * D + dim) = part;
+        if (dim == 0) a.part_sum[at] = make_float2(reference, total);
+      } else {
+        store_out<Tag, D>(a, my_out, dim, part, reference, total);
+      }
     }
 }
 
