@@ -37,13 +37,21 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// Place of 16-byte chunk `chunk` of row `row` in a wave's value tile: the 8 rows
-// x 2 chunks of half a transposed read, and the 16 rows of a store, fall on
-// different banks.
-template <int D>
-__device__ __forceinline__ uint32_t value_place(uint32_t row, uint32_t chunk) {
-  const uint32_t x = D == 64 ? (((row >> 1) & 3u) << 1) | ((row >> 3) & 1u) : ((row & 7u) << 1) | ((row >> 3) & 1u);
-  return row * (D * 2) + ((chunk ^ x) << 4);
+// Place of 16-byte chunk `chunk` of row `row` in a wave's key or value tile of
+// kBytes a row.  The chunks of a row are exchanged by an exclusive or with bits of
+// the row, so that the accesses served together fall on different banks: rows
+// stored 64 or 128 bytes at a time, 16 rows read at one chunk (keys), 8 rows at
+// two (half a transposed read of values).
+template <int kBytes>
+__device__ __forceinline__ uint32_t tile_place(uint32_t row, uint32_t chunk) {
+  uint32_t x;
+  if constexpr (kBytes == 64)
+    x = (row >> 2) & 3u;
+  else if constexpr (kBytes == 128)
+    x = (((row >> 1) & 1u) << 2) | (((row >> 2) & 1u) << 1) | ((row >> 3) & 1u);
+  else
+    x = ((row & 1u) << 3) | (((row >> 1) & 1u) << 2) | (((row >> 2) & 1u) << 1) | ((row >> 3) & 1u);
+  return row * kBytes + ((chunk ^ x) << 4);
 }
 
 template <uint32_t N>
@@ -51,21 +59,30 @@ struct Rounds {
   static constexpr uint32_t value = N;
 };
 
+// A step's rows on their way from the cache.  Neighbouring lanes load neighbouring
+// 16-byte runs of a row (kLanes of them, 128 bytes where the row has as many): one
+// load that touches a different row in every lane moves a quarter of the bytes a
+// cycle, and held a decode step of cached keys that are all in L2 to 8 TB/s.
 template <bool kFp8, int D>
 struct Tile {
-  static constexpr int kLoads = kFp8 ? D / 64 : D / 32;  // 16-byte loads per lane and 16-key tile
-  uint4 k[2][kLoads];
-  uint4 v[2][kLoads];
+  static constexpr int kBytes = kFp8 ? D : 2 * D;               // of a cache row
+  static constexpr int kLanes = kBytes < 128 ? kBytes / 16 : 8;  // that share a row
+  static constexpr int kRows = 64 / kLanes;                      // of one load
+  static constexpr int kPasses = kStep / kRows;
+  static constexpr int kLoads = kBytes / (16 * kLanes);          // of one row
+  u32x4 k[kPasses][kLoads];
+  u32x4 v[kPasses][kLoads];
   float scale;  // fp8: lane l < 32 the key scale of key l, else the value scale of key l - 32
 };
 
 template <class Tag, bool kFp8, int D, bool kSelected>
 __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAttentionArgs a) {
-  constexpr int kLoads = Tile<kFp8, D>::kLoads;
-  constexpr uint32_t kAhead = kFp8 ? 2 : 1;  // steps loaded ahead
+  using T = Tile<kFp8, D>;
+  constexpr uint32_t kAhead = kFp8 ? 2 : 1;  // steps on their way in registers
   constexpr int kQ = D / 32;  // k-steps of the first product
   constexpr int kO = D / 16;  // dim tiles of the second
   __shared__ __attribute__((aligned(16))) char values[4][kStep * D * 2];  // a wave's value tile; its output at the end
+  __shared__ __attribute__((aligned(16))) char keys[4][kStep * T::kBytes];
   __shared__ __attribute__((aligned(16))) int32_t table[kSpan];
   __shared__ __attribute__((aligned(16))) float scales[4][64];
   __shared__ float2 sums[4][16];
@@ -145,8 +162,10 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
       q[j] = *reinterpret_cast<const uint4*>(p + d * 2);
     }
   }
-  const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * quad;
-  const char* value_base = a.cache.values + g * a.cache.value_head + 16u * quad;
+  const uint32_t load_row = lane / T::kLanes;
+  const uint32_t load_chunk = lane % T::kLanes;
+  const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * load_chunk;
+  const char* value_base = a.cache.values + g * a.cache.value_head + 16u * load_chunk;
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
   const int64_t* list = kSelected ? a.indices + (int64_t)token0 * a.index_stride : nullptr;
 
@@ -156,22 +175,23 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   float reference = kNoKeys;
   float total = 0.f;  // of this lane's keys
   char* mine = values[wave];
+  char* my_keys = keys[wave];
   uint32_t tr_place[kO];
 #pragma unroll
   for (int i = 0; i < kO; ++i)
-    tr_place[i] = value_place<D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1)) + 8u * (col & 1u);
+    tr_place[i] = tile_place<2 * D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1)) + 8u * (col & 1u);
 
-  auto load = [&](Tile<kFp8, D>& t, uint32_t step) {
+  auto load = [&](T& t, uint32_t step) {
     const int32_t* at = table + step * kStep;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t row = (uint32_t)at[16 * h + col] & 0x7fffffffu;
+    for (int i = 0; i < T::kPasses; ++i) {
+      const uint32_t row = (uint32_t)at[T::kRows * i + load_row] & 0x7fffffffu;
       const char* kp = key_base + a.cache.key_offset(row);
       const char* vp = value_base + a.cache.value_offset(row);
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) t.k[h][j] = *reinterpret_cast<const uint4*>(kp + 64 * j);
+      for (int j = 0; j < T::kLoads; ++j) t.k[i][j] = *reinterpret_cast<const u32x4*>(kp + 16 * T::kLanes * j);
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) t.v[h][j] = *reinterpret_cast<const uint4*>(vp + 64 * j);
+      for (int j = 0; j < T::kLoads; ++j) t.v[i][j] = *reinterpret_cast<const u32x4*>(vp + 16 * T::kLanes * j);
     }
     if constexpr (kFp8) {
       const uint32_t row = (uint32_t)at[lane & 31u] & 0x7fffffffu;
@@ -179,36 +199,42 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     }
   };
 
-  auto compute = [&](const Tile<kFp8, D>& t, uint32_t step, uint32_t base) {
+  // Both tiles to LDS, rows as they are; fp8 values widened.
+  auto stage = [&](const T& t, uint32_t step) {
     const int32_t* at = table + step * kStep;
-    // Values to LDS, rows as they are.
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int i = 0; i < T::kPasses; ++i) {
+      const uint32_t r = T::kRows * i + load_row;
       bool drop = false;
-      if constexpr (kSelected) drop = at[16 * h + col] < 0;  // padding's weight is 0, which NaN would survive
+      if constexpr (kSelected) drop = at[r] < 0;  // padding's weight is 0, which NaN would survive
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        uint4 v = t.v[h][j];
-        if (kSelected && drop) v = make_uint4(0u, 0u, 0u, 0u);
+      for (int j = 0; j < T::kLoads; ++j) {
+        const uint32_t c = T::kLanes * j + load_chunk;
+        *reinterpret_cast<u32x4*>(my_keys + tile_place<T::kBytes>(r, c)) = t.k[i][j];
+        u32x4 v = t.v[i][j];
+        if (kSelected && drop) v = u32x4{0u, 0u, 0u, 0u};
         if constexpr (kFp8) {
-          const uint32_t c = 2u * (4u * j + quad);
-          *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
-          *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
+          *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
+          *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
         } else {
-          *reinterpret_cast<uint4*>(mine + value_place<D>(16u * h + col, 4u * j + quad)) = v;
+          *reinterpret_cast<u32x4*>(mine + tile_place<2 * D>(r, c)) = v;
         }
       }
     }
     if constexpr (kFp8) scales[wave][lane] = t.scale;
     wave_order();
+  };
+
+  auto compute = [&](uint32_t step, uint32_t base) {
+    const int32_t* at = table + step * kStep;
     // Scores of keys 16 h + 4 quad + i, in powers of two.
     float x[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       floatx4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const uint4 k = t.k[h][j];
+      for (int j = 0; j < T::kBytes / 64; ++j) {
+        const uint4 k = *reinterpret_cast<const uint4*>(my_keys + tile_place<T::kBytes>(16u * h + col, 4u * j + quad));
         if constexpr (kFp8) {
           s = mfma_16x16x32(Tag{}, fp8x8_to_bf16x8_paired(make_uint2(k.x, k.y)), q[2 * j], s);
           s = mfma_16x16x32(Tag{}, fp8x8_to_bf16x8_paired(make_uint2(k.z, k.w)), q[2 * j + 1], s);
@@ -306,26 +332,28 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     __syncthreads();
     if (steps <= 4u) {
       // one step a wave: nothing to load ahead
-      Tile<kFp8, D> tile;
+      T tile;
       if (wave < steps) {
         load(tile, wave);
-        compute(tile, wave, base);
+        stage(tile, wave);
+        compute(wave, base);
       }
     } else {
-      // kAhead steps' loads run under this one's products; past the end they
-      // repeat the last.
-      Tile<kFp8, D> tile[kAhead + 1];
+      // The tiles in registers are kAhead steps on their way while LDS holds the
+      // one at work; past the end they repeat the last.  (No way out of the loop
+      // but its end: with one after each step the compiler waits for every load
+      // in flight at its head.)
+      T tile[kAhead];
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; ++i) load(tile[i], min(wave + 4u * i, steps - 1u));
-      // (No way out of the loop but its end: with one after each step the
-      // compiler waits for every load in flight at its head.)
-      for (uint32_t first = wave; first < steps; first += 4u * (kAhead + 1u)) {
+      for (uint32_t first = wave; first < steps; first += 4u * kAhead) {
 #pragma unroll
-        for (uint32_t i = 0; i <= kAhead; ++i) {
+        for (uint32_t i = 0; i < kAhead; ++i) {
           const uint32_t step = first + 4u * i;
-          load(tile[(i + kAhead) % (kAhead + 1u)], min(step + 4u * kAhead, steps - 1u));
+          stage(tile[i], min(step, steps - 1u));
+          load(tile[i], min(step + 4u * kAhead, steps - 1u));
           __builtin_amdgcn_sched_barrier(0);
-          if (step < steps) compute(tile[i], step, base);
+          if (step < steps) compute(step, base);
         }
       }
     }
