@@ -21,8 +21,8 @@
 namespace dsa {
 namespace {
 
-constexpr int kSpan = 2048;  // keys whose cache rows are looked up at a time
-constexpr int kStep = 32;    // keys per wave and step
+constexpr uint32_t kStep = 32;   // keys per wave and step
+constexpr uint32_t kGroup = 8;   // steps whose cache rows a wave looks up at a time
 // Workgroups that run at a time: what the registers of each head_dim allow on 256
 // CUs.  Work is cut to fill them once.
 template <int D>
@@ -54,11 +54,6 @@ __device__ __forceinline__ uint32_t tile_place(uint32_t row, uint32_t chunk) {
   return row * kBytes + ((chunk ^ x) << 4);
 }
 
-template <uint32_t N>
-struct Rounds {
-  static constexpr uint32_t value = N;
-};
-
 // A step's rows on their way from the cache.  Neighbouring lanes load neighbouring
 // 16-byte runs of a row (kLanes of them, 128 bytes where the row has as many): one
 // load that touches a different row in every lane moves a quarter of the bytes a
@@ -81,9 +76,11 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   constexpr uint32_t kAhead = kFp8 ? 2 : 1;  // steps on their way in registers
   constexpr int kQ = D / 32;  // k-steps of the first product
   constexpr int kO = D / 16;  // dim tiles of the second
-  __shared__ __attribute__((aligned(16))) char values[4][kStep * D * 2];  // a wave's value tile; its output at the end
-  __shared__ __attribute__((aligned(16))) char keys[4][kStep * T::kBytes];
-  __shared__ __attribute__((aligned(16))) int32_t table[kSpan];
+  // A wave's value tile (at the end its output) and key tile, one offset apart.
+  constexpr uint32_t kValues = kStep * D * 2;
+  __shared__ __attribute__((aligned(16))) char tiles[4][kValues + kStep * T::kBytes];
+  // A wave's cache rows of this group of steps and the next; negative: padding.
+  __shared__ __attribute__((aligned(16))) int32_t table[4][2][kGroup * kStep];
   __shared__ __attribute__((aligned(16))) float scales[4][64];
   __shared__ float2 sums[4][16];
   __shared__ uint32_t last_piece;
@@ -174,15 +171,50 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   for (int i = 0; i < kO; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float reference = kNoKeys;
   float total = 0.f;  // of this lane's keys
-  char* mine = values[wave];
-  char* my_keys = keys[wave];
+  char* mine = tiles[wave];
+  char* my_keys = mine + kValues;
   uint32_t tr_place[kO];
 #pragma unroll
   for (int i = 0; i < kO; ++i)
     tr_place[i] = tile_place<2 * D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1)) + 8u * (col & 1u);
 
+  // The wave's steps are every fourth of the piece, step s at keys first_key(s).
+  const uint32_t steps = (end - begin + kStep - 1u) / kStep;
+  const uint32_t own = steps > wave ? (steps - wave + 3u) / 4u : 0u;
+  auto first_key = [&](uint32_t step) { return begin + (4u * step + wave) * kStep; };
+  auto rows_at = [&](uint32_t step) { return table[wave][step / kGroup % 2u] + step % kGroup * kStep; };
+
+  // The cache rows of a group of steps, in three parts so that a group's look-ups
+  // run under the steps before it: list entries, page ids, the table.  Lane l has
+  // keys l % 32 of steps 2 j + l / 32.
+  constexpr uint32_t kRounds = kGroup / 2;
+  uint32_t key[kRounds], page[kRounds];
+  auto look_keys = [&](uint32_t group) {
+#pragma unroll
+    for (uint32_t j = 0; j < kRounds; ++j) {
+      const uint32_t at = first_key(group * kGroup + 2u * j + lane / 32u) + lane % 32u;
+      key[j] = min(at, end - 1u);
+      if constexpr (kSelected) {
+        const int64_t named = list[key[j]];
+        key[j] = at < end && named >= 0 && named < (int64_t)length ? (uint32_t)named : 0x80000000u;
+      }
+    }
+  };
+  auto look_pages = [&]() {
+#pragma unroll
+    for (uint32_t j = 0; j < kRounds; ++j) page[j] = (uint32_t)pages[(key[j] & 0x7fffffffu) >> a.cache.shift];
+  };
+  auto look_rows = [&](uint32_t group) {
+#pragma unroll
+    for (uint32_t j = 0; j < kRounds; ++j)
+      table[wave][group % 2u][64u * j + lane] =
+          (int32_t)((min(page[j], a.cache.pages - 1u) << a.cache.shift) | (key[j] & ((1u << a.cache.shift) - 1u)) |
+                    (key[j] & 0x80000000u));
+    wave_order();
+  };
+
   auto load = [&](T& t, uint32_t step) {
-    const int32_t* at = table + step * kStep;
+    const int32_t* at = rows_at(step);
 #pragma unroll
     for (int i = 0; i < T::kPasses; ++i) {
       const uint32_t row = (uint32_t)at[T::kRows * i + load_row] & 0x7fffffffu;
@@ -201,7 +233,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
 
   // Both tiles to LDS, rows as they are; fp8 values widened.
   auto stage = [&](const T& t, uint32_t step) {
-    const int32_t* at = table + step * kStep;
+    const int32_t* at = rows_at(step);
 #pragma unroll
     for (int i = 0; i < T::kPasses; ++i) {
       const uint32_t r = T::kRows * i + load_row;
@@ -225,8 +257,8 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     wave_order();
   };
 
-  auto compute = [&](uint32_t step, uint32_t base) {
-    const int32_t* at = table + step * kStep;
+  auto compute = [&](uint32_t step) {
+    const int32_t* at = rows_at(step);
     // Scores of keys 16 h + 4 quad + i, in powers of two.
     float x[8];
 #pragma unroll
@@ -257,7 +289,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
         x[4 * h + 3] = r.w < 0 ? -INFINITY : x[4 * h + 3];
       }
     }
-    const uint32_t key0 = base + step * kStep;
+    const uint32_t key0 = first_key(step);
     if (!kSelected && key0 + kStep > min(all_see, end)) {
       const uint32_t limit = min(sees, end);
 #pragma unroll
@@ -300,61 +332,39 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     wave_order();
   };
 
-  for (uint32_t base = begin; base < end; base += kSpan) {
-    const uint32_t n = min((uint32_t)kSpan, end - base);
-    const uint32_t steps = (n + kStep - 1) / kStep;
-    if (base != begin) __syncthreads();
-    auto look_up = [&](auto rounds) {  // all under way before the first is waited for
-      constexpr uint32_t kRounds = decltype(rounds)::value;
-      uint32_t row[kRounds];
-      if constexpr (kSelected) {
-        int64_t key[kRounds];
+  if (own > 0) {
+    look_keys(0);
+    look_pages();
+    look_rows(0);
+  }
+  if (own == 1) {  // nothing to load ahead
+    T tile;
+    load(tile, 0);
+    stage(tile, 0);
+    compute(0);
+  } else if (own > 1) {
+    // The tiles in registers are kAhead steps on their way while LDS holds the one
+    // at work; past the end they repeat the last.  Look-ups are issued ahead of a
+    // step's loads, whose wait they then do not lengthen.  (No way out of the loop
+    // but its end: with one after each step the compiler waits for every load in
+    // flight at its head.)
+    T tile[kAhead];
 #pragma unroll
-        for (uint32_t j = 0; j < kRounds; ++j) {
-          const uint32_t i = threadIdx.x + 256u * j;
-          key[j] = list[base + min(i, n - 1u)];
-          if (i >= n || key[j] >= (int64_t)length) key[j] = -1;
+    for (uint32_t i = 0; i < kAhead; ++i) load(tile[i], min(i, own - 1u));
+    for (uint32_t first = 0; first < own; first += kAhead) {
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; ++i) {
+        const uint32_t step = first + i;
+        const uint32_t group = step / kGroup + 1u;
+        if (group * kGroup < own) {
+          if (step % kGroup == 0) look_keys(group);
+          if (step % kGroup == 2) look_pages();
+          if (step % kGroup == 5) look_rows(group);
         }
-#pragma unroll
-        for (uint32_t j = 0; j < kRounds; ++j)
-          row[j] = cache_row(a, pages, (uint32_t)max(key[j], (int64_t)0)) | (key[j] < 0 ? 0x80000000u : 0u);
-      } else {
-#pragma unroll
-        for (uint32_t j = 0; j < kRounds; ++j) row[j] = cache_row(a, pages, min(base + threadIdx.x + 256u * j, end - 1u));
-      }
-#pragma unroll
-      for (uint32_t j = 0; j < kRounds; ++j) table[threadIdx.x + 256u * j] = (int32_t)row[j];
-    };
-    if (n <= 256u)
-      look_up(Rounds<1>{});
-    else
-      look_up(Rounds<kSpan / 256>{});
-    __syncthreads();
-    if (steps <= 4u) {
-      // one step a wave: nothing to load ahead
-      T tile;
-      if (wave < steps) {
-        load(tile, wave);
-        stage(tile, wave);
-        compute(wave, base);
-      }
-    } else {
-      // The tiles in registers are kAhead steps on their way while LDS holds the
-      // one at work; past the end they repeat the last.  (No way out of the loop
-      // but its end: with one after each step the compiler waits for every load
-      // in flight at its head.)
-      T tile[kAhead];
-#pragma unroll
-      for (uint32_t i = 0; i < kAhead; ++i) load(tile[i], min(wave + 4u * i, steps - 1u));
-      for (uint32_t first = wave; first < steps; first += 4u * kAhead) {
-#pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-          const uint32_t step = first + 4u * i;
-          stage(tile[i], min(step, steps - 1u));
-          load(tile[i], min(step + 4u * kAhead, steps - 1u));
-          __builtin_amdgcn_sched_barrier(0);
-          if (step < steps) compute(step, base);
-        }
+        stage(tile[i], min(step, own - 1u));
+        load(tile[i], min(step + kAhead, own - 1u));
+        __builtin_amdgcn_sched_barrier(0);
+        if (step < own) compute(step);
       }
     }
   }
@@ -383,7 +393,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     float weight = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      sum += *reinterpret_cast<const floatx4*>(values[w] + r * (D * 4) + ((c ^ r) << 4));
+      sum += *reinterpret_cast<const floatx4*>(tiles[w] + r * (D * 4) + ((c ^ r) << 4));
       weight += sums[w][r].y * exp2_fast(sums[w][r].x - top);
     }
     if (pieces == 1u) {
@@ -422,9 +432,9 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   const uint32_t live = min(16u, rows - row0);
   const uint32_t cells = live * (D / 4);
   const uint32_t groups = max(1u, 256u / cells);
-  floatx4* joined = reinterpret_cast<floatx4*>(values[0]);  // [256]
+  floatx4* joined = reinterpret_cast<floatx4*>(tiles[0]);  // [256]
   floatx2* joined_sum = reinterpret_cast<floatx2*>(table);  // [256]
-  static_assert(sizeof(values) >= 256 * sizeof(floatx4) && sizeof(table) >= 256 * sizeof(floatx2), "join");
+  static_assert(sizeof(tiles) >= 256 * sizeof(floatx4) && sizeof(table) >= 256 * sizeof(floatx2), "join");
   const uint32_t group = threadIdx.x / cells;
   for (uint32_t cell = threadIdx.x % cells; cell < cells; cell += 256u) {
     const uint32_t r = cell / (D / 4);
