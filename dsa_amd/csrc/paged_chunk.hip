@@ -28,18 +28,25 @@ __device__ __forceinline__ floatx16 mfma_32x32x16(F16Tag, uint4 a, uint4 b, floa
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// LDS places of 16-byte chunk `chunk` of a row.  Keys are read 16 rows at one
-// chunk at a time, values 4 rows x 4 chunks: each fills 256 bytes of banks.
+// Keeps a value's computation where it stands: the compiler would move it past
+// the next branch, away from the products that it is to run under.
+__device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
+
+// The scheduling of the instructions so far in the block: `others` arithmetic ones
+// after each of `products` matrix ones.
+#define interleave(products, others)                          \
+  _Pragma("unroll") for (int n_ = 0; n_ < (products); ++n_) { \
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        \
+    __builtin_amdgcn_sched_group_barrier(0x402, (others), 0); \
+  }
+
+// Bytes between the rows of a tile in LDS.  Padded, not exchanged, so that every
+// address of a tile is one register and an offset: keys are read 16 rows at one
+// 16-byte chunk, values 4 rows at 64 bytes, and each falls on all banks once.
 template <int D>
-__device__ __forceinline__ uint32_t key_place(uint32_t row, uint32_t chunk) {
-  const uint32_t x = D == 64 ? (row >> 1) & 7u : row & 15u;
-  return row * (D * 2) + ((chunk ^ x) << 4);
-}
+constexpr int kKeyRow = 2 * D + 16;
 template <int D>
-__device__ __forceinline__ uint32_t tile_value_place(uint32_t row, uint32_t chunk) {
-  const uint32_t x = D == 64 ? ((row >> 1) & 1u) << 2 : (row & 3u) << 2;
-  return row * (D * 2) + ((chunk ^ x) << 4);
-}
+constexpr int kValueRow = 2 * D + 64;
 
 template <class Tag, bool kFp8, int D, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_chunk_kernel(PagedAttentionArgs a) {
@@ -48,11 +55,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
   constexpr uint32_t kChunks = kFp8 ? D / 16 : D / 8;       // 16-byte loads per cache row
   constexpr uint32_t kPass = kThreads / kChunks;            // cache rows per pass of the workgroup
   constexpr int kLoads = kTileKeys / kPass;                 // passes per tile
-  constexpr int kTileBytes = kTileKeys * D * 2;
+  constexpr int kKeyBytes = kTileKeys * kKeyRow<D>;
+  constexpr int kValueBytes = kTileKeys * kValueRow<D>;
   static_assert(kLoads >= 1 && kTileKeys % kPass == 0, "a tile is whole passes");
-  __shared__ __attribute__((aligned(16))) char key_tile[2][kTileBytes];
-  __shared__ __attribute__((aligned(16))) char value_tile[2][kTileBytes];
-  __shared__ __attribute__((aligned(16))) int32_t table[4][kTileKeys];  // cache rows of tiles t .. t + 2
+  __shared__ __attribute__((aligned(16))) char key_tile[2][kKeyBytes];
+  __shared__ __attribute__((aligned(16))) char value_tile[2][kValueBytes];
+  // Places in the cache of tiles t .. t + 2: offsets of the keys' and the values'
+  // row, and for fp8 the row itself.
+  __shared__ ulong2 table[4][kTileKeys];
+  __shared__ uint32_t table_row[4][kFp8 ? kTileKeys : 1];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kTileKeys];
   const uint32_t tid = threadIdx.x;
   const uint32_t lane = lane_id();
@@ -111,13 +122,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
   auto load = [&](uint32_t t) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t row = (uint32_t)table[t & 3u][load_row + kPass * i];
-      kr[i] = *reinterpret_cast<const u32x4*>(key_base + a.cache.key_offset(row));
-      vr[i] = *reinterpret_cast<const u32x4*>(value_base + a.cache.value_offset(row));
+      const ulong2 at = table[t & 3u][load_row + kPass * i];
+      kr[i] = *reinterpret_cast<const u32x4*>(key_base + at.x);
+      vr[i] = *reinterpret_cast<const u32x4*>(value_base + at.y);
     }
     if constexpr (kFp8) {
       if (tid < 2u * kTileKeys) {
-        const uint32_t row = (uint32_t)table[t & 3u][tid % kTileKeys];
+        const uint32_t row = table_row[t & 3u][tid % kTileKeys];
         sr = (tid < kTileKeys ? a.cache.key_scales : a.cache.value_scales)[(uint64_t)row * a.cache.kv_heads + g];
       }
     }
@@ -129,122 +140,180 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
     for (int i = 0; i < kLoads; ++i) {
       const uint32_t row = load_row + kPass * i;
       if constexpr (kFp8) {
-        *reinterpret_cast<uint4*>(keys + key_place<D>(row, 2u * load_chunk)) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].x, kr[i].y));
-        *reinterpret_cast<uint4*>(keys + key_place<D>(row, 2u * load_chunk + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].z, kr[i].w));
-        *reinterpret_cast<uint4*>(values + tile_value_place<D>(row, 2u * load_chunk)) = fp8x8_to_bf16x8_paired(make_uint2(vr[i].x, vr[i].y));
-        *reinterpret_cast<uint4*>(values + tile_value_place<D>(row, 2u * load_chunk + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(vr[i].z, vr[i].w));
+        *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + 32u * load_chunk) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].x, kr[i].y));
+        *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + 32u * load_chunk + 16u) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].z, kr[i].w));
+        *reinterpret_cast<uint4*>(values + row * kValueRow<D> + 32u * load_chunk) = fp8x8_to_bf16x8_paired(make_uint2(vr[i].x, vr[i].y));
+        *reinterpret_cast<uint4*>(values + row * kValueRow<D> + 32u * load_chunk + 16u) = fp8x8_to_bf16x8_paired(make_uint2(vr[i].z, vr[i].w));
       } else {
-        *reinterpret_cast<u32x4*>(keys + key_place<D>(row, load_chunk)) = kr[i];
-        *reinterpret_cast<u32x4*>(values + tile_value_place<D>(row, load_chunk)) = vr[i];
+        *reinterpret_cast<u32x4*>(keys + row * kKeyRow<D> + 16u * load_chunk) = kr[i];
+        *reinterpret_cast<u32x4*>(values + row * kValueRow<D> + 16u * load_chunk) = vr[i];
       }
     }
     if constexpr (kFp8) {
       if (tid < 2u * kTileKeys) scales[t & 1u][tid / kTileKeys][tid % kTileKeys] = sr;
     }
   };
-  // Places of this lane in a transposed read of 16 keys x 32 dims, by 32-dim block.
-  uint32_t tr_place[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-    tr_place[i] = tile_value_place<D>(4u * half + ((lane & 15u) >> 2), 4u * i + 2u * ((lane >> 4) & 1u) + ((lane & 3u) >> 1)) +
-                  8u * (lane & 1u);
+  // This lane's places: keys row `col`, chunk `half`; values in a transposed read
+  // of 16 keys x 32 dims.
+  const uint32_t key_at = col * kKeyRow<D> + 16u * half;
+  const uint32_t value_at = (4u * half + ((lane & 15u) >> 2)) * kValueRow<D> + 32u * ((lane >> 4) & 1u) + 8u * (lane & 3u);
 
+  // One tile for the wave's rows, 32 keys at a time, so that the products of one
+  // half run under the exponentials of the other: a dependent product holds up
+  // the wave, but between two of them other instructions issue.  Operands are
+  // read from LDS a batch ahead of their products.
   auto compute = [&](uint32_t t) {
     const uint32_t key0 = begin + t * kTileKeys;
     if (key0 >= some_see) return;
-    const char* keys = key_tile[t & 1u];
-    const char* values = value_tile[t & 1u];
+    const char* keys = key_tile[t & 1u] + key_at;
+    const char* values = value_tile[t & 1u] + value_at;
+    constexpr int kSteps = D / 16;
+    uint4 ka[kSteps], kb[kSteps];
     floatx16 x[2];
+    auto read_key = [&](uint32_t s, uint32_t step) {
+      return *reinterpret_cast<const uint4*>(keys + 32u * s * kKeyRow<D> + 32u * step);
+    };
+    // x[s][4 b + i]: key 32 s + 8 b + 4 half + i.  Scores less the reference, in
+    // powers of two, hidden ones -inf, and their maximum.
+    auto scores = [&](uint32_t s) {
+      float most = -INFINITY;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+      for (int b = 0; b < 4; ++b) {
+        floatx4 by = {a.scale, a.scale, a.scale, a.scale};
+        if constexpr (kFp8) by *= *reinterpret_cast<const floatx4*>(&scales[t & 1u][0][32 * s + 8 * b + 4 * half]);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-        x[s] = mfma_32x32x16(Tag{}, *reinterpret_cast<const uint4*>(keys + key_place<D>(32u * s + col, 2u * j + half)), q[j], x[s]);
-    }
-    // x[s][4 a + i]: key 32 s + 8 a + 4 half + i
-    if constexpr (kFp8) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const floatx4 ks = *reinterpret_cast<const floatx4*>(&scales[t & 1u][0][32 * s + 8 * b + 4 * half]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[s][4 * b + i] *= ks[i];
-        }
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[s][e] = fmaf(x[s][e], a.scale, -reference);
-    if (key0 + kTileKeys > all_see) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < 4; ++i) x[s][4 * b + i] = fmaf(x[s][4 * b + i], by[i], -reference);
+      }
+      if (key0 + 32u * s + 32u > all_see) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           x[s][e] = key0 + 32u * s + 8u * (e / 4) + 4u * half + (e % 4) < sees ? x[s][e] : -INFINITY;
-    }
-    float most = fmaxf(x[0][0], x[1][0]);
+      }
 #pragma unroll
-    for (int e = 1; e < 16; ++e) most = fmaxf(most, fmaxf(x[0][e], x[1][e]));
-    if (t == 0 || __any(most > kLift + kSlack)) {
+      for (int e = 0; e < 16; e += 2) most = fmaxf(fmaxf(most, x[s][e]), x[s][e + 1]);
+      return most;
+    };
+    auto raise_by = [&](float most, bool first) {
       most = fmaxf(most, __shfl_xor(most, 32, kWave)) - kLift;
-      const float raise = t == 0 ? (most == -INFINITY ? 0.f : most) : fmaxf(most, 0.f);
+      const float raise = first ? (most == -INFINITY ? 0.f : most) : fmaxf(most, 0.f);
       reference += raise;
       const float shrink = exp2_fast(-raise);
       total *= shrink;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) o[i] *= shrink;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) x[s] -= raise;
-    }
-    uint4 p[4];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
+      return raise;
+    };
+    float weight[2][16];
+    auto weigh = [&](uint32_t s) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        x[s][e] = exp2_fast(x[s][e]);
-        total += x[s][e];
+        weight[s][e] = exp2_fast(x[s][e]);
+        total += weight[s][e];
       }
+    };
+    auto packed = [&](uint32_t s, uint32_t u) {
+      const float* p = &weight[s][8 * u];
+      floatx4 w[2] = {{p[0], p[1], p[2], p[3]}, {p[4], p[5], p[6], p[7]}};
       if constexpr (kFp8) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const floatx4 vs = *reinterpret_cast<const floatx4*>(&scales[t & 1u][1][32 * s + 8 * b + 4 * half]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[s][4 * b + i] *= vs[i];
-        }
+        for (int b = 0; b < 2; ++b)
+          w[b] *= *reinterpret_cast<const floatx4*>(&scales[t & 1u][1][32 * s + 16 * u + 8 * b + 4 * half]);
       }
+      return make_uint4(pack2(Tag{}, w[0][0], w[0][1]), pack2(Tag{}, w[0][2], w[0][3]), pack2(Tag{}, w[1][0], w[1][1]),
+                        pack2(Tag{}, w[1][2], w[1][3]));
+    };
+    auto read_value = [&](uint32_t u, uint32_t i) {
+      const uint2 lo = read_transposed(values + 16u * u * kValueRow<D> + 64u * i);
+      const uint2 hi = read_transposed(values + (16u * u + 8u) * kValueRow<D> + 64u * i);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
+
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        p[2 * s + u] = make_uint4(pack2(Tag{}, x[s][8 * u], x[s][8 * u + 1]), pack2(Tag{}, x[s][8 * u + 2], x[s][8 * u + 3]),
-                                  pack2(Tag{}, x[s][8 * u + 4], x[s][8 * u + 5]), pack2(Tag{}, x[s][8 * u + 6], x[s][8 * u + 7]));
+    for (int j = 0; j < kSteps; ++j) ka[j] = read_key(0, j);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[0][e] = x[1][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      kb[j] = read_key(1, j);
+      x[0] = mfma_32x32x16(Tag{}, ka[j], q[j], x[0]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    const float most0 = scores(0);
+    // A row that sees any key of the piece sees its first: the first tile's first
+    // half sets the reference.
+    if (t == 0 || __any(most0 > kLift + kSlack)) x[0] -= raise_by(most0, t == 0);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+    for (int j = 0; j < kSteps; ++j) x[1] = mfma_32x32x16(Tag{}, kb[j], q[j], x[1]);
+    weigh(0);
+    uint4 va[D / 32], vb[D / 32];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint2 lo = read_transposed(values + tr_place[i] + (16 * u) * D * 2);
-        const uint2 hi = read_transposed(values + tr_place[i] + (16 * u + 8) * D * 2);
-        o[i] = mfma_32x32x16(Tag{}, make_uint4(lo.x, lo.y, hi.x, hi.y), p[u], o[i]);
+    for (int i = 0; i < D / 32; ++i) va[i] = read_value(0, i);
+    interleave(kSteps, 48 / kSteps);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) pin(weight[0][e]);
+    const float most1 = scores(1);
+    if (__any(most1 > kLift + kSlack)) {
+      const float raise = raise_by(most1, false);
+      const float shrink = exp2_fast(-raise);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) weight[0][e] *= shrink;
+      x[1] -= raise;
+    }
+    {
+      const uint4 p0 = packed(0, 0), p1 = packed(0, 1);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        vb[i] = read_value(1, i);
+        o[i] = mfma_32x32x16(Tag{}, va[i], p0, o[i]);
       }
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        va[i] = read_value(2, i);
+        o[i] = mfma_32x32x16(Tag{}, vb[i], p1, o[i]);
+      }
+      weigh(1);
+    }
+    {
+      const uint4 p0 = packed(1, 0), p1 = packed(1, 1);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        vb[i] = read_value(3, i);
+        o[i] = mfma_32x32x16(Tag{}, va[i], p0, o[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] = mfma_32x32x16(Tag{}, vb[i], p1, o[i]);
+    }
   };
 
   if (begin < end) {
     const uint32_t tiles = (end - begin + kTileKeys - 1u) / kTileKeys;
-    auto look_up = [&](uint32_t t) { return (int32_t)cache_row(a, pages, min(begin + t * kTileKeys + tid % kTileKeys, end - 1u)); };
-    if (tid < 2u * kTileKeys) table[tid / kTileKeys][tid % kTileKeys] = look_up(tid / kTileKeys);
+    // The look-up of a tile's cache rows, by its first 64 threads: the page id's
+    // load two tiles ahead of the rows' and before them, its use after the tile.
+    auto key_of = [&](uint32_t t) { return min(begin + t * kTileKeys + tid % kTileKeys, end - 1u); };
+    auto look_page = [&](uint32_t t) { return (uint32_t)pages[key_of(t) >> a.cache.shift]; };
+    auto place = [&](uint32_t t, uint32_t page) {
+      const uint32_t row = (min(page, a.cache.pages - 1u) << a.cache.shift) | (key_of(t) & ((1u << a.cache.shift) - 1u));
+      table[t & 3u][tid % kTileKeys] = ulong2{a.cache.key_offset(row), a.cache.value_offset(row)};
+      if constexpr (kFp8) table_row[t & 3u][tid % kTileKeys] = row;
+    };
+    if (tid < 2u * kTileKeys) place(tid / kTileKeys, look_page(tid / kTileKeys));
     __syncthreads();
     load(0);
     stage(0);
     __syncthreads();
     for (uint32_t t = 0; t < tiles; ++t) {
+      uint32_t page = 0;
+      if (wave == 0) page = look_page(t + 2u);
+      __builtin_amdgcn_sched_barrier(0);
       load(t + 1u);  // past the end: the last key again
-      int32_t next = 0;
-      if (tid < (uint32_t)kTileKeys) next = look_up(t + 2u);
+      __builtin_amdgcn_sched_barrier(0);
       compute(t);
       stage(t + 1u);
-      if (tid < (uint32_t)kTileKeys) table[(t + 2u) & 3u][tid] = next;
+      if (wave == 0) {
+        asm volatile("" : "+v"(page));  // nothing of what follows, and so no wait, moves up to the load
+        place(t + 2u, page);
+      }
       __syncthreads();
     }
   }
