@@ -22,6 +22,7 @@ namespace dsa {
 namespace {
 
 constexpr uint32_t kStep = 32;   // keys per wave and step
+constexpr uint32_t kLeastSteps = 4;  // of a piece: one for each wave
 constexpr uint32_t kGroup = 8;   // steps whose cache rows a wave looks up at a time
 // Workgroups that run at a time: what the registers of each head_dim allow on 256
 // CUs.  Work is cut to fill them once.
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     slot = item * a.splits;
   } else {
     Piece piece;
-    if (!find_piece(a, id, piece)) return;
+    if (!find_piece<16, kStep, kLeastSteps>(a, id, piece)) return;
     sequence = piece.sequence;
     token0 = piece.span.first;
     row0 = 0;
@@ -127,8 +128,8 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     length = piece.keys;
     // row r sees keys below seen0 + r / group + 1 of a causal chunk; the last sees all
     seen0 = length - piece.span.count;  // may wrap below zero: see `sees`
-    begin = min(piece.index * piece.units * kUnit, length);
-    end = min(begin + piece.units * kUnit, length);
+    begin = (uint32_t)min((uint64_t)piece.index * piece.units * kStep, (uint64_t)length);
+    end = (uint32_t)min((uint64_t)begin + (uint64_t)piece.units * kStep, (uint64_t)length);
     pieces = piece.count;
     index = piece.index;
     tile_slot = slot = piece.slot;
@@ -498,15 +499,18 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
     }
     if (tokens_of(a, low).count * a.group < a.least_rows) return;
   }
-  const float2* sums = a.part_sum + row * a.splits;
-  const float* parts = a.part_out + row * a.splits * D + dim;
+  const uint2 of = a.part_of[row];
+  if (of.y == 1u) return;
+  const uint32_t apart = a.cache.kv_heads * a.part_rows;
+  const float2* sums = a.part_sum + of.x;
+  const float* parts = a.part_out + (uint64_t)of.x * D + dim;
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};
   float top = kNoKeys;
   float total = 0.f;
 #pragma unroll 4
-  for (uint32_t p = 0; p < a.splits; ++p) {
-    const float2 s = sums[p];
-    const floatx4 v = *reinterpret_cast<const floatx4*>(parts + (uint64_t)p * D);
+  for (uint32_t p = 0; p < of.y; ++p) {
+    const float2 s = sums[p * apart];
+    const floatx4 v = *reinterpret_cast<const floatx4*>(parts + (uint64_t)p * apart * D);
     const float raised = fmaxf(top, s.x);
     const float keep = exp2_fast(top - raised);
     const float take = exp2_fast(s.x - raised);
@@ -539,7 +543,6 @@ void launch_combine(const PagedAttentionArgs& a, int32_t dim, hipStream_t s) {
 }
 
 int combine(const PagedAttentionArgs& a, int32_t dim, int32_t dtype, hipStream_t s) {
-  if (a.splits == 1) return 0;
   if (dtype == kBF16)
     launch_combine<Bf16Tag>(a, dim, s);
   else
@@ -613,27 +616,31 @@ int check_common(const dsa_paged_cache* cache, const void* queries, int64_t quer
 
 constexpr int64_t kStreamRows = 16;  // most rows of a sequence that the stream kernel takes
 
-// Workspace: the counters, at one place for every shape, then results of
-// `parts` rows and their sums.
-int64_t part_bytes(int64_t parts, int64_t dim) { return parts ? kCounters * 4 + parts * (dim + 2) * 4 : 0; }
+// Workspace: the counters, at one place for every shape, then `parts` outputs,
+// their sums and where `rows` rows have theirs.
+int64_t part_bytes(int64_t parts, int64_t rows, int64_t dim) {
+  return parts ? kCounters * 4 + parts * (dim + 2) * 4 + rows * 8 : 0;
+}
 
-int take_workspace(PagedAttentionArgs& a, int64_t parts, int64_t dim, void* workspace, int64_t bytes) {
+int take_workspace(PagedAttentionArgs& a, int64_t parts, int64_t rows, int64_t dim, void* workspace, int64_t bytes) {
   if (parts == 0) return 0;
-  if (!workspace || bytes < part_bytes(parts, dim) || reinterpret_cast<uintptr_t>(workspace) % 16)
+  if (!workspace || bytes < part_bytes(parts, rows, dim) || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(DSA_STATUS_WORKSPACE_TOO_SMALL, "paged attention needs %lld bytes of 16-byte aligned workspace",
-                (long long)part_bytes(parts, dim));
+                (long long)part_bytes(parts, rows, dim));
   a.arrived = static_cast<uint32_t*>(workspace);
   a.part_out = reinterpret_cast<float*>(a.arrived + kCounters);
   a.part_sum = reinterpret_cast<float2*>(a.part_out + parts * dim);
+  a.part_of = reinterpret_cast<uint2*>(a.part_sum + parts);
   return 0;
 }
 
+// Which kernels a call runs, and what it cuts.
 struct Plan {
-  int64_t stream_items, chunk_items;  // 0: no sequence of that kind
-  uint32_t cuts, part_rows;           // stream kernel
-  uint32_t chunk_splits;
-  int64_t stream_pieces;  // at most
-  int64_t parts;
+  uint32_t stream_cuts, stream_rows;  // rows of a part
+  int64_t stream_pieces;              // at most; 0: no sequence of few rows
+  uint32_t chunk_cuts;                // 0: more row tiles than could be cut to use
+  int64_t chunk_pieces;
+  int64_t parts, rows;
 };
 
 Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens, int64_t heads, int64_t capacity,
@@ -642,19 +649,28 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
   const int64_t group = heads / kv_heads;
   Plan p = {};
   const int64_t each = tokens / sequences * group;
-  if (!uniform || each <= kStreamRows) p.stream_items = uniform ? sequences : (tokens < sequences ? tokens : sequences);
-  if (!uniform || each > kStreamRows) p.chunk_items = row_tiles(sequences, tokens, group, uniform, kChunkRows);
-  if (p.stream_items) {
-    p.cuts = (uint32_t)((resident_workgroups(cache->head_dim) + kv_heads - 1) / kv_heads);
-    p.part_rows = (uint32_t)(uniform ? each : kStreamRows);
-    const int64_t least = kLeastUnits * kUnit;
-    p.stream_pieces = p.stream_items * ((capacity + least - 1) / least);
-    if (p.stream_pieces > p.stream_items + p.cuts) p.stream_pieces = p.stream_items + p.cuts;
-    p.parts = 2 * kv_heads * p.part_rows * p.cuts;
+  const int64_t cuts = (resident_workgroups(cache->head_dim) + kv_heads - 1) / kv_heads;
+  auto at_most = [&](int64_t tiles, int64_t least) {
+    const int64_t pieces = tiles * ((capacity + least - 1) / least);
+    return pieces < tiles + cuts ? pieces : tiles + cuts;
+  };
+  if (!uniform || each <= kStreamRows) {
+    const int64_t tiles = uniform ? sequences : (tokens < sequences ? tokens : sequences);
+    p.stream_cuts = (uint32_t)cuts;
+    p.stream_rows = (uint32_t)(uniform ? each : kStreamRows);
+    p.stream_pieces = at_most(tiles, kLeastSteps * kStep);
+    p.parts = 2 * cuts * kv_heads * p.stream_rows;
   }
-  if (p.chunk_items) {
-    p.chunk_splits = splits_for(p.chunk_items * kv_heads, 512, capacity, 256);
-    if (p.chunk_splits > 1 && p.parts < tokens * heads * p.chunk_splits) p.parts = tokens * heads * p.chunk_splits;
+  if (!uniform || each > kStreamRows) {
+    const int64_t tiles = row_tiles(sequences, tokens, group, uniform, kChunkRows);
+    if (tiles >= 2 * cuts) {
+      p.chunk_pieces = tiles;
+    } else {
+      p.chunk_cuts = (uint32_t)cuts;
+      p.chunk_pieces = at_most(tiles, kLeastChunkKeys);
+      p.rows = tokens * heads;
+      if (p.parts < 2 * cuts * kv_heads * kChunkRows) p.parts = 2 * cuts * kv_heads * kChunkRows;
+    }
   }
   return p;
 }
@@ -687,7 +703,7 @@ extern "C" int64_t dsa_paged_attention_workspace_bytes(const dsa_paged_cache* ca
                                                        int32_t heads, int64_t columns, int32_t uniform) {
   if (!sizes_valid(cache, sequences, tokens, heads)) return 0;
   const Plan p = dense_plan(cache, sequences, tokens, heads, columns * cache->page_size, uniform != 0);
-  return part_bytes(p.parts, cache->head_dim);
+  return part_bytes(p.parts, p.rows, cache->head_dim);
 }
 
 extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
@@ -707,22 +723,23 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
   hipStream_t s = static_cast<hipStream_t>(stream);
   // A sequence of few rows (one decoded token, a few drafted ones) is bound by
   // reading its cache, one of many by the products: a mixed batch has both.
-  if (int st = take_workspace(a, p.parts, cache->head_dim, workspace, workspace_bytes)) return st;
-  if (p.stream_items) {
-    a.cuts = p.cuts;
-    a.part_rows = p.part_rows;
+  if (int st = take_workspace(a, p.parts, p.rows, cache->head_dim, workspace, workspace_bytes)) return st;
+  if (p.stream_pieces) {
+    a.cuts = p.stream_cuts;
+    a.part_rows = p.stream_rows;
     a.least_rows = 1;
     a.most_rows = kStreamRows;
     if (int st = launch<false>(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
   }
-  if (p.chunk_items) {
-    a.splits = p.chunk_splits;
+  if (p.chunk_pieces) {
+    a.cuts = p.chunk_cuts;
+    a.part_rows = kChunkRows;
     a.least_rows = kStreamRows + 1;
     a.most_rows = 0xffffffffu;
-    const int64_t grid = p.chunk_items * a.splits * a.cache.kv_heads;
+    const int64_t grid = p.chunk_pieces * a.cache.kv_heads;
     DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
     if (int st = launch_paged_chunk(a, cache->head_dim, cache->dtype, (uint32_t)grid, s)) return st;
-    return combine(a, cache->head_dim, dtype, s);
+    if (p.chunk_cuts) return combine(a, cache->head_dim, dtype, s);
   }
   return 0;
 }
@@ -731,7 +748,7 @@ extern "C" int64_t dsa_paged_selected_workspace_bytes(const dsa_paged_cache* cac
                                                       int64_t k) {
   if (!sizes_valid(cache, 1, tokens, heads)) return 0;
   const SelectedPlan p = selected_plan(cache, tokens, heads, k);
-  return part_bytes(p.parts, cache->head_dim);
+  return part_bytes(p.parts, 0, cache->head_dim);
 }
 
 extern "C" int dsa_paged_selected_attention(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
@@ -755,6 +772,6 @@ extern "C" int dsa_paged_selected_attention(const dsa_paged_cache* cache, const 
   a.k = (uint32_t)k;
   a.out = static_cast<char*>(out);
   a.lse = lse;
-  if (int st = take_workspace(a, p.parts, cache->head_dim, workspace, workspace_bytes)) return st;
+  if (int st = take_workspace(a, p.parts, 0, cache->head_dim, workspace, workspace_bytes)) return st;
   return launch<true>(a, cache, dtype, p.items * p.splits, static_cast<hipStream_t>(stream));
 }

@@ -34,19 +34,20 @@ struct PagedAttentionArgs {
   uint32_t k;
   uint32_t sequences, tokens, heads;
   uint32_t group;           // query heads per kv head
-  uint32_t splits;          // pieces that a row's keys are cut into (not the dense stream kernel)
-  uint32_t cuts;            // dense stream kernel: pieces that the batch's keys are cut for
+  uint32_t splits;          // selected attention: pieces that a list is cut into
+  uint32_t cuts;            // else: pieces that the batch is cut for (0: no row tile is cut)
   uint32_t causal;
   uint32_t most_rows;       // sequences of more (token, head) rows per kv head are another kernel's
   uint32_t least_rows;
   float scale;              // times log2 e
   char* out;                // [tokens][heads][dim]
   float* lse;               // nullable: [tokens][heads]
-  // Pieces' results: the chunk kernel's by row, [tokens][heads][splits][dim]; the
-  // stream kernel's by piece, [slot][kv_heads][part_rows][dim].
+  // Results of the pieces of row tiles that have several, [slot][kv_heads]
+  // [part_rows]: outputs [dim], and {reference, sum}.
   float* part_out;
-  float2* part_sum;         // {reference, sum} of each
+  float2* part_sum;
   uint32_t part_rows;
+  uint2* part_of;           // chunk kernel: [tokens][heads] {part of the row's first piece, pieces}
   uint32_t* arrived;        // stream kernel: pieces of each row tile that are done; zero between calls
 };
 
@@ -77,63 +78,34 @@ __device__ __forceinline__ uint32_t cache_row(const PagedAttentionArgs& a, const
   return (page << a.cache.shift) | (key & ((1u << a.cache.shift) - 1u));
 }
 
-// A tile of `size` consecutive (token, head) rows of one kv head of a sequence.
-struct RowTile {
-  uint32_t sequence;
-  uint32_t index;  // of the tile among its sequence's
-  Span span;
-};
-
-// Tile `item` of the sequences of least_rows .. most_rows rows, counted over them
-// in order; every wave searches for itself.  False past the last.
-__device__ __forceinline__ bool find_row_tile(const PagedAttentionArgs& a, uint32_t item, uint32_t size, RowTile& tile) {
-  const uint32_t lane = lane_id();
-  for (uint32_t b = 0; b < a.sequences; b += kWave) {
-    Span s = {0, 0};
-    if (b + lane < a.sequences) s = tokens_of(a, b + lane);
-    const uint32_t n = s.count * a.group;
-    const uint32_t tiles = n < a.least_rows || n > a.most_rows ? 0u : (n + size - 1u) / size;
-    const uint32_t upto = wave_incl_scan(tiles);
-    const uint64_t owner = __ballot(item < upto);
-    if (owner) {
-      const int at = __builtin_ctzll(owner);
-      tile.sequence = b + (uint32_t)at;
-      tile.index = item - (uint32_t)__builtin_amdgcn_readlane(upto - tiles, at);
-      tile.span.first = (uint32_t)__builtin_amdgcn_readlane(s.first, at);
-      tile.span.count = (uint32_t)__builtin_amdgcn_readlane(s.count, at);
-      return true;
-    }
-    item -= (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
-  }
-  return false;
-}
-
-// One piece of the keys of a sequence of few rows (dense stream kernel).
-constexpr uint32_t kUnit = 32;         // keys that the batch is cut in
-constexpr uint32_t kLeastUnits = 4;    // of a piece: a step for each wave
-constexpr uint32_t kMostSplits = 256;  // pieces of a sequence
+// One piece of the work: a tile of a sequence's (token, head) rows of one kv head
+// against some of its keys.
+constexpr uint32_t kMostSplits = 256;  // pieces of a tile
 
 struct Piece {
   uint32_t sequence;
   Span span;
   uint32_t keys;   // of the sequence
-  uint32_t units;  // of every piece of the batch but a sequence's last
+  uint32_t tile;   // of the sequence's rows
+  uint32_t units;  // of every piece of the tile but the last
   uint32_t index, count;
-  uint32_t slot;   // of the sequence's first piece, where there are several
+  uint32_t slot;   // of the tile's first piece, where there are several
 };
 
-// Piece `id` of the batch.  All pieces are as long, whatever the sequences'
-// lengths, so every wave sums the batch's keys first: one load and a scan for up
-// to 64 sequences.  `cuts` pieces fill the GPU once, and a few more would run
-// alone after them (a batch of 128K to 56K fp8 keys took 194 us in 1040 pieces of
-// 1024 that run at a time); so for up to 64 sequences pieces are lengthened until
-// the sequences' last ones fit too.  At most cuts + sequences pieces, and at most
-// twice `cuts` of sequences that have several.
+// Piece `id` of the sequences of least_rows .. most_rows rows, in tiles of
+// kTileRows rows and units of kUnit keys, at least kLeast units a piece.  No piece
+// is longer than one length for the whole batch, whatever the sequences' lengths,
+// so every wave sums the batch's work first: one load and a scan for up to 64
+// sequences.  `cuts` pieces fill the GPU once, and a few more would run alone
+// after them; so for up to 64 sequences that length grows until the pieces fit.  A
+// tile is cut evenly (ragged fp16 chunks, us: 111, and 129 with the remainder in a
+// tile's last piece).  At most cuts + tiles pieces, and at most 2 cuts of tiles
+// that have several.
+template <uint32_t kTileRows, uint32_t kUnit, uint32_t kLeast>
 __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, uint32_t id, Piece& p) {
   const uint32_t lane = lane_id();
   Span span = {0, 0};
-  uint32_t keys = 0, units = 0;
-  bool mine = false;
+  uint32_t keys = 0, units = 0, tiles = 0;
   auto look = [&](uint32_t b) {
     span = {0, 0};
     keys = 0;
@@ -142,38 +114,48 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, uint32_t
       keys = keys_of(a, b + lane);
     }
     const uint32_t rows = span.count * a.group;
-    mine = rows >= a.least_rows && rows <= a.most_rows;
-    units = mine ? (keys + kUnit - 1u) / kUnit : 0u;
+    tiles = rows >= a.least_rows && rows <= a.most_rows ? (rows + kTileRows - 1u) / kTileRows : 0u;
+    units = tiles ? (keys + kUnit - 1u) / kUnit : 0u;
   };
-  uint64_t all = 0;
-  uint32_t most = 0;
-  for (uint32_t b = 0; b < a.sequences; b += kWave) {
-    look(b);
-    all += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(units), kWave - 1);
-    most = max(most, wave_max_u32(units));
-  }
-  p.units = max(max(kLeastUnits, (most + kMostSplits - 1u) / kMostSplits), (uint32_t)((all + a.cuts - 1u) / a.cuts));
-  if (a.sequences <= kWave) {
-    for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t pieces = mine ? max(1u, (units + p.units - 1u) / p.units) : 0u;
-      if ((uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(pieces), kWave - 1) <= a.cuts) break;
-      p.units += (p.units + 31u) / 32u;
+  auto pieces_of = [&](uint32_t each) { return max(1u, (units + each - 1u) / each); };
+  p.units = 0x7fffffffu;
+  if (a.cuts) {
+    uint64_t all = 0;
+    uint32_t most = 0;
+    for (uint32_t b = 0; b < a.sequences; b += kWave) {
+      look(b);
+      // (two scans: a sequence's tiles x units may pass 32 bits)
+      const uint64_t work = (uint64_t)tiles * units;
+      all += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan((uint32_t)(work & 0xffffffu)), kWave - 1);
+      all += (uint64_t)(uint32_t)__builtin_amdgcn_readlane(wave_incl_scan((uint32_t)(work >> 24)), kWave - 1) << 24;
+      most = max(most, wave_max_u32(units));
+    }
+    p.units = max(max(kLeast, (most + kMostSplits - 1u) / kMostSplits), (uint32_t)((all + a.cuts - 1u) / a.cuts));
+    if (a.sequences <= kWave) {
+      for (uint32_t i = 0; i < 8; ++i) {
+        if ((uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(tiles * pieces_of(p.units)), kWave - 1) <= a.cuts) break;
+        p.units += (p.units + 31u) / 32u;
+      }
     }
   }
   p.slot = 0;
   for (uint32_t b = 0; b < a.sequences; b += kWave) {
-    if (a.sequences > kWave) look(b);
-    const uint32_t pieces = mine ? max(1u, (units + p.units - 1u) / p.units) : 0u;
+    if (!a.cuts || a.sequences > kWave) look(b);
+    const uint32_t each = pieces_of(p.units);
+    const uint32_t pieces = tiles * each;
     const uint32_t upto = wave_incl_scan(pieces);
-    const uint32_t several = pieces > 1u ? pieces : 0u;
+    const uint32_t several = each > 1u ? pieces : 0u;
     const uint32_t slots = wave_incl_scan(several);
     const uint64_t owner = __ballot(id < upto);
     if (owner) {
       const int at = __builtin_ctzll(owner);
+      const uint32_t within = id - (uint32_t)__builtin_amdgcn_readlane(upto - pieces, at);
       p.sequence = b + (uint32_t)at;
-      p.index = id - (uint32_t)__builtin_amdgcn_readlane(upto - pieces, at);
-      p.count = (uint32_t)__builtin_amdgcn_readlane(pieces, at);
-      p.slot += (uint32_t)__builtin_amdgcn_readlane(slots - several, at);
+      p.count = (uint32_t)__builtin_amdgcn_readlane(each, at);
+      p.tile = within / p.count;
+      p.index = within % p.count;
+      p.slot += (uint32_t)__builtin_amdgcn_readlane(slots - several, at) + p.tile * p.count;
+      p.units = max(1u, ((uint32_t)__builtin_amdgcn_readlane(units, at) + p.count - 1u) / p.count);
       p.keys = (uint32_t)__builtin_amdgcn_readlane(keys, at);
       p.span.first = (uint32_t)__builtin_amdgcn_readlane(span.first, at);
       p.span.count = (uint32_t)__builtin_amdgcn_readlane(span.count, at);
@@ -227,7 +209,8 @@ __device__ __forceinline__ void store_out(const PagedAttentionArgs& a, uint64_t 
   if (a.lse && dim == 0) a.lse[row] = total == 0.f ? -INFINITY : (reference + log2f(total)) * kLn2;
 }
 
-constexpr int kChunkRows = 128;  // rows of a workgroup of the chunk kernel
+constexpr int kChunkRows = 128;        // rows of a workgroup of the chunk kernel
+constexpr int kLeastChunkKeys = 256;   // keys of a piece of it
 
 // paged_chunk.hip: the chunk kernel over `grid` workgroups.
 int launch_paged_chunk(const PagedAttentionArgs& a, int32_t dim, int32_t cache_dtype, uint32_t grid, hipStream_t s);

@@ -17,7 +17,8 @@
 namespace dsa {
 namespace {
 
-constexpr int kTileKeys = 64;
+constexpr uint32_t kTileKeys = 64;
+constexpr uint32_t kLeastTiles = kLeastChunkKeys / kTileKeys;  // of a piece
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
@@ -71,27 +72,27 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
   const uint32_t col = lane & 31u;
   const uint32_t half = lane >> 5;
 
+  // Heads vary fastest: workgroups go round-robin over the XCDs, so that a kv
+  // head's keys meet all of its rows in few L2s.
   const uint32_t g = blockIdx.x % a.cache.kv_heads;
-  const uint32_t rest = blockIdx.x / a.cache.kv_heads;
-  const uint32_t piece = rest % a.splits;
-  RowTile tile;
-  if (!find_row_tile(a, rest / a.splits, kRows, tile)) return;
-  const uint32_t length = keys_of(a, tile.sequence);
-  const uint32_t rows = tile.span.count * a.group;
+  Piece piece;
+  if (!find_piece<kRows, kTileKeys, kLeastTiles>(a, blockIdx.x / a.cache.kv_heads, piece)) return;
+  const Span span = piece.span;
+  const uint32_t length = piece.keys;
+  const uint32_t rows = span.count * a.group;
   // The last tile of a sequence first: a causal chunk's last rows see most.
-  const uint32_t row0 = ((rows + kRows - 1u) / kRows - 1u - tile.index) * kRows;
+  const uint32_t row0 = ((rows + kRows - 1u) / kRows - 1u - piece.tile) * kRows;
 
   // Row r sees keys below `seen(r)`.
   auto seen = [&](uint32_t r) {
-    return a.causal ? (uint32_t)max(0, (int32_t)(length - tile.span.count + r / a.group + 1u)) : length;
+    return a.causal ? (uint32_t)max(0, (int32_t)(length - span.count + r / a.group + 1u)) : length;
   };
   const uint32_t visible = seen(min(row0 + kRows, rows) - 1u);
-  const uint32_t chunk = max(256u, ((visible + a.splits - 1u) / a.splits + kTileKeys - 1u) & ~(kTileKeys - 1u));
-  const uint32_t begin = min(piece * chunk, visible);
-  const uint32_t end = min(begin + chunk, visible);
+  const uint32_t begin = (uint32_t)min((uint64_t)piece.index * piece.units * kTileKeys, (uint64_t)visible);
+  const uint32_t end = (uint32_t)min((uint64_t)begin + (uint64_t)piece.units * kTileKeys, (uint64_t)visible);
   const uint32_t wave_row = min(row0 + 32u * wave, rows - 1u);
   const uint32_t my_row = min(row0 + 32u * wave + col, rows - 1u);
-  const uint32_t my_token = tile.span.first + my_row / a.group;
+  const uint32_t my_token = span.first + my_row / a.group;
   const uint32_t my_head = g * a.group + my_row % a.group;
   const uint32_t sees = min(seen(my_row), end);
   const uint32_t all_see = min(seen(wave_row), end);                          // every row of the wave sees these
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
   float reference = 0.f;  // set by the first tile: a row that sees any key of the piece sees its first
   float total = 0.f;
 
-  const int32_t* pages = a.page_table + (int64_t)tile.sequence * a.table_stride;
+  const int32_t* pages = a.page_table + (int64_t)piece.sequence * a.table_stride;
   const uint32_t load_row = tid / kChunks;
   const uint32_t load_chunk = tid % kChunks;
   const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * load_chunk;
@@ -322,19 +323,21 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
   if (total == 0.f) reference = kNoKeys;
   if (row0 + 32u * wave + col >= rows) return;
   const uint64_t my_out = (uint64_t)my_token * a.heads + my_head;
+  const uint64_t part = ((uint64_t)(piece.slot + piece.index) * a.cache.kv_heads + g) * kRows + 32u * wave + col;
+  if (half == 0 && a.cuts) {
+    if (piece.index == 0) a.part_of[my_out] = make_uint2((uint32_t)part, piece.count);
+    if (piece.count > 1u) a.part_sum[part] = make_float2(reference, total);
+  }
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const uint32_t dim = 32u * i + 8u * b + 4u * half;
-      const floatx4 part = {o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
-      if (a.splits > 1) {
-        const uint64_t at = my_out * a.splits + piece;
-        *reinterpret_cast<floatx4*>(a.part_out + at * D + dim) = part;
-        if (dim == 0) a.part_sum[at] = make_float2(reference, total);
-      } else {
-        store_out<Tag, D>(a, my_out, dim, part, reference, total);
-      }
+      const floatx4 v = {o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
+      if (piece.count > 1u)
+        *reinterpret_cast<floatx4*>(a.part_out + part * D + dim) = v;
+      else
+        store_out<Tag, D>(a, my_out, dim, v, reference, total);
     }
 }
 
