@@ -71,9 +71,17 @@ struct Tile {
   float scale;  // fp8: lane l < 32 the key scale of key l, else the value scale of key l - 32
 };
 
-template <class Tag, bool kFp8, int D, bool kSelected>
+// What a workgroup of the stream kernel takes.
+enum Work {
+  kDense,     // a piece of a sequence's keys
+  kSelected,  // a piece of a token's list
+  kSolo,      // four tokens' lists, each wave one by itself
+};
+
+template <class Tag, bool kFp8, int D, Work kWork>
 __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAttentionArgs a) {
   using T = Tile<kFp8, D>;
+  constexpr bool kListed = kWork != kDense;
   constexpr uint32_t kAhead = kFp8 ? 2 : 1;  // steps on their way in registers
   constexpr int kQ = D / 32;  // k-steps of the first product
   constexpr int kO = D / 16;  // dim tiles of the second
@@ -94,18 +102,19 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   // rows meet in few L2s; but the heads of an fp8 piece, whose scales share cache
   // lines, follow each other on one XCD (16 bit / fp8 decode steps, us: heads
   // fastest 385 / 209, heads on one XCD 397 / 191).
-  constexpr bool kTogether = kFp8 && !kSelected;
+  constexpr bool kTogether = kFp8 && !kListed;
   const uint32_t turn = kTogether ? blockIdx.x / kXcds : blockIdx.x;
   const uint32_t g = turn % a.cache.kv_heads;
   const uint32_t id = kTogether ? turn / a.cache.kv_heads * kXcds + blockIdx.x % kXcds : turn / a.cache.kv_heads;
 
   uint32_t sequence, token0, row0, rows, length, begin, end, pieces, index, slot, tile_slot, seen0 = 0;
-  if constexpr (kSelected) {
+  if constexpr (kListed) {
     // a piece of the list of a tile of a token's heads
     const uint32_t tiles = (a.group + 15u) / 16u;
-    const uint32_t item = id / a.splits;
-    const uint32_t piece = id % a.splits;
+    const uint32_t item = kWork == kSolo ? 4u * id + wave : id / a.splits;
+    const uint32_t piece = kWork == kSolo ? 0u : id % a.splits;
     token0 = item / tiles;
+    if (kWork == kSolo && token0 >= a.tokens) return;
     row0 = item % tiles * 16u;
     rows = a.group;
     sequence = sequence_of(a, token0);
@@ -137,15 +146,15 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
 
   // This lane's row, and the keys it sees.
   const uint32_t my_row = min(row0 + col, rows - 1u);
-  const uint32_t my_token = kSelected ? token0 : token0 + my_row / a.group;
-  const uint32_t my_head = g * a.group + (kSelected ? my_row : my_row % a.group);
-  const bool partly = !kSelected && a.causal;
+  const uint32_t my_token = kListed ? token0 : token0 + my_row / a.group;
+  const uint32_t my_head = g * a.group + (kListed ? my_row : my_row % a.group);
+  const bool partly = !kListed && a.causal;
   const uint32_t sees = partly ? (uint32_t)max(0, (int32_t)(seen0 + my_row / a.group + 1u)) : end;
   const uint32_t all_see = partly ? (uint32_t)max(0, (int32_t)(seen0 + row0 / a.group + 1u)) : end;
 
   auto out_row = [&](uint32_t r) {
-    const uint64_t token = kSelected ? token0 : token0 + (row0 + r) / a.group;
-    return token * a.heads + g * a.group + (kSelected ? row0 + r : (row0 + r) % a.group);
+    const uint64_t token = kListed ? token0 : token0 + (row0 + r) / a.group;
+    return token * a.heads + g * a.group + (kListed ? row0 + r : (row0 + r) % a.group);
   };
   auto part_at = [&](uint32_t piece, uint32_t r) {
     return ((uint64_t)piece * a.cache.kv_heads + g) * a.part_rows + r;
@@ -165,7 +174,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * load_chunk;
   const char* value_base = a.cache.values + g * a.cache.value_head + 16u * load_chunk;
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
-  const int64_t* list = kSelected ? a.indices + (int64_t)token0 * a.index_stride : nullptr;
+  const int64_t* list = kListed ? a.indices + (int64_t)token0 * a.index_stride : nullptr;
 
   floatx4 o[kO];
 #pragma unroll
@@ -179,10 +188,13 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   for (int i = 0; i < kO; ++i)
     tr_place[i] = tile_place<2 * D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1)) + 8u * (col & 1u);
 
-  // The wave's steps are every fourth of the piece, step s at keys first_key(s).
+  // The wave's steps are every fourth of the piece (all of its own list), step s at
+  // keys first_key(s).
+  constexpr uint32_t kApart = kWork == kSolo ? 1 : 4;
+  const uint32_t from = kWork == kSolo ? 0u : wave;
   const uint32_t steps = (end - begin + kStep - 1u) / kStep;
-  const uint32_t own = steps > wave ? (steps - wave + 3u) / 4u : 0u;
-  auto first_key = [&](uint32_t step) { return begin + (4u * step + wave) * kStep; };
+  const uint32_t own = steps > from ? (steps - from + kApart - 1u) / kApart : 0u;
+  auto first_key = [&](uint32_t step) { return begin + (kApart * step + from) * kStep; };
   auto rows_at = [&](uint32_t step) { return table[wave][step / kGroup % 2u] + step % kGroup * kStep; };
 
   // The cache rows of a group of steps, in three parts so that a group's look-ups
@@ -195,7 +207,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     for (uint32_t j = 0; j < kRounds; ++j) {
       const uint32_t at = first_key(group * kGroup + 2u * j + lane / 32u) + lane % 32u;
       key[j] = min(at, end - 1u);
-      if constexpr (kSelected) {
+      if constexpr (kListed) {
         const int64_t named = list[key[j]];
         key[j] = at < end && named >= 0 && named < (int64_t)length ? (uint32_t)named : 0x80000000u;
       }
@@ -239,13 +251,13 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     for (int i = 0; i < T::kPasses; ++i) {
       const uint32_t r = T::kRows * i + load_row;
       bool drop = false;
-      if constexpr (kSelected) drop = at[r] < 0;  // padding's weight is 0, which NaN would survive
+      if constexpr (kListed) drop = at[r] < 0;  // padding's weight is 0, which NaN would survive
 #pragma unroll
       for (int j = 0; j < T::kLoads; ++j) {
         const uint32_t c = T::kLanes * j + load_chunk;
         *reinterpret_cast<u32x4*>(my_keys + tile_place<T::kBytes>(r, c)) = t.k[i][j];
         u32x4 v = t.v[i][j];
-        if (kSelected && drop) v = u32x4{0u, 0u, 0u, 0u};
+        if (kListed && drop) v = u32x4{0u, 0u, 0u, 0u};
         if constexpr (kFp8) {
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
@@ -282,7 +294,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[4 * h + i] *= ks[i];
       }
-      if constexpr (kSelected) {
+      if constexpr (kListed) {
         const int4 r = *reinterpret_cast<const int4*>(&at[16 * h + 4 * quad]);
         x[4 * h] = r.x < 0 ? -INFINITY : x[4 * h];
         x[4 * h + 1] = r.y < 0 ? -INFINITY : x[4 * h + 1];
@@ -291,7 +303,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
       }
     }
     const uint32_t key0 = first_key(step);
-    if (!kSelected && key0 + kStep > min(all_see, end)) {
+    if (!kListed && key0 + kStep > min(all_see, end)) {
       const uint32_t limit = min(sees, end);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = key0 + 16u * (i / 4) + 4u * quad + (i % 4) < limit ? x[i] : -INFINITY;
@@ -373,6 +385,13 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   // Join the four waves: every wave scales its sums to the largest reference.
   total += __shfl_xor(total, 16, kWave);
   total += __shfl_xor(total, 32, kWave);
+  if constexpr (kWork == kSolo) {
+    if (row0 + col < rows) {
+#pragma unroll
+      for (int i = 0; i < kO; ++i) store_out<Tag, D>(a, out_row(col), 16u * i + 4u * quad, o[i], reference, total);
+    }
+    return;
+  }
   if (quad == 0) sums[wave][col] = make_float2(reference, total);
   __syncthreads();
   float most = sums[0][col].x;
@@ -521,14 +540,14 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
   store_out<Tag, D>(a, row, dim, sum, top, total);
 }
 
-template <class Tag, bool kFp8, bool kSelected>
+template <class Tag, bool kFp8, Work kWork>
 void launch_stream(const PagedAttentionArgs& a, int32_t dim, uint32_t grid, hipStream_t s) {
   if (dim == 64)
-    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 64, kSelected>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 64, kWork>), dim3(grid), dim3(256), 0, s, a);
   else if (dim == 128)
-    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 128, kSelected>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 128, kWork>), dim3(grid), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 256, kSelected>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 256, kWork>), dim3(grid), dim3(256), 0, s, a);
 }
 
 template <class Tag>
@@ -550,17 +569,17 @@ int combine(const PagedAttentionArgs& a, int32_t dim, int32_t dtype, hipStream_t
   return check_launch("paged_combine_kernel");
 }
 
-template <bool kSelected>
+template <Work kWork>
 int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dtype, int64_t pieces, hipStream_t s) {
   const int64_t grid = pieces * a.cache.kv_heads;
   DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
   const int32_t dim = cache->head_dim;
   if (cache->dtype == kFP8E4M3)
-    launch_stream<Bf16Tag, true, kSelected>(a, dim, (uint32_t)grid, s);
+    launch_stream<Bf16Tag, true, kWork>(a, dim, (uint32_t)grid, s);
   else if (dtype == kBF16)
-    launch_stream<Bf16Tag, false, kSelected>(a, dim, (uint32_t)grid, s);
+    launch_stream<Bf16Tag, false, kWork>(a, dim, (uint32_t)grid, s);
   else
-    launch_stream<F16Tag, false, kSelected>(a, dim, (uint32_t)grid, s);
+    launch_stream<F16Tag, false, kWork>(a, dim, (uint32_t)grid, s);
   return check_launch("paged_stream_kernel");
 }
 
@@ -678,6 +697,7 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
 struct SelectedPlan {
   int64_t items;
   uint32_t splits, part_rows;
+  bool solo;
   int64_t parts;
 };
 
@@ -685,7 +705,12 @@ SelectedPlan selected_plan(const dsa_paged_cache* cache, int64_t tokens, int64_t
   const int64_t kv_heads = cache->kv_heads;
   const int64_t group = heads / kv_heads;
   const int64_t items = tokens * ((group + 15) / 16);
-  SelectedPlan p = {items, splits_for(items * kv_heads, resident_workgroups(cache->head_dim), k, 128), (uint32_t)(group < 16 ? group : 16), 0};
+  SelectedPlan p = {items, splits_for(items * kv_heads, resident_workgroups(cache->head_dim), k, 128), (uint32_t)(group < 16 ? group : 16), false, 0};
+  // A list to a wave, once they give every wave that runs at a time one: no joining
+  // of waves, and four times the steps for a start.  (Lists of 512 of bf16, 8 kv
+  // heads, us, by waves / by workgroups: 128 tokens 24.0 / 23.6, 256 33.5 / 42.9,
+  // 1024 118 / 151; of 2048: 82 / 61, 114 / 116, 426 / 449.)
+  p.solo = items * kv_heads >= 4 * resident_workgroups(cache->head_dim);
   if (p.splits > 1) p.parts = items * p.splits * kv_heads * p.part_rows;
   return p;
 }
@@ -729,7 +754,7 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
     a.part_rows = p.stream_rows;
     a.least_rows = 1;
     a.most_rows = kStreamRows;
-    if (int st = launch<false>(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
+    if (int st = launch<kDense>(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
   }
   if (p.chunk_pieces) {
     a.cuts = p.chunk_cuts;
@@ -773,5 +798,6 @@ extern "C" int dsa_paged_selected_attention(const dsa_paged_cache* cache, const 
   a.out = static_cast<char*>(out);
   a.lse = lse;
   if (int st = take_workspace(a, p.parts, 0, cache->head_dim, workspace, workspace_bytes)) return st;
-  return launch<true>(a, cache, dtype, p.items * p.splits, static_cast<hipStream_t>(stream));
+  if (p.solo) return launch<kSolo>(a, cache, dtype, (p.items + 3) / 4, static_cast<hipStream_t>(stream));
+  return launch<kSelected>(a, cache, dtype, p.items * p.splits, static_cast<hipStream_t>(stream));
 }
