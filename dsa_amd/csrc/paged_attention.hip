@@ -22,7 +22,9 @@ namespace dsa {
 namespace {
 
 constexpr uint32_t kStep = 32;   // keys per wave and step
-constexpr uint32_t kLeastSteps = 4;  // of a piece: one for each wave
+// Steps of a piece, at least: two for each wave.  (One sequence of 4096 bf16 keys,
+// us: 10.9, with one step 13.0, whose twice as many pieces take longer to join.)
+constexpr uint32_t kLeastSteps = 8;
 constexpr uint32_t kGroup = 8;   // steps whose cache rows a wave looks up at a time
 // Workgroups that run at a time: what the registers of each head_dim allow on 256
 // CUs.  Work is cut to fill them once.
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     sequence = sequence_of(a, token0);
     length = keys_of(a, sequence);
     const uint32_t visible = length ? a.k : 0u;
-    const uint32_t chunk = max(128u, ((a.k + a.splits - 1u) / a.splits + 31u) & ~31u);
+    const uint32_t chunk = max(kLeastSteps * kStep, ((a.k + a.splits - 1u) / a.splits + 31u) & ~31u);
     begin = min(piece * chunk, visible);
     end = min(begin + chunk, visible);
     pieces = a.splits;
@@ -705,7 +707,8 @@ SelectedPlan selected_plan(const dsa_paged_cache* cache, int64_t tokens, int64_t
   const int64_t kv_heads = cache->kv_heads;
   const int64_t group = heads / kv_heads;
   const int64_t items = tokens * ((group + 15) / 16);
-  SelectedPlan p = {items, splits_for(items * kv_heads, resident_workgroups(cache->head_dim), k, 128), (uint32_t)(group < 16 ? group : 16), false, 0};
+  SelectedPlan p = {items, splits_for(items * kv_heads, resident_workgroups(cache->head_dim), k,
+                                     kLeastSteps * kStep), (uint32_t)(group < 16 ? group : 16), false, 0};
   // A list to a wave, once they give every wave that runs at a time one: no joining
   // of waves, and four times the steps for a start.  (Lists of 512 of bf16, 8 kv
   // heads, us, by waves / by workgroups: 128 tokens 24.0 / 23.6, 256 33.5 / 42.9,

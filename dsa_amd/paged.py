@@ -41,7 +41,7 @@ class PagedCache:
     cache row r is slot ``r % page_size`` of page ``r // page_size``."""
 
     __slots__ = ("keys", "values", "key_scales", "value_scales", "pages", "page_size", "kv_heads", "head_dim", "dtype",
-                 "row_dtype", "_struct", "_address")
+                 "row_dtype", "device", "_index", "_code", "_struct", "_address", "_needs")
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor | None = None,
                  value_scales: torch.Tensor | None = None) -> None:
@@ -72,6 +72,10 @@ class PagedCache:
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.dtype = keys.dtype
         self.row_dtype = torch.bfloat16 if fp8 else keys.dtype  # of the queries and of appended rows
+        self.device = keys.device
+        self._index = keys.get_device()
+        self._code = _lib.dtype_code(self.row_dtype)
+        self._needs: dict[tuple, int] = {}
         self._struct = _lib.PagedCacheC(
             _lib.ptr(keys), _lib.ptr(values), _lib.ptr(key_scales), _lib.ptr(value_scales), pages, *keys.stride()[:3],
             *values.stride()[:3], page_size, kv_heads, head_dim, _lib.dtype_code(keys.dtype))
@@ -80,6 +84,18 @@ class PagedCache:
     @property
     def rows(self) -> int:
         return self.pages * self.page_size
+
+    def _workspace(self, stream: int, entry: str, *sizes: int) -> tuple[int | None, int]:
+        """Address and size of the workspace that ``entry`` asks for at these sizes."""
+
+        need = self._needs.get((entry, sizes))
+        if need is None:
+            if len(self._needs) >= 256:  # a serving loop's sizes; a prompt's do not pile up
+                self._needs.clear()
+            need = self._needs[entry, sizes] = _lib.query(entry, self._address, *sizes)
+        if need <= 0:
+            return None, 0
+        return _lib.workspace("paged_attention", self.device, stream, need, zeroed=True).data_ptr(), need
 
 
 def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, dtype: torch.dtype = torch.bfloat16,
@@ -112,11 +128,17 @@ def cache_rows(cache: PagedCache, page_table: torch.Tensor, positions: torch.Ten
     return page.long() * size + positions % size
 
 
-def _rows(x: torch.Tensor, dim: int) -> tuple[torch.Tensor, int]:
+# A short call is bound by the host, so its checks are the cheap ones where they
+# pass: sizes are unpacked once, devices compared by index, and only tensors that
+# are not as the kernels read them take another look.
+
+
+def _rows(x: torch.Tensor, heads: int, dim: int) -> tuple[torch.Tensor, int]:
     """``x`` ``[T, heads, dim]`` as rows the kernels read (heads packed, tokens
     16-byte aligned at any stride), and its token stride."""
 
-    heads = x.shape[1]
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, heads * dim
     stride, head, unit = x.stride()
     packed = unit == 1 and (head == dim or heads == 1)
     if x.shape[0] == 1 and packed:
@@ -129,23 +151,39 @@ def _rows(x: torch.Tensor, dim: int) -> tuple[torch.Tensor, int]:
     return x, stride
 
 
-def _dense_like(x: torch.Tensor, stride: int) -> torch.Tensor:
+def _like(x: torch.Tensor, stride: int, heads: int, dim: int) -> torch.Tensor:
     """An uninitialised dense tensor like the rows ``x`` (empty_like is the
     cheaper call by 0.6 us, a twentieth of a short call's host time)."""
 
-    return torch.empty_like(x) if stride == x.shape[1] * x.shape[2] else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    return torch.empty_like(x) if stride == heads * dim else torch.empty(x.shape, device=x.device, dtype=x.dtype)
 
 
-def _queries(queries: torch.Tensor, cache: PagedCache) -> tuple[torch.Tensor, int]:
-    if queries.ndim != 3 or queries.shape[2] != cache.head_dim:
+def _queries(queries: torch.Tensor, cache: PagedCache) -> tuple[torch.Tensor, int, int, int]:
+    """Checked queries, their token stride, tokens and heads."""
+
+    if queries.ndim != 3:
         raise ValueError("queries must be [tokens,heads,head_dim]")
-    if queries.shape[1] == 0 or queries.shape[1] % cache.kv_heads:
+    tokens, heads, dim = queries.shape
+    if dim != cache.head_dim:
+        raise ValueError("queries must be [tokens,heads,head_dim]")
+    if heads == 0 or heads % cache.kv_heads:
         raise ValueError("heads must be a multiple of the cache's kv_heads")
-    if queries.dtype != cache.row_dtype:
+    if queries.dtype is not cache.row_dtype:
         raise ValueError("queries must have the cache's dtype (BF16 for an FP8 cache)")
-    if queries.device != cache.keys.device:
+    if queries.get_device() != cache._index:
         raise ValueError("queries and cache must be on one GPU")
-    return _rows(queries, cache.head_dim)
+    queries, stride = _rows(queries, heads, dim)
+    return queries, stride, tokens, heads
+
+
+def _integers(x: torch.Tensor, dtype: torch.dtype, name: str, cache: PagedCache) -> torch.Tensor:
+    """``x`` as contiguous ``dtype`` on the cache's GPU."""
+
+    if x.dtype is dtype and x.get_device() == cache._index and x.is_contiguous():
+        return x
+    if x.is_floating_point() or x.is_complex():
+        raise ValueError(f"{name} must be integers")
+    return x.to(device=cache.device, dtype=dtype).contiguous()
 
 
 def append(
@@ -168,85 +206,66 @@ def append(
     cache scales each head by its largest magnitude.
     """
 
-    dim = cache.head_dim
-    tokens = keys.shape[0]
-    if keys.ndim != 3 or keys.shape[1:] != (cache.kv_heads, dim) or values.shape != keys.shape:
+    dim, kv_heads = cache.head_dim, cache.kv_heads
+    if keys.ndim != 3 or values.shape != keys.shape:
         raise ValueError("keys and values must both be [tokens,kv_heads,head_dim]")
-    if keys.dtype != cache.row_dtype or values.dtype != keys.dtype:
+    tokens, rows_heads, rows_dim = keys.shape
+    if rows_heads != kv_heads or rows_dim != dim:
+        raise ValueError("keys and values must both be [tokens,kv_heads,head_dim]")
+    if keys.dtype is not cache.row_dtype or values.dtype is not cache.row_dtype:
         raise ValueError("appended rows must have the cache's dtype (BF16 for an FP8 cache)")
-    if keys.device != cache.keys.device or values.device != keys.device:
+    if keys.get_device() != cache._index or values.get_device() != cache._index:
         raise ValueError("appended rows and cache must be on one GPU")
-    if rows.shape != (tokens,) or positions.shape != (tokens,):
+    if rows.ndim != 1 or len(rows) != tokens or positions.shape != rows.shape:
         raise ValueError("rows and positions must be [tokens]")
-    rope_dim = dim if rope_dim is None else rope_dim
+    if rope_dim is None:
+        rope_dim = dim
     if rope_dim % 16 or not 0 <= rope_dim <= dim:
         raise ValueError("rope_dim must be a multiple of 16 no larger than head_dim")
-    if not (theta > 0 and math.isfinite(theta)):
+    if not 0 < theta < math.inf:
         raise ValueError("theta must be positive")
-    rows, positions = _tokens(rows, keys.device), _tokens(positions, keys.device)
+    rows = _integers(rows, torch.int64, "rows", cache)
+    positions = _integers(positions, torch.int64, "positions", cache)
     out = None
     heads = query_stride = 0
     if queries is not None:
-        if queries.shape[0] != tokens:
+        queries, query_stride, query_tokens, heads = _queries(queries, cache)
+        if query_tokens != tokens:
             raise ValueError("queries must be [tokens,heads,head_dim]")
-        queries, query_stride = _queries(queries, cache)
-        heads = queries.shape[1]
-        out = _dense_like(queries, query_stride)
+        out = _like(queries, query_stride, heads, dim)
     if tokens == 0:
         return out
-    keys, key_stride = _rows(keys, dim)
-    values, value_stride = _rows(values, dim)
+    keys, key_stride = _rows(keys, kv_heads, dim)
+    values, value_stride = _rows(values, kv_heads, dim)
     _lib.call("dsa_paged_append", cache._address, keys.data_ptr(), key_stride, values.data_ptr(), value_stride,
-              _lib.ptr(queries), query_stride, _lib.ptr(out), heads, _lib.dtype_code(keys.dtype), rows.data_ptr(),
+              _lib.ptr(queries), query_stride, _lib.ptr(out), heads, cache._code, rows.data_ptr(),
               positions.data_ptr(), tokens, rope_dim, theta, _lib.stream_of(keys))
     return out
 
 
-def _tokens(x: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if x.dtype == torch.int64 and x.device == device and x.is_contiguous():
-        return x
-    if x.is_floating_point() or x.is_complex():
-        raise ValueError("rows and positions must be integers")
-    return x.to(device=device, dtype=torch.int64).contiguous()
+def _batch(tokens: int, cache: PagedCache, page_table, lengths, starts):
+    """Checked page table with its sizes and row stride, lengths and starts."""
 
-
-def _int32(x: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
-    if x.dtype == torch.int32 and x.device == device and x.is_contiguous():
-        return x
-    if x.is_floating_point() or x.is_complex():
-        raise ValueError(f"{name} must be integers")
-    return x.to(device=device, dtype=torch.int32).contiguous()
-
-
-def _batch(queries, cache, page_table, lengths, starts):
-    """Checked page table, lengths and starts of a call's sequences."""
-
-    device = cache.keys.device
-    if page_table.ndim != 2 or page_table.shape[1] == 0 or page_table.shape[0] == 0:
+    if page_table.ndim != 2 or 0 in page_table.shape:
         raise ValueError("page_table must be [sequences,columns]")
-    sequences = page_table.shape[0]
-    if lengths.shape != (sequences,):
+    sequences, columns = page_table.shape
+    if lengths.ndim != 1 or len(lengths) != sequences:
         raise ValueError("lengths must be [sequences]")
-    if page_table.dtype != torch.int32 or page_table.device != device or page_table.stride(1) != 1:
-        page_table = _int32(page_table, "page_table", device)
+    stride, unit = page_table.stride()
+    if (page_table.dtype is not torch.int32 or page_table.get_device() != cache._index or unit != 1
+            or (stride < columns and sequences > 1)):
+        page_table = _integers(page_table, torch.int32, "page_table", cache)
+        stride = columns
+    if sequences == 1:
+        stride = columns
     if starts is None:
-        if queries.shape[0] % sequences:
+        if tokens % sequences:
             raise ValueError("without starts every sequence has the same number of tokens")
-    elif starts.shape != (sequences + 1,):
+    elif starts.ndim != 1 or len(starts) != sequences + 1:
         raise ValueError("starts must be [sequences + 1]")
     else:
-        starts = _int32(starts, "starts", device)
-    stride = page_table.stride(0) if sequences > 1 else page_table.shape[1]
-    if stride < page_table.shape[1]:
-        page_table = page_table.contiguous()
-        stride = page_table.shape[1]
-    return page_table, stride, _int32(lengths, "lengths", device), starts
-
-
-def _workspace(cache: PagedCache, stream: int, need: int) -> torch.Tensor | None:
-    if need <= 0:
-        return None
-    return _lib.workspace("paged_attention", cache.keys.device, stream, need, zeroed=True)
+        starts = _integers(starts, torch.int32, "starts", cache)
+    return page_table, sequences, columns, stride, _integers(lengths, torch.int32, "lengths", cache), starts
 
 
 def attention(
@@ -274,22 +293,18 @@ def attention(
     ``[T, heads]``.  A row that sees no key gets zeros and -inf.
     """
 
-    queries, query_stride = _queries(queries, cache)
-    page_table, table_stride, lengths, starts = _batch(queries, cache, page_table, lengths, starts)
-    tokens, heads, dim = queries.shape
-    device = queries.device
-    out = _dense_like(queries, query_stride)
-    lse = torch.empty((tokens, heads), device=device, dtype=torch.float32) if return_lse else None
+    queries, query_stride, tokens, heads = _queries(queries, cache)
+    page_table, sequences, columns, table_stride, lengths, starts = _batch(tokens, cache, page_table, lengths, starts)
+    dim = cache.head_dim
+    out = _like(queries, query_stride, heads, dim)
+    lse = torch.empty((tokens, heads), device=cache.device, dtype=torch.float32) if return_lse else None
     if tokens:
-        sequences, columns = page_table.shape
         stream = _lib.stream_of(queries)
-        need = _lib.query("dsa_paged_attention_workspace_bytes", cache._address, sequences, tokens, heads, columns,
-                          starts is None)
-        ws = _workspace(cache, stream, need)
+        ws, need = cache._workspace(stream, "dsa_paged_attention_workspace_bytes", sequences, tokens, heads, columns,
+                                    starts is None)
         _lib.call("dsa_paged_attention", cache._address, queries.data_ptr(), query_stride, page_table.data_ptr(),
-                  table_stride, columns, lengths.data_ptr(), _lib.ptr(starts), sequences, tokens, heads,
-                  _lib.dtype_code(queries.dtype), dim**-0.5 if scale is None else scale, causal, out.data_ptr(),
-                  _lib.ptr(lse), _lib.ptr(ws), need, stream)
+                  table_stride, columns, lengths.data_ptr(), _lib.ptr(starts), sequences, tokens, heads, cache._code,
+                  dim**-0.5 if scale is None else scale, causal, out.data_ptr(), _lib.ptr(lse), ws, need, stream)
     return (out, lse) if return_lse else out
 
 
@@ -311,28 +326,23 @@ def selected_attention(
     with contiguous entries is read in place).
     """
 
-    queries, query_stride = _queries(queries, cache)
-    page_table, table_stride, lengths, starts = _batch(queries, cache, page_table, lengths, starts)
-    tokens, heads, dim = queries.shape
-    device = queries.device
+    queries, query_stride, tokens, heads = _queries(queries, cache)
+    page_table, sequences, columns, table_stride, lengths, starts = _batch(tokens, cache, page_table, lengths, starts)
+    dim = cache.head_dim
     if indices.ndim != 2 or indices.shape[0] != tokens:
         raise ValueError("indices must be [tokens,k]")
-    if indices.is_floating_point() or indices.is_complex():
-        raise ValueError("indices must be integers")
     k = indices.shape[1]
-    index_stride = indices.stride(0)
-    if indices.dtype != torch.int64 or indices.device != device or (k > 1 and indices.stride(1) != 1) or index_stride < k:
-        indices = indices.to(device=device, dtype=torch.int64).contiguous()
+    index_stride, unit = indices.stride()
+    if indices.dtype is not torch.int64 or indices.get_device() != cache._index or (k > 1 and unit != 1) or index_stride < k:
+        indices = _integers(indices, torch.int64, "indices", cache)
         index_stride = k
-    out = _dense_like(queries, query_stride)
-    lse = torch.empty((tokens, heads), device=device, dtype=torch.float32) if return_lse else None
+    out = _like(queries, query_stride, heads, dim)
+    lse = torch.empty((tokens, heads), device=cache.device, dtype=torch.float32) if return_lse else None
     if tokens:
-        sequences, columns = page_table.shape
         stream = _lib.stream_of(queries)
-        need = _lib.query("dsa_paged_selected_workspace_bytes", cache._address, tokens, heads, k)
-        ws = _workspace(cache, stream, need)
+        ws, need = cache._workspace(stream, "dsa_paged_selected_workspace_bytes", tokens, heads, k)
         _lib.call("dsa_paged_selected_attention", cache._address, queries.data_ptr(), query_stride,
                   page_table.data_ptr(), table_stride, columns, lengths.data_ptr(), _lib.ptr(starts), sequences, tokens,
-                  heads, _lib.dtype_code(queries.dtype), indices.data_ptr(), index_stride, k,
-                  dim**-0.5 if scale is None else scale, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need, stream)
+                  heads, cache._code, indices.data_ptr(), index_stride, k, dim**-0.5 if scale is None else scale,
+                  out.data_ptr(), _lib.ptr(lse), ws, need, stream)
     return (out, lse) if return_lse else out
