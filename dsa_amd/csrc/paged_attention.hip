@@ -659,6 +659,8 @@ int take_workspace(PagedAttentionArgs& a, int64_t parts, int64_t rows, int64_t d
 struct Plan {
   uint32_t stream_cuts, stream_rows;  // rows of a part
   int64_t stream_pieces;              // at most; 0: no sequence of few rows
+  bool prefill;                       // the prefill kernel takes the other sequences, else the chunk kernel
+  int32_t chunk_rows;                 // of a tile of theirs
   uint32_t chunk_cuts;                // 0: more row tiles than could be cut to use
   int64_t chunk_pieces;
   int64_t parts, rows;
@@ -670,27 +672,37 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
   const int64_t group = heads / kv_heads;
   Plan p = {};
   const int64_t each = tokens / sequences * group;
-  const int64_t cuts = (resident_workgroups(cache->head_dim) + kv_heads - 1) / kv_heads;
-  auto at_most = [&](int64_t tiles, int64_t least) {
+  auto at_most = [&](int64_t tiles, int64_t cuts, int64_t least) {
     const int64_t pieces = tiles * ((capacity + least - 1) / least);
     return pieces < tiles + cuts ? pieces : tiles + cuts;
   };
   if (!uniform || each <= kStreamRows) {
+    const int64_t cuts = (resident_workgroups(cache->head_dim) + kv_heads - 1) / kv_heads;
     const int64_t tiles = uniform ? sequences : (tokens < sequences ? tokens : sequences);
     p.stream_cuts = (uint32_t)cuts;
     p.stream_rows = (uint32_t)(uniform ? each : kStreamRows);
-    p.stream_pieces = at_most(tiles, kLeastSteps * kStep);
+    p.stream_pieces = at_most(tiles, cuts, kLeastSteps * kStep);
     p.parts = 2 * cuts * kv_heads * p.stream_rows;
   }
   if (!uniform || each > kStreamRows) {
-    const int64_t tiles = row_tiles(sequences, tokens, group, uniform, kChunkRows);
+    // The prefill kernel from more than 128 rows a sequence on, the chunk kernel, of
+    // half its rows a workgroup and two or three workgroups a CU, below; head_dim 256
+    // has the prefill kernel alone.  (us, chunk / prefill kernel, 32 heads on 8 of
+    // 128 dims, 64K keys: 64 rows 71 / 73, 128 rows 78 / 76, 256 rows 114 / 99, 2048
+    // rows 646 / 553; 8K keys: 128 rows 25.5 / 28.0, 256 rows 34.9 / 36.3; fp8, 64K:
+    // 128 rows 73 / 90, 256 rows 110 / 106; head_dim 256, 64K: 20 rows 118 / 74.)
+    p.prefill = cache->head_dim == 256 || tokens * group > 128 * sequences;
+    p.chunk_rows = p.prefill ? prefill_rows(cache->head_dim) : kChunkRows;
+    const int64_t fill = p.prefill ? 256 : resident_workgroups(cache->head_dim);
+    const int64_t cuts = (fill + kv_heads - 1) / kv_heads;
+    const int64_t tiles = row_tiles(sequences, tokens, group, uniform, p.chunk_rows);
     if (tiles >= 2 * cuts) {
       p.chunk_pieces = tiles;
     } else {
       p.chunk_cuts = (uint32_t)cuts;
-      p.chunk_pieces = at_most(tiles, kLeastChunkKeys);
+      p.chunk_pieces = at_most(tiles, cuts, kLeastChunkKeys);
       p.rows = tokens * heads;
-      if (p.parts < 2 * cuts * kv_heads * kChunkRows) p.parts = 2 * cuts * kv_heads * kChunkRows;
+      if (p.parts < 2 * cuts * kv_heads * p.chunk_rows) p.parts = 2 * cuts * kv_heads * p.chunk_rows;
     }
   }
   return p;
@@ -761,12 +773,13 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
   }
   if (p.chunk_pieces) {
     a.cuts = p.chunk_cuts;
-    a.part_rows = kChunkRows;
+    a.part_rows = (uint32_t)p.chunk_rows;
     a.least_rows = kStreamRows + 1;
     a.most_rows = 0xffffffffu;
     const int64_t grid = p.chunk_pieces * a.cache.kv_heads;
     DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
-    if (int st = launch_paged_chunk(a, cache->head_dim, cache->dtype, (uint32_t)grid, s)) return st;
+    const auto launch_rows = p.prefill ? launch_paged_prefill : launch_paged_chunk;
+    if (int st = launch_rows(a, cache->head_dim, cache->dtype, (uint32_t)grid, s)) return st;
     if (p.chunk_cuts) return combine(a, cache->head_dim, dtype, s);
   }
   return 0;

@@ -209,10 +209,35 @@ __device__ __forceinline__ void store_out(const PagedAttentionArgs& a, uint64_t 
   if (a.lse && dim == 0) a.lse[row] = total == 0.f ? -INFINITY : (reference + log2f(total)) * kLn2;
 }
 
+// The chunk kernels' products and tiles.
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ floatx16 mfma_32x32x16(Bf16Tag, uint4 a, uint4 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mfma_32x32x16(F16Tag, uint4 a, uint4 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+constexpr uint32_t kTileKeys = 64;
+
+// Bytes between the rows of a tile in LDS.  Padded, not exchanged, so that every
+// address of a tile is one register and an offset: keys are read 16 rows at one
+// 16-byte chunk, values 4 rows at 64 bytes, and each falls on all banks once.
+template <int D>
+constexpr int kKeyRow = 2 * D + 16;
+template <int D>
+constexpr int kValueRow = 2 * D + 64;
+
 constexpr int kChunkRows = 128;        // rows of a workgroup of the chunk kernel
 constexpr int kLeastChunkKeys = 256;   // keys of a piece of it
 
-// paged_chunk.hip: the chunk kernel over `grid` workgroups.
+// paged_prefill.hip: the kernel of many rows, over `grid` workgroups, and its rows a
+// workgroup.
+constexpr int32_t prefill_rows(int64_t dim) { return dim == 256 ? 128 : 256; }
+int launch_paged_prefill(const PagedAttentionArgs& a, int32_t dim, int32_t cache_dtype, uint32_t grid, hipStream_t s);
+
+// paged_chunk.hip: the chunk kernel (head_dim 64 or 128).
 int launch_paged_chunk(const PagedAttentionArgs& a, int32_t dim, int32_t cache_dtype, uint32_t grid, hipStream_t s);
 
 }  // namespace dsa

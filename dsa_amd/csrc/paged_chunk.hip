@@ -1,33 +1,26 @@
-// Attention over a paged key/value cache: many query rows, as in a prefill or a
-// chunk of a prompt, on the matrix cores.
+// Attention over a paged key/value cache: some query rows, as in the chunks of a
+// mixed batch, on the matrix cores.
 //
-// A workgroup takes 32 (token, head) rows of one kv head per wave against one
+// A workgroup takes 128 (token, head) rows of one kv head, 32 a wave, against one
 // piece of the keys, 64 keys at a time.  Keys and values of a tile go through
-// registers into LDS, the next tile's loads in flight under this one's
-// products; every wave reads all of them for its own rows.
+// registers into LDS, the next tile's loads in flight under this one's products;
+// every wave reads all of them for its own rows.
 //   scores^T = K Q^T   v_mfma_f32_32x32x16, keys the A operand: a lane holds 32
 //                      scores of one row, so maximum, weights and sum need no
 //                      other lane (the two halves of a wave meet only when the
 //                      running maximum is raised, and at the end)
 //   out^T += V^T P^T   the weights are the B operand as they stand, values read
 //                      transposed by ds_read_b64_tr_b16
-// Rescaling a row is one factor per lane for the same reason.
+// Rescaling a row is one factor per lane for the same reason.  Two workgroups a CU
+// (three at head_dim 64) hide each other's waits; at few rows that reads the cache at
+// 3.9 TB/s (20 rows a kv head of 64K bf16 keys, 268 MB: 68 us), at 128 it makes 440
+// TFLOP/s, and from there on the prefill kernel is the faster one.
 #include "paged_attention.hpp"
 
 namespace dsa {
 namespace {
 
-constexpr uint32_t kTileKeys = 64;
 constexpr uint32_t kLeastTiles = kLeastChunkKeys / kTileKeys;  // of a piece
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ floatx16 mfma_32x32x16(Bf16Tag, uint4 a, uint4 b, floatx16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ floatx16 mfma_32x32x16(F16Tag, uint4 a, uint4 b, floatx16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
 
 // Keeps a value's computation where it stands: the compiler would move it past
 // the next branch, away from the products that it is to run under.
@@ -41,18 +34,10 @@ __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
     __builtin_amdgcn_sched_group_barrier(0x402, (others), 0); \
   }
 
-// Bytes between the rows of a tile in LDS.  Padded, not exchanged, so that every
-// address of a tile is one register and an offset: keys are read 16 rows at one
-// 16-byte chunk, values 4 rows at 64 bytes, and each falls on all banks once.
-template <int D>
-constexpr int kKeyRow = 2 * D + 16;
-template <int D>
-constexpr int kValueRow = 2 * D + 64;
-
-template <class Tag, bool kFp8, int D, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_chunk_kernel(PagedAttentionArgs a) {
-  constexpr uint32_t kThreads = 64 * kWaves;
-  constexpr uint32_t kRows = 32 * kWaves;
+template <class Tag, bool kFp8, int D>
+__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs a) {
+  constexpr uint32_t kThreads = 256;
+  constexpr uint32_t kRows = kChunkRows;
   constexpr uint32_t kChunks = kFp8 ? D / 16 : D / 8;       // 16-byte loads per cache row
   constexpr uint32_t kPass = kThreads / kChunks;            // cache rows per pass of the workgroup
   constexpr int kLoads = kTileKeys / kPass;                 // passes per tile
@@ -345,13 +330,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? kWaves / 4 : 2) void paged_
 
 template <class Tag, bool kFp8>
 static void launch_dim(const PagedAttentionArgs& a, int32_t dim, uint32_t grid, hipStream_t s) {
-  constexpr int kThreads = 2 * kChunkRows;
   if (dim == 64)
-    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kFp8, 64, kChunkRows / 32>), dim3(grid), dim3(kThreads), 0, s, a);
-  else if (dim == 128)
-    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kFp8, 128, kChunkRows / 32>), dim3(grid), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kFp8, 64>), dim3(grid), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kFp8, 256, kChunkRows / 32>), dim3(grid), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kFp8, 128>), dim3(grid), dim3(256), 0, s, a);
 }
 
 int launch_paged_chunk(const PagedAttentionArgs& a, int32_t dim, int32_t cache_dtype, uint32_t grid, hipStream_t s) {
