@@ -247,8 +247,11 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   };
 
   // Both tiles to LDS, rows as they are; fp8 values widened.
+  bool dropped = false;
   auto stage = [&](const T& t, uint32_t step) {
     const int32_t* at = rows_at(step);
+    const uint32_t key0 = first_key(step);
+    const bool hides = !kListed && key0 + kStep > all_see;  // from some row
 #pragma unroll
     for (int i = 0; i < T::kPasses; ++i) {
       const uint32_t r = T::kRows * i + load_row;
@@ -260,6 +263,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
         *reinterpret_cast<u32x4*>(my_keys + tile_place<T::kBytes>(r, c)) = t.k[i][j];
         u32x4 v = t.v[i][j];
         if (kListed && drop) v = u32x4{0u, 0u, 0u, 0u};
+        if (hides && key0 + r >= all_see) dropped |= drop_nonfinite<Tag, kFp8>(v);
         if constexpr (kFp8) {
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
@@ -268,7 +272,15 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
         }
       }
     }
-    if constexpr (kFp8) scales[wave][lane] = t.scale;
+    if constexpr (kFp8) {
+      float scale = t.scale;
+      if (kListed && at[lane & 31u] < 0) scale = 0.f;
+      if (hides && lane >= 32u && key0 + lane - 32u >= all_see && !is_finite(scale)) {
+        scale = 0.f;
+        dropped = true;
+      }
+      scales[wave][lane] = scale;
+    }
     wave_order();
   };
 
@@ -382,6 +394,19 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
         if (step < own) compute(step);
       }
     }
+  }
+
+  if (!kListed && __any(dropped)) {
+    for (uint32_t k = max(begin, all_see); k < end; ++k)
+      if ((k - begin) / kStep % 4u == wave && k < sees) {
+        const uint32_t row = cache_row(a, pages, k);
+#pragma unroll
+        for (int i = 0; i < kO; ++i) {
+          float back[4] = {0.f, 0.f, 0.f, 0.f};
+          add_nonfinite<Tag, kFp8>(a, row, g, 16u * i + 4u * quad, back);
+          o[i] += floatx4{back[0], back[1], back[2], back[3]};
+        }
+      }
   }
 
   // Join the four waves: every wave scales its sums to the largest reference.

@@ -51,6 +51,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
   __shared__ ulong2 table[4][kTileKeys];
   __shared__ uint32_t table_row[4][kFp8 ? kTileKeys : 1];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kTileKeys];
+  // Whether a value was staged as 0 for not being finite: in the last row's padding.
+  uint32_t& dropped = *reinterpret_cast<uint32_t*>(key_tile[0] + kTileKeys * kKeyRow<D> - 16u);
   const uint32_t tid = threadIdx.x;
   const uint32_t lane = lane_id();
   const uint32_t wave = tid / kWave;
@@ -80,7 +82,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
   const uint32_t my_token = span.first + my_row / a.group;
   const uint32_t my_head = g * a.group + my_row % a.group;
   const uint32_t sees = min(seen(my_row), end);
-  const uint32_t all_see = min(seen(wave_row), end);                          // every row of the wave sees these
+  const uint32_t all_see = min(seen(wave_row), end);  // every row of the wave sees these
+  const uint32_t all_rows_see = seen(row0);  // of the workgroup
   const uint32_t some_see = row0 + 32u * wave < rows ? min(seen(min(wave_row + 31u, rows - 1u)), end) : 0u;
 
   uint4 q[D / 16];
@@ -120,6 +123,16 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
     }
   };
   auto stage = [&](uint32_t t) {
+    const uint32_t key0 = begin + t * kTileKeys;
+    if (key0 + kTileKeys > all_rows_see) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        if (key0 + load_row + kPass * i >= all_rows_see && drop_nonfinite<Tag, kFp8>(vr[i])) dropped = 1;
+      if (kFp8 && tid >= kTileKeys && key0 + tid - kTileKeys >= all_rows_see && !is_finite(sr)) {
+        sr = 0.f;
+        dropped = 1;
+      }
+    }
     char* keys = key_tile[t & 1u];
     char* values = value_tile[t & 1u];
 #pragma unroll
@@ -273,6 +286,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
   };
 
   if (begin < end) {
+    if (tid == 0) dropped = 0;
     const uint32_t tiles = (end - begin + kTileKeys - 1u) / kTileKeys;
     // The look-up of a tile's cache rows, by its first 64 threads: the page id's
     // load two tiles ahead of the rows' and before them, its use after the tile.
@@ -302,6 +316,23 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
       }
       __syncthreads();
     }
+  }
+
+  if (begin < end && all_rows_see < end && dropped) {
+    for (uint32_t k = max(begin, all_rows_see); k < end; ++k)
+      if (k < sees) {
+        const uint32_t row = cache_row(a, pages, k);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            float back[4] = {0.f, 0.f, 0.f, 0.f};
+            add_nonfinite<Tag, kFp8>(a, row, g, 32u * i + 8u * b + 4u * half, back);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][4 * b + e] += back[e];
+            __builtin_amdgcn_sched_barrier(0);  // few loads at a time: no registers for more
+          }
+      }
   }
 
   total += __shfl_xor(total, 32, kWave);

@@ -40,6 +40,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   __shared__ ulong2 table[4][kTileKeys];
   __shared__ uint32_t table_row[4][kFp8 ? kTileKeys : 1];
   __shared__ __attribute__((aligned(16))) float scales[2][4][kTileKeys];
+  // Whether a value was staged as 0 for not being finite: in the last row's padding.
+  uint32_t& dropped = *reinterpret_cast<uint32_t*>(key_tile[0] + kTileKeys * kKeyRow<D> - 16u);
   const uint32_t tid = threadIdx.x;
   const uint32_t lane = lane_id();
   const uint32_t wave = tid / kWave;
@@ -70,6 +72,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   const uint32_t my_head = g * a.group + my_row % a.group;
   const uint32_t sees = min(seen(my_row), end);
   const uint32_t all_see = min(seen(min(wave_row, rows - 1u)), end);  // every row of the wave sees these
+  const uint32_t all_rows_see = seen(row0);  // of the workgroup
   const uint32_t some_see = wave_row < rows ? min(seen(min(wave_row + 32u, rows) - 1u), end) : 0u;
 
   uint4 q[kSteps];
@@ -128,6 +131,16 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
     }
   };
   auto stage_values = [&](uint32_t t) {
+    const uint32_t key0 = begin + t * kTileKeys;
+    if (key0 + kTileKeys > all_rows_see) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        if (key0 + load_row + kPass * i >= all_rows_see && drop_nonfinite<Tag, kFp8>(vr[i])) dropped = 1;
+      if (kFp8 && key0 + tid >= all_rows_see && !is_finite(vs)) {
+        vs = 0.f;
+        dropped = 1;
+      }
+    }
     if (kPart && load_row >= kTileKeys) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) put(value_tile[t & 1u] + (load_row + kPass * i) * kValueRow<D>, vr[i]);
@@ -253,6 +266,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   };
 
   if (begin < end) {
+    if (tid == 0) dropped = 0;
     const uint32_t tiles = (end - begin + kTileKeys - 1u) / kTileKeys;
     const uint32_t mine = some_see > begin ? (some_see - begin + kTileKeys - 1u) / kTileKeys : 0u;  // tiles the wave sees
     if (tid < 3u * kTileKeys) place(tid / kTileKeys, look_page(tid / kTileKeys));
@@ -303,6 +317,23 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
       turn(t, x, y);
       if (t + 1u < tiles) turn(t + 1u, y, x);
     }
+  }
+
+  if (begin < end && all_rows_see < end && dropped) {
+    for (uint32_t k = max(begin, all_rows_see); k < end; ++k)
+      if (k < sees) {
+        const uint32_t row = cache_row(a, pages, k);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            float back[4] = {0.f, 0.f, 0.f, 0.f};
+            add_nonfinite<Tag, kFp8>(a, row, g, 32u * i + 8u * b + 4u * half, back);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][4 * b + e] += back[e];
+            __builtin_amdgcn_sched_barrier(0);  // few loads at a time: no registers for more
+          }
+      }
   }
 
   total += __shfl_xor(total, 32, kWave);

@@ -290,7 +290,8 @@ def attention(
 
     Returns ``[T, heads, head_dim]`` in the queries' dtype, and with
     ``return_lse`` the natural log of each row's softmax denominator, fp32
-    ``[T, heads]``.  A row that sees no key gets zeros and -inf.
+    ``[T, heads]``.  A row that sees no key gets zeros and -inf; what a row does
+    not see does not reach it, whatever it holds.
     """
 
     queries, query_stride, tokens, heads = _queries(queries, cache)

@@ -886,9 +886,10 @@ int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, int64_t key
  * keys, its new tokens' included, at most columns * page_size (itself at most 2^30).  With causal, the
  * i-th of n new tokens sees keys j <= lengths[s] - n + i, else every key of the
  * sequence.  A row that sees no key gets zeros and lse -inf.  lse (nullable,
- * [tokens][heads] fp32) is the natural log of the softmax's denominator.  Cache
- * rows past a sequence's length are never used.  Page ids outside the cache read
- * other rows of it.  Workspace (16-byte aligned): the bytes that the query below
+ * [tokens][heads] fp32) is the natural log of the softmax's denominator.  What a
+ * row does not see does not reach it, infinities and NaN of later tokens, of rows
+ * past a sequence's length and of other sequences included.  Page ids outside the
+ * cache read other rows of it.  Workspace (16-byte aligned): the bytes that the query below
  * gives for the same sizes, uniform = (starts == NULL); its first 16 KiB are zero
  * before the first call, and every call leaves them so.  Calls that share one are
  * ordered on one stream. */
