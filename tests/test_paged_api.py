@@ -144,3 +144,17 @@ def test_oracle_rotation_keeps_lengths_and_relative_angles() -> None:
     assert np.isclose(np.linalg.norm(at(x, 77)), np.linalg.norm(x))
     assert np.isclose(at(x, 105) @ at(y, 100), at(x, 1005) @ at(y, 1000))
     assert np.array_equal(at(x, 5)[8:], x[0, 0, 8:])
+
+
+def test_command_line_of_attend(tmp_path) -> None:
+    from dsa_amd.cli import build_parser
+
+    parser = build_parser()
+    args = parser.parse_args(["attend", "--output", str(tmp_path), "--cache-dtype", "fp8", "--k", "64"])
+    assert (args.length, args.steps, args.k, args.head_dim, args.cache_dtype) == (16384, 16, 64, 128, "fp8")
+    for bad in (["--cache-dtype", "int4"], ["--head-dim", "96"]):
+        with pytest.raises(SystemExit):
+            parser.parse_args(["attend", "--output", str(tmp_path), *bad])
+    with pytest.raises(ValueError, match="at least 1"):
+        args.steps = 0
+        args.function(args)
