@@ -13,6 +13,8 @@ the names of the reference package ``temporal_dsa``:
   approx              device own-trajectory policy state and step
   sidecar             LightningIndexerSidecar encoders and score_encoded
   certified           block_key_norms, temporal_score_radius
+  paged               paged key/value cache: append, attention, attention over
+                      selected keys (no counterpart in the reference)
   temporal            device temporal pruning (seed, hot-first, running top-K)
 """
 

@@ -27,4 +27,8 @@ Modules and what pins each restatement (tests under ``tests/``):
              covering inequality on random signed-weight inputs and by
              closed forms (zero drift gives radius 0, a single head reduces to
              Cauchy-Schwarz).
+  paged      append, attention and selected attention of a paged key/value
+             cache (no counterpart in the reference).  Pinned by closed forms:
+             equal scores average the values, rotations keep lengths and
+             depend on differences of positions only.
 """
