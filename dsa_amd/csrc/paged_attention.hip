@@ -134,13 +134,15 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
     if (!find_piece<16, kStep, kLeastSteps>(a, id, piece)) return;
     sequence = piece.sequence;
     token0 = piece.span.first;
-    row0 = 0;
-    rows = piece.span.count * a.group;  // at most 16
+    row0 = piece.tile * 16u;
+    rows = piece.span.count * a.group;
     length = piece.keys;
-    // row r sees keys below seen0 + r / group + 1 of a causal chunk; the last sees all
+    // row r sees keys below seen0 + r / group + 1 of a causal chunk; its tile's last sees most
     seen0 = length - piece.span.count;  // may wrap below zero: see `sees`
-    begin = (uint32_t)min((uint64_t)piece.index * piece.units * kStep, (uint64_t)length);
-    end = (uint32_t)min((uint64_t)begin + (uint64_t)piece.units * kStep, (uint64_t)length);
+    const uint32_t last = min(row0 + 16u, rows) - 1u;
+    const uint32_t visible = a.causal ? (uint32_t)max(0, (int32_t)(seen0 + last / a.group + 1u)) : length;
+    begin = (uint32_t)min((uint64_t)piece.index * piece.units * kStep, (uint64_t)visible);
+    end = (uint32_t)min((uint64_t)begin + (uint64_t)piece.units * kStep, (uint64_t)visible);
     pieces = piece.count;
     index = piece.index;
     tile_slot = slot = piece.slot;
@@ -683,6 +685,7 @@ int take_workspace(PagedAttentionArgs& a, int64_t parts, int64_t rows, int64_t d
 // Which kernels a call runs, and what it cuts.
 struct Plan {
   uint32_t stream_cuts, stream_rows;  // rows of a part
+  uint32_t stream_most;               // rows of a sequence of the stream kernel's
   int64_t stream_pieces;              // at most; 0: no sequence of few rows
   bool prefill;                       // the prefill kernel takes the other sequences, else the chunk kernel
   int32_t chunk_rows;                 // of a tile of theirs
@@ -701,15 +704,23 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
     const int64_t pieces = tiles * ((capacity + least - 1) / least);
     return pieces < tiles + cuts ? pieces : tiles + cuts;
   };
+  // Where only `starts` says how the tokens are dealt and there are no more of them
+  // than sequences, this is a decode step, and the stream kernel takes it all, some
+  // sequence of several tokens in several row tiles: two launches less.  (us, with /
+  // without the others' launches, 32 heads on 8 of 128 dims: 64 sequences of 4K keys,
+  // bf16 192 / 186, fp8 126 / 119; 16 of 2K 34 / 27, 26 / 21; but 16 tokens of one
+  // sequence of 32K and none of 15 others 43 / 68, 43 / 38.)
+  const bool few = !uniform && tokens <= sequences;
   if (!uniform || each <= kStreamRows) {
     const int64_t cuts = (resident_workgroups(cache->head_dim) + kv_heads - 1) / kv_heads;
-    const int64_t tiles = uniform ? sequences : (tokens < sequences ? tokens : sequences);
+    const int64_t tiles = (tokens < sequences ? tokens : sequences) + (few ? tokens * group / kStreamRows : 0);
+    p.stream_most = few ? 0xffffffffu : kStreamRows;
     p.stream_cuts = (uint32_t)cuts;
     p.stream_rows = (uint32_t)(uniform ? each : kStreamRows);
     p.stream_pieces = at_most(tiles, cuts, kLeastSteps * kStep);
     p.parts = 2 * cuts * kv_heads * p.stream_rows;
   }
-  if (!uniform || each > kStreamRows) {
+  if (uniform ? each > kStreamRows : !few) {
     // The prefill kernel from more than 128 rows a sequence on, the chunk kernel, of
     // half its rows a workgroup and two or three workgroups a CU, below; head_dim 256
     // has the prefill kernel alone.  (us, chunk / prefill kernel, 32 heads on 8 of
@@ -793,7 +804,7 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
     a.cuts = p.stream_cuts;
     a.part_rows = p.stream_rows;
     a.least_rows = 1;
-    a.most_rows = kStreamRows;
+    a.most_rows = p.stream_most;
     if (int st = launch<kDense>(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
   }
   if (p.chunk_pieces) {

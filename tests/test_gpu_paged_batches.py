@@ -52,6 +52,23 @@ def test_more_sequences_than_lanes(device, chunk, dim, dtype) -> None:
         c.check(out, lse, dim**-0.5)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("chunks,heads,kv_heads,dim,dtype", [
+    ([1, 1, 1, 1, 1], 8, 2, 128, BF16),
+    ([5, 0, 0, 0, 0], 10, 2, 128, BF16),       # 25 rows: two row tiles of one sequence
+    ([0, 3, 0, 0, 2], 12, 1, 64, F16),
+    ([0, 0, 0, 0, 4], 40, 2, 64, FP8),         # 80 rows
+    ([2, 0, 3, 0, 0], 11, 1, 256, FP8),        # an odd group: tiles end inside a token
+    ([0, 0, 4, 0, 0], 9, 1, 128, F16),
+])
+def test_no_more_tokens_than_sequences(device, chunks, heads, kv_heads, dim, dtype, causal) -> None:
+    print(f"few tokens {chunks} {heads}/{kv_heads}x{dim} {dtype} {causal}", flush=True)
+    for lengths in ([3000, 33, 900, 0, 1700], [3, 2, 1, 65, 2]):
+        c = Case(device, 33, lengths, chunks, heads, kv_heads, dim, 16, dtype, hot=True)
+        out, lse = paged.attention(c.q.to(device), c.cache, *c.device_args(), causal=causal, return_lse=True)
+        c.check(out, lse, dim**-0.5, causal=causal)
+
+
 def test_more_uneven_sequences_than_lanes(device) -> None:
     lengths = [(53 * b) % 307 for b in range(100)]
     chunks = [(0, 1, 2, 7, 30, 66)[b % 6] for b in range(100)]
