@@ -9,7 +9,9 @@
 // product, whose error then is of the output's own rounding.
 //
 // A workgroup takes 16 rows, which are (token, head) pairs of one kv head,
-// against one piece of the keys; its four waves take steps of 32 keys each.
+// against one piece of the keys; its four waves take steps of 32 keys each.  Bound
+// by HBM: 16 sequences of 32K bf16 keys (2.15 GB) take 368 us, 5.8 TB/s, where a
+// plain read of 2 GiB makes 5.9; 4 of up to 128K fp8 keys 160 us, 5.0 TB/s.
 // Keys are the A operand of v_mfma_f32_16x16x32 and queries the B operand, so a
 // lane ends with eight scores of ONE row (lane & 15) and those are, as they
 // stand, the B operand of the second product: its k index is any order of the
@@ -76,24 +78,34 @@ struct Tile {
 // What a workgroup of the stream kernel takes.
 enum Work {
   kDense,     // a piece of a sequence's keys
+  kBeside,    // the same for two heads that lie side by side, eight waves
   kSelected,  // a piece of a token's list
   kSolo,      // four tokens' lists, each wave one by itself
 };
 
+// Heads of a workgroup, four waves each, and waves that a SIMD holds.
+template <Work kWork>
+constexpr int kHeadsOf = kWork == kBeside ? 2 : 1;
+template <int D, Work kWork>
+constexpr int kPerSimd = kWork == kBeside ? 2 : kPerCu<D>;
+
 template <class Tag, bool kFp8, int D, Work kWork>
-__global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAttentionArgs a) {
+__global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void paged_stream_kernel(PagedAttentionArgs a) {
   using T = Tile<kFp8, D>;
-  constexpr bool kListed = kWork != kDense;
+  constexpr bool kListed = kWork == kSelected || kWork == kSolo;
+  constexpr int kHeads = kHeadsOf<kWork>;
+  constexpr uint32_t kWaves = 4;  // of a head
+  constexpr uint32_t kThreads = 64 * kWaves * kHeads;
   constexpr uint32_t kAhead = kFp8 ? 2 : 1;  // steps on their way in registers
   constexpr int kQ = D / 32;  // k-steps of the first product
   constexpr int kO = D / 16;  // dim tiles of the second
   // A wave's value tile (at the end its output) and key tile, one offset apart.
   constexpr uint32_t kValues = kStep * D * 2;
-  __shared__ __attribute__((aligned(16))) char tiles[4][kValues + kStep * T::kBytes];
+  __shared__ __attribute__((aligned(16))) char tiles[kWaves * kHeads][kValues + kStep * T::kBytes];
   // A wave's cache rows of this group of steps and the next; negative: padding.
-  __shared__ __attribute__((aligned(16))) int32_t table[4][2][kGroup * kStep];
-  __shared__ __attribute__((aligned(16))) float scales[4][64];
-  __shared__ float2 sums[4][16];
+  __shared__ __attribute__((aligned(16))) int32_t table[kWaves * kHeads][2][kGroup * kStep];
+  __shared__ __attribute__((aligned(16))) float scales[kWaves * kHeads][64];
+  __shared__ float2 sums[kWaves * kHeads][16];
   __shared__ uint32_t last_piece;
   const uint32_t lane = lane_id();
   const uint32_t wave = threadIdx.x / kWave;
@@ -106,8 +118,10 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   // fastest 385 / 209, heads on one XCD 397 / 191).
   constexpr bool kTogether = kFp8 && !kListed;
   const uint32_t turn = kTogether ? blockIdx.x / kXcds : blockIdx.x;
-  const uint32_t g = turn % a.cache.kv_heads;
-  const uint32_t id = kTogether ? turn / a.cache.kv_heads * kXcds + blockIdx.x % kXcds : turn / a.cache.kv_heads;
+  const uint32_t kinds = a.cache.kv_heads / kHeads;
+  const uint32_t g0 = turn % kinds * kHeads;
+  const uint32_t g = kHeads == 1 ? g0 : g0 + wave / kWaves;  // this wave's head
+  const uint32_t id = kTogether ? turn / kinds * kXcds + blockIdx.x % kXcds : turn / kinds;
 
   uint32_t sequence, token0, row0, rows, length, begin, end, pieces, index, slot, tile_slot, seen0 = 0;
   if constexpr (kListed) {
@@ -156,12 +170,12 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   const uint32_t sees = partly ? (uint32_t)max(0, (int32_t)(seen0 + my_row / a.group + 1u)) : end;
   const uint32_t all_see = partly ? (uint32_t)max(0, (int32_t)(seen0 + row0 / a.group + 1u)) : end;
 
-  auto out_row = [&](uint32_t r) {
+  auto out_row = [&](uint32_t h, uint32_t r) {
     const uint64_t token = kListed ? token0 : token0 + (row0 + r) / a.group;
-    return token * a.heads + g * a.group + (kListed ? row0 + r : (row0 + r) % a.group);
+    return token * a.heads + (g0 + h) * a.group + (kListed ? row0 + r : (row0 + r) % a.group);
   };
-  auto part_at = [&](uint32_t piece, uint32_t r) {
-    return ((uint64_t)piece * a.cache.kv_heads + g) * a.part_rows + r;
+  auto part_at = [&](uint32_t piece, uint32_t h, uint32_t r) {
+    return ((uint64_t)piece * a.cache.kv_heads + g0 + h) * a.part_rows + r;
   };
 
   uint4 q[kQ];
@@ -192,10 +206,10 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   for (int i = 0; i < kO; ++i)
     tr_place[i] = tile_place<2 * D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1)) + 8u * (col & 1u);
 
-  // The wave's steps are every fourth of the piece (all of its own list), step s at
-  // keys first_key(s).
-  constexpr uint32_t kApart = kWork == kSolo ? 1 : 4;
-  const uint32_t from = kWork == kSolo ? 0u : wave;
+  // The steps of a piece are dealt to its head's waves (a list of its own is all
+  // the wave's), step s at keys first_key(s).
+  constexpr uint32_t kApart = kWork == kSolo ? 1 : kWaves;
+  const uint32_t from = kWork == kSolo ? 0u : wave % kWaves;
   const uint32_t steps = (end - begin + kStep - 1u) / kStep;
   const uint32_t own = steps > from ? (steps - from + kApart - 1u) / kApart : 0u;
   auto first_key = [&](uint32_t step) { return begin + (kApart * step + from) * kStep; };
@@ -400,7 +414,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
 
   if (!kListed && __any(dropped)) {
     for (uint32_t k = max(begin, all_see); k < end; ++k)
-      if ((k - begin) / kStep % 4u == wave && k < sees) {
+      if ((k - begin) / kStep % kWaves == from && k < sees) {
         const uint32_t row = cache_row(a, pages, k);
 #pragma unroll
         for (int i = 0; i < kO; ++i) {
@@ -411,44 +425,47 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
       }
   }
 
-  // Join the four waves: every wave scales its sums to the largest reference.
+  // Join a head's waves: every wave scales its sums to the largest reference.
   total += __shfl_xor(total, 16, kWave);
   total += __shfl_xor(total, 32, kWave);
   if constexpr (kWork == kSolo) {
     if (row0 + col < rows) {
 #pragma unroll
-      for (int i = 0; i < kO; ++i) store_out<Tag, D>(a, out_row(col), 16u * i + 4u * quad, o[i], reference, total);
+      for (int i = 0; i < kO; ++i) store_out<Tag, D>(a, out_row(0, col), 16u * i + 4u * quad, o[i], reference, total);
     }
     return;
   }
   if (quad == 0) sums[wave][col] = make_float2(reference, total);
   __syncthreads();
-  float most = sums[0][col].x;
+  const uint32_t first_wave = wave / kWaves * kWaves;
+  float most = sums[first_wave][col].x;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) most = fmaxf(most, sums[w][col].x);
+  for (uint32_t w = 1; w < kWaves; ++w) most = fmaxf(most, sums[first_wave + w][col].x);
   const float shrink = exp2_fast(reference - most);
 #pragma unroll
   for (int i = 0; i < kO; ++i)
     *reinterpret_cast<floatx4*>(mine + col * (D * 4) + (((4u * i + quad) ^ col) << 4)) = o[i] * shrink;
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < 16u * (D / 4); i += 256u) {
-    const uint32_t r = i / (D / 4);
+  const uint32_t live = min(16u, rows - row0);
+  for (uint32_t i = threadIdx.x; i < kHeads * live * (D / 4); i += kThreads) {
     const uint32_t c = i % (D / 4);
-    if (row0 + r >= rows) break;
+    const uint32_t h = kHeads == 1 ? 0u : i / (D / 4) / live;
+    const uint32_t r = i / (D / 4) - h * live;
+    const uint32_t w0 = h * kWaves;
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-    float top = sums[0][r].x;
+    float top = sums[w0][r].x;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, sums[w][r].x);
+    for (uint32_t w = 1; w < kWaves; ++w) top = fmaxf(top, sums[w0 + w][r].x);
     float weight = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      sum += *reinterpret_cast<const floatx4*>(tiles[w] + r * (D * 4) + ((c ^ r) << 4));
-      weight += sums[w][r].y * exp2_fast(sums[w][r].x - top);
+    for (uint32_t w = 0; w < kWaves; ++w) {
+      sum += *reinterpret_cast<const floatx4*>(tiles[w0 + w] + r * (D * 4) + ((c ^ r) << 4));
+      weight += sums[w0 + w][r].y * exp2_fast(sums[w0 + w][r].x - top);
     }
     if (pieces == 1u) {
-      store_out<Tag, D>(a, out_row(r), 4u * c, sum, top, weight);
+      store_out<Tag, D>(a, out_row(h, r), 4u * c, sum, top, weight);
     } else {
-      const uint64_t at = part_at(slot + index, r);
+      const uint64_t at = part_at(slot + index, h, r);
       float2* to = reinterpret_cast<float2*>(a.part_out + at * D + 4u * c);
       store_shared(to, sum[0], sum[1]);
       store_shared(to + 1, sum[2], sum[3]);
@@ -466,7 +483,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    uint32_t* arrived = a.arrived + (tile_slot * a.cache.kv_heads + g);
+    uint32_t* arrived = a.arrived + (tile_slot * kinds + g0 / kHeads);
     const uint32_t before = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last_piece = before + 1u == pieces;
     if (before + 1u == pieces) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -478,15 +495,15 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
   // the rows leave, kPieces pieces' loads under way at a time.  (Kept short: it runs
   // once, from a cold instruction cache.)
   constexpr uint32_t kPieces = 8;
-  const uint32_t live = min(16u, rows - row0);
-  const uint32_t cells = live * (D / 4);
-  const uint32_t groups = max(1u, 256u / cells);
-  floatx4* joined = reinterpret_cast<floatx4*>(tiles[0]);  // [256]
-  floatx2* joined_sum = reinterpret_cast<floatx2*>(table);  // [256]
-  static_assert(sizeof(tiles) >= 256 * sizeof(floatx4) && sizeof(table) >= 256 * sizeof(floatx2), "join");
+  const uint32_t cells = kHeads * live * (D / 4);
+  const uint32_t groups = max(1u, kThreads / cells);
+  floatx4* joined = reinterpret_cast<floatx4*>(tiles[0]);  // [kThreads]
+  floatx2* joined_sum = reinterpret_cast<floatx2*>(table);  // [kThreads]
+  static_assert(sizeof(tiles) >= kThreads * sizeof(floatx4) && sizeof(table) >= kThreads * sizeof(floatx2), "join");
   const uint32_t group = threadIdx.x / cells;
-  for (uint32_t cell = threadIdx.x % cells; cell < cells; cell += 256u) {
-    const uint32_t r = cell / (D / 4);
+  for (uint32_t cell = threadIdx.x % cells; cell < cells; cell += kThreads) {
+    const uint32_t h = kHeads == 1 ? 0u : cell / (D / 4) / live;
+    const uint32_t r = cell / (D / 4) - h * live;
     const uint32_t dim = 4u * (cell % (D / 4));
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
     float top = kNoKeys;
@@ -503,7 +520,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
       float2 s[kPieces], lo[kPieces], hi[kPieces];
 #pragma unroll
       for (uint32_t j = 0; j < kPieces; ++j) {
-        const uint64_t at = part_at(slot + min(p + groups * j, pieces - 1u), r);
+        const uint64_t at = part_at(slot + min(p + groups * j, pieces - 1u), h, r);
         const float2* from = reinterpret_cast<const float2*>(a.part_out + at * D + dim);
         s[j] = load_shared(a.part_sum + at);
         lo[j] = load_shared(from);
@@ -523,7 +540,7 @@ __global__ __launch_bounds__(256, kPerCu<D>) void paged_stream_kernel(PagedAtten
         add(s[0], s[1], joined[i * cells + cell]);
       }
     }
-    if (group == 0) store_out<Tag, D>(a, out_row(r), dim, sum, top, weight);
+    if (group == 0) store_out<Tag, D>(a, out_row(h, r), dim, sum, top, weight);
   }
 }
 
@@ -569,14 +586,20 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
   store_out<Tag, D>(a, row, dim, sum, top, total);
 }
 
+template <class Tag, bool kFp8, int D, Work kWork>
+void launch_stream_of(const PagedAttentionArgs& a, uint32_t grid, hipStream_t s) {
+  if constexpr (kWork != kBeside || Tile<kFp8, D>::kBytes == 128)
+    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, D, kWork>), dim3(grid), dim3(256 * kHeadsOf<kWork>), 0, s, a);
+}
+
 template <class Tag, bool kFp8, Work kWork>
 void launch_stream(const PagedAttentionArgs& a, int32_t dim, uint32_t grid, hipStream_t s) {
   if (dim == 64)
-    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 64, kWork>), dim3(grid), dim3(256), 0, s, a);
+    launch_stream_of<Tag, kFp8, 64, kWork>(a, grid, s);
   else if (dim == 128)
-    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 128, kWork>), dim3(grid), dim3(256), 0, s, a);
+    launch_stream_of<Tag, kFp8, 128, kWork>(a, grid, s);
   else
-    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, 256, kWork>), dim3(grid), dim3(256), 0, s, a);
+    launch_stream_of<Tag, kFp8, 256, kWork>(a, grid, s);
 }
 
 template <class Tag>
@@ -600,7 +623,7 @@ int combine(const PagedAttentionArgs& a, int32_t dim, int32_t dtype, hipStream_t
 
 template <Work kWork>
 int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dtype, int64_t pieces, hipStream_t s) {
-  const int64_t grid = pieces * a.cache.kv_heads;
+  const int64_t grid = pieces * (a.cache.kv_heads / kHeadsOf<kWork>);
   DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
   const int32_t dim = cache->head_dim;
   if (cache->dtype == kFP8E4M3)
@@ -686,6 +709,7 @@ int take_workspace(PagedAttentionArgs& a, int64_t parts, int64_t rows, int64_t d
 struct Plan {
   uint32_t stream_cuts, stream_rows;  // rows of a part
   uint32_t stream_most;               // rows of a sequence of the stream kernel's
+  bool stream_beside;                 // it takes heads side by side
   int64_t stream_pieces;              // at most; 0: no sequence of few rows
   bool prefill;                       // the prefill kernel takes the other sequences, else the chunk kernel
   int32_t chunk_rows;                 // of a tile of theirs
@@ -693,6 +717,23 @@ struct Plan {
   int64_t chunk_pieces;
   int64_t parts, rows;
 };
+
+// Whether the stream kernel takes two heads a workgroup: heads of 128 bytes that lie
+// side by side, from 128 MiB of cache on.  HBM serves 256 contiguous bytes that one
+// workgroup asks for together faster than two requests of 128 at different times
+// (fp8 of 128 dims read at 4.6 TB/s, with a head's rows contiguous at 5.6); a cache
+// that the last-level cache holds is not bound by that, and eight waves a workgroup
+// start and join later.  (us, four waves / eight, 8 kv heads: fp8 of 128 dims, 4
+// sequences of up to 128K keys 178 / 160, 16 of 32K 239 / 212, 64 of 4K 119 / 107,
+// one of 32K, 67 MB, 27 / 32; 16-bit of 64 dims, 16 of 32K 212 / 191, 64 of 4K 122 /
+// 98, one of 32K 23 / 20; 2 kv heads of fp8, 64 of 4K, 128 MiB, 32 / 32, one of 32K
+// 25 / 35.  Heads of 64 bytes, fp8 of 64 dims, lose more by two waves a SIMD instead of
+// three: 16 of 32K 136 / 178.)
+bool heads_lie_beside(const dsa_paged_cache* cache, int64_t sequences, int64_t capacity) {
+  return cache->head_dim * (cache->dtype == kFP8E4M3 ? 1 : 2) == 128 && cache->kv_heads % 2 == 0 &&
+         cache->key_head_stride == cache->head_dim && cache->value_head_stride == cache->head_dim &&
+         sequences * capacity * cache->kv_heads >= 1LL << 19;
+}
 
 Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens, int64_t heads, int64_t capacity,
                 bool uniform) {
@@ -712,7 +753,10 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
   // sequence of 32K and none of 15 others 43 / 68, 43 / 38.)
   const bool few = !uniform && tokens <= sequences;
   if (!uniform || each <= kStreamRows) {
-    const int64_t cuts = (resident_workgroups(cache->head_dim) + kv_heads - 1) / kv_heads;
+    p.stream_beside = heads_lie_beside(cache, sequences, capacity);
+    const int64_t kinds = p.stream_beside ? kv_heads / 2 : kv_heads;
+    const int64_t fill = p.stream_beside ? 256 : resident_workgroups(cache->head_dim);
+    const int64_t cuts = (fill + kinds - 1) / kinds;
     const int64_t tiles = (tokens < sequences ? tokens : sequences) + (few ? tokens * group / kStreamRows : 0);
     p.stream_most = few ? 0xffffffffu : kStreamRows;
     p.stream_cuts = (uint32_t)cuts;
@@ -805,7 +849,8 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
     a.part_rows = p.stream_rows;
     a.least_rows = 1;
     a.most_rows = p.stream_most;
-    if (int st = launch<kDense>(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
+    const auto launch_stream = p.stream_beside ? launch<kBeside> : launch<kDense>;
+    if (int st = launch_stream(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
   }
   if (p.chunk_pieces) {
     a.cuts = p.chunk_cuts;

@@ -69,6 +69,41 @@ def test_no_more_tokens_than_sequences(device, chunks, heads, kv_heads, dim, dty
         c.check(out, lse, dim**-0.5, causal=causal)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(8, 4, 128, FP8), (6, 2, 64, BF16), (4, 4, 64, F16), (32, 2, 128, FP8)])
+@pytest.mark.parametrize("chunks", [[1, 1, 1, 1], [2, 0, 1, 1], [3, 2, 1, 0], [2, 2, 2, 2]])
+def test_heads_beside_each_other(device, chunks, heads, kv_heads, dim, dtype) -> None:
+    """Page tables of more than 128 MiB of cache, whatever the lengths."""
+
+    print(f"heads beside {chunks} {heads}/{kv_heads}x{dim} {dtype}", flush=True)
+    c = Case(device, 34, [2100, 40, 700, 0], chunks, heads, kv_heads, dim, 64, dtype, hot=True)
+    table, lengths, starts = c.device_args()
+    wide = torch.full((4, 2200), 1 << 30, dtype=torch.int32, device=device)
+    wide[:, :table.shape[1]] = table
+    assert 4 * wide.shape[1] * 64 * kv_heads * 256 >= 128 << 20
+    for causal in (True, False):
+        out, lse = paged.attention(c.q.to(device), c.cache, wide, lengths, starts, causal=causal, return_lse=True)
+        c.check(out, lse, dim**-0.5, causal=causal)
+
+
+def test_values_that_are_not_finite_beside(device) -> None:
+    """The eight-wave variant hides later tokens' values as the others do."""
+
+    c = Case(device, 35, [300], [4], 4, 2, 128, 64, FP8)
+    table, lengths, starts = c.device_args()
+    wide = torch.full((1, 4200), 1 << 30, dtype=torch.int32, device=device)
+    wide[:, :table.shape[1]] = table
+    q = c.q.to(device)
+    row = int(paged.cache_rows(c.cache, table, torch.tensor([298], device=device), torch.tensor([0], device=device)))
+    _poke(c.cache.values, row, [3, 77], 0.0)
+    clean = paged.attention(q, c.cache, wide, lengths, starts)
+    _poke(c.cache.values, row, [3, 77], math.nan)
+    got = paged.attention(q, c.cache, wide, lengths, starts)
+    assert torch.equal(got[:2], clean[:2])
+    want = clean[2:].float()
+    want[:, :, [3, 77]] = math.nan
+    assert torch.equal(torch.nan_to_num(got[2:].float(), 7e4), torch.nan_to_num(want, 7e4))
+
+
 def test_more_uneven_sequences_than_lanes(device) -> None:
     lengths = [(53 * b) % 307 for b in range(100)]
     chunks = [(0, 1, 2, 7, 30, 66)[b % 6] for b in range(100)]
