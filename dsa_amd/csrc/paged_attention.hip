@@ -714,6 +714,7 @@ struct Plan {
   bool prefill;                       // the prefill kernel takes the other sequences, else the chunk kernel
   int32_t chunk_rows;                 // of a tile of theirs
   uint32_t chunk_cuts;                // 0: more row tiles than could be cut to use
+  uint32_t chunk_whole;               // row tiles that are not cut all the same
   int64_t chunk_pieces;
   int64_t parts, rows;
 };
@@ -776,11 +777,26 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
     const int64_t fill = p.prefill ? 256 : resident_workgroups(cache->head_dim);
     const int64_t cuts = (fill + kv_heads - 1) / kv_heads;
     const int64_t tiles = row_tiles(sequences, tokens, group, uniform, p.chunk_rows);
-    if (tiles >= 2 * cuts) {
+    // One sequence: row tiles that fill the GPU some times over are not cut, those
+    // left over are, but for most of a prompt from its start, whose last tiles to run
+    // are its shortest.  (us, all whole / the rest cut, 32 heads on 8 of 128 dims, 32K
+    // keys, 32 tiles at a time: 33 tiles 1590 / 977, 48 1593 / 1411, 65 2459 / 1818, 136
+    // 3957 / 3538, 258 6087 / 6064; of 8K keys 65 472 / 395, 80, 5120 tokens, 471 / 483,
+    // 104 505 / 542.)
+    const int64_t rest = tiles % cuts;
+    const bool cut = sequences == 1 && tiles >= cuts
+                         ? rest > 0 && tiles < 8 * cuts && (tiles < 2 * cuts || 8 * tokens <= 5 * capacity)
+                         : tiles < 2 * cuts;
+    if (!cut) {
       p.chunk_pieces = tiles;
     } else {
       p.chunk_cuts = (uint32_t)cuts;
-      p.chunk_pieces = at_most(tiles, cuts, kLeastChunkKeys);
+      if (sequences == 1 && tiles >= cuts) {
+        p.chunk_whole = (uint32_t)(tiles - rest);
+        p.chunk_pieces = tiles - rest + (cuts > rest ? cuts : rest);
+      } else {
+        p.chunk_pieces = at_most(tiles, cuts, kLeastChunkKeys);
+      }
       p.rows = tokens * heads;
       if (p.parts < 2 * cuts * kv_heads * p.chunk_rows) p.parts = 2 * cuts * kv_heads * p.chunk_rows;
     }
@@ -854,6 +870,7 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
   }
   if (p.chunk_pieces) {
     a.cuts = p.chunk_cuts;
+    a.whole = p.chunk_whole;
     a.part_rows = (uint32_t)p.chunk_rows;
     a.least_rows = kStreamRows + 1;
     a.most_rows = 0xffffffffu;

@@ -41,6 +41,7 @@ struct PagedAttentionArgs {
   uint32_t causal;
   uint32_t most_rows;       // sequences of more (token, head) rows per kv head are another kernel's
   uint32_t least_rows;
+  uint32_t whole;           // row tiles of a single sequence that are not cut (see find_piece)
   float scale;              // times log2 e
   char* out;                // [tokens][heads][dim]
   float* lse;               // nullable: [tokens][heads]
@@ -102,10 +103,33 @@ struct Piece {
 // after them; so for up to 64 sequences that length grows until the pieces fit.  A
 // tile is cut evenly (ragged fp16 chunks, us: 111, and 129 with the remainder in a
 // tile's last piece).  At most cuts + tiles pieces, and at most 2 cuts of tiles
-// that have several.
+// that have several.  With `whole`, a multiple of cuts, there is one sequence: its
+// first `whole` tiles fill the GPU some times over, and only the others are cut, into
+// at most cuts pieces together.
 template <uint32_t kTileRows, uint32_t kUnit, uint32_t kLeast>
 __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, uint32_t id, Piece& p) {
   const uint32_t lane = lane_id();
+  if (a.whole) {
+    p.sequence = 0;
+    p.span = tokens_of(a, 0);
+    p.keys = keys_of(a, 0);
+    const uint32_t rows = p.span.count * a.group;
+    const uint32_t tiles = rows >= a.least_rows && rows <= a.most_rows ? (rows + kTileRows - 1u) / kTileRows : 0u;
+    const uint32_t units = (p.keys + kUnit - 1u) / kUnit;
+    p.tile = id;
+    p.units = max(1u, units);
+    p.index = 0;
+    p.count = 1;
+    p.slot = 0;
+    if (id < a.whole || tiles <= a.whole) return id < tiles;
+    const uint32_t rest = tiles - a.whole;
+    p.count = min(max(1u, min(a.cuts / rest, units / kLeast)), kMostSplits);
+    p.tile = a.whole + (id - a.whole) / p.count;
+    p.index = (id - a.whole) % p.count;
+    p.units = max(1u, (units + p.count - 1u) / p.count);
+    p.slot = (p.tile - a.whole) * p.count;
+    return p.tile < tiles;
+  }
   Span span = {0, 0};
   uint32_t keys = 0, units = 0, tiles = 0;
   auto look = [&](uint32_t b) {

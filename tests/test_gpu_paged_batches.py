@@ -211,3 +211,30 @@ def test_scales_of_rows_that_no_list_names(device) -> None:
     out, lse = paged.selected_attention(c.q.to(device), c.cache, *c.device_args()[:2],
                                         torch.from_numpy(lists).to(device), return_lse=True)
     c.check(out, lse, 128**-0.5, lists=lists)
+
+
+@pytest.mark.parametrize("length,chunk,heads,kv_heads,dim,dtype,causal", [
+    (1300, 1152, 64, 32, 64, BF16, True),      # nine row tiles of 256 rows where eight run at a time
+    (1300, 1152, 64, 32, 64, FP8, False),
+    (650, 600, 128, 64, 128, F16, True),       # five, four at a time: more room than keys for the last one
+    (2000, 800, 128, 64, 128, BF16, True),     # seven: three left over
+    (700, 530, 64, 64, 256, BF16, True),       # five of 128 rows
+    (600, 512, 64, 64, 256, FP8, True),        # four: none left over
+    (20, 600, 128, 64, 64, BF16, True),        # more tokens than keys
+    (0, 600, 128, 64, 64, BF16, True),
+    (300, 280, 256, 128, 64, F16, True),       # three, two at a time
+])
+def test_more_row_tiles_than_workgroups(device, length, chunk, heads, kv_heads, dim, dtype, causal) -> None:
+    """One sequence whose row tiles do not divide by the workgroups that run at a
+    time; the first and the last kv head are checked."""
+
+    print(f"row tiles {length} {chunk} {heads}/{kv_heads}x{dim} {dtype} {causal}", flush=True)
+    c = Case(device, 71, [length], [chunk], heads, kv_heads, dim, 16, dtype)
+    outs = [paged.attention(c.q.to(device), c.cache, *c.device_args(starts), causal=causal, return_lse=True)
+            for starts in (True, False)]
+    group = heads // kv_heads
+    keep = [*range(group), *range(heads - group, heads)]
+    c.q, c.heads = c.q[:, keep], 2 * group
+    c.keys64, c.values64 = c.keys64[:, :, [0, -1]], c.values64[:, :, [0, -1]]
+    for out, lse in outs:
+        c.check(out[:, keep], lse[:, keep], dim**-0.5, causal=causal)
