@@ -17,7 +17,7 @@
 // stand, the B operand of the second product: its k index is any order of the
 // 32 keys that both operands share, and here is the order the scores have.  The
 // values' transposed operand is read from LDS by ds_read_b64_tr_b16.  Every row
-// of the cache is read once, as 16-byte loads of 64 contiguous bytes a row.
+// of the cache is read once, as 16-byte loads of up to 128 contiguous bytes a row.
 #include "paged_attention.hpp"
 
 namespace dsa {
@@ -741,6 +741,7 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
   const int64_t kv_heads = cache->kv_heads;
   const int64_t group = heads / kv_heads;
   Plan p = {};
+  uniform |= sequences == 1;  // whose starts are 0 and tokens
   const int64_t each = tokens / sequences * group;
   auto at_most = [&](int64_t tiles, int64_t cuts, int64_t least) {
     const int64_t pieces = tiles * ((capacity + least - 1) / least);
