@@ -196,7 +196,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
       most = fmaxf(most, __shfl_xor(most, 32, kWave)) - kLift;
       const float raise = first ? (most == -INFINITY ? 0.f : most) : fmaxf(most, 0.f);
       reference += raise;
-      const float shrink = exp2_fast(-raise);
+      // (the first raise may be below zero, by any amount: its sums are 0 and must stay so)
+      const float shrink = exp2_fast(fminf(-raise, 0.f));
       total *= shrink;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) o[i] *= shrink;

@@ -197,7 +197,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
       const float top = fmaxf(x.most, __shfl_xor(x.most, 32, kWave)) - kLift;
       const float raise = first ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
       reference += raise;
-      const float shrink = exp2_fast(-raise);
+      // (the first raise may be below zero, by any amount: its sums are 0 and must stay so)
+      const float shrink = exp2_fast(fminf(-raise, 0.f));
       total *= shrink;
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) o[i] *= shrink;
