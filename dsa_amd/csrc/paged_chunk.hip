@@ -97,7 +97,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-  float reference = 0.f;  // set by the first tile: a row that sees any key of the piece sees its first
+  float reference = 0.f;  // set by the row's first keys whose scores are not all -inf
+  bool fresh = true;      // the row has no reference yet
   float total = 0.f;
 
   const int32_t* pages = a.page_table + (int64_t)piece.sequence * a.table_stride;
@@ -192,9 +193,11 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
       for (int e = 0; e < 16; e += 2) most = fmaxf(fmaxf(most, x[s][e]), x[s][e + 1]);
       return most;
     };
-    auto raise_by = [&](float most, bool first) {
+    auto raises = [&](float most) { return __any(most > (fresh ? -INFINITY : kLift + kSlack)); };
+    auto raise_by = [&](float most) {
       most = fmaxf(most, __shfl_xor(most, 32, kWave)) - kLift;
-      const float raise = first ? (most == -INFINITY ? 0.f : most) : fmaxf(most, 0.f);
+      const float raise = most > (fresh ? -INFINITY : 0.f) ? most : 0.f;
+      fresh = fresh && most == -INFINITY;
       reference += raise;
       // (the first raise may be below zero, by any amount: its sums are 0 and must stay so)
       const float shrink = exp2_fast(fminf(-raise, 0.f));
@@ -240,9 +243,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
     }
     __builtin_amdgcn_sched_barrier(0);
     const float most0 = scores(0);
-    // A row that sees any key of the piece sees its first: the first tile's first
-    // half sets the reference.
-    if (t == 0 || __any(most0 > kLift + kSlack)) x[0] -= raise_by(most0, t == 0);
+    if (raises(most0)) x[0] -= raise_by(most0);
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) x[1] = mfma_32x32x16(Tag{}, kb[j], q[j], x[1]);
     weigh(0);
@@ -253,9 +254,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
 #pragma unroll
     for (int e = 0; e < 16; ++e) pin(weight[0][e]);
     const float most1 = scores(1);
-    if (__any(most1 > kLift + kSlack)) {
-      const float raise = raise_by(most1, false);
-      const float shrink = exp2_fast(-raise);
+    if (raises(most1)) {
+      const float raise = raise_by(most1);
+      const float shrink = exp2_fast(fminf(-raise, 0.f));
 #pragma unroll
       for (int e = 0; e < 16; ++e) weight[0][e] *= shrink;
       x[1] -= raise;

@@ -56,3 +56,30 @@ def test_scores_far_below_zero(device, lengths, chunks, heads, kv_heads, dim, dt
     for causal in (True, False):
         out, lse = paged.attention(c.q.to(device), c.cache, *c.device_args(), causal=causal, return_lse=True)
         c.check(out, lse, scale, causal=causal)
+
+
+@pytest.mark.parametrize("below", [4.0, 60.0, 300.0])
+@pytest.mark.parametrize("lengths,chunks,heads,kv_heads,dim,dtype", [r for r in ROWS if r[-1] != FP8])
+def test_first_keys_that_score_minus_infinity(device, lengths, chunks, heads, kv_heads, dim, dtype, below) -> None:
+    """Keys with an infinity that the queries weigh negatively have weights of 0, however
+    far below zero the later keys' scores are."""
+
+    print(f"-inf, then about -{below}: {lengths} {chunks} {heads}/{kv_heads}x{dim} {dtype}", flush=True)
+    c = Case(device, 82, lengths, chunks, heads, kv_heads, dim, 16, dtype)
+    scale = dim**-0.5
+    _set_key_dim(c, 0, -16.0)
+    c.q[:, :, 0] = below / scale / 16.0
+    first = [min((3 * n) // 4, n - n_new) for n, n_new in zip(lengths, chunks)]  # every row sees its own key beyond them
+    for b, n in enumerate(first):
+        rows = paged.cache_rows(c.cache, c.table.to(device), torch.arange(n, device=device),
+                                torch.full((n,), b, dtype=torch.int64, device=device))
+        flat = c.cache.keys.view(-1, kv_heads, dim)
+        flat[rows, :, 0] = -math.inf
+    for causal in (True, False):
+        lists = np.full((sum(chunks), max(lengths)), -1, dtype=np.int64)
+        for b, n in enumerate(lengths):
+            for i in range(chunks[b]):
+                last = n - chunks[b] + i + 1 if causal else n
+                lists[c.starts[b] + i, first[b]:last] = np.arange(first[b], last)
+        out, lse = paged.attention(c.q.to(device), c.cache, *c.device_args(), causal=causal, return_lse=True)
+        c.check(out, lse, scale, lists=lists)
