@@ -562,11 +562,14 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
       const uint32_t mid = (low + high) / 2u;
       if (a.starts[mid] <= (int32_t)token) low = mid; else high = mid;
     }
-    if (tokens_of(a, low).count * a.group < a.least_rows) return;
+    const Span span = tokens_of(a, low);
+    if (token - span.first >= span.count || span.count * a.group < a.least_rows) return;
   }
+  // A token outside every sequence has no entry here (a batch padded to a fixed number
+  // of tokens), nor has one of `starts` that fall: what stands there is not an index.
   const uint2 of = a.part_of[row];
-  if (of.y == 1u) return;
   const uint32_t apart = a.cache.kv_heads * a.part_rows;
+  if (of.y < 2u || of.y > kMostSplits || of.x + (uint64_t)(of.y - 1u) * apart >= a.parts) return;
   const float2* sums = a.part_sum + of.x;
   const float* parts = a.part_out + (uint64_t)of.x * D + dim;
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -702,6 +705,7 @@ int take_workspace(PagedAttentionArgs& a, int64_t parts, int64_t rows, int64_t d
   a.part_out = reinterpret_cast<float*>(a.arrived + kCounters);
   a.part_sum = reinterpret_cast<float2*>(a.part_out + parts * dim);
   a.part_of = reinterpret_cast<uint2*>(a.part_sum + parts);
+  a.parts = (uint32_t)parts;
   return 0;
 }
 

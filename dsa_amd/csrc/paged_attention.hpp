@@ -49,6 +49,7 @@ struct PagedAttentionArgs {
   // [part_rows]: outputs [dim], and {reference, sum}.
   float* part_out;
   float2* part_sum;
+  uint32_t parts;           // rows that part_out and part_sum have room for
   uint32_t part_rows;
   uint2* part_of;           // chunk kernel: [tokens][heads] {part of the row's first piece, pieces}
   uint32_t* arrived;        // stream kernel: pieces of each row tile that are done; zero between calls

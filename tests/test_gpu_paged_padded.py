@@ -1,0 +1,63 @@
+"""Paged attention of batches padded to a fixed number of tokens: the last tokens, or
+the first ones, belong to no sequence.  The sequences' own rows are those of the batch
+without padding, in every kernel."""
+
+from __future__ import annotations
+
+import functools
+
+import pytest
+import torch
+
+from dsa_amd import paged
+from test_gpu_paged import BF16, F16, FP8, Case
+
+pytestmark = pytest.mark.gpu
+
+PADDED = [
+    # lengths, chunks, before, after, heads, kv_heads, dim, dtype
+    ([300, 40], [1, 1], 0, 6, 8, 2, 128, BF16),                  # a decode step of few sequences in many places
+    ([300, 40, 90, 9], [1, 1, 1, 1], 0, 0, 8, 2, 128, BF16),
+    ([900, 64, 1, 300], [1, 1, 0, 1], 0, 1, 8, 2, 64, FP8),
+    ([700, 515], [50, 50], 0, 100, 8, 2, 128, BF16),             # pieces that another launch joins
+    ([700, 515], [50, 50], 7, 93, 8, 2, 128, F16),
+    ([900, 64, 1, 300], [70, 1, 1, 30], 0, 154, 8, 2, 64, BF16),
+    ([515, 300, 1], [66, 67, 0], 3, 500, 8, 2, 128, FP8),
+    ([1000], [30], 0, 34, 8, 2, 256, BF16),                      # one sequence
+    ([700], [65], 5, 60, 8, 2, 128, BF16),
+    ([1900], [33], 0, 31, 8, 2, 128, F16),
+    ([650], [600], 0, 20, 128, 64, 128, BF16),                   # more row tiles than run at a time
+    ([650], [300], 0, 320, 128, 64, 128, BF16),
+]
+
+
+def _padded(c: Case, before: int, after: int, device):
+    """Queries and starts of a case with tokens of no sequence around its own."""
+
+    q = torch.full((before + len(c.q) + after, *c.q.shape[1:]), 3.0, dtype=c.q.dtype)
+    q[before:before + len(c.q)] = c.q
+    return q.to(device), torch.tensor(c.starts + before, dtype=torch.int32, device=device)
+
+
+@functools.lru_cache(maxsize=1)
+def _other_call(device):
+    c = Case(device, 93, [3000], [64], 32, 2, 128, 16, BF16)
+    return c.q.to(device), c.cache, *c.device_args()
+
+
+def _soil_workspace(device) -> None:
+    """Leaves numbers of another call's pieces all over the workspace."""
+
+    paged.attention(*_other_call(device))
+
+
+@pytest.mark.parametrize("lengths,chunks,before,after,heads,kv_heads,dim,dtype", PADDED)
+def test_attention_of_padded_batches(device, lengths, chunks, before, after, heads, kv_heads, dim, dtype) -> None:
+    print(f"padded: {lengths} {before}+{chunks}+{after} {heads}/{kv_heads}x{dim} {dtype}", flush=True)
+    c = Case(device, 91, lengths, chunks, heads, kv_heads, dim, 16, dtype)
+    q, starts = _padded(c, before, after, device)
+    own = slice(before, before + len(c.q))
+    for causal in (True, False):
+        _soil_workspace(device)
+        out, lse = paged.attention(q, c.cache, *c.device_args()[:2], starts, causal=causal, return_lse=True)
+        c.check(out[own], lse[own], dim**-0.5, causal=causal)
