@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
   float reference = 0.f;  // set by the row's first keys whose scores are not all -inf
-  bool fresh = true;      // the row has no reference yet
+  uint64_t fresh = __ballot(sees > begin);  // lanes whose row has no reference yet
   float total = 0.f;
 
   const int32_t* pages = a.page_table + (int64_t)piece.sequence * a.table_stride;
@@ -193,11 +193,11 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
       for (int e = 0; e < 16; e += 2) most = fmaxf(fmaxf(most, x[s][e]), x[s][e + 1]);
       return most;
     };
-    auto raises = [&](float most) { return __any(most > (fresh ? -INFINITY : kLift + kSlack)); };
+    auto raises = [&](float most) { return (__ballot(most > kLift + kSlack) | fresh) != 0; };
     auto raise_by = [&](float most) {
       most = fmaxf(most, __shfl_xor(most, 32, kWave)) - kLift;
-      const float raise = most > (fresh ? -INFINITY : 0.f) ? most : 0.f;
-      fresh = fresh && most == -INFINITY;
+      const float raise = most > (fresh >> lane & 1u ? -INFINITY : 0.f) ? most : 0.f;
+      fresh &= __ballot(most == -INFINITY);
       reference += raise;
       // (the first raise may be below zero, by any amount: its sums are 0 and must stay so)
       const float shrink = exp2_fast(fminf(-raise, 0.f));

@@ -87,7 +87,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
   float reference = 0.f;  // set by the row's first tile whose scores are not all -inf
-  bool fresh = true;      // the row has no reference yet
+  uint64_t fresh = __ballot(sees > begin);  // lanes whose row has no reference yet
   float total = 0.f;
 
   const int32_t* pages = a.page_table + (int64_t)piece.sequence * a.table_stride;
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
     x.s[e / 16][e % 16] = fmaf(x.s[e / 16][e % 16], by, -reference);
   };
   // Hides what the row does not see, and raises the reference if a score passes it.
-  auto settle = [&](Scores& x, uint32_t t) {
+  auto settle = [&](Scores& x, uint32_t t, bool first) {
     const uint32_t key0 = begin + t * kTileKeys;
     if (key0 + kTileKeys > all_see) {
       x.most = -INFINITY;
@@ -194,10 +194,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
           x.most = fmaxf(x.most, x.s[h][e]);
         }
     }
-    if (__any(x.most > (fresh ? -INFINITY : kLift + kSlack))) {
+    if (first || (__ballot(x.most > kLift + kSlack) | fresh) != 0) {
       const float top = fmaxf(x.most, __shfl_xor(x.most, 32, kWave)) - kLift;
-      const float raise = top > (fresh ? -INFINITY : 0.f) ? top : 0.f;
-      fresh = fresh && top == -INFINITY;
+      const float raise = top > (fresh >> lane & 1u ? -INFINITY : 0.f) ? top : 0.f;
+      fresh &= __ballot(top == -INFINITY);
       reference += raise;
       // (the first raise may be below zero, by any amount: its sums are 0 and must stay so)
       const float shrink = exp2_fast(fminf(-raise, 0.f));
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
       __builtin_amdgcn_sched_barrier(0);
     }
     y.most = most;
-    settle(y, t + 1u);
+    settle(y, t + 1u, false);
   };
 
   if (begin < end) {
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
         scale_score(x, 0, e);
         x.most = fmaxf(x.most, x.s[e / 16][e % 16]);
       }
-      settle(x, 0);
+      settle(x, 0, true);
     }
     __syncthreads();  // every wave has read the first tile's keys
     auto turn = [&](uint32_t t, Scores& now, Scores& next) {
