@@ -135,6 +135,10 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
     rows = a.group;
     sequence = sequence_of(a, token0);
     length = keys_of(a, sequence);
+    if (a.starts) {
+      const Span span = tokens_of(a, sequence);
+      if (token0 - span.first >= span.count) length = 0;  // no sequence's
+    }
     const uint32_t visible = length ? a.k : 0u;
     const uint32_t chunk = max(kLeastSteps * kStep, ((a.k + a.splits - 1u) / a.splits + 31u) & ~31u);
     begin = min(piece * chunk, visible);
@@ -145,7 +149,9 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
     slot = item * a.splits;
   } else {
     Piece piece;
-    if (!find_piece<16, kStep, kLeastSteps>(a, id, piece)) return;
+    const bool found = find_piece<16, kStep, kLeastSteps>(a, id, piece);
+    clear_unowned<D, kThreads>(a);
+    if (!found) return;
     sequence = piece.sequence;
     token0 = piece.span.first;
     row0 = piece.tile * 16u;
@@ -870,6 +876,7 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
     a.part_rows = p.stream_rows;
     a.least_rows = 1;
     a.most_rows = p.stream_most;
+    a.clears = starts != nullptr;
     const auto launch_stream = p.stream_beside ? launch<kBeside> : launch<kDense>;
     if (int st = launch_stream(a, cache, dtype, (p.stream_pieces + kXcds - 1) / kXcds * kXcds, s)) return st;
   }
@@ -879,6 +886,7 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
     a.part_rows = (uint32_t)p.chunk_rows;
     a.least_rows = kStreamRows + 1;
     a.most_rows = 0xffffffffu;
+    a.clears = starts && !p.stream_pieces;
     const int64_t grid = p.chunk_pieces * a.cache.kv_heads;
     DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
     const auto launch_rows = p.prefill ? launch_paged_prefill : launch_paged_chunk;

@@ -42,6 +42,7 @@ struct PagedAttentionArgs {
   uint32_t most_rows;       // sequences of more (token, head) rows per kv head are another kernel's
   uint32_t least_rows;
   uint32_t whole;           // row tiles of a single sequence that are not cut (see find_piece)
+  uint32_t clears;          // this launch answers the tokens that no sequence has (see clear_unowned)
   float scale;              // times log2 e
   char* out;                // [tokens][heads][dim]
   float* lse;               // nullable: [tokens][heads]
@@ -281,6 +282,27 @@ __device__ __forceinline__ void store_out(const PagedAttentionArgs& a, uint64_t 
   *reinterpret_cast<uint2*>(a.out + (row * D + dim) * 2) =
       make_uint2(pack2(Tag{}, o[0] * inv, o[1] * inv), pack2(Tag{}, o[2] * inv, o[3] * inv));
   if (a.lse && dim == 0) a.lse[row] = total == 0.f ? -INFINITY : (reference + log2f(total)) * kLn2;
+}
+
+// Results of the tokens before the first sequence's and past the last one's, which a
+// batch padded to a fixed number of tokens has: as rows without keys, 0 and -inf.
+// Dealt to the launch's threads, 16 bytes at a time.
+template <int D, uint32_t kThreads>
+__device__ __forceinline__ void clear_unowned(const PagedAttentionArgs& a) {
+  if (!a.clears) return;
+  const uint32_t first = tokens_of(a, 0).first;
+  const Span last = tokens_of(a, a.sequences - 1u);
+  const uint32_t end = max(first, last.first + last.count);
+  if (first == 0 && end == a.tokens) return;
+  const uint64_t count = ((uint64_t)first + a.tokens - end) * a.heads;  // rows
+  const uint64_t from = (uint64_t)first * a.heads;                      // those past it lie behind the sequences'
+  const uint64_t skip = (uint64_t)(end - first) * a.heads;
+  for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < count * (D / 8); i += (uint64_t)gridDim.x * kThreads) {
+    uint64_t row = i / (D / 8);
+    row += row < from ? 0u : skip;
+    *reinterpret_cast<uint4*>(a.out + (row * D + i % (D / 8) * 8u) * 2u) = make_uint4(0u, 0u, 0u, 0u);
+    if (a.lse && i % (D / 8) == 0) a.lse[row] = -INFINITY;
+  }
 }
 
 // The chunk kernels' products and tiles.

@@ -62,6 +62,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
   // Heads vary fastest: workgroups go round-robin over the XCDs, so that a kv
   // head's keys meet all of its rows in few L2s.
   const uint32_t g = blockIdx.x % a.cache.kv_heads;
+  clear_unowned<D, kThreads>(a);
   Piece piece;
   if (!find_piece<kRows, kTileKeys, kLeastTiles>(a, blockIdx.x / a.cache.kv_heads, piece)) return;
   const Span span = piece.span;

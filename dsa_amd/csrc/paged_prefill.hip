@@ -51,6 +51,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   // Heads vary fastest: workgroups go round-robin over the XCDs, so that a kv
   // head's keys meet all of its rows in few L2s.
   const uint32_t g = blockIdx.x % a.cache.kv_heads;
+  clear_unowned<D, kThreads>(a);
   Piece piece;
   if (!find_piece<kRows, kTileKeys, kLeastTiles>(a, blockIdx.x / a.cache.kv_heads, piece)) return;
   const Span span = piece.span;

@@ -284,8 +284,9 @@ def attention(
     queries ``[T, heads, head_dim]`` of the cache's dtype (bf16 for fp8), already
     rotated; ``page_table`` ``[B, columns]`` int32 page ids; ``lengths`` ``[B]``
     int32 keys of each sequence, the new tokens' own included.  Sequence b's
-    tokens are ``starts[b] .. starts[b + 1]`` (``[B + 1]`` int32); without
-    ``starts`` every sequence has T / B.  ``causal``: the i-th of n new tokens
+    tokens are ``starts[b] .. starts[b + 1]`` (``[B + 1]`` int32, ascending, within
+    0 .. T; tokens outside ``starts[0] .. starts[B]`` are padding, which sees no key);
+    without ``starts`` every sequence has T / B.  ``causal``: the i-th of n new tokens
     sees keys ``j <= lengths[b] - n + i``.  ``scale`` defaults to head_dim^-0.5.
 
     Returns ``[T, heads, head_dim]`` in the queries' dtype, and with

@@ -881,11 +881,12 @@ int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, int64_t key
  *   out[t][h] = sum_j softmax_j(scale q[t][h] . k[j][h / group]) v[j][h / group]
  * queries and out [tokens][heads][head_dim] (queries' token stride in elements,
  * out dense), heads a multiple of kv_heads, group = heads / kv_heads.  Sequence
- * s has tokens starts[s] .. starts[s + 1] (starts[0] = 0, ascending,
- * starts[sequences] = tokens; NULL: tokens / sequences each) and lengths[s]
- * keys, its new tokens' included, at most columns * page_size (itself at most 2^30).  With causal, the
- * i-th of n new tokens sees keys j <= lengths[s] - n + i, else every key of the
- * sequence.  A row that sees no key gets zeros and lse -inf.  lse (nullable,
+ * s has tokens starts[s] .. starts[s + 1] (ascending, 0 .. tokens; NULL: tokens /
+ * sequences each) and lengths[s] keys, its new tokens' included, at most columns *
+ * page_size (itself at most 2^30).  Tokens below starts[0] or from starts[sequences]
+ * on, as in a batch padded to a fixed number of tokens, belong to no sequence and see
+ * no key.  With causal, the i-th of n new tokens sees keys j <= lengths[s] - n + i,
+ * else every key of the sequence.  A row that sees no key gets zeros and lse -inf.  lse (nullable,
  * [tokens][heads] fp32) is the natural log of the softmax's denominator.  What a
  * row does not see does not reach it, infinities and NaN of later tokens, of rows
  * past a sequence's length and of other sequences included.  Page ids outside the

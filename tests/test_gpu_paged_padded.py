@@ -1,11 +1,13 @@
 """Paged attention of batches padded to a fixed number of tokens: the last tokens, or
 the first ones, belong to no sequence.  The sequences' own rows are those of the batch
-without padding, in every kernel."""
+without padding, in every kernel; the others are 0 and their log sums -inf."""
 
 from __future__ import annotations
 
 import functools
+import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -45,10 +47,18 @@ def _other_call(device):
     return c.q.to(device), c.cache, *c.device_args()
 
 
-def _soil_workspace(device) -> None:
-    """Leaves numbers of another call's pieces all over the workspace."""
+def _soil_memory(device, like) -> None:
+    """Leaves numbers of another call's pieces all over the workspace, and NaN where
+    the allocator will place the results."""
 
     paged.attention(*_other_call(device))
+    held = [torch.full_like(like, math.nan), torch.full(like.shape[:2], math.nan, device=device)]
+    del held
+
+
+def _check_padding(out, lse, own) -> None:
+    for outside in (slice(0, own.start), slice(own.stop, None)):
+        assert (out[outside] == 0).all() and (lse[outside] == -math.inf).all()
 
 
 @pytest.mark.parametrize("lengths,chunks,before,after,heads,kv_heads,dim,dtype", PADDED)
@@ -58,6 +68,32 @@ def test_attention_of_padded_batches(device, lengths, chunks, before, after, hea
     q, starts = _padded(c, before, after, device)
     own = slice(before, before + len(c.q))
     for causal in (True, False):
-        _soil_workspace(device)
+        _soil_memory(device, q)
         out, lse = paged.attention(q, c.cache, *c.device_args()[:2], starts, causal=causal, return_lse=True)
         c.check(out[own], lse[own], dim**-0.5, causal=causal)
+        _check_padding(out, lse, own)
+
+
+@pytest.mark.parametrize("lengths,chunks,before,after,heads,kv_heads,dim,dtype,k", [
+    ([300, 40], [1, 1], 0, 6, 8, 2, 128, BF16, 30),
+    ([3000, 700], [2, 1], 2, 5, 8, 2, 128, FP8, 1500),           # lists in pieces
+    ([150, 90], [700, 310], 10, 200, 4, 3, 64, BF16, 45),        # a list to a wave
+])
+def test_selected_attention_of_padded_batches(device, lengths, chunks, before, after, heads, kv_heads, dim, dtype, k) -> None:
+    """A list of a token that no sequence has names nothing."""
+
+    print(f"padded lists: {lengths} {before}+{chunks}+{after} {heads}/{kv_heads}x{dim} {dtype} {k}", flush=True)
+    heads = heads if heads % kv_heads == 0 else kv_heads
+    c = Case(device, 92, lengths, chunks, heads, kv_heads, dim, 16, dtype)
+    q, starts = _padded(c, before, after, device)
+    own = slice(before, before + len(c.q))
+    lists = np.random.default_rng(k).integers(-20, max(lengths) + 20, (len(q), k))
+    for b, n in enumerate(lengths):  # no position twice
+        for t in range(c.starts[b], c.starts[b + 1]):
+            row = lists[before + t]
+            row[np.setdiff1d(np.arange(k), np.unique(row, return_index=True)[1])] = -1
+    _soil_memory(device, q)
+    out, lse = paged.selected_attention(q, c.cache, *c.device_args()[:2], torch.from_numpy(lists).to(device), starts,
+                                        return_lse=True)
+    c.check(out[own], lse[own], dim**-0.5, lists=lists[own])
+    _check_padding(out, lse, own)
