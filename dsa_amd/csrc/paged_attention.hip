@@ -884,7 +884,7 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
     a.cuts = p.chunk_cuts;
     a.whole = p.chunk_whole;
     a.part_rows = (uint32_t)p.chunk_rows;
-    a.least_rows = kStreamRows + 1;
+    a.least_rows = p.stream_pieces ? kStreamRows + 1 : 1;  // fewer: the stream kernel's, if it ran
     a.most_rows = 0xffffffffu;
     a.clears = starts && !p.stream_pieces;
     const int64_t grid = p.chunk_pieces * a.cache.kv_heads;

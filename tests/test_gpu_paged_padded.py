@@ -30,6 +30,13 @@ PADDED = [
     ([1900], [33], 0, 31, 8, 2, 128, F16),
     ([650], [600], 0, 20, 128, 64, 128, BF16),                   # more row tiles than run at a time
     ([650], [300], 0, 320, 128, 64, 128, BF16),
+    ([300], [1], 0, 63, 8, 1, 128, BF16),                        # one sequence, most of the batch padding
+    ([300], [2], 3, 15, 8, 2, 64, F16),
+    ([1300], [1], 0, 40, 8, 2, 128, FP8),
+    ([700], [3], 10, 10, 4, 1, 256, BF16),
+    ([300], [1], 0, 599, 128, 64, 128, BF16),
+    ([300], [0], 0, 64, 8, 1, 128, BF16),                        # nothing but padding
+    ([300, 5], [0, 0], 0, 64, 8, 1, 128, BF16),
 ]
 
 
