@@ -107,7 +107,9 @@ struct Piece {
 // tile's last piece).  At most cuts + tiles pieces, and at most 2 cuts of tiles
 // that have several.  With `whole`, a multiple of cuts, there is one sequence: its
 // first `whole` tiles fill the GPU some times over, and only the others are cut, into
-// at most cuts pieces together.
+// at most cuts pieces together.  `starts` that fall would name tokens twice and make
+// more pieces than the launch has: there are none then, so that no tile is left with
+// some of its pieces done and its counter raised.
 template <uint32_t kTileRows, uint32_t kUnit, uint32_t kLeast>
 __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, uint32_t id, Piece& p) {
   const uint32_t lane = lane_id();
@@ -150,14 +152,17 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, uint32_t
   if (a.cuts) {
     uint64_t all = 0;
     uint32_t most = 0;
+    bool falls = false;
     for (uint32_t b = 0; b < a.sequences; b += kWave) {
       look(b);
+      falls |= a.starts && b + lane < a.sequences && a.starts[b + lane + 1u] < a.starts[b + lane];
       // (two scans: a sequence's tiles x units may pass 32 bits)
       const uint64_t work = (uint64_t)tiles * units;
       all += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan((uint32_t)(work & 0xffffffu)), kWave - 1);
       all += (uint64_t)(uint32_t)__builtin_amdgcn_readlane(wave_incl_scan((uint32_t)(work >> 24)), kWave - 1) << 24;
       most = max(most, wave_max_u32(units));
     }
+    if (__any(falls)) return false;
     p.units = max(max(kLeast, (most + kMostSplits - 1u) / kMostSplits), (uint32_t)((all + a.cuts - 1u) / a.cuts));
     if (a.sequences <= kWave) {
       for (uint32_t i = 0; i < 8; ++i) {

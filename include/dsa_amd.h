@@ -885,7 +885,7 @@ int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, int64_t key
  * sequences each) and lengths[s] keys, its new tokens' included, at most columns *
  * page_size (itself at most 2^30).  Tokens below starts[0] or from starts[sequences]
  * on, as in a batch padded to a fixed number of tokens, belong to no sequence and see
- * no key.  With causal, the i-th of n new tokens sees keys j <= lengths[s] - n + i,
+ * no key; `starts` that fall leave the results unspecified.  With causal, the i-th of n new tokens sees keys j <= lengths[s] - n + i,
  * else every key of the sequence.  A row that sees no key gets zeros and lse -inf.  lse (nullable,
  * [tokens][heads] fp32) is the natural log of the softmax's denominator.  What a
  * row does not see does not reach it, infinities and NaN of later tokens, of rows

@@ -104,3 +104,26 @@ def test_selected_attention_of_padded_batches(device, lengths, chunks, before, a
                                         return_lse=True)
     c.check(out[own], lse[own], dim**-0.5, lists=lists[own])
     _check_padding(out, lse, own)
+
+
+@pytest.mark.parametrize("lengths,chunk,heads,kv_heads,dim,dtype", [
+    ([900, 300] * 20, 1, 8, 2, 128, BF16),      # a decode step
+    ([900, 300] * 40, 1, 8, 2, 64, F16),        # of more sequences than lanes
+    ([700, 515], 40, 8, 2, 128, FP8),
+    ([300], 20, 8, 2, 256, BF16),
+])
+def test_starts_that_fall_leave_no_trace(device, lengths, chunk, heads, kv_heads, dim, dtype) -> None:
+    """Starts that name tokens again and again have unspecified results, but the next
+    call's are what they were."""
+
+    print(f"falling starts: {len(lengths)} x {chunk} {heads}/{kv_heads}x{dim} {dtype}", flush=True)
+    c = Case(device, 94, lengths, [chunk] * len(lengths), heads, kv_heads, dim, 16, dtype)
+    q = c.q.to(device)
+    table, keys, starts = c.device_args()
+    want = paged.attention(q, c.cache, table, keys, starts)
+    falling = torch.zeros_like(starts)
+    falling[1::2] = len(q)                      # 0, T, 0, T, ...
+    for bad in (falling, starts.flip(0), starts - 1000, starts + 1000, starts * 1000):
+        paged.attention(q, c.cache, table, keys, bad)
+        paged.selected_attention(q, c.cache, table, keys, torch.zeros(len(q), 3, dtype=torch.int64, device=device), bad)
+        assert torch.equal(paged.attention(q, c.cache, table, keys, starts), want)
