@@ -264,6 +264,7 @@ def _release() -> None:
     finally:
         with _workspace_lock:
             _workspace_cache.clear()
+            _outgrown.clear()
 
 
 def call(name: str, *args) -> None:
@@ -302,6 +303,7 @@ def stream_of(tensor: torch.Tensor) -> int:
 
 
 _workspace_cache: dict[tuple, torch.Tensor] = {}
+_outgrown: list[torch.Tensor] = []
 _workspace_lock = threading.Lock()
 
 
@@ -313,7 +315,11 @@ def workspace(kind: str, device: torch.device, stream: int, need: int, *, zeroed
     The entry points accept any workspace at least as large as they ask for,
     so one buffer serves every length.  It grows geometrically (at least
     doubling), so a decode loop whose context grows by one key per step
-    reallocates O(log L) times instead of keeping a buffer per length.
+    reallocates O(log L) times instead of keeping a buffer per length.  A
+    buffer that was outgrown is kept until the interpreter exits, since a
+    captured graph may hold its address: replayed after it was freed, the
+    graph would write into whatever the allocator had placed there.  Those of
+    a key are smaller together than its present one.
     ``zeroed`` buffers are zero-filled when allocated; the entry points that
     need zeros there (a per-row region at the start of the buffer) leave them
     zeroed after every call.  That region grows with the row count, over
@@ -326,6 +332,8 @@ def workspace(kind: str, device: torch.device, stream: int, need: int, *, zeroed
         ws = _workspace_cache.get(key)
         if ws is None or ws.numel() < need:
             size = max(int(need), 256, 2 * ws.numel() if ws is not None else 0)
+            if ws is not None:
+                _outgrown.append(ws)
             ws = (torch.zeros if zeroed else torch.empty)(size, device=device, dtype=torch.uint8)
             _workspace_cache[key] = ws
         return ws
