@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libdsa_amd.so"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -130,6 +130,7 @@ _SIGNATURES: dict[str, list] = {
     "dsa_sketch_scores": [_p, _p, _i64, _i32, _p, _i32, ctypes.c_float, _i32, _i64, _p, _p],
 }
 _RESTYPES: dict[str, object] = {
+    "dsa_stream_capture": (_i64, [_p]),
     "dsa_topk_long_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "dsa_score_topk_workspace_bytes": (_i64, [_i64, _i64]),
     "dsa_temporal_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
@@ -265,6 +266,7 @@ def _release() -> None:
         with _workspace_lock:
             _workspace_cache.clear()
             _outgrown.clear()
+            _captured.clear()
 
 
 def call(name: str, *args) -> None:
@@ -304,6 +306,8 @@ def stream_of(tensor: torch.Tensor) -> int:
 
 _workspace_cache: dict[tuple, torch.Tensor] = {}
 _outgrown: list[torch.Tensor] = []
+# (device index, stream): the id of the last capture there that needed buffers, and those
+_captured: dict[tuple, tuple[int, dict[tuple, torch.Tensor]]] = {}
 _workspace_lock = threading.Lock()
 
 
@@ -320,6 +324,11 @@ def workspace(kind: str, device: torch.device, stream: int, need: int, *, zeroed
     captured graph may hold its address: replayed after it was freed, the
     graph would write into whatever the allocator had placed there.  Those of
     a key are smaller together than its present one.
+
+    A call that is being captured takes the stream's buffer if that is large
+    enough.  Else it gets one of its capture's own, from the graph's memory, in
+    which the zero fill is recorded and so runs with every replay: no other
+    capture and no eager call may use it, since the fill has not run when they do.
     ``zeroed`` buffers are zero-filled when allocated; the entry points that
     need zeros there (a per-row region at the start of the buffer) leave them
     zeroed after every call.  That region grows with the row count, over
@@ -331,12 +340,29 @@ def workspace(kind: str, device: torch.device, stream: int, need: int, *, zeroed
     with _workspace_lock:
         ws = _workspace_cache.get(key)
         if ws is None or ws.numel() < need:
+            capture = capture_of(stream)
+            if capture:
+                ident, held = _captured.get((device.index, stream), (0, {}))
+                if ident != capture:
+                    held = {}
+                    _captured[device.index, stream] = (capture, held)
+                ws = held.get(key)
+                if ws is None or ws.numel() < need:
+                    ws = held[key] = (torch.zeros if zeroed else torch.empty)(max(int(need), 256), device=device,
+                                                                              dtype=torch.uint8)
+                return ws
             size = max(int(need), 256, 2 * ws.numel() if ws is not None else 0)
             if ws is not None:
                 _outgrown.append(ws)
             ws = (torch.zeros if zeroed else torch.empty)(size, device=device, dtype=torch.uint8)
             _workspace_cache[key] = ws
         return ws
+
+
+def capture_of(stream: int) -> int:
+    """The id of the graph capture that ``stream`` takes part in, 0 outside one."""
+
+    return query("dsa_stream_capture", stream)
 
 
 def workspace_count() -> int:

@@ -98,3 +98,11 @@ uint32_t env_limit(const char* name, uint32_t fallback, uint32_t limit) {
 extern "C" const char* dsa_last_error(void) { return dsa::g_message; }
 
 extern "C" int dsa_abi_version(void) { return DSA_ABI_VERSION; }
+
+extern "C" int64_t dsa_stream_capture(void* stream) {
+  if (!stream) return 0;  // the default stream cannot be captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) return 0;
+  return status == hipStreamCaptureStatusActive ? (int64_t)id : 0;
+}

@@ -18,6 +18,10 @@ attention.  Here the cache and that attention are operators of the library:
 
 Query heads share kv heads in equal groups: head h reads kv head
 h * kv_heads // heads.  Inference only: no autograd graph is kept.
+
+Every call may be captured in a HIP graph.  Attention calls on one stream share its
+workspace (:func:`dsa_amd._lib.workspace`), and so do graphs that were captured on
+it: replay them one after the other, not side by side on several streams.
 """
 
 from __future__ import annotations

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define DSA_ABI_VERSION 6
+#define DSA_ABI_VERSION 7
 
 #define DSA_STATUS_OK 0
 #define DSA_STATUS_INVALID_ARGUMENT 1
@@ -45,6 +45,11 @@ const char* dsa_last_error(void);
 
 /* DSA_ABI_VERSION of the loaded library. */
 int dsa_abi_version(void);
+
+/* The id of the graph capture that a stream takes part in, 0 outside one.  A
+ * workspace that has to start at zero and is allocated while its stream captures
+ * has its fill recorded, not run: it is that capture's alone. */
+int64_t dsa_stream_capture(void* stream);
 
 /* ------------------------------------------------------------------------
  * Dense indexer scores for a batch of independent decode sequences.

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from dsa_amd import paged
+from dsa_amd import _lib, paged
 from test_gpu_paged import BF16, FP8, Case
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,52 @@ def test_a_larger_call_after_the_capture(device, dtype) -> None:
             assert torch.equal(prompt(), large)
         stream.synchronize()
         assert all(bool((x == 77).all()) for x in junk)
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (2, 1, 0), (1, 2, 0)])
+def test_captures_without_a_call_before_on_their_stream(device, order) -> None:
+    """Three graphs of growing workspaces, captured on a stream that no call has run
+    on, replayed in any order, with eager calls on that stream before the first."""
+
+    calls = [_decode(device, 3), _decode(device, 4, FP8), _prompt(device, 5, 300)]
+    want = [call() for call in calls]                     # on another stream
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    graphs, got = [], []
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            got.append(call())
+    torch.cuda.synchronize()
+
+    def same(i, out):
+        return torch.equal(out, want[i]) if torch.is_tensor(out) else _same(out, want[i])
+
+    with torch.cuda.stream(stream):
+        assert same(0, calls[0]())
+    for turn in range(3):
+        for i in order:
+            for x in (got[i],) if torch.is_tensor(got[i]) else got[i]:
+                x.zero_()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert same(i, got[i]), (turn, i)
+        with torch.cuda.stream(stream):
+            assert same(2, calls[2]()) and same(1, calls[1]())
+        torch.cuda.synchronize()
+
+
+def test_captures_have_ids_of_their_own(device) -> None:
+    stream = torch.cuda.Stream()
+    x = torch.zeros(4, device=device)
+    ids = []
+    for _ in range(3):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            x += 1
+            ids.append(_lib.capture_of(stream.cuda_stream))
+        assert _lib.capture_of(stream.cuda_stream) == 0
+        graph.replay()
+    torch.cuda.synchronize()
+    assert len(set(ids)) == 3 and 0 not in ids
+    assert x.tolist() == [3.0] * 4
