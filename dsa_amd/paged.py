@@ -118,18 +118,29 @@ def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, dtype
 def cache_rows(cache: PagedCache, page_table: torch.Tensor, positions: torch.Tensor,
                sequences: torch.Tensor | None = None) -> torch.Tensor:
     """int64 cache rows of ``positions`` ``[T]``; token t belongs to sequence
-    ``sequences[t]`` (default: token t to sequence t)."""
+    ``sequences[t]`` (default: token t to sequence t).  Padding, which is any token
+    whose position or sequence is not in the page table (-1), has row -1."""
 
     if page_table.ndim != 2 or positions.ndim != 1:
         raise ValueError("page_table must be [sequences,columns] and positions [tokens]")
-    if sequences is None:
-        if positions.shape[0] != page_table.shape[0]:
-            raise ValueError("without sequences there is one token per sequence")
-        sequences = torch.arange(positions.shape[0], device=positions.device)
     size = cache.page_size
+    count, columns = page_table.shape
     positions = positions.long()
-    page = page_table[sequences.long(), torch.div(positions, size, rounding_mode="floor")]
-    return page.long() * size + positions % size
+    if page_table.numel() == 0:
+        return torch.full_like(positions, -1)
+    inside = positions.clamp(0, columns * size - 1)
+    column = inside >> (size.bit_length() - 1)
+    padding = inside != positions
+    if sequences is None:
+        if positions.shape[0] != count:
+            raise ValueError("without sequences there is one token per sequence")
+        page = page_table.gather(1, column.unsqueeze(1)).squeeze(1)
+    else:
+        sequences = sequences.to(positions.device, torch.int64)
+        at = sequences.clamp(0, count - 1)
+        padding = padding.logical_or_(at != sequences)
+        page = page_table.take(torch.add(column, at, alpha=columns))
+    return torch.add(inside & (size - 1), page, alpha=size).masked_fill_(padding, -1)
 
 
 # A short call is bound by the host, so its checks are the cheap ones where they
