@@ -133,17 +133,17 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
     }
   };
   auto stage_values = [&](uint32_t t) {
+    if (kPart && load_row >= kTileKeys) return;  // these threads have loaded nothing
     const uint32_t key0 = begin + t * kTileKeys;
     if (key0 + kTileKeys > all_rows_see) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
         if (key0 + load_row + kPass * i >= all_rows_see && drop_nonfinite<Tag, kFp8>(vr[i])) dropped = 1;
-      if (kFp8 && key0 + tid >= all_rows_see && !is_finite(vs)) {
+      if (kFp8 && tid < kTileKeys && key0 + tid >= all_rows_see && !is_finite(vs)) {
         vs = 0.f;
         dropped = 1;
       }
     }
-    if (kPart && load_row >= kTileKeys) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) put(value_tile[t & 1u] + (load_row + kPass * i) * kValueRow<D>, vr[i]);
     if constexpr (kFp8) {
