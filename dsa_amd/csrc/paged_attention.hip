@@ -5,8 +5,8 @@
 // over the keys a row sees: its sequence's first ones up to its own position,
 // or the positions its index list names.  One pass over the keys with the
 // running maximum and sum of the softmax; scores, weights' sum and output stay
-// in fp32, and the weights are rounded to the queries' type for the second
-// product, whose error then is of the output's own rounding.
+// in fp32, and the weights (times an fp8 value's scale) are rounded to the queries'
+// type for the second product, whose error then is of the output's own rounding.
 //
 // A workgroup takes 16 rows, which are (token, head) pairs of one kv head,
 // against one piece of the keys; its four waves take steps of 32 keys each.  Bound
@@ -730,7 +730,9 @@ struct Plan {
 };
 
 // Whether the stream kernel takes two heads a workgroup: heads of 128 bytes that lie
-// side by side, from 128 MiB of cache on.  HBM serves 256 contiguous bytes that one
+// side by side, from 128 MiB of cache on.  The lengths are the GPU's, so the page
+// table's room stands for them: short sequences in wide tables take this form too, at
+// the cost that the figures of one sequence show.  HBM serves 256 contiguous bytes that one
 // workgroup asks for together faster than two requests of 128 at different times
 // (fp8 of 128 dims read at 4.6 TB/s, with a head's rows contiguous at 5.6); a cache
 // that the last-level cache holds is not bound by that, and eight waves a workgroup
@@ -762,7 +764,8 @@ Plan dense_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
   // sequence of several tokens in several row tiles: two launches less.  (us, with /
   // without the others' launches, 32 heads on 8 of 128 dims: 64 sequences of 4K keys,
   // bf16 192 / 186, fp8 126 / 119; 16 of 2K 34 / 27, 26 / 21; but 16 tokens of one
-  // sequence of 32K and none of 15 others 43 / 68, 43 / 38.)
+  // sequence of 32K and none of 15 others 43 / 68, 43 / 38: that sequence's keys are
+  // read once for each 16 rows, and more tokens of it cost more.)
   const bool few = !uniform && tokens <= sequences;
   if (!uniform || each <= kStreamRows) {
     p.stream_beside = heads_lie_beside(cache, sequences, capacity);

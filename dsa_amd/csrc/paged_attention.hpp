@@ -17,7 +17,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 // and share no maximum between lanes.  The stored reference is the maximum at
 // the last raise less kLift: weights are 2^(score - reference), about 2^kLift
 // at that maximum and at most 2^(kLift + kSlack) = 2^14, inside fp16; the lift
-// keeps fp16's small weights above its subnormal range.
+// keeps fp16's small weights above its subnormal range.  They are divided out at the
+// end, so a row's sum overflows where its values reach 2^114 over the number of keys
+// that weigh alike, which only bf16 values can.
 constexpr float kLift = 6.f;
 constexpr float kSlack = 8.f;
 constexpr float kNoKeys = -FLT_MAX;  // reference of a row that has seen no key
@@ -102,8 +104,9 @@ struct Piece {
 // is longer than one length for the whole batch, whatever the sequences' lengths,
 // so every wave sums the batch's work first: one load and a scan for up to 64
 // sequences.  `cuts` pieces fill the GPU once, and a few more would run alone
-// after them; so for up to 64 sequences that length grows until the pieces fit.  A
-// tile is cut evenly (ragged fp16 chunks, us: 111, and 129 with the remainder in a
+// after them; so for up to 64 sequences that length grows, by up to 28 %, while the
+// pieces do not fit (many sequences of unlike lengths still may not).  A tile is cut
+// evenly (ragged fp16 chunks, us: 111, and 129 with the remainder in a
 // tile's last piece).  At most cuts + tiles pieces, and at most 2 cuts of tiles
 // that have several.  With `whole`, a multiple of cuts, there is one sequence: its
 // first `whole` tiles fill the GPU some times over, and only the others are cut, into

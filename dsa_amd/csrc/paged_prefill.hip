@@ -9,7 +9,7 @@
 // so that between two matrix instructions stand others that wait for neither.  Keys
 // are in LDS a tile ahead of the values.
 //
-// Bound by power: 2048 tokens over 32K keys (1.06 TFLOP) take 950 us, 1.12 PFLOP/s,
+// Bound by power: 2048 tokens over 32K keys (1.06 TFLOP) take 965 us, 1.1 PFLOP/s,
 // the matrix pipes busy 54 % of the time at the 1.88 GHz that the card then holds
 // (2.1 GHz in the chunk kernel, 1120 us); a plain 8192^3 product of the library makes
 // 1.44 PFLOP/s.  Operands read further ahead, half of the waves half a tile behind

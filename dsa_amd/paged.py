@@ -217,8 +217,11 @@ def append(
     non-interleaved RoPE of their first ``rope_dim`` dims (default: all; 0: none).
 
     With ``queries`` ``[T, heads, head_dim]`` the rotated queries are returned.
-    Tokens whose row is outside the cache (-1: padding) are not written.  An fp8
-    cache scales each head by its largest magnitude.
+    Tokens whose row is outside the cache (-1: padding) are not written; no two
+    tokens may have the same row.  An fp8 cache scales each head by its largest
+    magnitude.  The angles are exact to fp32 at any position; taken as an fp32
+    product, as the sidecar's encoders and many models take theirs, they are 0.0006
+    rad off at position 65535, so keys and queries are best rotated by one of the two.
     """
 
     dim, kv_heads = cache.head_dim, cache.kv_heads

@@ -871,8 +871,8 @@ typedef struct dsa_paged_cache {
  * position * theta^(-2 i / rope_dim), evaluated to fp32 accuracy at any
  * position; sidecar.py:10-28 takes the angle's product in fp32).  Products and
  * sums are fp32, rounded once to the cache's type.  Tokens whose row is outside
- * the cache are not written; two tokens with one row leave either's values.
- * fp8: scale = max(max|x| / 448, 2^-126) over a head, code = round-to-nearest
+ * the cache are not written; two tokens with one row leave either's values (on an
+ * fp8 cache any mixture of their codes and scales).  fp8: scale = max(max|x| / 448, 2^-126) over a head, code = round-to-nearest
  * (x / scale); rows must be finite.  queries (nullable, [tokens][heads]
  * [head_dim]) are turned by the same angles into out_queries (dense, may not
  * overlap).  dtype is that of keys, values and queries: the cache's, or bf16 for
