@@ -15,19 +15,21 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libdsa_amd.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
 DTYPE_FP8_E4M3 = 3
 DTYPE_F64 = 4  # score rows of dsa_topk_exact only
+DTYPE_FP4_E2M1 = 5  # paged caches only
 
 _TORCH_DTYPES = {
     torch.float32: DTYPE_F32,
     torch.float16: DTYPE_F16,
     torch.bfloat16: DTYPE_BF16,
     torch.float8_e4m3fn: DTYPE_FP8_E4M3,
+    torch.float4_e2m1fn_x2: DTYPE_FP4_E2M1,
 }
 
 _p = ctypes.c_void_p
@@ -117,6 +119,7 @@ _SIGNATURES: dict[str, list] = {
     "dsa_encode_queries_gemm": [_p, _i64, _i64, _i64, _p, _i32, _p, _p, ctypes.c_float, ctypes.c_float, _p, _p, _p,
                                 _i64, _p],
     "dsa_paged_append": [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _i32, _p, _p, _i64, _i32, ctypes.c_double, _p],
+    "dsa_paged_read": [_p, _p, _i64, _p, _p, _p],
     "dsa_paged_attention": [
         _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i32, _i32, ctypes.c_float, _i32, _p, _p, _p, _i64, _p,
     ],

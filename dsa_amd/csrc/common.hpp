@@ -31,7 +31,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 
-enum KeyDtype : int { kF32 = 0, kF16 = 1, kBF16 = 2, kFP8E4M3 = 3 };
+enum KeyDtype : int { kF32 = 0, kF16 = 1, kBF16 = 2, kFP8E4M3 = 3, kFP4E2M1 = 5 };  // (4: fp64 rows of the exact top-K)
 
 // ---------------------------------------------------------------------------
 // MFMA wrappers: one 16x16x32 product, fp32 accumulation.

@@ -5,6 +5,10 @@
 // page_table[p / page_size] * page_size + p % page_size.  Heads are contiguous
 // runs of head_dim elements, 16-byte aligned; pages, slots and heads lie at any
 // strides.  e4m3 caches keep one fp32 scale per (page, slot, head), contiguous.
+// e2m1 caches hold two codes a byte, the first in the low half, and one power of
+// two (e8m0, the byte less 127; 255: the block is NaN) per kPowerDims of them in
+// contiguous [pages][kv_heads][page_size][head_dim / kPowerDims]: a page's of one
+// head lie together, as one workgroup reads them.
 #pragma once
 
 #include <float.h>
@@ -15,11 +19,19 @@
 
 namespace dsa {
 
+// How a cache holds its elements.
+enum Store { k16Bit, kE4M3, kE2M1 };
+constexpr int kPowerDims = 32;  // dims that share a power of two of an e2m1 cache
+template <Store kStore, int D>
+constexpr int kRowBytes = kStore == kE2M1 ? D / 2 : kStore == kE4M3 ? D : 2 * D;  // of a head's keys or values
+
 struct PagedView {
   char* keys;
   char* values;
   float* key_scales;
   float* value_scales;
+  uint8_t* key_powers;
+  uint8_t* value_powers;
   uint64_t key_head, value_head;  // bytes between heads
   uint32_t key_page, key_slot;    // bytes between pages and slots
   uint32_t value_page, value_slot;
@@ -33,10 +45,20 @@ struct PagedView {
   __device__ __forceinline__ uint64_t value_offset(uint32_t row) const {
     return (uint64_t)(row >> shift) * value_page + (uint64_t)(row & ((1u << shift) - 1u)) * value_slot;
   }
+  // Of a head's first power of two.
+  template <int D>
+  __device__ __forceinline__ uint64_t power_offset(uint32_t row, uint32_t head) const {
+    return ((((uint64_t)(row >> shift) * kv_heads + head) << shift) | (row & ((1u << shift) - 1u))) * (D / kPowerDims);
+  }
 };
 
 // Checks a descriptor and fills the device view of it.
 int make_paged_view(const dsa_paged_cache* cache, PagedView& view);
+
+// The type of a cache's queries, and of the rows appended to it.
+inline int32_t row_type(int32_t cache_dtype) {
+  return cache_dtype == kFP8E4M3 || cache_dtype == kFP4E2M1 ? (int32_t)kBF16 : cache_dtype;
+}
 
 // 2^x by the hardware instruction (results below the normal range become 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -56,6 +78,27 @@ __device__ __forceinline__ uint4 fp8x8_to_bf16x8_paired(uint2 v) {
     return __builtin_bit_cast(uint32_t, p);
   };
   return make_uint4(two(v.x, Low{}), two(v.x, High{}), two(v.y, Low{}), two(v.y, High{}));
+}
+
+// 8 e2m1 codes times a power of two to 8 bf16, exactly (NaN for a power of NaN).
+__device__ __forceinline__ uint4 fp4x8_to_bf16x8(uint32_t w, float power) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  const pair p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, 0);
+  const pair p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, 1);
+  const pair p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, 2);
+  const pair p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, 3);
+  return make_uint4(__builtin_bit_cast(uint32_t, p0), __builtin_bit_cast(uint32_t, p1), __builtin_bit_cast(uint32_t, p2),
+                    __builtin_bit_cast(uint32_t, p3));
+}
+__device__ __forceinline__ float power_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+// Bytes of `w` that are 255, as 0x80 in their place.
+__device__ __forceinline__ uint32_t nan_powers(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+
+// LDS that the lanes of one wave share: a wave's LDS accesses are served in
+// order, so only the compiler has to keep them so.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // Two fp32 rounded to nearest-even bf16 or fp16, packed.

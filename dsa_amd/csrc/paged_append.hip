@@ -6,28 +6,40 @@
 //   x'[i + half] = x[i + half] cos a + x[i] sin a
 // in fp32, rounded once to the cache's type; values are stored as they are.
 // An e4m3 cache takes s = max(max|x| / 448, 2^-126) of each head and stores
-// rn(x / s) and s.  The queries' heads can be turned by the same angles in the
-// same launch.  The angle's turns are taken in double and reduced there: in fp32
-// an angle near 10^5 is off by 0.01.
+// rn(x / s) and s.  An e2m1 cache takes of each 32 dims the least power of two
+// under which the largest magnitude is 7 or less (2^-124 .. 2^125) and stores
+// rn(x / power): a largest magnitude of 6 to 7 is stored as 6, off by half a step
+// at most, as all others are.  A block with an infinity or NaN is NaN.  Its keys are
+// turned in double: a value that fp32 puts on the other side of a border
+// between two codes moves by a whole step.  The queries' heads can be turned by the
+// same angles in the same launch.  The angle's turns are taken in double and reduced
+// there: in fp32 an angle near 10^5 is off by 0.01.
 #include <math.h>
+
+#include <type_traits>
 
 #include "paged.hpp"
 
 namespace dsa {
 
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 int make_paged_view(const dsa_paged_cache* c, PagedView& v) {
   DSA_REQUIRE(c && c->keys && c->values, "the paged cache has no keys or values");
-  DSA_REQUIRE(c->dtype == kBF16 || c->dtype == kF16 || c->dtype == kFP8E4M3,
-              "a paged cache is bf16, fp16 or fp8 e4m3 (got %d)", c->dtype);
-  const bool fp8 = c->dtype == kFP8E4M3;
+  DSA_REQUIRE(c->dtype == kBF16 || c->dtype == kF16 || c->dtype == kFP8E4M3 || c->dtype == kFP4E2M1,
+              "a paged cache is bf16, fp16 or fp8 e4m3, or fp4 e2m1 (got %d)", c->dtype);
+  const bool fp8 = c->dtype == kFP8E4M3, fp4 = c->dtype == kFP4E2M1;
   DSA_REQUIRE(!fp8 || (c->key_scales && c->value_scales), "an fp8 paged cache needs key and value scales");
+  DSA_REQUIRE(!fp4 || (c->key_scales && c->value_scales), "an fp4 paged cache needs key and value scales");
+  DSA_REQUIRE(!fp4 || (aligned16(c->key_scales) && aligned16(c->value_scales)),
+              "the scales of an fp4 paged cache must be 16-byte aligned");
   DSA_REQUIRE(c->page_size > 0 && (c->page_size & (c->page_size - 1)) == 0, "page_size %d must be a power of two",
               c->page_size);
   DSA_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "head_dim %d must be 64, 128 or 256",
               c->head_dim);
   DSA_REQUIRE(c->kv_heads > 0 && c->kv_heads <= 1024, "kv_heads %d out of range", c->kv_heads);
   DSA_REQUIRE(c->pages > 0 && c->pages * (int64_t)c->page_size < (1LL << 31), "pages * page_size must be in 1..2^31 - 1");
-  const int64_t e = fp8 ? 1 : 2;
+  const int64_t e = fp8 || fp4 ? 1 : 2;
   const int64_t strides[6] = {c->key_page_stride, c->key_slot_stride, c->key_head_stride,
                               c->value_page_stride, c->value_slot_stride, c->value_head_stride};
   for (int i = 0; i < 6; ++i) {
@@ -38,8 +50,10 @@ int make_paged_view(const dsa_paged_cache* c, PagedView& v) {
               "the paged cache must be 16-byte aligned");
   v.keys = static_cast<char*>(c->keys);
   v.values = static_cast<char*>(c->values);
-  v.key_scales = fp8 ? c->key_scales : nullptr;
-  v.value_scales = fp8 ? c->value_scales : nullptr;
+  v.key_scales = fp8 ? static_cast<float*>(c->key_scales) : nullptr;
+  v.value_scales = fp8 ? static_cast<float*>(c->value_scales) : nullptr;
+  v.key_powers = fp4 ? static_cast<uint8_t*>(c->key_scales) : nullptr;
+  v.value_powers = fp4 ? static_cast<uint8_t*>(c->value_scales) : nullptr;
   v.key_page = (uint32_t)(c->key_page_stride * e);
   v.key_slot = (uint32_t)(c->key_slot_stride * e);
   v.key_head = (uint64_t)(c->key_head_stride * e);
@@ -75,16 +89,34 @@ struct AppendArgs {
   double octaves;       // log2(theta) / half
 };
 
+// The powers of two that an e2m1 cache holds, as their bytes: 0.5 * 2^-124 is normal
+// in bf16 and 6 * 2^125 finite.
+constexpr int kLeastPower = 127 - 124;
+constexpr int kMostPower = 127 + 125;
+
+// The nearest fp32, of the two next to an inexact x the one with an odd last bit: a
+// later rounding to fewer bits goes as it would from x.
+__device__ __forceinline__ float rounded_to_odd(double x) {
+  const float f = (float)x;
+  const double off = x - (double)f;
+  const uint32_t bits = __float_as_uint(f);
+  if (off == 0.0 || !(off == off) || (bits & 1u)) return f;
+  return __uint_as_float((off > 0.0) == (x > 0.0) ? bits + 1u : bits - 1u);
+}
+
 // A thread serves a unit, 16 elements of one head: two 8-element runs that turn
 // into each other (i.. and i + half..), or 16 consecutive ones where nothing turns.
 // So it loads and stores 16 bytes at a time, and a head's D/16 units are
 // neighbouring lanes, which share its largest magnitude by shuffles.  A workgroup
 // takes 256 units of one token, or as many whole tokens as it has threads for.
 // HBM bound: 8192 tokens of 48 bf16 heads, 202 MB, 39 us (5.1 TB/s).
-template <class Tag, bool kFp8, int D>
+template <class Tag, Store kStore, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr uint32_t kUnits = D / 16;
-  __shared__ float2 turn[1024];  // [tokens of the workgroup][half], at most 256 / (2 kUnits) of D / 2
+  using Angle = typename std::conditional<kStore == kE2M1, double2, float2>::type;
+  __shared__ Angle turn[1024];  // [tokens of the workgroup][half], at most 256 / (2 kUnits) of D / 2
+  // Magnitudes of each head's runs of 8, by their dims (e2m1).
+  __shared__ __attribute__((aligned(16))) uint32_t most_of[kStore == kE2M1 ? 512 : 1];
   const uint32_t half = a.rope_dim / 2;
   const uint32_t my = a.pack > 1u ? threadIdx.x / a.units : 0u;
   const uint32_t unit = a.pack > 1u ? threadIdx.x % a.units : blockIdx.y * 256u + threadIdx.x;
@@ -112,9 +144,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     const uint32_t at = i / half;
     const int64_t position = a.positions[min(first + at, (int64_t)a.tokens - 1)];
     const double turns = (double)position * exp2(-a.octaves * (double)(i - at * half)) * 0.15915494309189535;
-    float s, co;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &co);
-    turn[i] = make_float2(co, s);
+    if constexpr (kStore == kE2M1) {
+      double s, co;
+      sincospi(2.0 * (turns - rint(turns)), &s, &co);
+      turn[i] = make_double2(co, s);
+    } else {
+      float s, co;
+      sincospif((float)(2.0 * (turns - rint(turns))), &s, &co);
+      turn[i] = make_float2(co, s);
+    }
   }
   __syncthreads();
   if (!live) return;
@@ -132,10 +170,17 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   if (turned) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 t = turn[my * half + 8 * c + i];
-      const float first = x[i], second = x[8 + i];
-      x[i] = first * t.x - second * t.y;
-      x[8 + i] = second * t.x + first * t.y;
+      const Angle t = turn[my * half + 8 * c + i];
+      if (kStore == kE2M1 && is_key) {
+        const double first = x[i], second = x[8 + i];
+        x[i] = rounded_to_odd(first * t.x - second * t.y);
+        x[8 + i] = rounded_to_odd(second * t.x + first * t.y);
+      } else {
+        const float first = x[i], second = x[8 + i];
+        const float co = (float)t.x, s = (float)t.y;
+        x[i] = first * co - second * s;
+        x[8 + i] = second * co + first * s;
+      }
     }
   }
   const bool in_cache = row >= 0 && row < a.row_limit;
@@ -143,7 +188,38 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     const uint32_t r = in_cache ? (uint32_t)row : 0u;
     char* to = is_key ? a.cache.keys + a.cache.key_offset(r) + h * a.cache.key_head
                       : a.cache.values + a.cache.value_offset(r) + h * a.cache.value_head;
-    if constexpr (kFp8) {
+    if constexpr (kStore == kE2M1) {
+      uint32_t* mine = most_of + threadIdx.x / kUnits * (D / 8);  // this head's: its units are lanes of one wave
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[8 * p + i]) & 0x7fffffffu);
+        mine[(p ? d1 : d0) / 8u] = most;
+      }
+      wave_order();
+      uint8_t* powers = (is_key ? a.cache.key_powers : a.cache.value_powers) + a.cache.power_offset<D>(r, h);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t d = p ? d1 : d0;
+        const uint4 runs = *reinterpret_cast<const uint4*>(mine + d / 32u * 4u);
+        const uint32_t most = max(max(runs.x, runs.y), max(runs.z, runs.w));
+        // 1.75 * 2^n, which is 7 * 2^(n - 2), is the last that n - 2 holds
+        const int least = (int)((most + 0x1fffffu) >> 23) - 2;
+        const uint32_t byte = most >= 0x7f800000u ? 255u : (uint32_t)min(max(least, kLeastPower), kMostPower);
+        const float inverse = __uint_as_float((254u - min(byte, 254u)) << 23);
+        uint32_t code = 0;
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[8 * p] * inverse, x[8 * p + 1] * inverse, 1.f, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[8 * p + 2] * inverse, x[8 * p + 3] * inverse, 1.f, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[8 * p + 4] * inverse, x[8 * p + 5] * inverse, 1.f, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[8 * p + 6] * inverse, x[8 * p + 7] * inverse, 1.f, 3);
+        if (!in_cache) continue;
+        *reinterpret_cast<uint32_t*>(to + d / 2u) = code;
+        if (d % 32u == 0) powers[d / 32u] = (uint8_t)byte;
+      }
+      return;
+    }
+    if constexpr (kStore == kE4M3) {
       float most = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(x[i]));
@@ -184,17 +260,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
                                                       pack2(Tag{}, x[12], x[13]), pack2(Tag{}, x[14], x[15]));
 }
 
-template <class Tag, bool kFp8>
+template <class Tag, Store kStore>
 void launch_append(const AppendArgs& a, int32_t dim, dim3 grid, hipStream_t stream) {
   if (dim == 64)
-    hipLaunchKernelGGL((paged_append_kernel<Tag, kFp8, 64>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((paged_append_kernel<Tag, kStore, 64>), grid, dim3(256), 0, stream, a);
   else if (dim == 128)
-    hipLaunchKernelGGL((paged_append_kernel<Tag, kFp8, 128>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((paged_append_kernel<Tag, kStore, 128>), grid, dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_append_kernel<Tag, kFp8, 256>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((paged_append_kernel<Tag, kStore, 256>), grid, dim3(256), 0, stream, a);
 }
-
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 }  // namespace dsa
@@ -213,8 +287,7 @@ extern "C" int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, 
   DSA_REQUIRE(!queries == !out_queries && (!queries || (heads > 0 && heads <= 65536)),
               "queries need an output and 1..65536 heads");
   DSA_REQUIRE(dtype == kBF16 || dtype == kF16, "appended rows are bf16 or fp16 (got %d)", dtype);
-  DSA_REQUIRE(dtype == (cache->dtype == kFP8E4M3 ? kBF16 : cache->dtype),
-              "appended rows must have the cache's type (bf16 for an fp8 cache)");
+  DSA_REQUIRE(dtype == row_type(cache->dtype), "appended rows must have the cache's type (bf16 for an fp8 or fp4 cache)");
   const int32_t dim = cache->head_dim;
   DSA_REQUIRE(rope_dim >= 0 && rope_dim <= dim && rope_dim % 16 == 0, "rope_dim %d must be a multiple of 16 up to head_dim",
               rope_dim);
@@ -244,11 +317,13 @@ extern "C" int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, 
   a.tokens = tokens;
   const dim3 grid((unsigned)((tokens + a.pack - 1) / a.pack), (a.units + 255) / 256);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (cache->dtype == kFP8E4M3)
-    launch_append<Bf16Tag, true>(a, dim, grid, s);
+  if (cache->dtype == kFP4E2M1)
+    launch_append<Bf16Tag, kE2M1>(a, dim, grid, s);
+  else if (cache->dtype == kFP8E4M3)
+    launch_append<Bf16Tag, kE4M3>(a, dim, grid, s);
   else if (dtype == kBF16)
-    launch_append<Bf16Tag, false>(a, dim, grid, s);
+    launch_append<Bf16Tag, k16Bit>(a, dim, grid, s);
   else
-    launch_append<F16Tag, false>(a, dim, grid, s);
+    launch_append<F16Tag, k16Bit>(a, dim, grid, s);
   return check_launch("paged_append_kernel");
 }

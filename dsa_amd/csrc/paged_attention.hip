@@ -35,13 +35,6 @@ constexpr int kPerCu = D == 64 ? 3 : D == 128 ? 2 : 1;
 constexpr int64_t resident_workgroups(int64_t dim) { return 256 * (dim == 64 ? kPerCu<64> : dim == 128 ? kPerCu<128> : kPerCu<256>); }
 constexpr int kCounters = 4096;  // of row tiles that are cut, by kv head
 
-// LDS that the lanes of one wave share: a wave's LDS accesses are served in
-// order, so only the compiler has to keep them so.
-__device__ __forceinline__ void wave_order() {
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-}
-
 // Place of 16-byte chunk `chunk` of row `row` in a wave's key or value tile of
 // kBytes a row.  The chunks of a row are exchanged by an exclusive or with bits of
 // the row, so that the accesses served together fall on different banks: rows
@@ -50,7 +43,9 @@ __device__ __forceinline__ void wave_order() {
 template <int kBytes>
 __device__ __forceinline__ uint32_t tile_place(uint32_t row, uint32_t chunk) {
   uint32_t x;
-  if constexpr (kBytes == 64)
+  if constexpr (kBytes == 32)
+    x = (row >> 3) & 1u;
+  else if constexpr (kBytes == 64)
     x = (row >> 2) & 3u;
   else if constexpr (kBytes == 128)
     x = (((row >> 1) & 1u) << 2) | (((row >> 2) & 1u) << 1) | ((row >> 3) & 1u);
@@ -59,20 +54,29 @@ __device__ __forceinline__ uint32_t tile_place(uint32_t row, uint32_t chunk) {
   return row * kBytes + ((chunk ^ x) << 4);
 }
 
+// The powers of two of one head's row of an e2m1 cache.
+template <int D>
+struct Powers {
+  static constexpr int kWords = D == 256 ? 2 : 1;
+  typename std::conditional<D == 64, uint16_t, uint32_t>::type w[kWords];
+};
+
 // A step's rows on their way from the cache.  Neighbouring lanes load neighbouring
 // 16-byte runs of a row (kLanes of them, 128 bytes where the row has as many): one
 // load that touches a different row in every lane moves a quarter of the bytes a
 // cycle, and held a decode step of cached keys that are all in L2 to 8 TB/s.
-template <bool kFp8, int D>
+template <Store kStore, int D>
 struct Tile {
-  static constexpr int kBytes = kFp8 ? D : 2 * D;               // of a cache row
+  static constexpr int kBytes = kRowBytes<kStore, D>;           // of a cache row
   static constexpr int kLanes = kBytes < 128 ? kBytes / 16 : 8;  // that share a row
   static constexpr int kRows = 64 / kLanes;                      // of one load
   static constexpr int kPasses = kStep / kRows;
   static constexpr int kLoads = kBytes / (16 * kLanes);          // of one row
   u32x4 k[kPasses][kLoads];
   u32x4 v[kPasses][kLoads];
-  float scale;  // fp8: lane l < 32 the key scale of key l, else the value scale of key l - 32
+  // Lane l < 32 has that of key l, else of the value of key l - 32: the scale of an
+  // e4m3 cache, the powers of two of an e2m1 cache.
+  typename std::conditional<kStore == kE2M1, Powers<D>, float>::type scale;
 };
 
 // What a workgroup of the stream kernel takes.
@@ -89,14 +93,16 @@ constexpr int kHeadsOf = kWork == kBeside ? 2 : 1;
 template <int D, Work kWork>
 constexpr int kPerSimd = kWork == kBeside ? 2 : kPerCu<D>;
 
-template <class Tag, bool kFp8, int D, Work kWork>
+template <class Tag, Store kStore, int D, Work kWork>
 __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void paged_stream_kernel(PagedAttentionArgs a) {
-  using T = Tile<kFp8, D>;
+  using T = Tile<kStore, D>;
+  constexpr bool kFp8 = kStore == kE4M3;
+  constexpr bool kFp4 = kStore == kE2M1;
   constexpr bool kListed = kWork == kSelected || kWork == kSolo;
   constexpr int kHeads = kHeadsOf<kWork>;
   constexpr uint32_t kWaves = 4;  // of a head
   constexpr uint32_t kThreads = 64 * kWaves * kHeads;
-  constexpr uint32_t kAhead = kFp8 ? 2 : 1;  // steps on their way in registers
+  constexpr uint32_t kAhead = kStore == k16Bit ? 1 : 2;  // steps on their way in registers
   constexpr int kQ = D / 32;  // k-steps of the first product
   constexpr int kO = D / 16;  // dim tiles of the second
   // A wave's value tile (at the end its output) and key tile, one offset apart.
@@ -104,7 +110,9 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
   __shared__ __attribute__((aligned(16))) char tiles[kWaves * kHeads][kValues + kStep * T::kBytes];
   // A wave's cache rows of this group of steps and the next; negative: padding.
   __shared__ __attribute__((aligned(16))) int32_t table[kWaves * kHeads][2][kGroup * kStep];
-  __shared__ __attribute__((aligned(16))) float scales[kWaves * kHeads][64];
+  // Of a step's keys, then its values: e4m3's scales, or each row's e2m1 powers.
+  constexpr uint32_t kPowers = D / kPowerDims;
+  __shared__ __attribute__((aligned(16))) float scales[kWaves * kHeads][kFp4 ? 16 * kPowers : 64];
   __shared__ float2 sums[kWaves * kHeads][16];
   __shared__ uint32_t last_piece;
   const uint32_t lane = lane_id();
@@ -189,7 +197,9 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
     const char* p = a.queries + (int64_t)my_token * a.query_stride + (uint64_t)my_head * D * 2;
 #pragma unroll
     for (int j = 0; j < kQ; ++j) {
-      const uint32_t d = kFp8 ? 64u * (j / 2) + 16u * quad + 8u * (j % 2) : 32u * j + 8u * quad;
+      const uint32_t d = kFp4   ? D / 4u * quad + 8u * j
+                         : kFp8 ? 64u * (j / 2) + 16u * quad + 8u * (j % 2)
+                                : 32u * j + 8u * quad;
       q[j] = *reinterpret_cast<const uint4*>(p + d * 2);
     }
   }
@@ -266,6 +276,11 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
       const uint32_t row = (uint32_t)at[lane & 31u] & 0x7fffffffu;
       t.scale = (lane < 32u ? a.cache.key_scales : a.cache.value_scales)[(uint64_t)row * a.cache.kv_heads + g];
     }
+    if constexpr (kFp4) {
+      const uint32_t row = (uint32_t)at[lane & 31u] & 0x7fffffffu;
+      t.scale = *reinterpret_cast<const Powers<D>*>((lane < 32u ? a.cache.key_powers : a.cache.value_powers) +
+                                                    a.cache.power_offset<D>(row, g));
+    }
   };
 
   // Both tiles to LDS, rows as they are; fp8 values widened.
@@ -274,6 +289,20 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
     const int32_t* at = rows_at(step);
     const uint32_t key0 = first_key(step);
     const bool hides = !kListed && key0 + kStep > all_see;  // from some row
+    if constexpr (kFp4) {
+      Powers<D> powers = t.scale;
+#pragma unroll
+      for (int i = 0; i < Powers<D>::kWords; ++i) {
+        if (kListed && at[lane & 31u] < 0) powers.w[i] = 0;  // of padding: what NaN is there has no weight
+        if (hides && lane >= 32u && key0 + lane - 32u >= all_see) {
+          const uint32_t found = nan_powers(powers.w[i]);
+          powers.w[i] &= ~((found >> 7) * 0xffu);
+          dropped |= found != 0;
+        }
+      }
+      reinterpret_cast<Powers<D>*>(scales[wave])[lane] = powers;
+      wave_order();
+    }
 #pragma unroll
     for (int i = 0; i < T::kPasses; ++i) {
       const uint32_t r = T::kRows * i + load_row;
@@ -285,8 +314,15 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
         *reinterpret_cast<u32x4*>(my_keys + tile_place<T::kBytes>(r, c)) = t.k[i][j];
         u32x4 v = t.v[i][j];
         if (kListed && drop) v = u32x4{0u, 0u, 0u, 0u};
-        if (hides && key0 + r >= all_see) dropped |= drop_nonfinite<Tag, kFp8>(v);
-        if constexpr (kFp8) {
+        if constexpr (!kFp4) {
+          if (hides && key0 + r >= all_see) dropped |= drop_nonfinite<Tag, kStore>(v);
+        }
+        if constexpr (kFp4) {
+          const float power = power_of(reinterpret_cast<const uint8_t*>(scales[wave])[(32u + r) * kPowers + c]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 4u * c + w)) = fp4x8_to_bf16x8(v[w], power);
+        } else if constexpr (kFp8) {
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
         } else {
@@ -313,8 +349,26 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       floatx4 s = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (kFp4) {
+        // this lane's quarter of key 16 h + col
+        uint32_t codes[kQ];
+        if constexpr (D == 64) {
+          const uint2 k = *reinterpret_cast<const uint2*>(my_keys + tile_place<T::kBytes>(16u * h + col, quad >> 1) + 8u * (quad & 1u));
+          codes[0] = k.x, codes[1] = k.y;
+        } else {
 #pragma unroll
-      for (int j = 0; j < T::kBytes / 64; ++j) {
+          for (int i = 0; i < D / 128; ++i) {
+            const uint4 k = *reinterpret_cast<const uint4*>(my_keys + tile_place<T::kBytes>(16u * h + col, D / 128u * quad + i));
+            codes[4 * i] = k.x, codes[4 * i + 1] = k.y, codes[4 * i + 2] = k.z, codes[4 * i + 3] = k.w;
+          }
+        }
+        const uint8_t* powers = reinterpret_cast<const uint8_t*>(scales[wave]) + (16u * h + col) * kPowers;
+#pragma unroll
+        for (int j = 0; j < kQ; ++j)
+          s = mfma_16x16x32(Tag{}, fp4x8_to_bf16x8(codes[j], power_of(powers[(D / 4u * quad + 8u * j) / kPowerDims])), q[j], s);
+      }
+#pragma unroll
+      for (int j = 0; j < (kFp4 ? 0 : T::kBytes / 64); ++j) {
         const uint4 k = *reinterpret_cast<const uint4*>(my_keys + tile_place<T::kBytes>(16u * h + col, 4u * j + quad));
         if constexpr (kFp8) {
           s = mfma_16x16x32(Tag{}, fp8x8_to_bf16x8_paired(make_uint2(k.x, k.y)), q[2 * j], s);
@@ -425,7 +479,7 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
 #pragma unroll
         for (int i = 0; i < kO; ++i) {
           float back[4] = {0.f, 0.f, 0.f, 0.f};
-          add_nonfinite<Tag, kFp8>(a, row, g, 16u * i + 4u * quad, back);
+          add_nonfinite<Tag, kStore, D>(a, row, g, 16u * i + 4u * quad, back);
           o[i] += floatx4{back[0], back[1], back[2], back[3]};
         }
       }
@@ -595,20 +649,20 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttentionArgs a
   store_out<Tag, D>(a, row, dim, sum, top, total);
 }
 
-template <class Tag, bool kFp8, int D, Work kWork>
+template <class Tag, Store kStore, int D, Work kWork>
 void launch_stream_of(const PagedAttentionArgs& a, uint32_t grid, hipStream_t s) {
-  if constexpr (kWork != kBeside || Tile<kFp8, D>::kBytes == 128)
-    hipLaunchKernelGGL((paged_stream_kernel<Tag, kFp8, D, kWork>), dim3(grid), dim3(256 * kHeadsOf<kWork>), 0, s, a);
+  if constexpr (kWork != kBeside || (kStore != kE2M1 && kRowBytes<kStore, D> == 128))
+    hipLaunchKernelGGL((paged_stream_kernel<Tag, kStore, D, kWork>), dim3(grid), dim3(256 * kHeadsOf<kWork>), 0, s, a);
 }
 
-template <class Tag, bool kFp8, Work kWork>
+template <class Tag, Store kStore, Work kWork>
 void launch_stream(const PagedAttentionArgs& a, int32_t dim, uint32_t grid, hipStream_t s) {
   if (dim == 64)
-    launch_stream_of<Tag, kFp8, 64, kWork>(a, grid, s);
+    launch_stream_of<Tag, kStore, 64, kWork>(a, grid, s);
   else if (dim == 128)
-    launch_stream_of<Tag, kFp8, 128, kWork>(a, grid, s);
+    launch_stream_of<Tag, kStore, 128, kWork>(a, grid, s);
   else
-    launch_stream_of<Tag, kFp8, 256, kWork>(a, grid, s);
+    launch_stream_of<Tag, kStore, 256, kWork>(a, grid, s);
 }
 
 template <class Tag>
@@ -635,12 +689,14 @@ int launch(const PagedAttentionArgs& a, const dsa_paged_cache* cache, int32_t dt
   const int64_t grid = pieces * (a.cache.kv_heads / kHeadsOf<kWork>);
   DSA_REQUIRE(grid < (1LL << 31), "too many tokens for one call");
   const int32_t dim = cache->head_dim;
-  if (cache->dtype == kFP8E4M3)
-    launch_stream<Bf16Tag, true, kWork>(a, dim, (uint32_t)grid, s);
+  if (cache->dtype == kFP4E2M1)
+    launch_stream<Bf16Tag, kE2M1, kWork>(a, dim, (uint32_t)grid, s);
+  else if (cache->dtype == kFP8E4M3)
+    launch_stream<Bf16Tag, kE4M3, kWork>(a, dim, (uint32_t)grid, s);
   else if (dtype == kBF16)
-    launch_stream<Bf16Tag, false, kWork>(a, dim, (uint32_t)grid, s);
+    launch_stream<Bf16Tag, k16Bit, kWork>(a, dim, (uint32_t)grid, s);
   else
-    launch_stream<F16Tag, false, kWork>(a, dim, (uint32_t)grid, s);
+    launch_stream<F16Tag, k16Bit, kWork>(a, dim, (uint32_t)grid, s);
   return check_launch("paged_stream_kernel");
 }
 
@@ -670,8 +726,7 @@ int check_common(const dsa_paged_cache* cache, const void* queries, int64_t quer
   DSA_REQUIRE(heads > 0 && heads <= 65536 && heads % cache->kv_heads == 0, "%d heads do not share %d kv heads evenly",
               heads, cache->kv_heads);
   DSA_REQUIRE(dtype == kBF16 || dtype == kF16, "queries are bf16 or fp16 (got %d)", dtype);
-  DSA_REQUIRE(dtype == (cache->dtype == kFP8E4M3 ? kBF16 : cache->dtype),
-              "queries must have the cache's type (bf16 for an fp8 cache)");
+  DSA_REQUIRE(dtype == row_type(cache->dtype), "queries must have the cache's type (bf16 for an fp8 or fp4 cache)");
   DSA_REQUIRE(starts || tokens % sequences == 0, "without starts every sequence has as many tokens");
   DSA_REQUIRE(columns > 0 && columns < (1LL << 31) && columns * cache->page_size <= (1LL << 30) && table_stride >= columns,
               "page table of %lld columns out of range", (long long)columns);
@@ -743,7 +798,7 @@ struct Plan {
 // 25 / 35.  Heads of 64 bytes, fp8 of 64 dims, lose more by two waves a SIMD instead of
 // three: 16 of 32K 136 / 178.)
 bool heads_lie_beside(const dsa_paged_cache* cache, int64_t sequences, int64_t capacity) {
-  return cache->head_dim * (cache->dtype == kFP8E4M3 ? 1 : 2) == 128 && cache->kv_heads % 2 == 0 &&
+  return cache->dtype != kFP4E2M1 && cache->head_dim * (cache->dtype == kFP8E4M3 ? 1 : 2) == 128 && cache->kv_heads % 2 == 0 &&
          cache->key_head_stride == cache->head_dim && cache->value_head_stride == cache->head_dim &&
          sequences * capacity * cache->kv_heads >= 1LL << 19;
 }

@@ -34,22 +34,25 @@ __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
     __builtin_amdgcn_sched_group_barrier(0x402, (others), 0); \
   }
 
-template <class Tag, bool kFp8, int D>
+template <class Tag, Store kStore, int D>
 __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs a) {
+  constexpr bool kFp8 = kStore == kE4M3;
+  constexpr bool kFp4 = kStore == kE2M1;  // widened with its powers of two: the tiles are exact
   constexpr uint32_t kThreads = 256;
   constexpr uint32_t kRows = kChunkRows;
-  constexpr uint32_t kChunks = kFp8 ? D / 16 : D / 8;       // 16-byte loads per cache row
+  constexpr uint32_t kChunks = kRowBytes<kStore, D> / 16;   // 16-byte loads per cache row
   constexpr uint32_t kPass = kThreads / kChunks;            // cache rows per pass of the workgroup
-  constexpr int kLoads = kTileKeys / kPass;                 // passes per tile
+  constexpr bool kPart = kPass > kTileKeys;                 // fewer loads than threads
+  constexpr int kLoads = kPart ? 1 : kTileKeys / kPass;     // passes per tile
   constexpr int kKeyBytes = kTileKeys * kKeyRow<D>;
   constexpr int kValueBytes = kTileKeys * kValueRow<D>;
-  static_assert(kLoads >= 1 && kTileKeys % kPass == 0, "a tile is whole passes");
+  static_assert(kPart || kTileKeys % kPass == 0, "a tile is whole passes");
   __shared__ __attribute__((aligned(16))) char key_tile[2][kKeyBytes];
   __shared__ __attribute__((aligned(16))) char value_tile[2][kValueBytes];
   // Places in the cache of tiles t .. t + 2: offsets of the keys' and the values'
-  // row, and for fp8 the row itself.
+  // row, and for fp8 and fp4 the row itself.
   __shared__ ulong2 table[4][kTileKeys];
-  __shared__ uint32_t table_row[4][kFp8 ? kTileKeys : 1];
+  __shared__ uint32_t table_row[4][kFp8 || kFp4 ? kTileKeys : 1];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kTileKeys];
   // Whether a value was staged as 0 for not being finite: in the last row's padding.
   uint32_t& dropped = *reinterpret_cast<uint32_t*>(key_tile[0] + kTileKeys * kKeyRow<D> - 16u);
@@ -110,9 +113,16 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
 
   u32x4 kr[kLoads], vr[kLoads];
   float sr = 0.f;
+  uint32_t kp[kLoads] = {}, vp[kLoads] = {};  // fp4: each run's power of two
   auto load = [&](uint32_t t) {
+    if (kPart && load_row >= kTileKeys) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
+      if constexpr (kFp4) {
+        const uint64_t power = a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk;
+        kp[i] = a.cache.key_powers[power];
+        vp[i] = a.cache.value_powers[power];
+      }
       const ulong2 at = table[t & 3u][load_row + kPass * i];
       kr[i] = *reinterpret_cast<const u32x4*>(key_base + at.x);
       vr[i] = *reinterpret_cast<const u32x4*>(value_base + at.y);
@@ -125,11 +135,21 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
     }
   };
   auto stage = [&](uint32_t t) {
+    if (kPart && load_row >= kTileKeys) return;  // these threads have loaded nothing
     const uint32_t key0 = begin + t * kTileKeys;
     if (key0 + kTileKeys > all_rows_see) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        if (key0 + load_row + kPass * i >= all_rows_see && drop_nonfinite<Tag, kFp8>(vr[i])) dropped = 1;
+      for (int i = 0; i < kLoads; ++i) {
+        if (key0 + load_row + kPass * i < all_rows_see) continue;
+        if constexpr (kFp4) {
+          if (vp[i] == 255u) {
+            vp[i] = 0;
+            dropped = 1;
+          }
+        } else {
+          if (drop_nonfinite<Tag, kStore>(vr[i])) dropped = 1;
+        }
+      }
       if (kFp8 && tid >= kTileKeys && key0 + tid - kTileKeys >= all_rows_see && !is_finite(sr)) {
         sr = 0.f;
         dropped = 1;
@@ -140,7 +160,13 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const uint32_t row = load_row + kPass * i;
-      if constexpr (kFp8) {
+      if constexpr (kFp4) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + 64u * load_chunk + 16u * w) = fp4x8_to_bf16x8(kr[i][w], power_of(kp[i]));
+          *reinterpret_cast<uint4*>(values + row * kValueRow<D> + 64u * load_chunk + 16u * w) = fp4x8_to_bf16x8(vr[i][w], power_of(vp[i]));
+        }
+      } else if constexpr (kFp8) {
         *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + 32u * load_chunk) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].x, kr[i].y));
         *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + 32u * load_chunk + 16u) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].z, kr[i].w));
         *reinterpret_cast<uint4*>(values + row * kValueRow<D> + 32u * load_chunk) = fp8x8_to_bf16x8_paired(make_uint2(vr[i].x, vr[i].y));
@@ -298,7 +324,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
     auto place = [&](uint32_t t, uint32_t page) {
       const uint32_t row = (min(page, a.cache.pages - 1u) << a.cache.shift) | (key_of(t) & ((1u << a.cache.shift) - 1u));
       table[t & 3u][tid % kTileKeys] = ulong2{a.cache.key_offset(row), a.cache.value_offset(row)};
-      if constexpr (kFp8) table_row[t & 3u][tid % kTileKeys] = row;
+      if constexpr (kFp8 || kFp4) table_row[t & 3u][tid % kTileKeys] = row;
     };
     if (tid < 2u * kTileKeys) place(tid / kTileKeys, look_page(tid / kTileKeys));
     __syncthreads();
@@ -330,7 +356,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
             float back[4] = {0.f, 0.f, 0.f, 0.f};
-            add_nonfinite<Tag, kFp8>(a, row, g, 32u * i + 8u * b + 4u * half, back);
+            add_nonfinite<Tag, kStore, D>(a, row, g, 32u * i + 8u * b + 4u * half, back);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][4 * b + e] += back[e];
             __builtin_amdgcn_sched_barrier(0);  // few loads at a time: no registers for more
@@ -362,21 +388,23 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
 
 }  // namespace
 
-template <class Tag, bool kFp8>
+template <class Tag, Store kStore>
 static void launch_dim(const PagedAttentionArgs& a, int32_t dim, uint32_t grid, hipStream_t s) {
   if (dim == 64)
-    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kFp8, 64>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kStore, 64>), dim3(grid), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kFp8, 128>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<Tag, kStore, 128>), dim3(grid), dim3(256), 0, s, a);
 }
 
 int launch_paged_chunk(const PagedAttentionArgs& a, int32_t dim, int32_t cache_dtype, uint32_t grid, hipStream_t s) {
-  if (cache_dtype == kFP8E4M3)
-    launch_dim<Bf16Tag, true>(a, dim, grid, s);
+  if (cache_dtype == kFP4E2M1)
+    launch_dim<Bf16Tag, kE2M1>(a, dim, grid, s);
+  else if (cache_dtype == kFP8E4M3)
+    launch_dim<Bf16Tag, kE4M3>(a, dim, grid, s);
   else if (cache_dtype == kBF16)
-    launch_dim<Bf16Tag, false>(a, dim, grid, s);
+    launch_dim<Bf16Tag, k16Bit>(a, dim, grid, s);
   else
-    launch_dim<F16Tag, false>(a, dim, grid, s);
+    launch_dim<F16Tag, k16Bit>(a, dim, grid, s);
   return check_launch("paged_chunk_kernel");
 }
 

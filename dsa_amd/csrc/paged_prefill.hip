@@ -21,11 +21,13 @@ namespace {
 
 constexpr uint32_t kLeastTiles = kLeastChunkKeys / kTileKeys;  // of a piece
 
-template <class Tag, bool kFp8, int D, int kWaves>
+template <class Tag, Store kStore, int D, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(PagedAttentionArgs a) {
+  constexpr bool kFp8 = kStore == kE4M3;
+  constexpr bool kFp4 = kStore == kE2M1;  // widened with its powers of two: the tiles are exact
   constexpr uint32_t kThreads = 64 * kWaves;
   constexpr uint32_t kRows = 32 * kWaves;
-  constexpr uint32_t kChunks = kFp8 ? D / 16 : D / 8;  // 16-byte loads per cache row
+  constexpr uint32_t kChunks = kRowBytes<kStore, D> / 16;  // 16-byte loads per cache row
   constexpr uint32_t kPass = kThreads / kChunks;       // cache rows per pass of the workgroup
   constexpr bool kPart = kPass > kTileKeys;            // fewer loads than threads
   constexpr int kLoads = kPart ? 1 : kTileKeys / kPass;  // passes per tile
@@ -36,9 +38,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   __shared__ __attribute__((aligned(16))) char key_tile[2][kTileKeys * kKeyRow<D>];
   __shared__ __attribute__((aligned(16))) char value_tile[2][kTileKeys * kValueRow<D>];
   // Places in the cache of tiles t + 1 .. t + 3: offsets of the keys' and the
-  // values' row, and for fp8 the row itself.
+  // values' row, and for fp8 and fp4 the row itself.
   __shared__ ulong2 table[4][kTileKeys];
-  __shared__ uint32_t table_row[4][kFp8 ? kTileKeys : 1];
+  __shared__ uint32_t table_row[4][kFp8 || kFp4 ? kTileKeys : 1];
   __shared__ __attribute__((aligned(16))) float scales[2][4][kTileKeys];
   // Whether a value was staged as 0 for not being finite: in the last row's padding.
   uint32_t& dropped = *reinterpret_cast<uint32_t*>(key_tile[0] + kTileKeys * kKeyRow<D> - 16u);
@@ -98,11 +100,15 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   const char* value_base = a.cache.values + g * a.cache.value_head + 16u * load_chunk;
   u32x4 kr[kLoads], vr[kLoads];
   float ks = 0.f, vs = 0.f;
+  uint32_t kp[kLoads] = {}, vp[kLoads] = {};  // fp4: each run's power of two
   auto load_keys = [&](uint32_t t) {
     if (kPart && load_row >= kTileKeys) return;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
+    for (int i = 0; i < kLoads; ++i) {
+      if constexpr (kFp4)
+        kp[i] = a.cache.key_powers[a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk];
       kr[i] = *reinterpret_cast<const u32x4*>(key_base + table[t & 3u][load_row + kPass * i].x);
+    }
     if constexpr (kFp8) {
       if (tid < kTileKeys) ks = a.cache.key_scales[(uint64_t)table_row[t & 3u][tid] * a.cache.kv_heads + g];
     }
@@ -110,14 +116,21 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   auto load_values = [&](uint32_t t) {
     if (kPart && load_row >= kTileKeys) return;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
+    for (int i = 0; i < kLoads; ++i) {
+      if constexpr (kFp4)
+        vp[i] = a.cache.value_powers[a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk];
       vr[i] = *reinterpret_cast<const u32x4*>(value_base + table[t & 3u][load_row + kPass * i].y);
+    }
     if constexpr (kFp8) {
       if (tid < kTileKeys) vs = a.cache.value_scales[(uint64_t)table_row[t & 3u][tid] * a.cache.kv_heads + g];
     }
   };
-  auto put = [&](char* row, const u32x4& v) {
-    if constexpr (kFp8) {
+  auto put = [&](char* row, const u32x4& v, uint32_t power) {
+    if constexpr (kFp4) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        *reinterpret_cast<uint4*>(row + 64u * load_chunk + 16u * w) = fp4x8_to_bf16x8(v[w], power_of(power));
+    } else if constexpr (kFp8) {
       *reinterpret_cast<uint4*>(row + 32u * load_chunk) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
       *reinterpret_cast<uint4*>(row + 32u * load_chunk + 16u) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
     } else {
@@ -127,7 +140,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   auto stage_keys = [&](uint32_t t) {
     if (kPart && load_row >= kTileKeys) return;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) put(key_tile[t & 1u] + (load_row + kPass * i) * kKeyRow<D>, kr[i]);
+    for (int i = 0; i < kLoads; ++i) put(key_tile[t & 1u] + (load_row + kPass * i) * kKeyRow<D>, kr[i], kp[i]);
     if constexpr (kFp8) {
       if (tid < kTileKeys) scales[0][t & 3u][tid] = ks;
     }
@@ -137,15 +150,24 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
     const uint32_t key0 = begin + t * kTileKeys;
     if (key0 + kTileKeys > all_rows_see) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        if (key0 + load_row + kPass * i >= all_rows_see && drop_nonfinite<Tag, kFp8>(vr[i])) dropped = 1;
+      for (int i = 0; i < kLoads; ++i) {
+        if (key0 + load_row + kPass * i < all_rows_see) continue;
+        if constexpr (kFp4) {
+          if (vp[i] == 255u) {
+            vp[i] = 0;
+            dropped = 1;
+          }
+        } else {
+          if (drop_nonfinite<Tag, kStore>(vr[i])) dropped = 1;
+        }
+      }
       if (kFp8 && tid < kTileKeys && key0 + tid >= all_rows_see && !is_finite(vs)) {
         vs = 0.f;
         dropped = 1;
       }
     }
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) put(value_tile[t & 1u] + (load_row + kPass * i) * kValueRow<D>, vr[i]);
+    for (int i = 0; i < kLoads; ++i) put(value_tile[t & 1u] + (load_row + kPass * i) * kValueRow<D>, vr[i], vp[i]);
     if constexpr (kFp8) {
       if (tid < kTileKeys) scales[1][t & 3u][tid] = vs;
     }
@@ -156,7 +178,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   auto place = [&](uint32_t t, uint32_t page) {
     const uint32_t row = (min(page, a.cache.pages - 1u) << a.cache.shift) | (key_of(t) & ((1u << a.cache.shift) - 1u));
     table[t & 3u][tid % kTileKeys] = ulong2{a.cache.key_offset(row), a.cache.value_offset(row)};
-    if constexpr (kFp8) table_row[t & 3u][tid % kTileKeys] = row;
+    if constexpr (kFp8 || kFp4) table_row[t & 3u][tid % kTileKeys] = row;
   };
 
   // This lane's places: keys row `col`, chunk `half`; values in a transposed read
@@ -332,7 +354,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
             float back[4] = {0.f, 0.f, 0.f, 0.f};
-            add_nonfinite<Tag, kFp8>(a, row, g, 32u * i + 8u * b + 4u * half, back);
+            add_nonfinite<Tag, kStore, D>(a, row, g, 32u * i + 8u * b + 4u * half, back);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][4 * b + e] += back[e];
             __builtin_amdgcn_sched_barrier(0);  // few loads at a time: no registers for more
@@ -362,25 +384,27 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
     }
 }
 
-template <class Tag, bool kFp8>
+template <class Tag, Store kStore>
 void launch_dim(const PagedAttentionArgs& a, int32_t dim, uint32_t grid, hipStream_t s) {
   if (dim == 64)
-    hipLaunchKernelGGL((paged_prefill_kernel<Tag, kFp8, 64, 8>), dim3(grid), dim3(512), 0, s, a);
+    hipLaunchKernelGGL((paged_prefill_kernel<Tag, kStore, 64, 8>), dim3(grid), dim3(512), 0, s, a);
   else if (dim == 128)
-    hipLaunchKernelGGL((paged_prefill_kernel<Tag, kFp8, 128, 8>), dim3(grid), dim3(512), 0, s, a);
+    hipLaunchKernelGGL((paged_prefill_kernel<Tag, kStore, 128, 8>), dim3(grid), dim3(512), 0, s, a);
   else
-    hipLaunchKernelGGL((paged_prefill_kernel<Tag, kFp8, 256, 4>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_prefill_kernel<Tag, kStore, 256, 4>), dim3(grid), dim3(256), 0, s, a);
 }
 
 }  // namespace
 
 int launch_paged_prefill(const PagedAttentionArgs& a, int32_t dim, int32_t cache_dtype, uint32_t grid, hipStream_t s) {
-  if (cache_dtype == kFP8E4M3)
-    launch_dim<Bf16Tag, true>(a, dim, grid, s);
+  if (cache_dtype == kFP4E2M1)
+    launch_dim<Bf16Tag, kE2M1>(a, dim, grid, s);
+  else if (cache_dtype == kFP8E4M3)
+    launch_dim<Bf16Tag, kE4M3>(a, dim, grid, s);
   else if (cache_dtype == kBF16)
-    launch_dim<Bf16Tag, false>(a, dim, grid, s);
+    launch_dim<Bf16Tag, k16Bit>(a, dim, grid, s);
   else
-    launch_dim<F16Tag, false>(a, dim, grid, s);
+    launch_dim<F16Tag, k16Bit>(a, dim, grid, s);
   return check_launch("paged_prefill_kernel");
 }
 

@@ -4,12 +4,14 @@ The reference scores the cached keys (sidecar.py:89-107), selects each query's
 top-k (metrics.py:9-22) and hands the positions back to the model's own
 attention.  Here the cache and that attention are operators of the library:
 
-  PagedCache          the cache: pages of key and value rows, bf16, fp16 or fp8
-                      e4m3 with one fp32 scale per row and head
+  PagedCache          the cache: pages of key and value rows, bf16, fp16, fp8
+                      e4m3 with one fp32 scale per row and head, or fp4 e2m1
+                      with a power of two (e8m0) per 32 dims
   new_cache           an empty one
   cache_rows          the cache rows of positions, through a page table
   append              new tokens' keys and values, rotated to their positions,
                       into cache rows (``dsa_paged_append``)
+  read                what cache rows stand for (``dsa_paged_read``)
   attention           each sequence's newest tokens, one or a chunk, over its
                       whole cache (``dsa_paged_attention``)
   selected_attention  each token over the positions its index list names, as
@@ -34,14 +36,19 @@ import torch
 from . import _lib
 
 HEAD_DIMS = (64, 128, 256)
-_CACHE_DTYPES = (torch.bfloat16, torch.float16, torch.float8_e4m3fn)
+POWER_DIMS = 32  # dims of an fp4 head that share a power of two
+FP4 = torch.float4_e2m1fn_x2
+_CACHE_DTYPES = (torch.bfloat16, torch.float16, torch.float8_e4m3fn, FP4)
 
 
 class PagedCache:
     """Keys and values ``[pages, page_size, kv_heads, head_dim]``, of any page,
     slot and head strides (16-byte aligned heads of contiguous dims), with
     ``key_scales`` / ``value_scales`` ``[pages, page_size, kv_heads]`` fp32 when
-    they are fp8 e4m3fn.  The tensors are the caller's and are written in place;
+    they are fp8 e4m3fn.  Of fp4 e2m1 (``torch.float4_e2m1fn_x2``, two codes an
+    element, the first in the low half) they are ``[pages, page_size, kv_heads,
+    head_dim / 2]``, and the scales e8m0 (``torch.float8_e8m0fnu``) ``[pages, kv_heads,
+    page_size, head_dim / 32]``.  The tensors are the caller's and are written in place;
     cache row r is slot ``r % page_size`` of page ``r // page_size``."""
 
     __slots__ = ("keys", "values", "key_scales", "value_scales", "pages", "page_size", "kv_heads", "head_dim", "dtype",
@@ -52,10 +59,13 @@ class PagedCache:
         if keys.ndim != 4 or values.shape != keys.shape:
             raise ValueError("keys and values must both be [pages,page_size,kv_heads,head_dim]")
         if keys.dtype not in _CACHE_DTYPES or values.dtype != keys.dtype:
-            raise ValueError("a paged cache is BF16, FP16 or FP8 e4m3fn")
+            raise ValueError("a paged cache is BF16, FP16 or FP8 e4m3fn, or FP4 e2m1fn_x2")
         if not (keys.is_cuda and values.is_cuda) or keys.device != values.device:
             raise ValueError("HIP kernels require GPU tensors")
         pages, page_size, kv_heads, head_dim = keys.shape
+        fp4 = keys.dtype == FP4
+        if fp4:
+            head_dim *= 2
         if page_size < 1 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two")
         if head_dim not in HEAD_DIMS:
@@ -70,12 +80,17 @@ class PagedCache:
             if fp8 and (t is None or t.shape != keys.shape[:3] or t.dtype != torch.float32 or not t.is_contiguous()
                         or t.device != keys.device):
                 raise ValueError("an fp8 cache needs contiguous fp32 scales [pages,page_size,kv_heads]")
-            if not fp8 and t is not None:
-                raise ValueError("only an fp8 cache has scales")
+            if fp4 and (t is None or t.shape != (pages, kv_heads, page_size, head_dim // POWER_DIMS)
+                        or t.dtype != torch.float8_e8m0fnu or not t.is_contiguous() or t.data_ptr() % 16
+                        or t.device != keys.device):
+                raise ValueError("an fp4 cache needs contiguous, 16-byte aligned e8m0 scales "
+                                 "[pages,kv_heads,page_size,head_dim/32]")
+            if not (fp8 or fp4) and t is not None:
+                raise ValueError("only an fp8 or fp4 cache has scales")
         self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.dtype = keys.dtype
-        self.row_dtype = torch.bfloat16 if fp8 else keys.dtype  # of the queries and of appended rows
+        self.row_dtype = torch.bfloat16 if fp8 or fp4 else keys.dtype  # of the queries and of appended rows
         self.device = keys.device
         self._index = keys.get_device()
         self._code = _lib.dtype_code(self.row_dtype)
@@ -105,8 +120,16 @@ class PagedCache:
 def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, dtype: torch.dtype = torch.bfloat16,
               device: torch.device | str = "cuda") -> PagedCache:
     """An empty cache.  Its rows are uninitialised: attention reads none that
-    was not appended."""
+    was not appended.  In an fp4 one a page's rows of one head lie together: a row
+    of its own is 64 bytes at head_dim 128, half of what memory serves well."""
 
+    if dtype == FP4:
+        if head_dim not in HEAD_DIMS:
+            raise ValueError("head_dim must be 64, 128 or 256")
+        parts = [torch.empty((pages, kv_heads, page_size, n), dtype=torch.uint8, device=device)
+                 for n in (head_dim // 2, head_dim // 2, head_dim // POWER_DIMS, head_dim // POWER_DIMS)]
+        return PagedCache(*(x.transpose(1, 2).view(FP4) for x in parts[:2]),
+                          *(x.view(torch.float8_e8m0fnu) for x in parts[2:]))
     shape = (pages, page_size, kv_heads, head_dim)
     keys, values = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
     if dtype != torch.float8_e4m3fn:
@@ -184,7 +207,7 @@ def _queries(queries: torch.Tensor, cache: PagedCache) -> tuple[torch.Tensor, in
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError("heads must be a multiple of the cache's kv_heads")
     if queries.dtype is not cache.row_dtype:
-        raise ValueError("queries must have the cache's dtype (BF16 for an FP8 cache)")
+        raise ValueError("queries must have the cache's dtype (BF16 for an FP8 or FP4 cache)")
     if queries.get_device() != cache._index:
         raise ValueError("queries and cache must be on one GPU")
     queries, stride = _rows(queries, heads, dim)
@@ -219,7 +242,9 @@ def append(
     With ``queries`` ``[T, heads, head_dim]`` the rotated queries are returned.
     Tokens whose row is outside the cache (-1: padding) are not written; no two
     tokens may have the same row.  An fp8 cache scales each head by its largest
-    magnitude.  The angles are exact to fp32 at any position; taken as an fp32
+    magnitude, an fp4 one each 32 dims by the least power of two under which theirs is
+    7 or less: no value is then off by more than half a step of the codes, and what
+    is not finite makes its 32 dims NaN.  The angles are exact to fp32 at any position; taken as an fp32
     product, as the sidecar's encoders and many models take theirs, they are 0.0006
     rad off at position 65535, so keys and queries are best rotated by one of the two.
     """
@@ -231,7 +256,7 @@ def append(
     if rows_heads != kv_heads or rows_dim != dim:
         raise ValueError("keys and values must both be [tokens,kv_heads,head_dim]")
     if keys.dtype is not cache.row_dtype or values.dtype is not cache.row_dtype:
-        raise ValueError("appended rows must have the cache's dtype (BF16 for an FP8 cache)")
+        raise ValueError("appended rows must have the cache's dtype (BF16 for an FP8 or FP4 cache)")
     if keys.get_device() != cache._index or values.get_device() != cache._index:
         raise ValueError("appended rows and cache must be on one GPU")
     if rows.ndim != 1 or len(rows) != tokens or positions.shape != rows.shape:
@@ -259,6 +284,24 @@ def append(
               _lib.ptr(queries), query_stride, _lib.ptr(out), heads, cache._code, rows.data_ptr(),
               positions.data_ptr(), tokens, rope_dim, theta, _lib.stream_of(keys))
     return out
+
+
+def read(cache: PagedCache, rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and the values ``[n, kv_heads, head_dim]`` that cache rows ``rows``
+    ``[n]`` stand for, in the type that rows are appended in: the rows themselves
+    of a 16-bit cache, bf16 for fp8 (rounded) and fp4 (exact).  Rows outside the cache
+    (-1: padding) give zeros."""
+
+    if rows.ndim != 1:
+        raise ValueError("rows must be [n]")
+    rows = _integers(rows, torch.int64, "rows", cache)
+    count = len(rows)
+    keys, values = (torch.empty((count, cache.kv_heads, cache.head_dim), dtype=cache.row_dtype, device=cache.device)
+                    for _ in range(2))
+    if count:
+        _lib.call("dsa_paged_read", cache._address, rows.data_ptr(), count, keys.data_ptr(), values.data_ptr(),
+                  _lib.stream_of(keys))
+    return keys, values
 
 
 def _batch(tokens: int, cache: PagedCache, page_table, lengths, starts):
@@ -299,7 +342,7 @@ def attention(
 ):
     """Softmax attention of each sequence's newest tokens over its cached keys.
 
-    queries ``[T, heads, head_dim]`` of the cache's dtype (bf16 for fp8), already
+    queries ``[T, heads, head_dim]`` of the cache's dtype (bf16 for fp8 and fp4), already
     rotated; ``page_table`` ``[B, columns]`` int32 page ids; ``lengths`` ``[B]``
     int32 keys of each sequence, the new tokens' own included.  Sequence b's
     tokens are ``starts[b] .. starts[b + 1]`` (``[B + 1]`` int32, ascending, within

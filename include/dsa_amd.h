@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define DSA_ABI_VERSION 7
+#define DSA_ABI_VERSION 8
 
 #define DSA_STATUS_OK 0
 #define DSA_STATUS_INVALID_ARGUMENT 1
@@ -39,6 +39,7 @@ extern "C" {
 #define DSA_DTYPE_BF16 2
 #define DSA_DTYPE_FP8_E4M3 3 /* keys only; queries are bf16 */
 #define DSA_DTYPE_F64 4      /* score rows of dsa_topk_exact only */
+#define DSA_DTYPE_FP4_E2M1 5 /* paged caches only; queries are bf16 */
 
 /* Message describing the last failure on the calling thread. */
 const char* dsa_last_error(void);
@@ -848,8 +849,12 @@ int dsa_encode_queries_gemm(const void* hidden, int64_t hidden_stride, int64_t t
  * slot, head, d) of the keys lies at page * key_page_stride + slot *
  * key_slot_stride + head * key_head_stride + d elements, the values' likewise:
  * any order of pages, slots and heads, head_dim contiguous elements.  dtype is
- * bf16, fp16 or fp8 e4m3; an fp8 cache stands for code * scale, with one fp32
- * scale per (page, slot, head) in contiguous [pages][page_size][kv_heads].
+ * bf16, fp16, fp8 e4m3 or fp4 e2m1; an fp8 cache stands for
+ * code * scale, with one fp32 scale per (page, slot, head) in contiguous
+ * [pages][page_size][kv_heads].  An fp4 cache holds two codes a byte, the first in
+ * the low half, its strides count those bytes, and it stands for code * 2^(power -
+ * 127), with one power byte (e8m0; 255: NaN) per 32 dims in contiguous, 16-byte
+ * aligned [pages][kv_heads][page_size][head_dim / 32].
  * page_size a power of two, head_dim 64, 128 or 256, pages * page_size below
  * 2^31; pointers and strides 16-byte aligned, page and slot strides below 4 GiB.
  * Offsets are 64-bit.  The descriptor is host memory, read during the call.
@@ -857,8 +862,8 @@ int dsa_encode_queries_gemm(const void* hidden, int64_t hidden_stride, int64_t t
 typedef struct dsa_paged_cache {
   void* keys;
   void* values;
-  float* key_scales;   /* fp8 only, else ignored */
-  float* value_scales;
+  void* key_scales;    /* fp8 (float) and fp4 (uint8_t) only, else ignored */
+  void* value_scales;
   int64_t pages;
   int64_t key_page_stride, key_slot_stride, key_head_stride;
   int64_t value_page_stride, value_slot_stride, value_head_stride;
@@ -873,14 +878,23 @@ typedef struct dsa_paged_cache {
  * sums are fp32, rounded once to the cache's type.  Tokens whose row is outside
  * the cache are not written; two tokens with one row leave either's values (on an
  * fp8 cache any mixture of their codes and scales).  fp8: scale = max(max|x| / 448, 2^-126) over a head, code = round-to-nearest
- * (x / scale); rows must be finite.  queries (nullable, [tokens][heads]
+ * (x / scale); rows must be finite.  fp4: the power of 32 dims is the least under
+ * which the largest magnitude is 7 or less, from 2^-124 to 2^125, code =
+ * round-to-nearest-even(x / 2^power), at most 6; 32 dims of which one is not finite
+ * become NaN; keys are turned in double and rounded once.  queries (nullable, [tokens][heads]
  * [head_dim]) are turned by the same angles into out_queries (dense, may not
  * overlap).  dtype is that of keys, values and queries: the cache's, or bf16 for
- * an fp8 cache.  rope_dim a multiple of 16 up to head_dim (0: no rotation). */
+ * an fp8 or fp4 cache.  rope_dim a multiple of 16 up to head_dim (0: no rotation). */
 int dsa_paged_append(const dsa_paged_cache* cache, const void* keys, int64_t key_stride, const void* values,
                      int64_t value_stride, const void* queries, int64_t query_stride, void* out_queries,
                      int32_t heads, int32_t dtype, const int64_t* rows, const int64_t* positions, int64_t tokens,
                      int32_t rope_dim, double theta, void* stream);
+
+/* What count cache rows stand for: out_keys and out_values [count][kv_heads]
+ * [head_dim], dense, of the cache's type (bf16 for an fp8 cache, rounded, and for
+ * an fp4 cache, exact), either of them NULL.  Rows outside the cache give zeros. */
+int dsa_paged_read(const dsa_paged_cache* cache, const int64_t* rows, int64_t count, void* out_keys, void* out_values,
+                   void* stream);
 
 /* Attention of each sequence's newest tokens over its whole cache:
  *   out[t][h] = sum_j softmax_j(scale q[t][h] . k[j][h / group]) v[j][h / group]

@@ -71,3 +71,38 @@ def attention(q, keys, values, table, lengths, starts, scale, *, causal=True, li
                 out[t, h], lse[t, h], weighted[t, h], sizes[t, h] = attend(q[t, h], keys[page, slot, g],
                                                                            values[page, slot, g], scale)
     return out, lse, weighted, sizes
+
+
+E2M1 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+POWERS = (-124, 125)  # of an fp4 cache
+
+
+def fp4_values(codes: np.ndarray, powers: np.ndarray) -> np.ndarray:
+    """What packed codes ``[..., D / 2]`` under e8m0 bytes ``[..., D / 32]`` stand for."""
+
+    code = np.stack([codes & 15, codes >> 4], axis=-1).reshape(*codes.shape[:-1], -1)
+    x = np.where(code > 7, -1.0, 1.0) * E2M1[code & 7]
+    unit = np.where(powers == 255, np.nan, 2.0 ** (powers.astype(np.float64) - 127))
+    return x * np.repeat(unit, 32, axis=-1)
+
+
+def fp4(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """Values and e8m0 bytes ``[..., D / 32]`` that an fp4 cache holds of ``x``
+    ``[..., D]``: the nearest of the values below (ties to the even code) under the
+    least power of two by which the largest magnitude is 7 or less."""
+
+    blocks = x.reshape(*x.shape[:-1], -1, 32)
+    out, powers = np.empty_like(blocks, dtype=np.float64), np.empty(blocks.shape[:-1], dtype=np.int64)
+    for at in np.ndindex(blocks.shape[:-1]):
+        b = blocks[at].astype(np.float64)
+        if not np.isfinite(b).all():
+            out[at], powers[at] = np.nan, 255
+            continue
+        e = POWERS[0]
+        while e < POWERS[1] and np.abs(b).max() > 7 * 2.0**e:
+            e += 1
+        away = np.abs(np.abs(b)[:, None] / 2.0**e - E2M1)
+        least = away.min(axis=1, keepdims=True)
+        code = np.argmax((away == least) * (2 - np.arange(8) % 2), axis=1)
+        out[at], powers[at] = np.sign(b) * E2M1[code] * 2.0**e, e + 127
+    return out.reshape(x.shape), powers
