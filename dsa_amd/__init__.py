@@ -15,6 +15,8 @@ the names of the reference package ``temporal_dsa``:
   certified           block_key_norms, temporal_score_radius
   paged               paged key/value cache: append, attention, attention over
                       selected keys (no counterpart in the reference)
+  eviction            accumulated attention weights of cached keys, and the
+                      eviction of those that have least
   temporal            device temporal pruning (seed, hot-first, running top-K)
 """
 

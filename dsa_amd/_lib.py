@@ -127,6 +127,10 @@ _SIGNATURES: dict[str, list] = {
         _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i32, _i32, _p, _i64, _i64, ctypes.c_float, _p, _p, _p, _i64,
         _p,
     ],
+    "dsa_paged_weights": [
+        _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i32, _i32, ctypes.c_float, _i32, _p, _p, _p, _i64, _p,
+    ],
+    "dsa_paged_evict": [_p, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _i64, _p],
     "dsa_dim_sketch": [_p, _i64, _i32, _i32, _p, _i32, _i32, _i32, ctypes.c_float, _p, _i32, _p],
     "dsa_abs_max": [_p, _i64, _i32, _p, _p],
     "dsa_fake_quantize": [_p, _i64, _i32, _i32, ctypes.c_float, _p, _p, _p],
@@ -144,6 +148,8 @@ _RESTYPES: dict[str, object] = {
     "dsa_encode_queries_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "dsa_paged_attention_workspace_bytes": (_i64, [_p, _i64, _i64, _i32, _i64, _i32]),
     "dsa_paged_selected_workspace_bytes": (_i64, [_p, _i64, _i32, _i64]),
+    "dsa_paged_weights_workspace_bytes": (_i64, [_p, _i64, _i64, _i32, _i64, _i32]),
+    "dsa_paged_evict_workspace_bytes": (_i64, [_p, _i64, _i64, _i64, _i32]),
 }
 
 

@@ -716,10 +716,12 @@ int64_t row_tiles(int64_t sequences, int64_t tokens, int64_t group, bool uniform
   return (tokens * group + (size - 1) * most) / size;
 }
 
-int check_common(const dsa_paged_cache* cache, const void* queries, int64_t query_stride, const int32_t* page_table,
-                 int64_t table_stride, int64_t columns, const int32_t* lengths, const int32_t* starts,
-                 int64_t sequences, int64_t tokens, int32_t heads, int32_t dtype, float scale, const void* out,
-                 PagedAttentionArgs& a) {
+}  // namespace
+
+int check_paged_batch(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
+                      const int32_t* page_table, int64_t table_stride, int64_t columns, const int32_t* lengths,
+                      const int32_t* starts, int64_t sequences, int64_t tokens, int32_t heads, int32_t dtype,
+                      float scale, const void* out, PagedAttentionArgs& a) {
   if (int st = make_paged_view(cache, a.cache)) return st;
   DSA_REQUIRE(sequences > 0 && sequences <= (1 << 20) && tokens >= 0 && tokens < (1LL << 28), "sequences/tokens out of range");
   DSA_REQUIRE(queries && page_table && lengths && out, "null pointer argument");
@@ -748,6 +750,8 @@ int check_common(const dsa_paged_cache* cache, const void* queries, int64_t quer
   a.scale = scale * kLog2E;
   return 0;
 }
+
+namespace {
 
 constexpr int64_t kStreamRows = 16;  // most rows of a sequence that the stream kernel takes
 
@@ -917,7 +921,7 @@ extern "C" int dsa_paged_attention(const dsa_paged_cache* cache, const void* que
                                    int32_t heads, int32_t dtype, float scale, int32_t causal, void* out, float* lse,
                                    void* workspace, int64_t workspace_bytes, void* stream) {
   PagedAttentionArgs a = {};
-  if (int st = check_common(cache, queries, query_stride, page_table, table_stride, columns, lengths, starts, sequences,
+  if (int st = check_paged_batch(cache, queries, query_stride, page_table, table_stride, columns, lengths, starts, sequences,
                             tokens, heads, dtype, scale, out, a))
     return st;
   if (tokens == 0) return 0;
@@ -968,7 +972,7 @@ extern "C" int dsa_paged_selected_attention(const dsa_paged_cache* cache, const 
                                             int64_t index_stride, int64_t k, float scale, void* out, float* lse,
                                             void* workspace, int64_t workspace_bytes, void* stream) {
   PagedAttentionArgs a = {};
-  if (int st = check_common(cache, queries, query_stride, page_table, table_stride, columns, lengths, starts, sequences,
+  if (int st = check_paged_batch(cache, queries, query_stride, page_table, table_stride, columns, lengths, starts, sequences,
                             tokens, heads, dtype, scale, out, a))
     return st;
   DSA_REQUIRE(k >= 0 && k < (1LL << 31) - 64 && (indices || k == 0) && index_stride >= k, "index lists of %lld out of range",

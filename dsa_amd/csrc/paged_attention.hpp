@@ -340,6 +340,12 @@ constexpr int kKeyRow = 2 * D + 16;
 template <int D>
 constexpr int kValueRow = 2 * D + 64;
 
+// Checks a call's arguments and fills what every kernel over a batch's queries needs.
+int check_paged_batch(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
+                      const int32_t* page_table, int64_t table_stride, int64_t columns, const int32_t* lengths,
+                      const int32_t* starts, int64_t sequences, int64_t tokens, int32_t heads, int32_t dtype,
+                      float scale, const void* out, PagedAttentionArgs& a);
+
 constexpr int kChunkRows = 128;        // rows of a workgroup of the chunk kernel
 constexpr int kLeastChunkKeys = 256;   // keys of a piece of it
 

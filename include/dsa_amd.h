@@ -935,6 +935,39 @@ int dsa_paged_selected_attention(const dsa_paged_cache* cache, const void* queri
                                  float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
                                  void* stream);
 
+/* What each cached key has of the softmax weights of each sequence's newest tokens,
+ * added to weights [kv_heads][pages * page_size] (fp32, by cache row):
+ *   weights[g][row(j)] += sum over tokens t and heads h of kv head g that see key j
+ *                         of exp(scale q[t][h] . k[j][g] - lse[t][h])
+ * Arguments as of dsa_paged_attention, lse [tokens][heads] as it returns them.  Sums
+ * are fp32 in an order that the sizes alone set, so two calls on the same inputs give
+ * the same bits unless two sequences share a page, whose sums are both added.  What a
+ * row does not see does not reach a weight.  Workspace: the bytes of the query. */
+int64_t dsa_paged_weights_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
+                                          int32_t heads, int64_t columns, int32_t uniform);
+int dsa_paged_weights(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
+                      const int32_t* page_table, int64_t table_stride, int64_t columns, const int32_t* lengths,
+                      const int32_t* starts, int64_t sequences, int64_t tokens, int32_t heads, int32_t dtype,
+                      float scale, int32_t causal, const float* lse, float* weights, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* Cuts each sequence of n = lengths[s] keys to m = min(n, keep), in place: its newest
+ * `recent` ones (at most m) and those of largest weight among the others (ties: the
+ * lowest position; NaN counts as the least).  Kept keys below position m stay; those
+ * from m on go, in order, to the positions below m that are freed.  per_head: each kv
+ * head keeps keys of its own, by its own weights; else all keep the same, by their
+ * weights' sum (held in fp64, rounded to fp32).  Weights move with their keys, those of
+ * positions m .. n become 0.  out_lengths[s] = m; kept [sequences][kv_heads if
+ * per_head else 1][keep] is the former position of the key now at each position, -1
+ * from m on.  No other byte of the cache is written.  A page may be of one
+ * sequence alone.  Workspace (16-byte aligned): the bytes of the query. */
+int64_t dsa_paged_evict_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t columns, int64_t keep,
+                                        int32_t per_head);
+int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t columns,
+                    const int32_t* lengths, int64_t sequences, float* weights, int64_t keep, int64_t recent,
+                    int32_t per_head, int32_t* out_lengths, int64_t* kept, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
 /* ------------------------------------------------------------------------
  * Measurement utility (no counterpart in the reference; it serves the
  * roofline's measured peak): one launch that only reads `bytes` of device
