@@ -8,10 +8,14 @@
 // order, so that nothing else has to move, and no move's source is another's
 // destination: the moves need no order either.
 //
-// Two launches.  The first finds each list's threshold (a list is a sequence's, or one
-// kv head's of it) by three passes over the weights' order-preserving 32-bit keys,
-// 11, 11 and 10 bits, and from it the list of moves; the second moves keys, values,
-// scales and weights.
+// A list (a sequence's, or one kv head's of it) has a threshold, found by three passes
+// over the weights' order-preserving 32-bit keys, 11, 11 and 10 bits, and from it its
+// holes and its sources, the i-th of either being one move; the last launch moves keys,
+// values, scales and weights.  Up to 16K positions a list is one workgroup's, beyond
+// that the passes are launches.
+#include <algorithm>
+#include <type_traits>
+
 #include "paged.hpp"
 #include "waveops.hpp"
 
@@ -19,8 +23,6 @@ namespace dsa {
 namespace {
 
 constexpr uint32_t kThreads = 1024;
-constexpr uint32_t kEach = 4;                  // positions of a thread and pass
-constexpr uint32_t kSpan = kThreads * kEach;   // of the workgroup
 
 struct EvictArgs {
   PagedView cache;
@@ -34,14 +36,15 @@ struct EvictArgs {
   uint32_t lists;         // of a sequence: kv_heads or 1
   int32_t* out_lengths;
   int64_t* kept;          // [sequences][lists][keep]
-  // Workspace, for each list: {holes that were filled}, the keys' order, the moves
-  // {to, from}; key_stride and keep entries apart.
+  // Workspace, for each list: the three passes' bins (zero between calls), its moves
+  // {to, from} (keep apart) and how many there are, and for long lists each chunk's
+  // counts and the order of every weight.
+  uint32_t* bins;
+  uint2* moves;
   uint32_t* counts;
+  uint4* chunks;
   uint32_t* order;
   uint64_t order_stride;
-  uint2* moves;
-  uint32_t pieces;        // bytes / 16 of a head's keys
-  uint32_t head_powers;   // of an e2m1 head
 };
 
 __device__ __forceinline__ uint32_t cache_row(const EvictArgs& a, const int32_t* table, uint32_t key) {
@@ -57,185 +60,480 @@ __device__ __forceinline__ uint32_t keys_of(const EvictArgs& a, uint32_t sequenc
 // Larger for larger weights; 0 for NaN.
 __device__ __forceinline__ uint32_t order_of(float w) { return w == w ? float_to_ordered(w) : 0u; }
 
+// A list: its sequence's keys before and after, and what is chosen among.
+struct List {
+  const int32_t* pages;
+  uint32_t sequence, g, n, m;
+  uint32_t old;   // positions that are chosen from: the first
+  uint32_t want;  // of them, fewer than there are
+};
+
+__device__ __forceinline__ List list_of(const EvictArgs& a, uint32_t list) {
+  List l;
+  l.sequence = list / a.lists;
+  l.g = list % a.lists;
+  l.pages = a.page_table + (int64_t)l.sequence * a.table_stride;
+  l.n = keys_of(a, l.sequence);
+  l.m = min(l.n, a.keep);
+  l.old = l.n - min(a.recent, l.m);
+  l.want = l.m - (l.n - l.old);
+  return l;
+}
+
+// The orders of positions first + stride * e of those that are chosen from; 0 past them.
+template <int kEach>
+__device__ __forceinline__ void orders_of(const EvictArgs& a, const List& l, uint32_t first, uint32_t stride,
+                                          uint32_t (&key)[kEach]) {
+  uint32_t row[kEach];
+#pragma unroll
+  for (uint32_t e = 0; e < kEach; ++e) row[e] = cache_row(a, l.pages, min(first + stride * e, l.n - 1u));
+  if (a.lists > 1u || a.cache.kv_heads == 1u) {
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) key[e] = order_of(a.weights[l.g * a.row_count + row[e]]);
+  } else {
+    double sum[kEach];
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) sum[e] = 0.0;
+    for (uint32_t h = 0; h < a.cache.kv_heads; ++h)
+#pragma unroll
+      for (uint32_t e = 0; e < kEach; ++e) sum[e] += (double)a.weights[h * a.row_count + row[e]];
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) key[e] = order_of((float)sum[e]);
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < kEach; ++e) key[e] = first + stride * e < l.old ? key[e] : 0u;
+}
+
+// Where the want-th largest of a list's orders lies: its digits so far, how many with
+// those digits are still wanted, and whether there are more of them.
+struct Threshold {
+  uint32_t prefix, rest;
+  bool ties;
+};
+constexpr uint32_t kShift[3] = {21u, 10u, 0u};  // of each pass's digit
+constexpr uint32_t kBins = 2048;
+
+// Counts a lane's bin; the lanes that share the first one's are one addition (a list of
+// zeros counts one bin).
+__device__ __forceinline__ void count_bin(uint32_t* bins, uint32_t bin, bool counts) {
+  const uint64_t all = __ballot(counts);
+  if (!all) return;
+  const uint32_t leader = (uint32_t)__builtin_ctzll(all);
+  const uint64_t same = __ballot(counts && bin == (uint32_t)__builtin_amdgcn_readlane(bin, leader));
+  if (lane_id() == leader)
+    atomicAdd(&bins[bin], (uint32_t)__popcll(same));
+  else if (counts && !(same >> lane_id() & 1u))
+    atomicAdd(&bins[bin], 1u);
+}
+
+// The digit of `pass` added to the threshold.
+__device__ __forceinline__ void locate_digit(const uint32_t* bins, uint32_t pass, Locate& shared, Threshold& t) {
+  if (threadIdx.x < kWave) {
+    const Locate l = wave_locate<32>(bins, t.rest, false);
+    if (threadIdx.x == 0) shared = l;
+  }
+  __syncthreads();
+  t.prefix |= shared.digit << kShift[pass];
+  t.rest = shared.rem;
+  t.ties = shared.count > shared.rem;
+  __syncthreads();
+}
+
+// A bit for each of a thread's positions that lies below `end`.  (No difference is taken
+// under a condition here, as in `end > at ? end - at : 0`: the compiler takes it for one
+// that never wraps, and concludes at <= end for comparisons further on.)
+template <int kEach>
+__device__ __forceinline__ uint32_t bits_below(uint32_t at, uint32_t end) {
+  return (1u << min(end - min(end, at), (uint32_t)kEach)) - 1u;
+}
+
+// Which of a thread's kEach positions from `at` on are kept; `rank` is that of its first
+// key at the threshold among all of those.
+template <int kEach>
+__device__ __forceinline__ uint32_t kept_of(const List& l, const Threshold& t, const uint32_t (&key)[kEach], uint32_t at,
+                                            uint32_t rank) {
+  const uint32_t old = l.want > 0 ? bits_below<kEach>(at, l.old) : 0u;
+  uint32_t keeps = bits_below<kEach>(at, l.n) & ~bits_below<kEach>(at, l.old);  // the newest
+#pragma unroll
+  for (uint32_t e = 0; e < kEach; ++e) {
+    const uint32_t level = (key[e] == t.prefix) & (old >> e & 1u);
+    const uint32_t chosen = (key[e] > t.prefix) | (level & (uint32_t)(!t.ties || rank < t.rest));
+    rank += level;
+    keeps |= (chosen & (old >> e & 1u)) << e;
+  }
+  return keeps;
+}
+
+// Records what the workgroup's positions from `first` on do, kEach neighbouring ones a
+// thread, its kept ones the bits of `keeps`: kept ones below m stay, the others there
+// are holes; kept ones from m on are sources; evicted ones there lose their weight.
+// `before`: the workgroup's holes and, in the upper half, sources before the thread's,
+// `all` of them; `hole`, `source`: the list's before the workgroup's.  Through LDS, so
+// that neighbouring lanes store to neighbouring places.
+template <int kEach>
+__device__ __forceinline__ void settle(const EvictArgs& a, const List& l, uint32_t list, uint32_t first, uint32_t keeps,
+                                       uint32_t before, uint32_t all, uint32_t hole, uint32_t source,
+                                       uint32_t* moving, uint32_t* masks) {
+  const uint32_t tid = threadIdx.x;
+  const uint32_t at = first + tid * kEach;
+  const uint32_t below = bits_below<kEach>(at, l.m);
+  const uint32_t holes = all & 0xffffu, sources = all >> 16;
+  uint32_t my_hole = before & 0xffffu, my_source = holes + (before >> 16);
+  masks[tid] = keeps;
+#pragma unroll
+  for (uint32_t e = 0; e < kEach; ++e) {
+    if ((~keeps & below) >> e & 1u) moving[my_hole++] = at + e;
+    if ((keeps & ~below) >> e & 1u) moving[my_source++] = at + e;
+  }
+  __syncthreads();
+  int64_t* kept = a.kept + (uint64_t)list * a.keep;
+  uint2* moves = a.moves + (uint64_t)list * a.keep;
+  for (uint32_t i = tid; i < holes; i += kThreads) moves[hole + i].x = moving[i];
+  for (uint32_t i = tid; i < sources; i += kThreads) moves[source + i].y = moving[holes + i];
+  uint32_t row[kEach];
+  uint32_t evicted = 0;
+#pragma unroll
+  for (uint32_t e = 0; e < kEach; ++e) {
+    const uint32_t within = tid + kThreads * e, i = first + within;
+    const uint32_t keep = masks[within / kEach] >> within % kEach & 1u;
+    if (keep & (uint32_t)(i < l.m)) kept[i] = i;
+    evicted |= ((keep ^ 1u) & (uint32_t)(i >= l.m) & (uint32_t)(i < l.n)) << e;
+    row[e] = cache_row(a, l.pages, min(i, l.n - 1u));
+  }
+  const uint32_t heads = a.lists > 1u ? 1u : a.cache.kv_heads;
+  for (uint32_t h = 0; h < heads; ++h)
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e)
+      if (evicted >> e & 1u) a.weights[(l.g + h) * a.row_count + row[e]] = 0.f;
+}
+
+// Holes and, in the upper half, sources among a thread's positions.
+template <int kEach>
+__device__ __forceinline__ uint32_t count_moves(const List& l, uint32_t at, uint32_t keeps) {
+  const uint32_t below = bits_below<kEach>(at, l.m);
+  return (uint32_t)__popc(~keeps & below) | (uint32_t)__popc(keeps & ~below) << 16;
+}
+
+// Positions that keep theirs where nothing is evicted, and those that a list has no key
+// for.
+__device__ __forceinline__ void fill_kept(const EvictArgs& a, const List& l, uint32_t list, uint32_t first, uint32_t step) {
+  int64_t* kept = a.kept + (uint64_t)list * a.keep;
+  for (uint32_t i = (l.n > l.m ? l.m : 0u) + first; i < a.keep; i += step) kept[i] = i < l.m ? (int64_t)i : -1;
+}
+
+// One workgroup a list, whose orders lie in LDS: kEach neighbouring positions a thread,
+// so that every rank is one scan.  Latency bound.
+template <int kEach>
 __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs a) {
-  __shared__ __attribute__((aligned(16))) uint32_t bins[2048];
+  __shared__ __attribute__((aligned(16))) uint32_t order[kThreads * (kEach + 1)];  // a thread's, then one word of room
+  __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
   __shared__ __attribute__((aligned(16))) uint32_t scan[2][16];
   __shared__ Locate found;
   const uint32_t tid = threadIdx.x;
   const uint32_t list = blockIdx.x;
-  const uint32_t sequence = list / a.lists, g = list % a.lists;
-  const uint32_t n = keys_of(a, sequence);
-  const uint32_t m = min(n, a.keep);
-  const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
-  int64_t* kept = a.kept + (uint64_t)list * a.keep;
+  const List l = list_of(a, list);
   if (tid == 0) {
-    if (g == 0) a.out_lengths[sequence] = (int32_t)m;
-    a.counts[list] = 0;
+    if (l.g == 0) a.out_lengths[l.sequence] = (int32_t)l.m;
+    if (l.n == l.m) a.counts[list] = 0;
   }
-  for (uint32_t i = (n > m ? m : 0u) + tid; i < a.keep; i += kThreads) kept[i] = i < m ? (int64_t)i : -1;
-  if (n == m) return;
-  const uint32_t old = n - min(a.recent, m);   // positions that are chosen from
-  const uint32_t want = m - (n - old);         // of them, fewer than there are
-  uint32_t* order = a.order + (uint64_t)list * a.order_stride;
-  uint2* moves = a.moves + (uint64_t)list * a.keep;
-
-  // The weights' order, and the want-th largest of it digit by digit.
-  uint32_t prefix = 0, rest = want;
-  bool ties = false;  // more keys are at the threshold than are kept
-  auto clear = [&]() {
-    for (uint32_t i = tid; i < 2048u; i += kThreads) bins[i] = 0;
-    __syncthreads();
-  };
-  clear();
-  for (uint32_t i = tid; i < old; i += kThreads) {
-    const uint32_t row = cache_row(a, pages, i);
-    uint32_t key;
-    if (a.lists > 1u || a.cache.kv_heads == 1u) {
-      key = order_of(a.weights[g * a.row_count + row]);
-    } else {
-      double sum = 0.0;
-      for (uint32_t h = 0; h < a.cache.kv_heads; ++h) sum += (double)a.weights[h * a.row_count + row];
-      key = order_of((float)sum);
-    }
-    order[i] = key;
-    atomicAdd(&bins[key >> 21], 1u);
+  fill_kept(a, l, list, tid, kThreads);
+  if (l.n == l.m) return;
+  for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
+  uint32_t key[kEach];
+  orders_of<kEach>(a, l, tid, kThreads, key);
+#pragma unroll
+  for (uint32_t e = 0; e < kEach; ++e) {
+    const uint32_t i = tid + kThreads * e;
+    order[i / kEach * (kEach + 1) + i % kEach] = key[e];
   }
-  if (want > 0) {
-    for (int pass = 0; pass < 3; ++pass) {
-      const uint32_t shift = pass == 0 ? 21u : pass == 1 ? 10u : 0u;
-      const uint32_t mask = pass == 2 ? 1023u : 2047u;
+  __syncthreads();
+  const uint32_t at = tid * kEach;
+#pragma unroll
+  for (uint32_t e = 0; e < kEach; ++e) key[e] = order[tid * (kEach + 1) + e];
+  Threshold t = {0u, l.want, false};
+  if (l.want > 0) {
+    for (uint32_t pass = 0; pass < 3; ++pass) {
       if (pass > 0) {
-        clear();
-        const uint32_t above = pass == 1 ? 21u : 10u;
-        for (uint32_t i = tid; i < old; i += kThreads) {
-          const uint32_t key = order[i];
-          if (key >> above == prefix >> above) atomicAdd(&bins[(key >> shift) & mask], 1u);
-        }
+        for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
+        __syncthreads();
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < kEach; ++e) {
+        const bool counts = at + e < l.old && (pass == 0 || key[e] >> kShift[pass - 1] == t.prefix >> kShift[pass - 1]);
+        count_bin(bins, key[e] >> kShift[pass] & (pass == 2 ? 1023u : 2047u), counts);
       }
       __syncthreads();
-      if (tid < kWave) {
-        const Locate l = wave_locate<32>(bins, rest, false);
-        if (tid == 0) found = l;
-      }
-      __syncthreads();
-      prefix |= found.digit << shift;
-      rest = found.rem;
-      ties = found.count > found.rem;
+      locate_digit(bins, pass, found, t);
     }
   }
-  __syncthreads();  // the order, as every thread has written it
-
-  // What is kept, position by position.  Every hole lies below every source, so the
-  // i-th source finds the i-th hole written.
-  uint32_t tied = 0, holes = 0, sources = 0;
-  for (uint32_t base = 0; base < n; base += kSpan) {
-    const uint32_t at = base + kEach * tid;
-    uint32_t key[kEach];
+  uint32_t rank = 0, all;
+  if (t.ties) {
     uint32_t level = 0;
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) {
-      key[e] = at + e < old ? order[at + e] : 0u;
-      level += want > 0 && at + e < old && key[e] == prefix;
-    }
-    uint32_t rank = tied;
-    if (ties) {
-      uint32_t all;
-      rank += block_excl_scan<16>(level, scan[0], all);
-      tied += all;
-    }
-    bool keeps[kEach];
-    uint32_t moved = 0;  // holes and, in the upper half, sources
-#pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) {
-      const bool chosen = want > 0 && (key[e] > prefix || (key[e] == prefix && (!ties || rank < rest)));
-      rank += want > 0 && at + e < old && key[e] == prefix;
-      keeps[e] = at + e < n && (at + e >= old || chosen);
-      if (at + e < m && !keeps[e]) moved += 1u;
-      if (at + e >= m && keeps[e]) moved += 1u << 16;
-    }
-    uint32_t all;
-    const uint32_t rank_moved = block_excl_scan<16>(moved, scan[1], all);
-    uint32_t hole = holes + (rank_moved & 0xffffu), source = sources + (rank_moved >> 16);
-    holes += all & 0xffffu;
-    sources += all >> 16;
-#pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) {
-      if (at + e >= m) break;
-      if (keeps[e])
-        kept[at + e] = at + e;
-      else
-        moves[hole++].x = at + e;
-    }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) {
-      if (at + e < m || at + e >= n) continue;
-      if (keeps[e]) {
-        kept[moves[source].x] = at + e;
-        moves[source++].y = at + e;
-      } else {
-        const uint32_t row = cache_row(a, pages, at + e);
-        if (a.lists > 1u || a.cache.kv_heads == 1u)
-          a.weights[g * a.row_count + row] = 0.f;
-        else
-          for (uint32_t h = 0; h < a.cache.kv_heads; ++h) a.weights[h * a.row_count + row] = 0.f;
-      }
-    }
-    __syncthreads();
+    for (uint32_t e = 0; e < kEach; ++e) level += at + e < l.old && key[e] == t.prefix;
+    rank = block_excl_scan<16>(level, scan[0], all);
   }
+  const uint32_t keeps = kept_of<kEach>(l, t, key, at, rank);
+  const uint32_t before = block_excl_scan<16>(count_moves<kEach>(l, at, keeps), scan[1], all);
+  const uint32_t holes = all & 0xffffu;
+  settle<kEach>(a, l, list, 0, keeps, before, all, 0, 0, order, bins);
+  int64_t* kept = a.kept + (uint64_t)list * a.keep;
+  for (uint32_t i = tid; i < holes; i += kThreads) kept[order[i]] = order[holes + i];
   if (tid == 0) a.counts[list] = holes;
 }
 
-// 16 bytes of a move a thread: first the keys, then the values of a head.  The thread
-// of a head's first 16 has its scales and weight too.
-template <Store kStore>
+// Longer lists: a chunk of one a workgroup, one launch a pass.  The passes' counts meet
+// in global memory, where the last launch leaves zeros.
+constexpr uint32_t kChunkEach = 8;
+constexpr uint32_t kChunk = kThreads * kChunkEach;
+
+template <int kPass>
+__device__ __forceinline__ Threshold threshold_of(const EvictArgs& a, const List& l, uint32_t list, Locate& found) {
+  Threshold t = {0u, l.want, false};
+  if (l.want > 0)
+#pragma unroll
+    for (uint32_t pass = 0; pass < kPass; ++pass) locate_digit(a.bins + ((uint64_t)list * 3u + pass) * kBins, pass, found, t);
+  return t;
+}
+
+template <int kPass>
+__global__ __launch_bounds__(kThreads) void paged_evict_count_kernel(EvictArgs a) {
+  __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
+  __shared__ Locate found;
+  const uint32_t tid = threadIdx.x;
+  const uint32_t list = blockIdx.y;
+  const List l = list_of(a, list);
+  const uint32_t first = blockIdx.x * kChunk;
+  if (kPass == 0) {
+    if (blockIdx.x == 0 && tid == 0) {
+      if (l.g == 0) a.out_lengths[l.sequence] = (int32_t)l.m;
+      a.counts[list] = 0;
+    }
+    fill_kept(a, l, list, blockIdx.x * kThreads + tid, gridDim.x * kThreads);
+  }
+  if (l.n == l.m || first >= l.old || l.want == 0) return;
+  const Threshold t = threshold_of<kPass>(a, l, list, found);
+  for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
+  __syncthreads();
+  uint32_t* order = a.order + (uint64_t)list * a.order_stride;
+  uint32_t own[kChunkEach];
+  if (kPass == 0) orders_of<kChunkEach>(a, l, first + tid, kThreads, own);
+#pragma unroll
+  for (uint32_t e = 0; e < kChunkEach; ++e) {
+    const uint32_t i = first + tid + kThreads * e;  // (inside the chunk's room, past the list's end too)
+    if (kPass == 0)
+      order[i] = own[e];
+    else
+      own[e] = order[i];
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < kChunkEach; ++e) {
+    const uint32_t i = first + tid + kThreads * e;
+    const uint32_t key = own[e];
+    const bool counts = i < l.old && (kPass == 0 || key >> kShift[kPass ? kPass - 1 : 0] == t.prefix >> kShift[kPass ? kPass - 1 : 0]);
+    count_bin(bins, key >> kShift[kPass] & (kPass == 2 ? 1023u : 2047u), counts);
+  }
+  __syncthreads();
+  uint32_t* to = a.bins + ((uint64_t)list * 3u + kPass) * kBins;
+  for (uint32_t i = tid; i < kBins; i += kThreads)
+    if (bins[i]) atomicAdd(&to[i], bins[i]);
+}
+
+// A thread's orders in a chunk: kChunkEach neighbouring positions.
+__device__ __forceinline__ void load_orders(const EvictArgs& a, const List& l, uint32_t list, uint32_t at,
+                                            uint32_t (&key)[kChunkEach]) {
+  const uint32_t* order = a.order + (uint64_t)list * a.order_stride;
+  if (at < l.old && l.want > 0) {  // the chunk's room ends on a multiple of kChunkEach, and holds 0 past the list
+    const uint4 lo = *reinterpret_cast<const uint4*>(order + at), hi = *reinterpret_cast<const uint4*>(order + at + 4u);
+    key[0] = lo.x, key[1] = lo.y, key[2] = lo.z, key[3] = lo.w;
+    key[4] = hi.x, key[5] = hi.y, key[6] = hi.z, key[7] = hi.w;
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < kChunkEach; ++e) key[e] = 0;
+  }
+}
+
+// Of each chunk: keys at the threshold, and above it or newest, below position m and
+// from there on.
+__global__ __launch_bounds__(kThreads) void paged_evict_chunk_kernel(EvictArgs a) {
+  __shared__ Locate found;
+  __shared__ uint32_t sums[4];
+  const uint32_t list = blockIdx.y;
+  const List l = list_of(a, list);
+  const uint32_t first = blockIdx.x * kChunk;
+  if (l.n == l.m || first >= l.n) return;
+  const Threshold t = threshold_of<3>(a, l, list, found);
+  if (threadIdx.x < 4u) sums[threadIdx.x] = 0;
+  __syncthreads();
+  const uint32_t at = first + threadIdx.x * kChunkEach;
+  uint32_t key[kChunkEach];
+  load_orders(a, l, list, at, key);
+  uint32_t count[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (uint32_t e = 0; e < kChunkEach; ++e) {
+    const uint32_t past = at + e >= l.m ? 2u : 0u;
+    const bool level = l.want > 0 && at + e < l.old && key[e] == t.prefix;
+    const bool sure = at + e < l.n && (at + e >= l.old || (l.want > 0 && key[e] > t.prefix));
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) count[c] += (c == past && level) || (c == past + 1u && sure);
+  }
+#pragma unroll
+  for (uint32_t c = 0; c < 4; ++c) {
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(count[c]), kWave - 1);
+    if (lane_id() == 0 && all) atomicAdd(&sums[c], all);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    a.chunks[(uint64_t)list * gridDim.x + blockIdx.x] = make_uint4(sums[0], sums[1], sums[2], sums[3]);
+}
+
+// What is kept, a chunk a workgroup, from the counts of the chunks before it.
+__global__ __launch_bounds__(kThreads) void paged_evict_settle_kernel(EvictArgs a) {
+  __shared__ Locate found;
+  __shared__ __attribute__((aligned(16))) uint32_t scan[2][16];
+  __shared__ uint32_t moving[kChunk], masks[kThreads];
+  __shared__ uint32_t start[3];  // ranks of the chunk's first: key at the threshold, hole, source
+  const uint32_t list = blockIdx.y;
+  const List l = list_of(a, list);
+  const uint32_t first = blockIdx.x * kChunk;
+  if (l.n == l.m || first >= l.n) return;
+  const Threshold t = threshold_of<3>(a, l, list, found);
+  if (threadIdx.x < kWave) {
+    // Keys at the threshold are kept while their rank is below t.rest; that rank follows
+    // the chunks, so a chunk keeps as many as are left of them.
+    uint32_t level = 0, kept_below = 0, kept_past = 0;
+    for (uint32_t base = 0; base < blockIdx.x; base += kWave) {
+      const uint32_t c = base + lane_id();
+      const uint4 v = c < blockIdx.x ? a.chunks[(uint64_t)list * gridDim.x + c] : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t upto = level + wave_incl_scan(v.x + v.z);
+      const uint32_t from = upto - v.x - v.z;
+      const uint32_t limit = t.ties ? t.rest : 0xffffffffu;
+      const uint32_t below = min(v.x, limit - min(limit, from));
+      const uint32_t past = min(v.z, limit - min(limit, from + v.x));
+      kept_below += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(v.y + below), kWave - 1);
+      kept_past += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(v.w + past), kWave - 1);
+      level = (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    if (threadIdx.x == 0) {
+      start[0] = level;
+      start[1] = min(first, l.m) - kept_below;
+      start[2] = kept_past;
+    }
+  }
+  __syncthreads();
+  const uint32_t at = first + threadIdx.x * kChunkEach;
+  uint32_t key[kChunkEach];
+  load_orders(a, l, list, at, key);
+  uint32_t rank = start[0], all;
+  if (t.ties) {
+    uint32_t level = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < kChunkEach; ++e) level += at + e < l.old && key[e] == t.prefix;
+    rank += block_excl_scan<16>(level, scan[0], all);
+  }
+  const uint32_t keeps = kept_of<kChunkEach>(l, t, key, at, rank);
+  const uint32_t before = block_excl_scan<16>(count_moves<kChunkEach>(l, at, keeps), scan[1], all);
+  settle<kChunkEach>(a, l, list, first, keeps, before, all, start[1], start[2], moving, masks);
+  if (threadIdx.x == 0 && first < l.m && l.m <= first + kChunk) a.counts[list] = start[1] + (all & 0xffffu);
+}
+
+// Moves of one head: 16 bytes of its key and of its value a thread, two moves at a time.
+// The first thread of a move has its scales and weight too.
+template <Store kStore, int kPieces>
 __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a) {
+  constexpr uint32_t kMoves = 256 / kPieces;  // of the workgroup at a time
+  constexpr uint32_t kBlocks = kStore == kE2M1 ? kPieces * 32 / kPowerDims : 1;  // powers of a head
+  typedef typename std::conditional<kBlocks == 8, uint2, typename std::conditional<kBlocks == 4, uint32_t, uint16_t>::type>::type Powers;
   const uint32_t list = blockIdx.y;
   const uint32_t sequence = list / a.lists;
-  const uint32_t heads = a.lists > 1u ? 1u : a.cache.kv_heads;
+  const uint32_t g = a.lists > 1u ? list % a.lists : blockIdx.z;
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
   const uint2* moves = a.moves + (uint64_t)list * a.keep;
-  const uint32_t units = 2u * a.pieces * heads;
-  const uint64_t all = (uint64_t)a.counts[list] * units;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
-    const uint2 move = moves[i / units];
-    uint32_t unit = (uint32_t)(i % units);
-    const uint32_t g = a.lists > 1u ? list % a.lists : unit / (2u * a.pieces);
-    unit %= 2u * a.pieces;
-    const bool value = unit >= a.pieces;
-    unit -= value ? a.pieces : 0u;
-    const uint32_t to = cache_row(a, pages, move.x), from = cache_row(a, pages, move.y);
-    char* base = value ? a.cache.values + g * a.cache.value_head : a.cache.keys + g * a.cache.key_head;
-    const uint64_t source = value ? a.cache.value_offset(from) : a.cache.key_offset(from);
-    const uint64_t target = value ? a.cache.value_offset(to) : a.cache.key_offset(to);
-    *reinterpret_cast<uint4*>(base + target + 16u * unit) = *reinterpret_cast<const uint4*>(base + source + 16u * unit);
-    if (unit > 0) continue;
-    if constexpr (kStore == kE4M3) {
-      float* scales = value ? a.cache.value_scales : a.cache.key_scales;
-      scales[(uint64_t)to * a.cache.kv_heads + g] = scales[(uint64_t)from * a.cache.kv_heads + g];
+  const uint32_t count = a.counts[list];
+  if (a.chunks && blockIdx.z == 0) {
+    for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < 3u * kBins; i += gridDim.x * 256u) a.bins[(uint64_t)list * 3u * kBins + i] = 0;
+    for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < count; i += gridDim.x * 256u)
+      a.kept[(uint64_t)list * a.keep + moves[i].x] = moves[i].y;
+  }
+  const uint32_t piece = threadIdx.x % kPieces;
+  char* keys = a.cache.keys + g * a.cache.key_head + 16u * piece;
+  char* values = a.cache.values + g * a.cache.value_head + 16u * piece;
+  float* weights = a.weights + g * a.row_count;
+  const uint32_t step = gridDim.x * kMoves;
+  for (uint32_t i = blockIdx.x * kMoves + threadIdx.x / kPieces; i < count; i += 2u * step) {
+    const bool both = i + step < count;
+    const uint2 move[2] = {moves[i], moves[both ? i + step : i]};
+    uint32_t to[2], from[2];
+    uint4 k[2], v[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      to[m] = cache_row(a, pages, move[m].x);
+      from[m] = cache_row(a, pages, move[m].y);
     }
-    if constexpr (kStore == kE2M1) {
-      uint8_t* powers = value ? a.cache.value_powers : a.cache.key_powers;
-      const uint64_t t = a.cache.power_offset<kPowerDims>(to, g), f = a.cache.power_offset<kPowerDims>(from, g);
-      for (uint32_t p = 0; p < a.head_powers; ++p) powers[t * a.head_powers + p] = powers[f * a.head_powers + p];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      k[m] = *reinterpret_cast<const uint4*>(keys + a.cache.key_offset(from[m]));
+      v[m] = *reinterpret_cast<const uint4*>(values + a.cache.value_offset(from[m]));
     }
-    if (!value) {
-      float* weights = a.weights + g * a.row_count;
-      weights[to] = weights[from];
-      weights[from] = 0.f;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if (m == 1 && !both) break;
+      *reinterpret_cast<uint4*>(keys + a.cache.key_offset(to[m])) = k[m];
+      *reinterpret_cast<uint4*>(values + a.cache.value_offset(to[m])) = v[m];
+      if (piece > 0) continue;
+      if constexpr (kStore == kE4M3) {
+        const uint64_t t = (uint64_t)to[m] * a.cache.kv_heads + g, f = (uint64_t)from[m] * a.cache.kv_heads + g;
+        a.cache.key_scales[t] = a.cache.key_scales[f];
+        a.cache.value_scales[t] = a.cache.value_scales[f];
+      }
+      if constexpr (kStore == kE2M1) {
+        const uint64_t t = a.cache.power_offset<kBlocks * kPowerDims>(to[m], g), f = a.cache.power_offset<kBlocks * kPowerDims>(from[m], g);
+        *reinterpret_cast<Powers*>(a.cache.key_powers + t) = *reinterpret_cast<const Powers*>(a.cache.key_powers + f);
+        *reinterpret_cast<Powers*>(a.cache.value_powers + t) = *reinterpret_cast<const Powers*>(a.cache.value_powers + f);
+      }
+      weights[to[m]] = weights[from[m]];
+      weights[from[m]] = 0.f;
     }
   }
 }
 
+template <Store kStore>
+void launch_move(const EvictArgs& a, int32_t pieces, dim3 grid, hipStream_t s) {
+  if constexpr (kStore == kE2M1) {
+    if (pieces == 2) hipLaunchKernelGGL((paged_evict_move_kernel<kStore, 2>), grid, dim3(256), 0, s, a);
+  }
+  if constexpr (kStore != k16Bit) {
+    if (pieces == 4) hipLaunchKernelGGL((paged_evict_move_kernel<kStore, 4>), grid, dim3(256), 0, s, a);
+  }
+  if (pieces == 8) hipLaunchKernelGGL((paged_evict_move_kernel<kStore, 8>), grid, dim3(256), 0, s, a);
+  if constexpr (kStore != kE2M1) {
+    if (pieces == 16) hipLaunchKernelGGL((paged_evict_move_kernel<kStore, 16>), grid, dim3(256), 0, s, a);
+  }
+  if constexpr (kStore == k16Bit) {
+    if (pieces == 32) hipLaunchKernelGGL((paged_evict_move_kernel<kStore, 32>), grid, dim3(256), 0, s, a);
+  }
+}
+
+// A list in one workgroup's LDS up to this room in the page table: 64 KiB of orders.
+constexpr int64_t kMostInLds = 16 * kThreads;
+
 struct EvictPlan {
-  int64_t lists, order_stride, bytes;
+  int64_t lists, chunks, order_stride;  // no chunks: one workgroup a list
+  int64_t bins, moves, counts, chunk_counts, bytes;  // offsets
 };
 
 EvictPlan evict_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t columns, int64_t keep, bool per_head) {
-  EvictPlan p;
+  EvictPlan p = {};
+  const int64_t capacity = columns * cache->page_size;
   p.lists = sequences * (per_head ? cache->kv_heads : 1);
-  p.order_stride = columns * cache->page_size;
-  p.bytes = p.lists * 8 * keep + p.lists * 4 * p.order_stride + p.lists * 4;
+  if (capacity > kMostInLds) {
+    p.chunks = (capacity + kChunk - 1) / kChunk;
+    p.order_stride = p.chunks * kChunk;
+  }
+  p.moves = p.lists * 3 * kBins * 4;  // kept clear of where there are no chunks: others share the workspace
+  p.counts = p.moves + p.lists * keep * 8;
+  p.chunk_counts = (p.counts + p.lists * 4 + 15) / 16 * 16;
+  p.bytes = p.chunk_counts + p.lists * p.chunks * 16 + p.lists * p.order_stride * 4;
   return p;
 }
 
@@ -278,30 +576,47 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
   a.lists = per_head ? (uint32_t)cache->kv_heads : 1u;
   a.out_lengths = out_lengths;
   a.kept = kept;
-  a.moves = static_cast<uint2*>(workspace);
-  a.order = reinterpret_cast<uint32_t*>(a.moves + p.lists * keep);
+  char* base = static_cast<char*>(workspace);
+  a.bins = reinterpret_cast<uint32_t*>(base);
+  a.moves = reinterpret_cast<uint2*>(base + p.moves);
+  a.counts = reinterpret_cast<uint32_t*>(base + p.counts);
+  a.chunks = p.chunks ? reinterpret_cast<uint4*>(base + p.chunk_counts) : nullptr;
+  a.order = reinterpret_cast<uint32_t*>(base + p.chunk_counts + p.lists * p.chunks * 16);
   a.order_stride = (uint64_t)p.order_stride;
-  a.counts = a.order + p.lists * p.order_stride;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t capacity = columns * cache->page_size;
+  const dim3 lists((unsigned)p.lists);
+  if (p.chunks) {
+    const dim3 chunks((unsigned)p.chunks, (unsigned)p.lists);
+    hipLaunchKernelGGL(paged_evict_count_kernel<0>, chunks, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(paged_evict_count_kernel<1>, chunks, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(paged_evict_count_kernel<2>, chunks, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(paged_evict_chunk_kernel, chunks, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(paged_evict_settle_kernel, chunks, dim3(kThreads), 0, s, a);
+  } else if (capacity > 8 * kThreads) {
+    hipLaunchKernelGGL(paged_evict_select_kernel<16>, lists, dim3(kThreads), 0, s, a);
+  } else if (capacity > 2 * kThreads) {
+    hipLaunchKernelGGL(paged_evict_select_kernel<8>, lists, dim3(kThreads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(paged_evict_select_kernel<2>, lists, dim3(kThreads), 0, s, a);
+  }
+  if (int st = check_launch("paged_evict_select_kernel")) return st;
+  // A list moves at most keep keys, and no more than lie past it.
+  const int64_t most = std::min(keep, capacity - keep);
+  if (most <= 0 && !p.chunks) return 0;  // (the move kernel leaves the bins zero)
   const int32_t bytes = cache->dtype == kFP4E2M1   ? cache->head_dim / 2
                         : cache->dtype == kFP8E4M3 ? cache->head_dim
                                                    : 2 * cache->head_dim;
-  a.pieces = (uint32_t)bytes / 16;
-  a.head_powers = (uint32_t)cache->head_dim / kPowerDims;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(paged_evict_select_kernel, dim3((unsigned)p.lists), dim3(kThreads), 0, s, a);
-  if (int st = check_launch("paged_evict_select_kernel")) return st;
-  // A list moves at most keep keys, and no more than lie past it.
-  const int64_t most = keep < p.order_stride - keep ? keep : p.order_stride - keep;
-  if (most <= 0) return 0;
-  const int64_t units = most * 2 * a.pieces * (per_head ? 1 : cache->kv_heads);
-  const int64_t fill = (4096 + p.lists - 1) / p.lists;
-  const int64_t blocks = (units + 255) / 256 < fill ? (units + 255) / 256 : fill;
-  const dim3 grid((unsigned)blocks, (unsigned)p.lists);
+  const int32_t pieces = bytes / 16;
+  const int64_t heads = per_head ? 1 : cache->kv_heads;
+  const int64_t fill = (4096 + p.lists * heads - 1) / (p.lists * heads);
+  const int64_t blocks = std::min((std::max(most, (int64_t)1) * pieces + 511) / 512, fill);
+  const dim3 grid((unsigned)blocks, (unsigned)p.lists, (unsigned)heads);
   if (cache->dtype == kFP4E2M1)
-    hipLaunchKernelGGL((paged_evict_move_kernel<kE2M1>), grid, dim3(256), 0, s, a);
+    launch_move<kE2M1>(a, pieces, grid, s);
   else if (cache->dtype == kFP8E4M3)
-    hipLaunchKernelGGL((paged_evict_move_kernel<kE4M3>), grid, dim3(256), 0, s, a);
+    launch_move<kE4M3>(a, pieces, grid, s);
   else
-    hipLaunchKernelGGL((paged_evict_move_kernel<k16Bit>), grid, dim3(256), 0, s, a);
+    launch_move<k16Bit>(a, pieces, grid, s);
   return check_launch("paged_evict_move_kernel");
 }

@@ -10,9 +10,10 @@
 // share them.  A lane's scores are all of one row, whose log sum is one register, and
 // the 16 lanes of a key add theirs once, at the end.
 //
-// Few rows (a decoded token) are bound by reading the keys, many by the exponentials
-// and the products.  Where the keys are too few workgroups for many rows, the rows are
-// cut into pieces, whose sums a second kernel adds in order.
+// That is the kernel of many rows, bound by the exponentials and the products.  Where
+// the keys are too few workgroups for them, the rows are cut into pieces, whose sums a
+// second kernel adds in order.  Few rows (a decoded token) are bound by reading the
+// keys: there the rows stay, in LDS, and the keys pass by, loaded a step ahead.
 #include "paged_attention.hpp"
 
 namespace dsa {
@@ -27,17 +28,30 @@ struct WeightArgs {
   float* parts;       // of several pieces: [sequences][kv_heads][pieces][tiles * keys of a tile]
   uint32_t tiles;     // of keys, of the longest sequence that the page table has room for
   uint32_t pieces;    // of each tile's rows
+  uint32_t steps;     // few rows: of a wave
   uint64_t row_count;
 };
+
+__device__ __forceinline__ float* weights_of(const WeightArgs& a, uint32_t g) { return a.weights + g * a.row_count; }
+
+// The sum over the 16 lanes of a row, in each of them.
+__device__ __forceinline__ float row16_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));  // row_ror:8
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, false));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, false));
+  return v;
+}
 
 // Adds to a weight.  (An atomic, since sequences may share a page; else each weight is
 // added to once.)
 __device__ __forceinline__ void add_weight(const WeightArgs& a, const int32_t* pages, uint32_t g, uint32_t key, float v) {
-  float* to = a.weights + g * a.row_count + cache_row(a.batch, pages, key);
-  __hip_atomic_fetch_add(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_fetch_add(weights_of(a, g) + cache_row(a.batch, pages, key), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <class Tag, Store kStore, int D, int kSets>
+constexpr int kSets = 4;  // of 16 keys, of a wave
+
+template <class Tag, Store kStore, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(WeightArgs w) {
   const PagedAttentionArgs& a = w.batch;
   constexpr bool kFp8 = kStore == kE4M3;
@@ -121,7 +135,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
       }
     }
 
-    uint4 staged[kLoads];
+    u32x4 staged[kLoads];
     float2 staged_of;
     auto load = [&](uint32_t r0) {
 #pragma unroll
@@ -129,7 +143,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
         const uint32_t at = tid + 256u * i;
         const uint32_t r = min(r0 + at / kRuns, end - 1u);
         const uint64_t token = span.first + first + r / a.group;
-        staged[i] = *reinterpret_cast<const uint4*>(a.queries + (int64_t)token * a.query_stride +
+        staged[i] = *reinterpret_cast<const u32x4*>(a.queries + (int64_t)token * a.query_stride +
                                                     ((uint64_t)(g * a.group + r % a.group) * D + at % kRuns * 8u) * 2u);
       }
       if (tid < kStage) {
@@ -144,7 +158,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
 #pragma unroll
       for (uint32_t i = 0; i < kLoads; ++i) {
         const uint32_t at = tid + 256u * i;
-        *reinterpret_cast<uint4*>(rows_tile[slot] + at / kRuns * kRow + at % kRuns * 16u) = staged[i];
+        *reinterpret_cast<u32x4*>(rows_tile[slot] + at / kRuns * kRow + at % kRuns * 16u) = staged[i];
       }
       if (tid < kStage) row_of[slot][tid] = staged_of;
     };
@@ -190,9 +204,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
 #pragma unroll
   for (int s = 0; s < kSets; ++s) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) sum[s][i] += __shfl_xor(sum[s][i], off, kWave);
+    for (int i = 0; i < 4; ++i) sum[s][i] = row16_sum(sum[s][i]);
     if (col < 4u) {
       const float v = col == 0 ? sum[s][0] : col == 1 ? sum[s][1] : col == 2 ? sum[s][2] : sum[s][3];
       const uint32_t key = key0 + 16u * s + 4u * quad + col;
@@ -201,6 +213,168 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
       } else if (key < length && begin < end) {
         add_weight(w, pages, g, key, v);
       }
+    }
+  }
+}
+
+// Few rows: kStage of a sequence lie in LDS while its keys pass by, 32 a wave and step,
+// loaded a step ahead as 128 neighbouring bytes by eight lanes, through LDS of the
+// wave's own.  A workgroup takes w.steps steps of each of its four waves.
+template <class Tag, Store kStore, int D>
+__global__ __launch_bounds__(256, D < 256 ? 3 : kStore == k16Bit ? 1 : 2) void paged_weights_few_kernel(WeightArgs w) {
+  const PagedAttentionArgs& a = w.batch;
+  constexpr bool kFp8 = kStore == kE4M3;
+  constexpr bool kFp4 = kStore == kE2M1;
+  constexpr int kQ = D / 32;
+  constexpr uint32_t kStep = 32;
+  constexpr uint32_t kRow = 2 * D + 16;                       // bytes of a row in LDS
+  constexpr uint32_t kRuns = D / 8;
+  constexpr int kBytes = kRowBytes<kStore, D>;                // of a key
+  constexpr uint32_t kLanes = kBytes < 128 ? kBytes / 16 : 8;  // that share one
+  constexpr uint32_t kRows = 64 / kLanes;                     // of one load
+  constexpr int kPasses = kStep / kRows;
+  constexpr int kLoads = kBytes / (16 * kLanes);              // of one key
+  constexpr uint32_t kKeyRow = kBytes + 16;
+  __shared__ __attribute__((aligned(16))) char rows_tile[kStage * kRow];
+  __shared__ float2 row_of[kStage];
+  __shared__ __attribute__((aligned(16))) char key_tile[4][kStep * kKeyRow];
+  const uint32_t tid = threadIdx.x, lane = lane_id(), wave = tid / kWave, col = lane & 15u, quad = lane >> 4;
+
+  uint32_t id = blockIdx.x;
+  const uint32_t g = id % a.cache.kv_heads;
+  id /= a.cache.kv_heads;
+  const uint32_t sequence = id % a.sequences;
+  const uint32_t length = keys_of(a, sequence);
+  const uint32_t tile0 = id / a.sequences * (4u * kStep * w.steps);
+  if (tile0 >= length) return;
+  const Span span = tokens_of(a, sequence);
+  const int64_t before = (int64_t)length - span.count;
+  const uint32_t rows = span.count * a.group;
+  const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
+  const uint32_t steps = min(w.steps, (length - tile0 + 4u * kStep - 1u) / (4u * kStep));
+  const uint32_t load_row = lane / kLanes, load_chunk = lane % kLanes;
+  const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * load_chunk;
+  auto first_key = [&](uint32_t step) { return tile0 + (4u * step + wave) * kStep; };
+
+  struct Tile {
+    u32x4 k[kPasses][kLoads];
+    float scale;       // e4m3: of key `lane`
+    uint32_t page;     // of key `lane` of the step after
+  };
+  auto look = [&](uint32_t step) { return (uint32_t)pages[min(first_key(step) + (lane & 31u), length - 1u) >> a.cache.shift]; };
+  auto row_at = [&](uint32_t step, uint32_t page) {
+    const uint32_t key = min(first_key(step) + (lane & 31u), length - 1u);
+    return (min(page, a.cache.pages - 1u) << a.cache.shift) | (key & ((1u << a.cache.shift) - 1u));
+  };
+  // `row`: the cache row of key `lane` of the step.
+  auto load = [&](Tile& t, uint32_t row) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const uint32_t r = (uint32_t)__shfl((int)row, kRows * i + load_row, kWave);
+      const char* from = key_base + a.cache.key_offset(r);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) t.k[i][j] = *reinterpret_cast<const u32x4*>(from + 16 * kLanes * j);
+    }
+    if constexpr (kFp8) t.scale = a.cache.key_scales[(uint64_t)row * a.cache.kv_heads + g];
+  };
+
+  for (uint32_t r0 = 0; r0 < rows; r0 += kStage) {
+    const uint32_t live = min(kStage, rows - r0);
+    uint32_t row = row_at(0, look(0));
+    uint32_t page = look(1u);
+    Tile t;
+    load(t, row);
+    if (r0 > 0) __syncthreads();
+    for (uint32_t at = tid; at < live * kRuns; at += 256u) {
+      const uint32_t r = r0 + at / kRuns;
+      const uint64_t token = span.first + r / a.group;
+      *reinterpret_cast<uint4*>(rows_tile + at / kRuns * kRow + at % kRuns * 16u) =
+          *reinterpret_cast<const uint4*>(a.queries + (int64_t)token * a.query_stride +
+                                          ((uint64_t)(g * a.group + r % a.group) * D + at % kRuns * 8u) * 2u);
+    }
+    if (tid < kStage) {
+      const uint32_t r = min(r0 + tid, rows - 1u);
+      const uint32_t i = r / a.group;
+      const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
+      const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r % a.group];
+      row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(r0 + tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
+    }
+    __syncthreads();
+    for (uint32_t step = 0; step < steps; ++step) {
+      const uint32_t key0 = first_key(step);
+      char* mine = key_tile[wave];
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j)
+          *reinterpret_cast<u32x4*>(mine + (kRows * i + load_row) * kKeyRow + (kLanes * j + load_chunk) * 16u) = t.k[i][j];
+      const uint32_t now = row;
+      const float scale = kFp8 ? t.scale * a.scale : a.scale;
+      wave_order();
+      row = row_at(step + 1u, page);  // past the end: the last key again
+      load(t, row);
+      page = look(step + 2u);
+      __builtin_amdgcn_sched_barrier(0);
+      uint4 k[2][kQ];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const char* key = mine + (16u * h + col) * kKeyRow;
+        if constexpr (kFp4) {
+          const uint32_t of = (uint32_t)__shfl((int)now, 16 * h + col, kWave);
+          const uint8_t* powers = a.cache.key_powers + a.cache.power_offset<D>(of, g);
+#pragma unroll
+          for (int j = 0; j < kQ; ++j)
+            k[h][j] = fp4x8_to_bf16x8(*reinterpret_cast<const uint32_t*>(key + D / 8u * quad + 4u * j),
+                                      power_of(powers[(D / 4u * quad + 8u * j) / kPowerDims]));
+        } else if constexpr (kFp8) {
+#pragma unroll
+          for (int j = 0; j < kQ / 2; ++j) {
+            const uint4 v = *reinterpret_cast<const uint4*>(key + 64u * j + 16u * quad);
+            k[h][2 * j] = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
+            k[h][2 * j + 1] = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kQ; ++j) k[h][j] = *reinterpret_cast<const uint4*>(key + 64u * j + 16u * quad);
+        }
+      }
+      float by[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) by[e] = kFp8 ? __shfl(scale, 16 * (e / 4) + 4 * quad + e % 4, kWave) : a.scale;
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (uint32_t sub = 0; sub < live; sub += 16u) {
+        const char* from = rows_tile + (sub + col) * kRow;
+        const float2 of = row_of[sub + col];
+        const uint32_t sees = __float_as_uint(of.y);
+        floatx4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int j = 0; j < kQ; ++j) {
+          const uint32_t d = kFp4   ? D / 4u * quad + 8u * j
+                             : kFp8 ? 64u * (j / 2) + 16u * quad + 8u * (j % 2)
+                                    : 32u * j + 8u * quad;
+          const uint4 q = *reinterpret_cast<const uint4*>(from + 2u * d);
+          x[0] = mfma_16x16x32(Tag{}, k[0][j], q, x[0]);
+          x[1] = mfma_16x16x32(Tag{}, k[1][j], q, x[1]);
+        }
+        const bool partly = __any(sees < key0 + kStep);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float p = exp2_fast(fmaf(x[e / 4][e % 4], by[e], -of.x));
+          if (partly) p = key0 + 16u * (e / 4) + 4u * quad + e % 4 < sees ? p : 0.f;
+          sum[e] += p;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = row16_sum(sum[e]);
+      const uint32_t of = 16u * (col % 8u / 4u) + 4u * quad + col % 4u;  // the key that this lane adds to
+      const uint32_t to = (uint32_t)__shfl((int)now, of, kWave);  // (every lane takes part: an idle one would give 0)
+      if (col < 8u) {
+        float v = sum[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) v = col == (uint32_t)e ? sum[e] : v;
+        if (key0 + of < length) __hip_atomic_fetch_add(weights_of(w, g) + to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      wave_order();
     }
   }
 }
@@ -218,46 +392,50 @@ __global__ __launch_bounds__(256) void paged_weights_join_kernel(WeightArgs w, u
 }
 
 struct WeightPlan {
-  int sets;
-  int64_t tiles, pieces, part_bytes;
+  bool few;
+  int64_t tiles, steps, pieces, part_bytes;
 };
 
 WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens, int64_t heads, int64_t capacity,
                        bool uniform) {
   const int64_t group = heads / cache->kv_heads;
-  const int64_t rows = (uniform ? tokens / sequences : tokens) * group;  // of a sequence, at most
   WeightPlan p = {};
-  const int64_t wide = (capacity + 255) / 256 * cache->kv_heads * sequences;
-  p.sets = rows <= 64 && wide < 512 ? 1 : 4;
-  p.tiles = (capacity + 64 * p.sets - 1) / (64 * p.sets);
-  const int64_t most = (rows + 4 * kStage - 1) / (4 * kStage);
-  p.pieces = (kManyWorkgroups + wide - 1) / wide;
-  if (p.pieces > most) p.pieces = most;
-  if (p.pieces < 1) p.pieces = 1;
-  if (p.pieces > 1) p.part_bytes = sequences * cache->kv_heads * p.pieces * p.tiles * 64 * p.sets * 4;
+  p.few = tokens * group <= kStage * sequences;
+  const int64_t keys = p.few ? 128 : 64 * kSets;  // of a tile, at least
+  p.tiles = (capacity + keys - 1) / keys;
+  const int64_t wide = p.tiles * cache->kv_heads * sequences;
+  p.pieces = 1;
+  if (p.few) {
+    // Steps that leave the GPU some rounds of workgroups, up to what hides a start.
+    p.steps = wide / kManyWorkgroups;
+    p.steps = p.steps < 1 ? 1 : p.steps > 32 ? 32 : p.steps;
+    p.tiles = (p.tiles + p.steps - 1) / p.steps;
+  } else {
+    const int64_t rows = (uniform ? tokens / sequences : tokens) * group;  // of a sequence, at most
+    const int64_t most = (rows + 4 * kStage - 1) / (4 * kStage);
+    const int64_t pieces = (kManyWorkgroups + wide - 1) / wide;
+    p.pieces = pieces < most ? pieces : most;
+    if (p.pieces > 1) p.part_bytes = sequences * cache->kv_heads * p.pieces * p.tiles * keys * 4;
+  }
   return p;
 }
 
-template <class Tag, Store kStore, int kSets>
-void launch_weights(const WeightArgs& w, int32_t dim, uint32_t grid, hipStream_t s) {
-  if (dim == 64)
-    hipLaunchKernelGGL((paged_weights_kernel<Tag, kStore, 64, kSets>), dim3(grid), dim3(256), 0, s, w);
-  else if (dim == 128)
-    hipLaunchKernelGGL((paged_weights_kernel<Tag, kStore, 128, kSets>), dim3(grid), dim3(256), 0, s, w);
+template <class Tag, Store kStore, int D>
+void launch_dim(const WeightArgs& w, uint32_t grid, hipStream_t s) {
+  if (w.steps)
+    hipLaunchKernelGGL((paged_weights_few_kernel<Tag, kStore, D>), dim3(grid), dim3(256), 0, s, w);
   else
-    hipLaunchKernelGGL((paged_weights_kernel<Tag, kStore, 256, kSets>), dim3(grid), dim3(256), 0, s, w);
+    hipLaunchKernelGGL((paged_weights_kernel<Tag, kStore, D>), dim3(grid), dim3(256), 0, s, w);
 }
 
-template <int kSets>
-void launch_weights(const WeightArgs& w, const dsa_paged_cache* cache, uint32_t grid, hipStream_t s) {
-  if (cache->dtype == kFP4E2M1)
-    launch_weights<Bf16Tag, kE2M1, kSets>(w, cache->head_dim, grid, s);
-  else if (cache->dtype == kFP8E4M3)
-    launch_weights<Bf16Tag, kE4M3, kSets>(w, cache->head_dim, grid, s);
-  else if (cache->dtype == kBF16)
-    launch_weights<Bf16Tag, k16Bit, kSets>(w, cache->head_dim, grid, s);
+template <class Tag, Store kStore>
+void launch_weights(const WeightArgs& w, int32_t dim, uint32_t grid, hipStream_t s) {
+  if (dim == 64)
+    launch_dim<Tag, kStore, 64>(w, grid, s);
+  else if (dim == 128)
+    launch_dim<Tag, kStore, 128>(w, grid, s);
   else
-    launch_weights<F16Tag, k16Bit, kSets>(w, cache->head_dim, grid, s);
+    launch_dim<Tag, kStore, 256>(w, grid, s);
 }
 
 }  // namespace
@@ -295,17 +473,22 @@ extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queri
   w.parts = static_cast<float*>(workspace);
   w.tiles = (uint32_t)p.tiles;
   w.pieces = (uint32_t)p.pieces;
+  w.steps = (uint32_t)p.steps;
   w.row_count = (uint64_t)cache->pages * cache->page_size;
   const int64_t grid = p.tiles * sequences * p.pieces * cache->kv_heads;
   DSA_REQUIRE(grid < (1LL << 24), "too many keys for one call");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p.sets == 1)
-    launch_weights<1>(w, cache, (uint32_t)grid, s);
+  if (cache->dtype == kFP4E2M1)
+    launch_weights<Bf16Tag, kE2M1>(w, cache->head_dim, (uint32_t)grid, s);
+  else if (cache->dtype == kFP8E4M3)
+    launch_weights<Bf16Tag, kE4M3>(w, cache->head_dim, (uint32_t)grid, s);
+  else if (cache->dtype == kBF16)
+    launch_weights<Bf16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, s);
   else
-    launch_weights<4>(w, cache, (uint32_t)grid, s);
+    launch_weights<F16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, s);
   if (int st = check_launch("paged_weights_kernel")) return st;
   if (p.pieces == 1) return 0;
-  const uint32_t keys = (uint32_t)(p.tiles * 64 * p.sets);
+  const uint32_t keys = (uint32_t)(p.tiles * 64 * kSets);
   DSA_REQUIRE(sequences < 65536, "too many sequences for one call");
   const dim3 join((keys + 255) / 256, (unsigned)cache->kv_heads, (unsigned)sequences);
   hipLaunchKernelGGL(paged_weights_join_kernel, join, dim3(256), 0, s, w, keys);

@@ -75,7 +75,7 @@ def accumulate_weights(
     lse = lse.contiguous()
     stream = _lib.stream_of(queries)
     ws, need = cache._workspace(stream, "dsa_paged_weights_workspace_bytes", sequences, tokens, heads, columns,
-                                starts is None, kind="paged_weights")
+                                starts is None, kind="paged_weights", zeroed_rows=None)
     _lib.call("dsa_paged_weights", cache._address, queries.data_ptr(), query_stride, page_table.data_ptr(), table_stride,
               columns, lengths.data_ptr(), _lib.ptr(starts), sequences, tokens, heads, cache._code,
               cache.head_dim**-0.5 if scale is None else scale, causal, lse.data_ptr(), weights.data_ptr(), ws, need,
@@ -109,8 +109,6 @@ def evict(
     """
 
     weights = _weights(weights, cache)
-    if page_table.ndim != 2:
-        raise ValueError("page_table must be [sequences,columns]")
     page_table, sequences, columns, table_stride, lengths, _ = _batch(0, cache, page_table, lengths, None)
     if isinstance(keep, bool) or not isinstance(keep, int) or not 0 < keep <= 1 << 30:
         raise ValueError("keep must be a positive integer")
@@ -120,8 +118,9 @@ def evict(
     kept = torch.empty((sequences, cache.kv_heads, keep) if per_head else (sequences, keep), dtype=torch.int64,
                        device=cache.device)
     stream = _lib.stream_of(weights)
+    lists = sequences * (cache.kv_heads if per_head else 1)
     ws, need = cache._workspace(stream, "dsa_paged_evict_workspace_bytes", sequences, columns, keep, bool(per_head),
-                                kind="paged_evict")
+                                kind="paged_evict", zeroed_rows=lists)
     _lib.call("dsa_paged_evict", cache._address, page_table.data_ptr(), table_stride, columns, lengths.data_ptr(),
               sequences, weights.data_ptr(), keep, recent, bool(per_head), out.data_ptr(), kept.data_ptr(), ws, need,
               stream)

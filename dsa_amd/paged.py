@@ -104,9 +104,10 @@ class PagedCache:
     def rows(self) -> int:
         return self.pages * self.page_size
 
-    def _workspace(self, stream: int, entry: str, *sizes: int, kind: str = "paged_attention") -> tuple[int | None, int]:
-        """Address and size of the workspace that ``entry`` asks for at these sizes.  The
-        attentions' is zeroed once."""
+    def _workspace(self, stream: int, entry: str, *sizes: int, kind: str = "paged_attention",
+                   zeroed_rows: int | None = 0) -> tuple[int | None, int]:
+        """Address and size of the workspace that ``entry`` asks for at these sizes;
+        ``zeroed_rows`` as :func:`dsa_amd._lib.workspace`'s rows, None if it needs no zeros."""
 
         need = self._needs.get((entry, sizes))
         if need is None:
@@ -115,7 +116,8 @@ class PagedCache:
             need = self._needs[entry, sizes] = _lib.query(entry, self._address, *sizes)
         if need <= 0:
             return None, 0
-        return _lib.workspace(kind, self.device, stream, need, zeroed=kind == "paged_attention").data_ptr(), need
+        return _lib.workspace(kind, self.device, stream, need, zeroed=zeroed_rows is not None,
+                              rows=zeroed_rows or 0).data_ptr(), need
 
 
 def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, dtype: torch.dtype = torch.bfloat16,

@@ -960,7 +960,9 @@ int dsa_paged_weights(const dsa_paged_cache* cache, const void* queries, int64_t
  * positions m .. n become 0.  out_lengths[s] = m; kept [sequences][kv_heads if
  * per_head else 1][keep] is the former position of the key now at each position, -1
  * from m on.  No other byte of the cache is written.  A page may be of one
- * sequence alone.  Workspace (16-byte aligned): the bytes of the query. */
+ * sequence alone.  Workspace (16-byte aligned): the bytes of the query; its first
+ * 24576 per list (sequences, times kv_heads if per_head) are zero before the first
+ * call, and every call of as many lists leaves them so. */
 int64_t dsa_paged_evict_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t columns, int64_t keep,
                                         int32_t per_head);
 int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t columns,

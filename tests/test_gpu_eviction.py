@@ -164,6 +164,9 @@ def _check_eviction(device, c, weights, keep, recent, per_head) -> None:
     ([5000, 4097, 4096], 2, 64, 32, FP4, 4000, 77, "paged"),
     ([9000], 3, 128, 16, FP4, 700, 5, "rows"),
     ([333, 20], 8, 256, 4, FP4, 332, 0, "wide"),
+    ([20000, 100, 16385], 2, 64, 64, BF16, 9000, 50, "nhd"),     # lists of several workgroups
+    ([40001], 3, 64, 16, FP4, 8192, 8192, "paged"),
+    ([17000, 5], 1, 128, 256, FP8, 16999, 1, "hnd"),
     ([400], 8, 128, 16, BF16, 500, 3, "nhd"),        # nothing to evict
 ])
 def test_evict(device, lengths, kv_heads, dim, page, dtype, keep, recent, layout, per_head) -> None:
@@ -175,12 +178,13 @@ def test_evict(device, lengths, kv_heads, dim, page, dtype, keep, recent, layout
 
 
 @pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("n", [6001, 25003])
 @pytest.mark.parametrize("kind", ["ties", "zeros", "nan", "signs", "infinite", "near", "rising", "falling"])
-def test_evict_by_any_weights(device, kind, per_head) -> None:
+def test_evict_by_any_weights(device, kind, n, per_head) -> None:
     """Ties go to the lowest position, also where nothing has any weight; keys whose
     sums overflow or are NaN have their place too."""
 
-    n, kv_heads = 6001, 3
+    kv_heads = 3
     c = _case(device, 4, [n, 100], [0, 0], kv_heads, kv_heads, 64, 16, BF16)
     gen = torch.Generator().manual_seed(5)
     shape = (kv_heads, c.cache.rows)
@@ -204,7 +208,7 @@ def test_evict_by_any_weights(device, kind, per_head) -> None:
         rows = paged.cache_rows(c.cache, c.table, torch.arange(n), torch.zeros(n, dtype=torch.int64))
         at[rows] = torch.arange(n).float()
         weights = (at if kind == "rising" else -at).expand(shape).contiguous()
-    for keep, recent in ((1000, 17), (1, 0), (n - 1, 2), (4096, 4096)):
+    for keep, recent in ((1000, 17), (1, 0), (n - 1, 2), (4096, 4096), (2 * n // 3, 0)):
         _check_eviction(device, c, weights.to(device), keep, recent, per_head)
 
 
