@@ -91,14 +91,26 @@ __device__ __forceinline__ void orders_of(const EvictArgs& a, const List& l, uin
 #pragma unroll
     for (uint32_t e = 0; e < kEach; ++e) key[e] = order_of(a.weights[l.g * a.row_count + row[e]]);
   } else {
-    double sum[kEach];
+    // eight heads of four positions under way at a time: a head after the other waits
+    // for memory as often as there are heads
+    constexpr int kTogether = kEach < 4 ? kEach : 4;
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) sum[e] = 0.0;
-    for (uint32_t h = 0; h < a.cache.kv_heads; ++h)
+    for (uint32_t e = 0; e < kEach; e += kTogether) {
+      double sum[kTogether] = {};
+      for (uint32_t h0 = 0; h0 < a.cache.kv_heads; h0 += 8u) {
+        float w[8][kTogether];
 #pragma unroll
-      for (uint32_t e = 0; e < kEach; ++e) sum[e] += (double)a.weights[h * a.row_count + row[e]];
+        for (uint32_t h = 0; h < 8; ++h)
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) key[e] = order_of((float)sum[e]);
+          for (int i = 0; i < kTogether; ++i) w[h][i] = a.weights[min(h0 + h, a.cache.kv_heads - 1u) * a.row_count + row[e + i]];
+#pragma unroll
+        for (uint32_t h = 0; h < 8; ++h)
+#pragma unroll
+          for (int i = 0; i < kTogether; ++i) sum[i] += h0 + h < a.cache.kv_heads ? (double)w[h][i] : 0.0;
+      }
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) key[e + i] = order_of((float)sum[i]);
+    }
   }
 #pragma unroll
   for (uint32_t e = 0; e < kEach; ++e) key[e] = first + stride * e < l.old ? key[e] : 0u;
@@ -113,17 +125,16 @@ struct Threshold {
 constexpr uint32_t kShift[3] = {21u, 10u, 0u};  // of each pass's digit
 constexpr uint32_t kBins = 2048;
 
-// Counts a lane's bin; the lanes that share the first one's are one addition (a list of
-// zeros counts one bin).
+// Counts a lane's bin; a wave whose lanes share one (a list of zeros) adds once.
 __device__ __forceinline__ void count_bin(uint32_t* bins, uint32_t bin, bool counts) {
   const uint64_t all = __ballot(counts);
   if (!all) return;
   const uint32_t leader = (uint32_t)__builtin_ctzll(all);
-  const uint64_t same = __ballot(counts && bin == (uint32_t)__builtin_amdgcn_readlane(bin, leader));
-  if (lane_id() == leader)
-    atomicAdd(&bins[bin], (uint32_t)__popcll(same));
-  else if (counts && !(same >> lane_id() & 1u))
+  if (__ballot(counts && bin == (uint32_t)__builtin_amdgcn_readlane(bin, leader)) == all) {
+    if (lane_id() == leader) atomicAdd(&bins[bin], (uint32_t)__popcll(all));
+  } else if (counts) {
     atomicAdd(&bins[bin], 1u);
+  }
 }
 
 // The digit of `pass` added to the threshold.
@@ -240,11 +251,17 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
   if (l.n == l.m) return;
   for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
   uint32_t key[kEach];
-  orders_of<kEach>(a, l, tid, kThreads, key);
+  // (eight at a time, which leaves the registers of 1024 threads room)
+  constexpr uint32_t kPart = kEach < 8 ? kEach : 8;
+#pragma unroll 1
+  for (uint32_t e0 = 0; e0 < kEach; e0 += kPart) {
+    uint32_t part[kPart];
+    orders_of<kPart>(a, l, tid + kThreads * e0, kThreads, part);
 #pragma unroll
-  for (uint32_t e = 0; e < kEach; ++e) {
-    const uint32_t i = tid + kThreads * e;
-    order[i / kEach * (kEach + 1) + i % kEach] = key[e];
+    for (uint32_t e = 0; e < kPart; ++e) {
+      const uint32_t i = tid + kThreads * (e0 + e);
+      order[i / kEach * (kEach + 1) + i % kEach] = part[e];
+    }
   }
   __syncthreads();
   const uint32_t at = tid * kEach;
@@ -264,10 +281,11 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
       }
       __syncthreads();
       locate_digit(bins, pass, found, t);
+      if (!t.ties) break;  // every key with these digits is kept: the least that they can stand for is the threshold
     }
   }
   uint32_t rank = 0, all;
-  if (t.ties) {
+  if (t.ties) {  // keys of equal weight, of which some are kept
     uint32_t level = 0;
 #pragma unroll
     for (uint32_t e = 0; e < kEach; ++e) level += at + e < l.old && key[e] == t.prefix;
@@ -437,34 +455,54 @@ __global__ __launch_bounds__(kThreads) void paged_evict_settle_kernel(EvictArgs 
   if (threadIdx.x == 0 && first < l.m && l.m <= first + kChunk) a.counts[list] = start[1] + (all & 0xffffu);
 }
 
-// Moves of one head: 16 bytes of its key and of its value a thread, two moves at a time.
-// The first thread of a move has its scales and weight too.
+// Moves: 16 bytes of a head's key and of its value a thread, two at a time; a move's
+// heads are neighbouring threads, so that what heads share, a row's scales in one cache
+// line, is written by one workgroup (with a workgroup a head 7800 moves of 8 fp8 heads
+// took 20 us, and 8 so).  The first thread of a head has its scales and weight too.
 template <Store kStore, int kPieces>
 __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a) {
-  constexpr uint32_t kMoves = 256 / kPieces;  // of the workgroup at a time
+  constexpr uint32_t kPairs = 256 / kPieces;  // of a move and a head, of the workgroup at a time
   constexpr uint32_t kBlocks = kStore == kE2M1 ? kPieces * 32 / kPowerDims : 1;  // powers of a head
-  typedef typename std::conditional<kBlocks == 8, uint2, typename std::conditional<kBlocks == 4, uint32_t, uint16_t>::type>::type Powers;
+  typedef typename std::conditional<kBlocks == 8, uint64_t, typename std::conditional<kBlocks == 4, uint32_t, uint16_t>::type>::type Powers;
   const uint32_t list = blockIdx.y;
   const uint32_t sequence = list / a.lists;
-  const uint32_t g = a.lists > 1u ? list % a.lists : blockIdx.z;
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
   const uint2* moves = a.moves + (uint64_t)list * a.keep;
   const uint32_t count = a.counts[list];
-  if (a.chunks && blockIdx.z == 0) {
+  if (a.chunks) {
     for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < 3u * kBins; i += gridDim.x * 256u) a.bins[(uint64_t)list * 3u * kBins + i] = 0;
     for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < count; i += gridDim.x * 256u)
       a.kept[(uint64_t)list * a.keep + moves[i].x] = moves[i].y;
   }
   const uint32_t piece = threadIdx.x % kPieces;
-  char* keys = a.cache.keys + g * a.cache.key_head + 16u * piece;
-  char* values = a.cache.values + g * a.cache.value_head + 16u * piece;
-  float* weights = a.weights + g * a.row_count;
-  const uint32_t step = gridDim.x * kMoves;
-  for (uint32_t i = blockIdx.x * kMoves + threadIdx.x / kPieces; i < count; i += 2u * step) {
-    const bool both = i + step < count;
-    const uint2 move[2] = {moves[i], moves[both ? i + step : i]};
+  const uint32_t heads = a.lists > 1u ? 1u : a.cache.kv_heads;
+  const uint32_t step = gridDim.x * kPairs;
+  const uint32_t pair = blockIdx.x * kPairs + threadIdx.x / kPieces;  // (the grid is small: both fit)
+  uint32_t i = pair / heads, h = pair % heads;
+  auto next = [&]() {
+    i += step / heads;
+    h += step % heads;
+    if (h >= heads) {
+      h -= heads;
+      ++i;
+    }
+  };
+  while (i < count) {
+    u32x2 move[2];
+    uint32_t g[2];
+    move[0] = *reinterpret_cast<const u32x2*>(moves + i);
+    g[0] = a.lists > 1u ? list % a.lists : h;
+    next();
+    const bool both = i < count;
+    move[1] = *reinterpret_cast<const u32x2*>(moves + (both ? i : count - 1u));
+    g[1] = a.lists > 1u ? list % a.lists : h;
+    next();
     uint32_t to[2], from[2];
-    uint4 k[2], v[2];
+    char *keys[2], *values[2];
+    float* weights[2];
+    u32x4 k[2], v[2];
+    float weight[2], key_scale[2], value_scale[2];
+    Powers key_powers[2], value_powers[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       to[m] = cache_row(a, pages, move[m].x);
@@ -472,27 +510,42 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a) {
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      k[m] = *reinterpret_cast<const uint4*>(keys + a.cache.key_offset(from[m]));
-      v[m] = *reinterpret_cast<const uint4*>(values + a.cache.value_offset(from[m]));
+      keys[m] = a.cache.keys + g[m] * a.cache.key_head + 16u * piece;
+      values[m] = a.cache.values + g[m] * a.cache.value_head + 16u * piece;
+      weights[m] = a.weights + g[m] * a.row_count;
+      k[m] = *reinterpret_cast<const u32x4*>(keys[m] + a.cache.key_offset(from[m]));
+      v[m] = *reinterpret_cast<const u32x4*>(values[m] + a.cache.value_offset(from[m]));
+      if (piece > 0) continue;
+      weight[m] = weights[m][from[m]];
+      if constexpr (kStore == kE4M3) {
+        const uint64_t f = (uint64_t)from[m] * a.cache.kv_heads + g[m];
+        key_scale[m] = a.cache.key_scales[f];
+        value_scale[m] = a.cache.value_scales[f];
+      }
+      if constexpr (kStore == kE2M1) {
+        const uint64_t f = a.cache.power_offset<kBlocks * kPowerDims>(from[m], g[m]);
+        key_powers[m] = *reinterpret_cast<const Powers*>(a.cache.key_powers + f);
+        value_powers[m] = *reinterpret_cast<const Powers*>(a.cache.value_powers + f);
+      }
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       if (m == 1 && !both) break;
-      *reinterpret_cast<uint4*>(keys + a.cache.key_offset(to[m])) = k[m];
-      *reinterpret_cast<uint4*>(values + a.cache.value_offset(to[m])) = v[m];
+      *reinterpret_cast<u32x4*>(keys[m] + a.cache.key_offset(to[m])) = k[m];
+      *reinterpret_cast<u32x4*>(values[m] + a.cache.value_offset(to[m])) = v[m];
       if (piece > 0) continue;
+      weights[m][to[m]] = weight[m];
+      weights[m][from[m]] = 0.f;
       if constexpr (kStore == kE4M3) {
-        const uint64_t t = (uint64_t)to[m] * a.cache.kv_heads + g, f = (uint64_t)from[m] * a.cache.kv_heads + g;
-        a.cache.key_scales[t] = a.cache.key_scales[f];
-        a.cache.value_scales[t] = a.cache.value_scales[f];
+        const uint64_t t = (uint64_t)to[m] * a.cache.kv_heads + g[m];
+        a.cache.key_scales[t] = key_scale[m];
+        a.cache.value_scales[t] = value_scale[m];
       }
       if constexpr (kStore == kE2M1) {
-        const uint64_t t = a.cache.power_offset<kBlocks * kPowerDims>(to[m], g), f = a.cache.power_offset<kBlocks * kPowerDims>(from[m], g);
-        *reinterpret_cast<Powers*>(a.cache.key_powers + t) = *reinterpret_cast<const Powers*>(a.cache.key_powers + f);
-        *reinterpret_cast<Powers*>(a.cache.value_powers + t) = *reinterpret_cast<const Powers*>(a.cache.value_powers + f);
+        const uint64_t t = a.cache.power_offset<kBlocks * kPowerDims>(to[m], g[m]);
+        *reinterpret_cast<Powers*>(a.cache.key_powers + t) = key_powers[m];
+        *reinterpret_cast<Powers*>(a.cache.value_powers + t) = value_powers[m];
       }
-      weights[to[m]] = weights[from[m]];
-      weights[from[m]] = 0.f;
     }
   }
 }
@@ -609,9 +662,9 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
                                                    : 2 * cache->head_dim;
   const int32_t pieces = bytes / 16;
   const int64_t heads = per_head ? 1 : cache->kv_heads;
-  const int64_t fill = (4096 + p.lists * heads - 1) / (p.lists * heads);
-  const int64_t blocks = std::min((std::max(most, (int64_t)1) * pieces + 511) / 512, fill);
-  const dim3 grid((unsigned)blocks, (unsigned)p.lists, (unsigned)heads);
+  const int64_t fill = (4096 + p.lists - 1) / p.lists;
+  const int64_t blocks = std::min((std::max(most, (int64_t)1) * heads * pieces + 511) / 512, fill);
+  const dim3 grid((unsigned)blocks, (unsigned)p.lists);
   if (cache->dtype == kFP4E2M1)
     launch_move<kE2M1>(a, pieces, grid, s);
   else if (cache->dtype == kFP8E4M3)

@@ -14,16 +14,31 @@
 // the keys are too few workgroups for them, the rows are cut into pieces, whose sums a
 // second kernel adds in order.  Few rows (a decoded token) are bound by reading the
 // keys: there the rows stay, in LDS, and the keys pass by, loaded a step ahead.
+#include <algorithm>
+
 #include "paged_attention.hpp"
 
 namespace dsa {
 namespace {
 
 constexpr uint32_t kStage = 64;  // rows in LDS at a time
-constexpr int64_t kManyWorkgroups = 2048;  // that rows are cut for: about four rounds of what runs at a time
+constexpr int64_t kManyWorkgroups = 2048;  // that the work is dealt to, where there is as much
+
+// Quotients of numbers below 2^31 by one divisor: a product and a shift.
+struct Quotient {
+  uint32_t factor, shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)((uint64_t)x * factor >> shift); }
+};
+
+Quotient quotient_by(uint32_t divisor) {
+  uint32_t shift = 31;
+  while ((1ull << (shift - 31)) < divisor) ++shift;
+  return {(uint32_t)(((1ull << shift) + divisor - 1) / divisor), shift};
+}
 
 struct WeightArgs {
   PagedAttentionArgs batch;
+  Quotient by_group;  // of a row: its token
   float* weights;     // [kv_heads][cache rows]
   float* parts;       // of several pieces: [sequences][kv_heads][pieces][tiles * keys of a tile]
   uint32_t tiles;     // of keys, of the longest sequence that the page table has room for
@@ -50,6 +65,7 @@ __device__ __forceinline__ void add_weight(const WeightArgs& a, const int32_t* p
 }
 
 constexpr int kSets = 4;  // of 16 keys, of a wave
+constexpr uint32_t kTile = 4 * 16 * kSets;  // keys of a workgroup
 
 template <class Tag, Store kStore, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(WeightArgs w) {
@@ -78,7 +94,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
   const uint32_t tile0 = tile * 4u * kKeys;
   if (tile0 >= length) return;
   const Span span = tokens_of(a, sequence);
-  // The first token that sees the tile's first key, and this piece's rows from there on.
+  // This piece's rows, from those on that see the tile's first key.
   const int64_t before = (int64_t)length - span.count;  // keys that token 0 sees, less its own
   const uint32_t first = a.causal ? (uint32_t)min((int64_t)span.count, max((int64_t)0, (int64_t)tile0 - before)) : 0u;
   const uint32_t rows_all = (span.count - first) * a.group;
@@ -94,6 +110,51 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
     for (int i = 0; i < 4; ++i) sum[s][i] = 0.f;
 
   if (begin < end) {
+    // A stage's rows.  Where whole tokens fill it and it ends within the sequence, a
+    // thread's places are the same in every stage, past a base that all threads share;
+    // else each row's token and head are worked out (for every stage that took a third
+    // of the time).
+    const char* base = a.queries + (int64_t)(span.first + first) * a.query_stride + (uint64_t)g * a.group * D * 2u;
+    const float* base_lse = a.lse + (uint64_t)(span.first + first) * a.heads + g * a.group;
+    const bool whole = kStage % a.group == 0;
+    uint64_t place[kLoads];
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const uint32_t at = tid + 256u * i, t = w.by_group(at / kRuns);
+      place[i] = (uint64_t)t * a.query_stride + ((at / kRuns - t * a.group) * D + at % kRuns * 8u) * 2u;
+    }
+    u32x4 staged[kLoads];
+    float2 staged_of;
+    auto load = [&](uint32_t r0) {
+      const uint32_t t0 = w.by_group(r0);
+      if (whole && r0 + kStage <= rows_all) {
+        const char* from = base + (int64_t)t0 * a.query_stride;
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) staged[i] = *reinterpret_cast<const u32x4*>(from + place[i]);
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+          const uint32_t at = tid + 256u * i, r = min(r0 + at / kRuns, rows_all - 1u), t = w.by_group(r);
+          staged[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)t * a.query_stride + ((r - t * a.group) * D + at % kRuns * 8u) * 2u);
+        }
+      }
+      if (tid < kStage) {
+        const uint32_t r = min(r0 + tid, rows_all - 1u), t = w.by_group(r);
+        const int64_t sees = a.causal ? before + first + t + 1 : (int64_t)length;
+        const float lse = base_lse[(uint64_t)t * a.heads + (r - t * a.group)];
+        staged_of = make_float2(lse * kLog2E, __uint_as_float(r0 + tid < end ? (uint32_t)max((int64_t)0, sees) : 0u));
+      }
+    };
+    auto stage = [&](uint32_t slot) {
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) {
+        const uint32_t at = tid + 256u * i;
+        *reinterpret_cast<u32x4*>(rows_tile[slot] + at / kRuns * kRow + at % kRuns * 16u) = staged[i];
+      }
+      if (tid < kStage) row_of[slot][tid] = staged_of;
+    };
+    load(begin);
+    __builtin_amdgcn_sched_barrier(0);  // under way before the keys are waited for
     // This wave's keys.  A lane has of key 16 s + col the dims that its quarter of each
     // product takes; the order of the dims is the store's.
     uint4 k[kSets][kQ];
@@ -135,65 +196,82 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
       }
     }
 
-    u32x4 staged[kLoads];
-    float2 staged_of;
-    auto load = [&](uint32_t r0) {
+    // Row sub + col of a stage, in the order of dims that the keys have.
+    auto read_row = [&](uint32_t slot, uint32_t sub, uint4 (&q)[kQ]) {
+      const char* row = rows_tile[slot] + (sub + col) * kRow;
 #pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) {
-        const uint32_t at = tid + 256u * i;
-        const uint32_t r = min(r0 + at / kRuns, end - 1u);
-        const uint64_t token = span.first + first + r / a.group;
-        staged[i] = *reinterpret_cast<const u32x4*>(a.queries + (int64_t)token * a.query_stride +
-                                                    ((uint64_t)(g * a.group + r % a.group) * D + at % kRuns * 8u) * 2u);
-      }
-      if (tid < kStage) {
-        const uint32_t r = min(r0 + tid, end - 1u);
-        const uint32_t t = first + r / a.group;
-        const int64_t sees = a.causal ? before + t + 1 : (int64_t)length;
-        const float lse = a.lse[(uint64_t)(span.first + t) * a.heads + g * a.group + r % a.group];
-        staged_of = make_float2(lse * kLog2E, __uint_as_float(r0 + tid < end ? (uint32_t)max((int64_t)0, sees) : 0u));
+      for (int j = 0; j < kQ; ++j) {
+        const uint32_t d = kFp4   ? D / 4u * quad + 8u * j
+                           : kFp8 ? 64u * (j / 2) + 16u * quad + 8u * (j % 2)
+                                  : 32u * j + 8u * quad;
+        q[j] = *reinterpret_cast<const uint4*>(row + 2u * d);
       }
     };
-    auto stage = [&](uint32_t slot) {
+    auto multiply = [&](const uint4 (&q)[kQ], floatx4 (&x)[kSets]) {
 #pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) {
-        const uint32_t at = tid + 256u * i;
-        *reinterpret_cast<u32x4*>(rows_tile[slot] + at / kRuns * kRow + at % kRuns * 16u) = staged[i];
-      }
-      if (tid < kStage) row_of[slot][tid] = staged_of;
+      for (int j = 0; j < kQ; ++j)
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+          x[s] = mfma_16x16x32(Tag{}, k[s][j], q[j], j == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : x[s]);
     };
-    load(begin);
     stage(0);
     __syncthreads();
     uint32_t slot = 0;
     for (uint32_t r0 = begin; r0 < end; r0 += kStage, slot ^= 1u) {
       const bool more = r0 + kStage < end;
       if (more) load(r0 + kStage);
-      for (uint32_t sub = 0; sub < kStage && r0 + sub < end; sub += 16u) {
-        const char* row = rows_tile[slot] + (sub + col) * kRow;
-        const float2 of = row_of[slot][sub + col];
-        const uint32_t sees = __float_as_uint(of.y);
-        floatx4 x[kSets];
+      // Rows ascend by token, so the first sees least.
+      const uint32_t least = (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(row_of[slot][0].y));
+      if (r0 + kStage <= end && least >= (uint32_t)__builtin_amdgcn_readfirstlane((int)key0) + kKeys) {
+        // Every row sees every key: the products of 16 rows under the exponentials of
+        // the 16 before, operands read from LDS a turn ahead.
+        constexpr uint32_t kTurns = kStage / 16u;
+        constexpr int kProducts = kSets * kQ;
+        uint4 q[2][kQ];
+        floatx4 x[2][kSets];
+        float lse[2];
+        read_row(slot, 0, q[0]);
+        float last = 0.f;  // a weight that is added a product later: an exponential's result has to wait
 #pragma unroll
-        for (int s = 0; s < kSets; ++s) x[s] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t n = 0; n <= kTurns; ++n) {
+          if (n + 1u < kTurns) read_row(slot, 16u * (n + 1u), q[(n + 1) % 2]);
+          if (n < kTurns) lse[n % 2] = row_of[slot][16u * n + col].x;  // for the next turn
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < kQ; ++j) {
-          const uint32_t d = kFp4   ? D / 4u * quad + 8u * j
-                             : kFp8 ? 64u * (j / 2) + 16u * quad + 8u * (j % 2)
-                                    : 32u * j + 8u * quad;
-          const uint4 q = *reinterpret_cast<const uint4*>(row + 2u * d);
+          for (int m = 0; m < kProducts; ++m) {
+            const int j = m / kSets, s = m % kSets;
+            if (n < kTurns)
+              x[n % 2][s] = mfma_16x16x32(Tag{}, k[s][j], q[n % 2][j], j == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : x[n % 2][s]);
+            if (n > 0) {
 #pragma unroll
-          for (int s = 0; s < kSets; ++s) x[s] = mfma_16x16x32(Tag{}, k[s][j], q, x[s]);
-        }
-        const bool partly = __any(sees < key0 + kKeys);
-#pragma unroll
-        for (int s = 0; s < kSets; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float p = exp2_fast(fmaf(x[s][i], kFp8 ? by[kFp8 ? s : 0][i] : a.scale, -of.x));
-            if (partly) p = key0 + 16u * s + 4u * quad + i < sees ? p : 0.f;
-            sum[s][i] += p;
+              for (int e = 4 * kSets * m / kProducts; e < 4 * kSets * (m + 1) / kProducts; ++e) {
+                const float p = exp2_fast(fmaf(x[(n + 1) % 2][e / 4][e % 4], kFp8 ? by[kFp8 ? e / 4 : 0][e % 4] : a.scale, -lse[(n + 1) % 2]));
+                const int before_e = e == 0 ? 4 * kSets - 1 : e - 1;
+                sum[before_e / 4][before_e % 4] += last;
+                last = p;
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
+        }
+        sum[kSets - 1][3] += last;
+      } else {
+        for (uint32_t sub = 0; sub < kStage && r0 + sub < end; sub += 16u) {
+          const float2 of = row_of[slot][sub + col];
+          const uint32_t sees = __float_as_uint(of.y);
+          if (!__any(sees > key0)) continue;  // these rows see none of the wave's keys
+          uint4 q[kQ];
+          floatx4 x[kSets];
+          read_row(slot, sub, q);
+          multiply(q, x);
+#pragma unroll
+          for (int s = 0; s < kSets; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = exp2_fast(fmaf(x[s][i], kFp8 ? by[kFp8 ? s : 0][i] : a.scale, -of.x));
+              sum[s][i] += key0 + 16u * s + 4u * quad + i < sees ? p : 0.f;
+            }
+        }
       }
       if (more) stage(slot ^ 1u);
       __syncthreads();
@@ -387,6 +465,7 @@ __global__ __launch_bounds__(256) void paged_weights_join_kernel(WeightArgs w, u
   if (key >= keys_of(a, sequence)) return;
   const float* from = w.parts + ((uint64_t)sequence * a.cache.kv_heads + g) * w.pieces * keys + key;
   float sum = 0.f;
+#pragma unroll 4
   for (uint32_t p = 0; p < w.pieces; ++p) sum += from[(uint64_t)p * keys];
   add_weight(w, a.page_table + (int64_t)sequence * a.table_stride, g, key, sum);
 }
@@ -401,7 +480,7 @@ WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t 
   const int64_t group = heads / cache->kv_heads;
   WeightPlan p = {};
   p.few = tokens * group <= kStage * sequences;
-  const int64_t keys = p.few ? 128 : 64 * kSets;  // of a tile, at least
+  const int64_t keys = p.few ? 128 : kTile;  // of a tile, at least
   p.tiles = (capacity + keys - 1) / keys;
   const int64_t wide = p.tiles * cache->kv_heads * sequences;
   p.pieces = 1;
@@ -411,10 +490,12 @@ WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t 
     p.steps = p.steps < 1 ? 1 : p.steps > 32 ? 32 : p.steps;
     p.tiles = (p.tiles + p.steps - 1) / p.steps;
   } else {
+    // As many pieces of every tile's rows, a causal tile's fewer rows in shorter ones:
+    // the longest come first, and the short ones fill what they leave.  (Prompt of 4096
+    // tokens over as many 4-bit keys, 32 heads on 8, us: 16 pieces a tile 92, 8 98;
+    // pieces of one length, twice or four times what runs at a time, 120 and 108.)
     const int64_t rows = (uniform ? tokens / sequences : tokens) * group;  // of a sequence, at most
-    const int64_t most = (rows + 4 * kStage - 1) / (4 * kStage);
-    const int64_t pieces = (kManyWorkgroups + wide - 1) / wide;
-    p.pieces = pieces < most ? pieces : most;
+    p.pieces = std::min((kManyWorkgroups + wide - 1) / wide, (rows + 4 * kStage - 1) / (4 * kStage));
     if (p.pieces > 1) p.part_bytes = sequences * cache->kv_heads * p.pieces * p.tiles * keys * 4;
   }
   return p;
@@ -467,6 +548,7 @@ extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queri
   if (p.part_bytes && (!workspace || workspace_bytes < p.part_bytes || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(DSA_STATUS_WORKSPACE_TOO_SMALL, "paged weights need %lld bytes of 16-byte aligned workspace",
                 (long long)p.part_bytes);
+  w.by_group = quotient_by(w.batch.group);
   w.batch.causal = causal != 0;
   w.batch.lse = const_cast<float*>(lse);
   w.weights = weights;
@@ -488,7 +570,7 @@ extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queri
     launch_weights<F16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, s);
   if (int st = check_launch("paged_weights_kernel")) return st;
   if (p.pieces == 1) return 0;
-  const uint32_t keys = (uint32_t)(p.tiles * 64 * kSets);
+  const uint32_t keys = (uint32_t)(p.tiles * kTile);
   DSA_REQUIRE(sequences < 65536, "too many sequences for one call");
   const dim3 join((keys + 255) / 256, (unsigned)cache->kv_heads, (unsigned)sequences);
   hipLaunchKernelGGL(paged_weights_join_kernel, join, dim3(256), 0, s, w, keys);
