@@ -296,26 +296,33 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
 }
 
 // Few rows: kStage of a sequence lie in LDS while its keys pass by, 32 a wave and step,
-// loaded a step ahead as 128 neighbouring bytes by eight lanes, through LDS of the
-// wave's own.  A workgroup takes w.steps steps of each of its four waves.
+// loaded as 128 neighbouring bytes by eight lanes, through LDS of the wave's own.  A
+// workgroup takes w.steps steps of each of its four waves.  A wave has 16 KiB of keys on
+// their way, whatever their type (8 KiB: 227 us for 16 sequences of 32K bf16 keys), and
+// nothing that the steps wait for is loaded after them: cache rows are looked up a group
+// of steps ahead, a row's powers of two come with it.
 template <class Tag, Store kStore, int D>
-__global__ __launch_bounds__(256, D < 256 ? 3 : kStore == k16Bit ? 1 : 2) void paged_weights_few_kernel(WeightArgs w) {
+__global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void paged_weights_few_kernel(WeightArgs w) {
   const PagedAttentionArgs& a = w.batch;
   constexpr bool kFp8 = kStore == kE4M3;
   constexpr bool kFp4 = kStore == kE2M1;
   constexpr int kQ = D / 32;
   constexpr uint32_t kStep = 32;
+  constexpr uint32_t kGroup = 8;                              // steps that are looked up at a time
   constexpr uint32_t kRow = 2 * D + 16;                       // bytes of a row in LDS
   constexpr uint32_t kRuns = D / 8;
   constexpr int kBytes = kRowBytes<kStore, D>;                // of a key
-  constexpr uint32_t kLanes = kBytes < 128 ? kBytes / 16 : 8;  // that share one
+  constexpr uint32_t kAhead = kBytes >= 512 ? 1 : kBytes >= 256 ? 2 : 4;  // steps on their way
+  constexpr uint32_t kLanes = kBytes < 128 ? kBytes / 16 : 8;  // that share a key
   constexpr uint32_t kRows = 64 / kLanes;                     // of one load
   constexpr int kPasses = kStep / kRows;
   constexpr int kLoads = kBytes / (16 * kLanes);              // of one key
   constexpr uint32_t kKeyRow = kBytes + 16;
+  constexpr int kPowerWords = D == 256 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) char rows_tile[kStage * kRow];
   __shared__ float2 row_of[kStage];
   __shared__ __attribute__((aligned(16))) char key_tile[4][kStep * kKeyRow];
+  __shared__ uint32_t table[4][2][kGroup * kStep];            // a wave's cache rows of this group of steps and the next
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = tid / kWave, col = lane & 15u, quad = lane >> 4;
 
   uint32_t id = blockIdx.x;
@@ -336,74 +343,87 @@ __global__ __launch_bounds__(256, D < 256 ? 3 : kStore == k16Bit ? 1 : 2) void p
 
   struct Tile {
     u32x4 k[kPasses][kLoads];
-    float scale;       // e4m3: of key `lane`
-    uint32_t page;     // of key `lane` of the step after
+    float scale;                  // e4m3: of key `lane`
+    uint32_t power[kPowerWords];  // e2m1: of key `lane`
   };
-  auto look = [&](uint32_t step) { return (uint32_t)pages[min(first_key(step) + (lane & 31u), length - 1u) >> a.cache.shift]; };
-  auto row_at = [&](uint32_t step, uint32_t page) {
-    const uint32_t key = min(first_key(step) + (lane & 31u), length - 1u);
-    return (min(page, a.cache.pages - 1u) << a.cache.shift) | (key & ((1u << a.cache.shift) - 1u));
+  // Lane l looks up keys l % 32 of steps 2 j + l / 32 of a group; past the end, the last.
+  uint32_t page[kGroup / 2];
+  auto key_at = [&](uint32_t group, uint32_t j) {
+    return min(first_key(group * kGroup + 2u * j + lane / 32u) + lane % 32u, length - 1u);
   };
-  // `row`: the cache row of key `lane` of the step.
-  auto load = [&](Tile& t, uint32_t row) {
+  auto look = [&](uint32_t group) {
+#pragma unroll
+    for (uint32_t j = 0; j < kGroup / 2; ++j) page[j] = (uint32_t)pages[key_at(group, j) >> a.cache.shift];
+  };
+  auto place = [&](uint32_t group) {
+#pragma unroll
+    for (uint32_t j = 0; j < kGroup / 2; ++j)
+      table[wave][group % 2u][64u * j + lane] =
+          (min(page[j], a.cache.pages - 1u) << a.cache.shift) | (key_at(group, j) & ((1u << a.cache.shift) - 1u));
+    wave_order();
+  };
+  auto rows_at = [&](uint32_t step) { return table[wave][step / kGroup % 2u] + step % kGroup * kStep; };
+  auto load = [&](Tile& t, uint32_t step) {
+    const uint32_t* at = rows_at(step);
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const uint32_t r = (uint32_t)__shfl((int)row, kRows * i + load_row, kWave);
-      const char* from = key_base + a.cache.key_offset(r);
+      const char* from = key_base + a.cache.key_offset(at[kRows * i + load_row]);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) t.k[i][j] = *reinterpret_cast<const u32x4*>(from + 16 * kLanes * j);
     }
-    if constexpr (kFp8) t.scale = a.cache.key_scales[(uint64_t)row * a.cache.kv_heads + g];
+    if constexpr (kFp8) t.scale = a.cache.key_scales[(uint64_t)at[lane & 31u] * a.cache.kv_heads + g];
+    if constexpr (kFp4) {
+      const uint8_t* powers = a.cache.key_powers + a.cache.power_offset<D>(at[lane & 31u], g);
+      if constexpr (D == 64) {
+        t.power[0] = *reinterpret_cast<const uint16_t*>(powers);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPowerWords; ++i) t.power[i] = reinterpret_cast<const uint32_t*>(powers)[i];
+      }
+    }
   };
 
   for (uint32_t r0 = 0; r0 < rows; r0 += kStage) {
     const uint32_t live = min(kStage, rows - r0);
-    uint32_t row = row_at(0, look(0));
-    uint32_t page = look(1u);
-    Tile t;
-    load(t, row);
+    Tile t[kAhead];
+    look(0);
+    place(0);
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) load(t[i], min(i, steps - 1u));
     if (r0 > 0) __syncthreads();
     for (uint32_t at = tid; at < live * kRuns; at += 256u) {
       const uint32_t r = r0 + at / kRuns;
-      const uint64_t token = span.first + r / a.group;
-      *reinterpret_cast<uint4*>(rows_tile + at / kRuns * kRow + at % kRuns * 16u) =
-          *reinterpret_cast<const uint4*>(a.queries + (int64_t)token * a.query_stride +
-                                          ((uint64_t)(g * a.group + r % a.group) * D + at % kRuns * 8u) * 2u);
+      const uint32_t i = w.by_group(r);
+      *reinterpret_cast<u32x4*>(rows_tile + at / kRuns * kRow + at % kRuns * 16u) =
+          *reinterpret_cast<const u32x4*>(a.queries + (int64_t)(span.first + i) * a.query_stride +
+                                          ((uint64_t)(g * a.group + r - i * a.group) * D + at % kRuns * 8u) * 2u);
     }
     if (tid < kStage) {
       const uint32_t r = min(r0 + tid, rows - 1u);
-      const uint32_t i = r / a.group;
+      const uint32_t i = w.by_group(r);
       const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
-      const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r % a.group];
+      const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r - i * a.group];
       row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(r0 + tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
     }
     __syncthreads();
-    for (uint32_t step = 0; step < steps; ++step) {
+    auto compute = [&](uint32_t step, float scale, const uint32_t (&power)[kPowerWords]) {
+      const char* mine = key_tile[wave];
       const uint32_t key0 = first_key(step);
-      char* mine = key_tile[wave];
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i)
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j)
-          *reinterpret_cast<u32x4*>(mine + (kRows * i + load_row) * kKeyRow + (kLanes * j + load_chunk) * 16u) = t.k[i][j];
-      const uint32_t now = row;
-      const float scale = kFp8 ? t.scale * a.scale : a.scale;
-      wave_order();
-      row = row_at(step + 1u, page);  // past the end: the last key again
-      load(t, row);
-      page = look(step + 2u);
-      __builtin_amdgcn_sched_barrier(0);
       uint4 k[2][kQ];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const char* key = mine + (16u * h + col) * kKeyRow;
         if constexpr (kFp4) {
-          const uint32_t of = (uint32_t)__shfl((int)now, 16 * h + col, kWave);
-          const uint8_t* powers = a.cache.key_powers + a.cache.power_offset<D>(of, g);
+          uint32_t of[kPowerWords];
+#pragma unroll
+          for (int i = 0; i < kPowerWords; ++i) of[i] = (uint32_t)__shfl((int)power[i], 16 * h + col, kWave);
+          // this lane's quarter of the key's blocks: half a block, one, or two
+          const uint32_t mine_of = D == 256 ? (quad < 2u ? of[0] : of[kPowerWords - 1]) : of[0];
+          const uint32_t at = D == 64 ? quad / 2u : D == 128 ? quad : 2u * (quad & 1u);
 #pragma unroll
           for (int j = 0; j < kQ; ++j)
             k[h][j] = fp4x8_to_bf16x8(*reinterpret_cast<const uint32_t*>(key + D / 8u * quad + 4u * j),
-                                      power_of(powers[(D / 4u * quad + 8u * j) / kPowerDims]));
+                                      power_of(mine_of >> 8u * (at + j / 4) & 0xffu));
         } else if constexpr (kFp8) {
 #pragma unroll
           for (int j = 0; j < kQ / 2; ++j) {
@@ -418,7 +438,7 @@ __global__ __launch_bounds__(256, D < 256 ? 3 : kStore == k16Bit ? 1 : 2) void p
       }
       float by[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) by[e] = kFp8 ? __shfl(scale, 16 * (e / 4) + 4 * quad + e % 4, kWave) : a.scale;
+      for (int e = 0; e < 8; ++e) by[e] = kFp8 ? __shfl(scale, 16 * (e / 4) + 4 * quad + e % 4, kWave) * a.scale : a.scale;
       float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (uint32_t sub = 0; sub < live; sub += 16u) {
         const char* from = rows_tile + (sub + col) * kRow;
@@ -444,15 +464,40 @@ __global__ __launch_bounds__(256, D < 256 ? 3 : kStore == k16Bit ? 1 : 2) void p
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] = row16_sum(sum[e]);
-      const uint32_t of = 16u * (col % 8u / 4u) + 4u * quad + col % 4u;  // the key that this lane adds to
-      const uint32_t to = (uint32_t)__shfl((int)now, of, kWave);  // (every lane takes part: an idle one would give 0)
       if (col < 8u) {
         float v = sum[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) v = col == (uint32_t)e ? sum[e] : v;
-        if (key0 + of < length) __hip_atomic_fetch_add(weights_of(w, g) + to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t of = 16u * (col / 4u) + 4u * quad + col % 4u;  // the key that this lane adds to
+        if (key0 + of < length)
+          __hip_atomic_fetch_add(weights_of(w, g) + rows_at(step)[of], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       wave_order();
+    };
+    for (uint32_t step0 = 0; step0 < steps; step0 += kAhead) {
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; ++i) {
+        const uint32_t step = step0 + i;
+        const uint32_t group = step / kGroup + 1u;
+        if (group * kGroup < steps) {
+          if (step % kGroup == 0) look(group);
+          if (step % kGroup == 3) place(group);
+        }
+        char* mine = key_tile[wave];
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j)
+            *reinterpret_cast<u32x4*>(mine + (kRows * p + load_row) * kKeyRow + (kLanes * j + load_chunk) * 16u) = t[i].k[p][j];
+        const float scale = t[i].scale;
+        uint32_t power[kPowerWords];
+#pragma unroll
+        for (int p = 0; p < kPowerWords; ++p) power[p] = t[i].power[p];
+        wave_order();
+        load(t[i], min(step + kAhead, steps - 1u));
+        __builtin_amdgcn_sched_barrier(0);
+        if (step < steps) compute(step, scale, power);
+      }
     }
   }
 }
