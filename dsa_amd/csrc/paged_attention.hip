@@ -54,6 +54,24 @@ __device__ __forceinline__ uint32_t tile_place(uint32_t row, uint32_t chunk) {
   return row * kBytes + ((chunk ^ x) << 4);
 }
 
+// The same for the values of an e2m1 cache, which a lane stores four chunks apart, one
+// after the other: 16 lanes have 4 neighbouring rows at head_dim 128 (8 at 64, 2 at
+// 256), so the row's bits go into the chunk's last two, beside those that the transposed
+// reads need in the others.  (As above those stores met at a quarter of the banks, and
+// 38 % of a decode step's time was conflicts.)
+template <int D>
+__device__ __forceinline__ uint32_t widened_place(uint32_t row, uint32_t chunk) {
+  const uint32_t r0 = row & 1u, r1 = (row >> 1) & 1u, r2 = (row >> 2) & 1u;
+  uint32_t x;
+  if constexpr (D == 64)
+    x = (r2 << 2) | (r1 << 1) | r2;
+  else if constexpr (D == 128)
+    x = (r2 << 3) | (r1 << 2) | (r0 << 1) | r1;
+  else
+    x = (r2 << 3) | (r1 << 2) | (r0 << 1) | (r0 ^ (chunk >> 4));
+  return row * (2 * D) + ((chunk ^ x) << 4);
+}
+
 // The powers of two of one head's row of an e2m1 cache.
 template <int D>
 struct Powers {
@@ -220,7 +238,9 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
   uint32_t tr_place[kO];
 #pragma unroll
   for (int i = 0; i < kO; ++i)
-    tr_place[i] = tile_place<2 * D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1)) + 8u * (col & 1u);
+    tr_place[i] = (kFp4 ? widened_place<D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1))
+                        : tile_place<2 * D>(4u * quad + (col >> 2), 2u * i + ((col & 3u) >> 1))) +
+                  8u * (col & 1u);
 
   // The steps of a piece are dealt to its head's waves (a list of its own is all
   // the wave's), step s at keys first_key(s).
@@ -321,7 +341,7 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
           const float power = power_of(reinterpret_cast<const uint8_t*>(scales[wave])[(32u + r) * kPowers + c]);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 4u * c + w)) = fp4x8_to_bf16x8(v[w], power);
+            *reinterpret_cast<uint4*>(mine + widened_place<D>(r, 4u * c + w)) = fp4x8_to_bf16x8(v[w], power);
         } else if constexpr (kFp8) {
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
