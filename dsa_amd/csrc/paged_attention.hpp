@@ -346,6 +346,13 @@ int check_paged_batch(const dsa_paged_cache* cache, const void* queries, int64_t
                       const int32_t* starts, int64_t sequences, int64_t tokens, int32_t heads, int32_t dtype,
                       float scale, const void* out, PagedAttentionArgs& a);
 
+// 4-byte words of a cache row that a thread loads at a time: four, but of an e2m1 head of
+// 64 dims as few as let every thread load some of a tile.  (A tile loaded and widened by
+// a quarter of the threads: ragged chunks of 64 dims 125 us, by all 122; of 128 dims by
+// half of them 1050, by all 1075.)
+template <Store kStore, int D, uint32_t kThreads>
+constexpr uint32_t kRunWords = kStore == kE2M1 && D == 64 ? kTileKeys * kRowBytes<kStore, D> / 4 / kThreads : 4u;
+
 constexpr int kChunkRows = 128;        // rows of a workgroup of the chunk kernel
 constexpr int kLeastChunkKeys = 256;   // keys of a piece of it
 

@@ -40,13 +40,14 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
   constexpr bool kFp4 = kStore == kE2M1;  // widened with its powers of two: the tiles are exact
   constexpr uint32_t kThreads = 256;
   constexpr uint32_t kRows = kChunkRows;
-  constexpr uint32_t kChunks = kRowBytes<kStore, D> / 16;   // 16-byte loads per cache row
+  constexpr uint32_t kWords = kRunWords<kStore, D, kThreads>;
+  constexpr uint32_t kChunks = kRowBytes<kStore, D> / (4 * kWords);  // loads per cache row
   constexpr uint32_t kPass = kThreads / kChunks;            // cache rows per pass of the workgroup
-  constexpr bool kPart = kPass > kTileKeys;                 // fewer loads than threads
-  constexpr int kLoads = kPart ? 1 : kTileKeys / kPass;     // passes per tile
+  constexpr int kLoads = kTileKeys / kPass;                 // passes per tile
+  typedef uint32_t Run __attribute__((ext_vector_type(kWords)));
   constexpr int kKeyBytes = kTileKeys * kKeyRow<D>;
   constexpr int kValueBytes = kTileKeys * kValueRow<D>;
-  static_assert(kPart || kTileKeys % kPass == 0, "a tile is whole passes");
+  static_assert(kLoads >= 1 && kTileKeys % kPass == 0, "a tile is whole passes");
   __shared__ __attribute__((aligned(16))) char key_tile[2][kKeyBytes];
   __shared__ __attribute__((aligned(16))) char value_tile[2][kValueBytes];
   // Places in the cache of tiles t .. t + 2: offsets of the keys' and the values'
@@ -108,24 +109,23 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
   const int32_t* pages = a.page_table + (int64_t)piece.sequence * a.table_stride;
   const uint32_t load_row = tid / kChunks;
   const uint32_t load_chunk = tid % kChunks;
-  const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * load_chunk;
-  const char* value_base = a.cache.values + g * a.cache.value_head + 16u * load_chunk;
+  const char* key_base = a.cache.keys + g * a.cache.key_head + 4u * kWords * load_chunk;
+  const char* value_base = a.cache.values + g * a.cache.value_head + 4u * kWords * load_chunk;
 
-  u32x4 kr[kLoads], vr[kLoads];
+  Run kr[kLoads], vr[kLoads];
   float sr = 0.f;
   uint32_t kp[kLoads] = {}, vp[kLoads] = {};  // fp4: each run's power of two
   auto load = [&](uint32_t t) {
-    if (kPart && load_row >= kTileKeys) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       if constexpr (kFp4) {
-        const uint64_t power = a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk;
+        const uint64_t power = a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk * kWords / 4u;
         kp[i] = a.cache.key_powers[power];
         vp[i] = a.cache.value_powers[power];
       }
       const ulong2 at = table[t & 3u][load_row + kPass * i];
-      kr[i] = *reinterpret_cast<const u32x4*>(key_base + at.x);
-      vr[i] = *reinterpret_cast<const u32x4*>(value_base + at.y);
+      kr[i] = *reinterpret_cast<const Run*>(key_base + at.x);
+      vr[i] = *reinterpret_cast<const Run*>(value_base + at.y);
     }
     if constexpr (kFp8) {
       if (tid < 2u * kTileKeys) {
@@ -135,7 +135,6 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
     }
   };
   auto stage = [&](uint32_t t) {
-    if (kPart && load_row >= kTileKeys) return;  // these threads have loaded nothing
     const uint32_t key0 = begin + t * kTileKeys;
     if (key0 + kTileKeys > all_rows_see) {
 #pragma unroll
@@ -162,9 +161,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttentionArgs 
       const uint32_t row = load_row + kPass * i;
       if constexpr (kFp4) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + 64u * load_chunk + 16u * w) = fp4x8_to_bf16x8(kr[i][w], power_of(kp[i]));
-          *reinterpret_cast<uint4*>(values + row * kValueRow<D> + 64u * load_chunk + 16u * w) = fp4x8_to_bf16x8(vr[i][w], power_of(vp[i]));
+        for (uint32_t w = 0; w < kWords; ++w) {
+          const uint32_t at = 16u * (kWords * load_chunk + w);
+          *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + at) = fp4x8_to_bf16x8(kr[i][w], power_of(kp[i]));
+          *reinterpret_cast<uint4*>(values + row * kValueRow<D> + at) = fp4x8_to_bf16x8(vr[i][w], power_of(vp[i]));
         }
       } else if constexpr (kFp8) {
         *reinterpret_cast<uint4*>(keys + row * kKeyRow<D> + 32u * load_chunk) = fp8x8_to_bf16x8_paired(make_uint2(kr[i].x, kr[i].y));

@@ -27,10 +27,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   constexpr bool kFp4 = kStore == kE2M1;  // widened with its powers of two: the tiles are exact
   constexpr uint32_t kThreads = 64 * kWaves;
   constexpr uint32_t kRows = 32 * kWaves;
-  constexpr uint32_t kChunks = kRowBytes<kStore, D> / 16;  // 16-byte loads per cache row
+  constexpr uint32_t kWords = kRunWords<kStore, D, kThreads>;
+  constexpr uint32_t kChunks = kRowBytes<kStore, D> / (4 * kWords);  // loads per cache row
   constexpr uint32_t kPass = kThreads / kChunks;       // cache rows per pass of the workgroup
   constexpr bool kPart = kPass > kTileKeys;            // fewer loads than threads
   constexpr int kLoads = kPart ? 1 : kTileKeys / kPass;  // passes per tile
+  typedef uint32_t Run __attribute__((ext_vector_type(kWords)));
   constexpr int kSteps = D / 16;                       // of a 32 x 32 block of scores
   constexpr int kBlocks = D / 32;                      // of an output row
   constexpr int kRing = 4;                             // operands read ahead of their products, and one at work
@@ -96,9 +98,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
   const int32_t* pages = a.page_table + (int64_t)piece.sequence * a.table_stride;
   const uint32_t load_row = tid / kChunks;
   const uint32_t load_chunk = tid % kChunks;
-  const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * load_chunk;
-  const char* value_base = a.cache.values + g * a.cache.value_head + 16u * load_chunk;
-  u32x4 kr[kLoads], vr[kLoads];
+  const char* key_base = a.cache.keys + g * a.cache.key_head + 4u * kWords * load_chunk;
+  const char* value_base = a.cache.values + g * a.cache.value_head + 4u * kWords * load_chunk;
+  Run kr[kLoads], vr[kLoads];
   float ks = 0.f, vs = 0.f;
   uint32_t kp[kLoads] = {}, vp[kLoads] = {};  // fp4: each run's power of two
   auto load_keys = [&](uint32_t t) {
@@ -106,8 +108,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       if constexpr (kFp4)
-        kp[i] = a.cache.key_powers[a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk];
-      kr[i] = *reinterpret_cast<const u32x4*>(key_base + table[t & 3u][load_row + kPass * i].x);
+        kp[i] = a.cache.key_powers[a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk * kWords / 4u];
+      kr[i] = *reinterpret_cast<const Run*>(key_base + table[t & 3u][load_row + kPass * i].x);
     }
     if constexpr (kFp8) {
       if (tid < kTileKeys) ks = a.cache.key_scales[(uint64_t)table_row[t & 3u][tid] * a.cache.kv_heads + g];
@@ -118,18 +120,18 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       if constexpr (kFp4)
-        vp[i] = a.cache.value_powers[a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk];
-      vr[i] = *reinterpret_cast<const u32x4*>(value_base + table[t & 3u][load_row + kPass * i].y);
+        vp[i] = a.cache.value_powers[a.cache.power_offset<D>(table_row[t & 3u][load_row + kPass * i], g) + load_chunk * kWords / 4u];
+      vr[i] = *reinterpret_cast<const Run*>(value_base + table[t & 3u][load_row + kPass * i].y);
     }
     if constexpr (kFp8) {
       if (tid < kTileKeys) vs = a.cache.value_scales[(uint64_t)table_row[t & 3u][tid] * a.cache.kv_heads + g];
     }
   };
-  auto put = [&](char* row, const u32x4& v, uint32_t power) {
+  auto put = [&](char* row, const Run& v, uint32_t power) {
     if constexpr (kFp4) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
-        *reinterpret_cast<uint4*>(row + 64u * load_chunk + 16u * w) = fp4x8_to_bf16x8(v[w], power_of(power));
+      for (uint32_t w = 0; w < kWords; ++w)
+        *reinterpret_cast<uint4*>(row + 16u * (kWords * load_chunk + w)) = fp4x8_to_bf16x8(v[w], power_of(power));
     } else if constexpr (kFp8) {
       *reinterpret_cast<uint4*>(row + 32u * load_chunk) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
       *reinterpret_cast<uint4*>(row + 32u * load_chunk + 16u) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
