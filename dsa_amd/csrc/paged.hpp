@@ -25,6 +25,18 @@ constexpr int kPowerDims = 32;  // dims that share a power of two of an e2m1 cac
 template <Store kStore, int D>
 constexpr int kRowBytes = kStore == kE2M1 ? D / 2 : kStore == kE4M3 ? D : 2 * D;  // of a head's keys or values
 
+// Quotients of numbers below 2^31 by one divisor: a product and a shift.
+struct Quotient {
+  uint32_t factor, shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)((uint64_t)x * factor >> shift); }
+};
+
+inline Quotient quotient_by(uint32_t divisor) {
+  uint32_t shift = 31;
+  while ((1ull << (shift - 31)) < divisor) ++shift;
+  return {(uint32_t)(((1ull << shift) + divisor - 1) / divisor), shift};
+}
+
 struct PagedView {
   char* keys;
   char* values;

@@ -24,6 +24,8 @@ namespace {
 
 constexpr uint32_t kThreads = 1024;
 
+struct Threshold;
+
 struct EvictArgs {
   PagedView cache;
   const int32_t* page_table;
@@ -43,6 +45,7 @@ struct EvictArgs {
   uint2* moves;
   uint32_t* counts;
   uint4* chunks;
+  Threshold* thresholds;  // after each pass
   uint32_t* order;
   uint64_t order_stride;
 };
@@ -119,23 +122,10 @@ __device__ __forceinline__ void orders_of(const EvictArgs& a, const List& l, uin
 // Where the want-th largest of a list's orders lies: its digits so far, how many with
 // those digits are still wanted, and whether there are more of them.
 struct Threshold {
-  uint32_t prefix, rest;
-  bool ties;
+  uint32_t prefix, rest, ties;
 };
 constexpr uint32_t kShift[3] = {21u, 10u, 0u};  // of each pass's digit
 constexpr uint32_t kBins = 2048;
-
-// Counts a lane's bin; a wave whose lanes share one (a list of zeros) adds once.
-__device__ __forceinline__ void count_bin(uint32_t* bins, uint32_t bin, bool counts) {
-  const uint64_t all = __ballot(counts);
-  if (!all) return;
-  const uint32_t leader = (uint32_t)__builtin_ctzll(all);
-  if (__ballot(counts && bin == (uint32_t)__builtin_amdgcn_readlane(bin, leader)) == all) {
-    if (lane_id() == leader) atomicAdd(&bins[bin], (uint32_t)__popcll(all));
-  } else if (counts) {
-    atomicAdd(&bins[bin], 1u);
-  }
-}
 
 // The digit of `pass` added to the threshold.
 __device__ __forceinline__ void locate_digit(const uint32_t* bins, uint32_t pass, Locate& shared, Threshold& t) {
@@ -267,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
   const uint32_t at = tid * kEach;
 #pragma unroll
   for (uint32_t e = 0; e < kEach; ++e) key[e] = order[tid * (kEach + 1) + e];
-  Threshold t = {0u, l.want, false};
+  Threshold t = {0u, l.want, 0u};
   if (l.want > 0) {
     for (uint32_t pass = 0; pass < 3; ++pass) {
       if (pass > 0) {
@@ -277,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
 #pragma unroll
       for (uint32_t e = 0; e < kEach; ++e) {
         const bool counts = at + e < l.old && (pass == 0 || key[e] >> kShift[pass - 1] == t.prefix >> kShift[pass - 1]);
-        count_bin(bins, key[e] >> kShift[pass] & (pass == 2 ? 1023u : 2047u), counts);
+        if (counts) atomicAdd(&bins[key[e] >> kShift[pass] & (pass == 2 ? 1023u : 2047u)], 1u);
       }
       __syncthreads();
       locate_digit(bins, pass, found, t);
@@ -305,12 +295,16 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
 constexpr uint32_t kChunkEach = 8;
 constexpr uint32_t kChunk = kThreads * kChunkEach;
 
+// The threshold after kPass passes: what the launch before this one's left of it, and
+// the digit that its bins say.
 template <int kPass>
 __device__ __forceinline__ Threshold threshold_of(const EvictArgs& a, const List& l, uint32_t list, Locate& found) {
-  Threshold t = {0u, l.want, false};
-  if (l.want > 0)
-#pragma unroll
-    for (uint32_t pass = 0; pass < kPass; ++pass) locate_digit(a.bins + ((uint64_t)list * 3u + pass) * kBins, pass, found, t);
+  Threshold t = {0u, l.want, 0u};
+  if (kPass == 0 || l.want == 0) return t;
+  Threshold* kept = a.thresholds + (uint64_t)list * 3u;
+  if (kPass > 1) t = kept[kPass > 1 ? kPass - 2 : 0];
+  locate_digit(a.bins + ((uint64_t)list * 3u + kPass - 1) * kBins, kPass - 1, found, t);
+  if (blockIdx.x == 0 && threadIdx.x == 0) kept[kPass - 1] = t;
   return t;
 }
 
@@ -349,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_count_kernel(EvictArgs a
     const uint32_t i = first + tid + kThreads * e;
     const uint32_t key = own[e];
     const bool counts = i < l.old && (kPass == 0 || key >> kShift[kPass ? kPass - 1 : 0] == t.prefix >> kShift[kPass ? kPass - 1 : 0]);
-    count_bin(bins, key >> kShift[kPass] & (kPass == 2 ? 1023u : 2047u), counts);
+    if (counts) atomicAdd(&bins[key >> kShift[kPass] & (kPass == 2 ? 1023u : 2047u)], 1u);
   }
   __syncthreads();
   uint32_t* to = a.bins + ((uint64_t)list * 3u + kPass) * kBins;
@@ -407,7 +401,6 @@ __global__ __launch_bounds__(kThreads) void paged_evict_chunk_kernel(EvictArgs a
 
 // What is kept, a chunk a workgroup, from the counts of the chunks before it.
 __global__ __launch_bounds__(kThreads) void paged_evict_settle_kernel(EvictArgs a) {
-  __shared__ Locate found;
   __shared__ __attribute__((aligned(16))) uint32_t scan[2][16];
   __shared__ uint32_t moving[kChunk], masks[kThreads];
   __shared__ uint32_t start[3];  // ranks of the chunk's first: key at the threshold, hole, source
@@ -415,7 +408,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_settle_kernel(EvictArgs 
   const List l = list_of(a, list);
   const uint32_t first = blockIdx.x * kChunk;
   if (l.n == l.m || first >= l.n) return;
-  const Threshold t = threshold_of<3>(a, l, list, found);
+  const Threshold t = l.want > 0 ? a.thresholds[(uint64_t)list * 3u + 2u] : Threshold{0u, 0u, 0u};
   if (threadIdx.x < kWave) {
     // Keys at the threshold are kept while their rank is below t.rest; that rank follows
     // the chunks, so a chunk keeps as many as are left of them.
@@ -572,7 +565,7 @@ constexpr int64_t kMostInLds = 16 * kThreads;
 
 struct EvictPlan {
   int64_t lists, chunks, order_stride;  // no chunks: one workgroup a list
-  int64_t bins, moves, counts, chunk_counts, bytes;  // offsets
+  int64_t bins, moves, counts, thresholds, chunk_counts, bytes;  // offsets
 };
 
 EvictPlan evict_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t columns, int64_t keep, bool per_head) {
@@ -585,7 +578,8 @@ EvictPlan evict_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t co
   }
   p.moves = p.lists * 3 * kBins * 4;  // kept clear of where there are no chunks: others share the workspace
   p.counts = p.moves + p.lists * keep * 8;
-  p.chunk_counts = (p.counts + p.lists * 4 + 15) / 16 * 16;
+  p.thresholds = p.counts + p.lists * 4;
+  p.chunk_counts = (p.thresholds + p.lists * 36 + 15) / 16 * 16;
   p.bytes = p.chunk_counts + p.lists * p.chunks * 16 + p.lists * p.order_stride * 4;
   return p;
 }
@@ -633,6 +627,7 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
   a.bins = reinterpret_cast<uint32_t*>(base);
   a.moves = reinterpret_cast<uint2*>(base + p.moves);
   a.counts = reinterpret_cast<uint32_t*>(base + p.counts);
+  a.thresholds = reinterpret_cast<Threshold*>(base + p.thresholds);
   a.chunks = p.chunks ? reinterpret_cast<uint4*>(base + p.chunk_counts) : nullptr;
   a.order = reinterpret_cast<uint32_t*>(base + p.chunk_counts + p.lists * p.chunks * 16);
   a.order_stride = (uint64_t)p.order_stride;

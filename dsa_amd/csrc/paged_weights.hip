@@ -24,18 +24,6 @@ namespace {
 constexpr uint32_t kStage = 64;  // rows in LDS at a time
 constexpr int64_t kManyWorkgroups = 2048;  // that the work is dealt to, where there is as much
 
-// Quotients of numbers below 2^31 by one divisor: a product and a shift.
-struct Quotient {
-  uint32_t factor, shift;
-  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)((uint64_t)x * factor >> shift); }
-};
-
-Quotient quotient_by(uint32_t divisor) {
-  uint32_t shift = 31;
-  while ((1ull << (shift - 31)) < divisor) ++shift;
-  return {(uint32_t)(((1ull << shift) + divisor - 1) / divisor), shift};
-}
-
 struct WeightArgs {
   PagedAttentionArgs batch;
   Quotient by_group;  // of a row: its token

@@ -299,8 +299,8 @@ def read(cache: PagedCache, rows: torch.Tensor) -> tuple[torch.Tensor, torch.Ten
         raise ValueError("rows must be [n]")
     rows = _integers(rows, torch.int64, "rows", cache)
     count = len(rows)
-    keys, values = (torch.empty((count, cache.kv_heads, cache.head_dim), dtype=cache.row_dtype, device=cache.device)
-                    for _ in range(2))
+    keys = torch.empty((count, cache.kv_heads, cache.head_dim), dtype=cache.row_dtype, device=cache.device)
+    values = torch.empty_like(keys)
     if count:
         _lib.call("dsa_paged_read", cache._address, rows.data_ptr(), count, keys.data_ptr(), values.data_ptr(),
                   _lib.stream_of(keys))
