@@ -115,8 +115,10 @@ def attend(args: argparse.Namespace) -> None:
     import pandas as pd
     import torch
 
-    from . import decode, paged
+    from . import decode, eviction, paged
 
+    if args.budget is not None and args.budget < 2:
+        raise ValueError("the budget must be at least 2 keys")
     if args.steps < 1 or args.length < 1 or args.batch < 1 or args.k < 1:
         raise ValueError("length, steps, batch and k must be at least 1")
     device = torch.device("cuda", 0)
@@ -124,7 +126,8 @@ def attend(args: argparse.Namespace) -> None:
     batch, heads, kv_heads, dim = args.batch, args.heads, args.kv_heads, args.head_dim
     longest = args.length + args.steps
     columns = -(-longest // args.page_size)
-    dtype = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp8": torch.float8_e4m3fn}[args.cache_dtype]
+    dtype = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp8": torch.float8_e4m3fn,
+             "fp4": torch.float4_e2m1fn_x2}[args.cache_dtype]
     cache = paged.new_cache(batch * columns, args.page_size, kv_heads, dim, dtype=dtype, device=device)
     table = torch.randperm(batch * columns, generator=gen, device=device).to(torch.int32).view(batch, columns)
     # A token's keys of every head share a part, which is the indexer's key and which
@@ -151,14 +154,16 @@ def attend(args: argparse.Namespace) -> None:
     index_weights = torch.full((batch, 64), 1 / 64, device=device)
     sequences = torch.arange(batch, device=device)
 
-    def write(first: int, n: int):
-        """Appends tokens first .. first + n of every sequence; their rotated queries."""
+    def write(first: int, n: int, cached: int):
+        """Appends tokens first .. first + n of every sequence behind its cached keys; their
+        rotated queries."""
 
         part, keys, values = tokens_of(n)
-        index_keys[:, first:first + n, :shared] = part.to(torch.bfloat16)
+        index_keys[:, cached:cached + n, :shared] = part.to(torch.bfloat16)
+        places = torch.arange(cached, cached + n, device=device).repeat(batch)
+        rows = paged.cache_rows(cache, table, places, sequences.repeat_interleave(n))
         positions = torch.arange(first, first + n, device=device).repeat(batch)
-        rows = paged.cache_rows(cache, table, positions, sequences.repeat_interleave(n))
-        queries = queries_of(index_keys[:, :first + n, :shared].float(), n)
+        queries = queries_of(index_keys[:, :cached + n, :shared].float(), n)
         plain = queries[:, :, rope_dim:rope_dim + shared]
         return paged.append(cache, keys, values, rows, positions, queries=queries, rope_dim=rope_dim), plain
 
@@ -171,32 +176,46 @@ def attend(args: argparse.Namespace) -> None:
         stop.synchronize()
         return out, 1e3 * start.elapsed_time(stop)
 
-    queries, _ = write(0, args.length)
+    queries, _ = write(0, args.length, 0)
     lengths = torch.full((batch,), args.length, dtype=torch.int32, device=device)
-    _, prompt_us = timed(lambda: paged.attention(queries, cache, table, lengths))
+    (_, prompt_lse), prompt_us = timed(lambda: paged.attention(queries, cache, table, lengths, return_lse=True))
+    cached, evictions, weights = args.length, 0, None
+    if args.budget is not None:  # the prompt's own rows say first what its keys are worth
+        weights = eviction.new_weights(cache)
+        eviction.accumulate_weights(weights, queries, cache, table, lengths, prompt_lse)
     print(f"prompt: {batch} x {args.length} tokens, {prompt_us:.0f} us of attention", flush=True)
     frames = []
     for step in range(args.steps):
-        position = args.length + step
-        queries, plain = write(position, 1)
+        if args.budget is not None and cached >= args.budget:
+            # to seven eighths of the budget, so that not every step evicts
+            cached = max(1, args.budget - args.budget // 8 - 1)
+            lengths, kept = eviction.evict(cache, table, lengths, weights, cached, recent=cached // 8)
+            index_keys[:, :cached] = index_keys.gather(1, kept[..., None].expand(-1, -1, 128))
+            evictions += 1
+        queries, plain = write(args.length + step, 1, cached)
+        cached += 1
         lengths = lengths + 1
         index_queries = torch.zeros(batch, 64, 128, device=device, dtype=torch.bfloat16)
         index_queries[..., :shared] = plain[:, torch.arange(64, device=device) * heads // 64].to(torch.bfloat16)
-        chosen = decode.indexer_topk(index_queries, index_weights, index_keys[:, :position + 1].contiguous(), args.k)
+        chosen = decode.indexer_topk(index_queries, index_weights, index_keys[:, :cached].contiguous(), args.k)
         (few, few_lse), few_us = timed(
             lambda: paged.selected_attention(queries, cache, table, lengths, chosen, return_lse=True))
         (full, full_lse), full_us = timed(
             lambda: paged.attention(queries, cache, table, lengths, return_lse=True))
-        kept = torch.exp(few_lse - full_lse)
+        if weights is not None:
+            eviction.accumulate_weights(weights, queries, cache, table, lengths, full_lse)
+        mass = torch.exp(few_lse - full_lse)
         off = torch.linalg.vector_norm(few.float() - full.float(), dim=(1, 2)) / torch.linalg.vector_norm(full.float(), dim=(1, 2))
         frames.append(pd.DataFrame({
-            "step": step, "sequence": range(batch), "keys": position + 1, "selected": (chosen >= 0).sum(1).cpu(),
-            "mass_kept_mean": kept.mean(1).cpu(), "mass_kept_least": kept.amin(1).cpu(), "output_error": off.cpu(),
+            "step": step, "sequence": range(batch), "keys": cached, "selected": (chosen >= 0).sum(1).cpu(),
+            "mass_kept_mean": mass.mean(1).cpu(), "mass_kept_least": mass.amin(1).cpu(), "output_error": off.cpu(),
             "selected_us": few_us, "dense_us": full_us}))
     frame = pd.concat(frames, ignore_index=True)
     args.output.mkdir(parents=True, exist_ok=True)
     frame.to_csv(args.output / "attention_steps.csv", index=False)
     print(frame.drop(columns=["step", "sequence"]).mean().to_string(float_format=lambda x: f"{x:.4g}"), flush=True)
+    if args.budget is not None:
+        print(f"evicted {evictions} times to a budget of {args.budget} keys", flush=True)
     print(f"wrote {len(frame)} rows to {args.output}", flush=True)
 
 
@@ -228,7 +247,9 @@ def build_parser() -> argparse.ArgumentParser:
     t.add_argument("--kv-heads", type=int, default=8)
     t.add_argument("--head-dim", type=int, default=128, choices=(64, 128, 256))
     t.add_argument("--page-size", type=int, default=64)
-    t.add_argument("--cache-dtype", default="bf16", choices=("bf16", "fp16", "fp8"))
+    t.add_argument("--cache-dtype", default="bf16", choices=("bf16", "fp16", "fp8", "fp4"))
+    t.add_argument("--budget", type=int, default=None,
+                   help="cached keys of a sequence: those of least accumulated attention weight are evicted")
     t.add_argument("--seed", type=int, default=1582)
     t.set_defaults(function=attend)
     return parser

@@ -38,7 +38,7 @@ struct EvictArgs {
   uint32_t lists;         // of a sequence: kv_heads or 1
   int32_t* out_lengths;
   int64_t* kept;          // [sequences][lists][keep]
-  // Workspace, for each list: the three passes' bins (zero between calls), its moves
+  // Workspace, for each list: the three passes' bins, its moves
   // {to, from} (keep apart) and how many there are, and for long lists each chunk's
   // counts and the order of every weight.
   uint32_t* bins;
@@ -291,9 +291,22 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
 }
 
 // Longer lists: a chunk of one a workgroup, one launch a pass.  The passes' counts meet
-// in global memory, where the last launch leaves zeros.
+// in global memory.
 constexpr uint32_t kChunkEach = 8;
 constexpr uint32_t kChunk = kThreads * kChunkEach;
+
+// What a call's other launches add to, and what stays as it is.
+__global__ __launch_bounds__(256) void paged_evict_begin_kernel(EvictArgs a) {
+  const uint32_t list = blockIdx.y;
+  const List l = list_of(a, list);
+  const uint32_t at = blockIdx.x * 256u + threadIdx.x, step = gridDim.x * 256u;
+  if (at == 0) {
+    if (l.g == 0) a.out_lengths[l.sequence] = (int32_t)l.m;
+    a.counts[list] = 0;
+  }
+  for (uint32_t i = at; i < 3u * kBins; i += step) a.bins[(uint64_t)list * 3u * kBins + i] = 0;
+  fill_kept(a, l, list, at, step);
+}
 
 // The threshold after kPass passes: what the launch before this one's left of it, and
 // the digit that its bins say.
@@ -316,13 +329,6 @@ __global__ __launch_bounds__(kThreads) void paged_evict_count_kernel(EvictArgs a
   const uint32_t list = blockIdx.y;
   const List l = list_of(a, list);
   const uint32_t first = blockIdx.x * kChunk;
-  if (kPass == 0) {
-    if (blockIdx.x == 0 && tid == 0) {
-      if (l.g == 0) a.out_lengths[l.sequence] = (int32_t)l.m;
-      a.counts[list] = 0;
-    }
-    fill_kept(a, l, list, blockIdx.x * kThreads + tid, gridDim.x * kThreads);
-  }
   if (l.n == l.m || first >= l.old || l.want == 0) return;
   const Threshold t = threshold_of<kPass>(a, l, list, found);
   for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
@@ -463,7 +469,6 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a) {
   const uint2* moves = a.moves + (uint64_t)list * a.keep;
   const uint32_t count = a.counts[list];
   if (a.chunks) {
-    for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < 3u * kBins; i += gridDim.x * 256u) a.bins[(uint64_t)list * 3u * kBins + i] = 0;
     for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < count; i += gridDim.x * 256u)
       a.kept[(uint64_t)list * a.keep + moves[i].x] = moves[i].y;
   }
@@ -576,7 +581,7 @@ EvictPlan evict_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t co
     p.chunks = (capacity + kChunk - 1) / kChunk;
     p.order_stride = p.chunks * kChunk;
   }
-  p.moves = p.lists * 3 * kBins * 4;  // kept clear of where there are no chunks: others share the workspace
+  p.moves = p.chunks ? p.lists * 3 * kBins * 4 : 0;
   p.counts = p.moves + p.lists * keep * 8;
   p.thresholds = p.counts + p.lists * 4;
   p.chunk_counts = (p.thresholds + p.lists * 36 + 15) / 16 * 16;
@@ -636,6 +641,7 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
   const dim3 lists((unsigned)p.lists);
   if (p.chunks) {
     const dim3 chunks((unsigned)p.chunks, (unsigned)p.lists);
+    hipLaunchKernelGGL(paged_evict_begin_kernel, dim3(4, (unsigned)p.lists), dim3(256), 0, s, a);
     hipLaunchKernelGGL(paged_evict_count_kernel<0>, chunks, dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL(paged_evict_count_kernel<1>, chunks, dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL(paged_evict_count_kernel<2>, chunks, dim3(kThreads), 0, s, a);
@@ -651,14 +657,14 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
   if (int st = check_launch("paged_evict_select_kernel")) return st;
   // A list moves at most keep keys, and no more than lie past it.
   const int64_t most = std::min(keep, capacity - keep);
-  if (most <= 0 && !p.chunks) return 0;  // (the move kernel leaves the bins zero)
+  if (most <= 0) return 0;
   const int32_t bytes = cache->dtype == kFP4E2M1   ? cache->head_dim / 2
                         : cache->dtype == kFP8E4M3 ? cache->head_dim
                                                    : 2 * cache->head_dim;
   const int32_t pieces = bytes / 16;
   const int64_t heads = per_head ? 1 : cache->kv_heads;
   const int64_t fill = (4096 + p.lists - 1) / p.lists;
-  const int64_t blocks = std::min((std::max(most, (int64_t)1) * heads * pieces + 511) / 512, fill);
+  const int64_t blocks = std::min((most * heads * pieces + 511) / 512, fill);
   const dim3 grid((unsigned)blocks, (unsigned)p.lists);
   if (cache->dtype == kFP4E2M1)
     launch_move<kE2M1>(a, pieces, grid, s);

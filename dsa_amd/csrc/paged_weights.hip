@@ -576,6 +576,7 @@ extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queri
     return st;
   DSA_REQUIRE(lse && weights, "null pointer argument");
   if (tokens == 0) return 0;
+  DSA_REQUIRE(tokens * w.batch.group < (1LL << 31), "too many rows for one call");
   const int64_t capacity = columns * cache->page_size;
   const WeightPlan p = weight_plan(cache, sequences, tokens, heads, capacity, !starts);
   if (p.part_bytes && (!workspace || workspace_bytes < p.part_bytes || reinterpret_cast<uintptr_t>(workspace) % 16))

@@ -118,9 +118,8 @@ def evict(
     kept = torch.empty((sequences, cache.kv_heads, keep) if per_head else (sequences, keep), dtype=torch.int64,
                        device=cache.device)
     stream = _lib.stream_of(weights)
-    lists = sequences * (cache.kv_heads if per_head else 1)
     ws, need = cache._workspace(stream, "dsa_paged_evict_workspace_bytes", sequences, columns, keep, bool(per_head),
-                                kind="paged_evict", zeroed_rows=lists)
+                                kind="paged_evict", zeroed_rows=None)
     _lib.call("dsa_paged_evict", cache._address, page_table.data_ptr(), table_stride, columns, lengths.data_ptr(),
               sequences, weights.data_ptr(), keep, recent, bool(per_head), out.data_ptr(), kept.data_ptr(), ws, need,
               stream)

@@ -877,7 +877,7 @@ typedef struct dsa_paged_cache {
  * position; sidecar.py:10-28 takes the angle's product in fp32).  Products and
  * sums are fp32, rounded once to the cache's type.  Tokens whose row is outside
  * the cache are not written; two tokens with one row leave either's values (on an
- * fp8 cache any mixture of their codes and scales).  fp8: scale = max(max|x| / 448, 2^-126) over a head, code = round-to-nearest
+ * fp8 or fp4 cache any mixture of their codes and scales).  fp8: scale = max(max|x| / 448, 2^-126) over a head, code = round-to-nearest
  * (x / scale); rows must be finite.  fp4: the power of 32 dims is the least under
  * which the largest magnitude is 7 or less, from 2^-124 to 2^125, code =
  * round-to-nearest-even(x / 2^power), at most 6; 32 dims of which one is not finite
@@ -960,9 +960,7 @@ int dsa_paged_weights(const dsa_paged_cache* cache, const void* queries, int64_t
  * positions m .. n become 0.  out_lengths[s] = m; kept [sequences][kv_heads if
  * per_head else 1][keep] is the former position of the key now at each position, -1
  * from m on.  No other byte of the cache is written.  A page may be of one
- * sequence alone.  Workspace (16-byte aligned): the bytes of the query; its first
- * 24576 per list (sequences, times kv_heads if per_head) are zero before the first
- * call, and every call of as many lists leaves them so. */
+ * sequence alone.  Workspace (16-byte aligned): the bytes of the query. */
 int64_t dsa_paged_evict_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t columns, int64_t keep,
                                         int32_t per_head);
 int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t columns,

@@ -100,3 +100,14 @@ def test_oracle_eviction_keeps_what_it_says() -> None:
     assert oracle.choose(w, 8, 3, 3) == [5, 6, 7]
     assert oracle.choose(w, 8, 7, 0) == [0, 1, 2, 3, 7, 5, 6]
     assert oracle.choose(w, 5, 8, 2) == [0, 1, 2, 3, 4]
+
+
+def test_command_line_of_the_budget(tmp_path) -> None:
+    from dsa_amd.cli import build_parser
+
+    args = build_parser().parse_args(["attend", "--output", str(tmp_path), "--cache-dtype", "fp4", "--budget", "4096"])
+    assert (args.cache_dtype, args.budget) == ("fp4", 4096)
+    assert build_parser().parse_args(["attend", "--output", str(tmp_path)]).budget is None
+    args.budget = 1
+    with pytest.raises(ValueError, match="budget"):
+        args.function(args)
