@@ -83,40 +83,45 @@ __device__ __forceinline__ List list_of(const EvictArgs& a, uint32_t list) {
   return l;
 }
 
-// The orders of positions first + stride * e of those that are chosen from; 0 past them.
+// The orders of positions first + kThreads * e + (this thread) of those that are chosen
+// from; 0 past them.  Four positions under way at a time, of eight heads where a key's
+// weight is their sum: a head after the other waits for memory as often as there are
+// heads.
 template <int kEach>
-__device__ __forceinline__ void orders_of(const EvictArgs& a, const List& l, uint32_t first, uint32_t stride,
-                                          uint32_t (&key)[kEach]) {
-  uint32_t row[kEach];
+__device__ __forceinline__ void orders_of(const EvictArgs& a, const List& l, uint32_t first, uint32_t (&key)[kEach]) {
+  constexpr int kTogether = kEach < 4 ? kEach : 4;
 #pragma unroll
-  for (uint32_t e = 0; e < kEach; ++e) row[e] = cache_row(a, l.pages, min(first + stride * e, l.n - 1u));
-  if (a.lists > 1u || a.cache.kv_heads == 1u) {
+  for (uint32_t e = 0; e < kEach; e += kTogether) {
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) key[e] = order_of(a.weights[l.g * a.row_count + row[e]]);
-  } else {
-    // eight heads of four positions under way at a time: a head after the other waits
-    // for memory as often as there are heads
-    constexpr int kTogether = kEach < 4 ? kEach : 4;
+    for (int i = 0; i < kTogether; ++i) key[e + i] = 0;
+    if (first + kThreads * e >= l.old) continue;  // for all threads
+    uint32_t row[kTogether];
+    float w[8][kTogether];
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; e += kTogether) {
+    for (int i = 0; i < kTogether; ++i)
+      row[i] = cache_row(a, l.pages, min(first + threadIdx.x + kThreads * (e + i), l.n - 1u));
+    if (a.lists > 1u || a.cache.kv_heads == 1u) {
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) w[0][i] = a.weights[l.g * a.row_count + row[i]];
+    } else {
       double sum[kTogether] = {};
       for (uint32_t h0 = 0; h0 < a.cache.kv_heads; h0 += 8u) {
-        float w[8][kTogether];
 #pragma unroll
         for (uint32_t h = 0; h < 8; ++h)
 #pragma unroll
-          for (int i = 0; i < kTogether; ++i) w[h][i] = a.weights[min(h0 + h, a.cache.kv_heads - 1u) * a.row_count + row[e + i]];
+          for (int i = 0; i < kTogether; ++i) w[h][i] = a.weights[min(h0 + h, a.cache.kv_heads - 1u) * a.row_count + row[i]];
 #pragma unroll
         for (uint32_t h = 0; h < 8; ++h)
 #pragma unroll
           for (int i = 0; i < kTogether; ++i) sum[i] += h0 + h < a.cache.kv_heads ? (double)w[h][i] : 0.0;
       }
 #pragma unroll
-      for (int i = 0; i < kTogether; ++i) key[e + i] = order_of((float)sum[i]);
+      for (int i = 0; i < kTogether; ++i) w[0][i] = (float)sum[i];
     }
-  }
 #pragma unroll
-  for (uint32_t e = 0; e < kEach; ++e) key[e] = first + stride * e < l.old ? key[e] : 0u;
+    for (int i = 0; i < kTogether; ++i)
+      if (first + threadIdx.x + kThreads * (e + i) < l.old) key[e + i] = order_of(w[0][i]);
+  }
 }
 
 // Where the want-th largest of a list's orders lies: its digits so far, how many with
@@ -246,7 +251,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
 #pragma unroll 1
   for (uint32_t e0 = 0; e0 < kEach; e0 += kPart) {
     uint32_t part[kPart];
-    orders_of<kPart>(a, l, tid + kThreads * e0, kThreads, part);
+    orders_of<kPart>(a, l, kThreads * e0, part);
 #pragma unroll
     for (uint32_t e = 0; e < kPart; ++e) {
       const uint32_t i = tid + kThreads * (e0 + e);
@@ -335,7 +340,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_count_kernel(EvictArgs a
   __syncthreads();
   uint32_t* order = a.order + (uint64_t)list * a.order_stride;
   uint32_t own[kChunkEach];
-  if (kPass == 0) orders_of<kChunkEach>(a, l, first + tid, kThreads, own);
+  if (kPass == 0) orders_of<kChunkEach>(a, l, first, own);
 #pragma unroll
   for (uint32_t e = 0; e < kChunkEach; ++e) {
     const uint32_t i = first + tid + kThreads * e;  // (inside the chunk's room, past the list's end too)
