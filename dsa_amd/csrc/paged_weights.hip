@@ -15,15 +15,27 @@
 // the keys are too few workgroups for them, the rows are cut into pieces, whose sums a
 // second kernel adds in order.  Few rows (a decoded token) are bound by reading the
 // keys: there the rows stay, in LDS, and the keys pass by, loaded a step ahead.
+//
+// Which of the two takes a sequence is known to the device alone where `starts` says how
+// many tokens each has.  There the kernel of few rows also lists the sequences that it
+// leaves to the other, which deals its workgroups to what is listed.
 #include <algorithm>
 
 #include "paged_attention.hpp"
+#include "waveops.hpp"
 
 namespace dsa {
 namespace {
 
 constexpr uint32_t kStage = 64;  // rows in LDS at a time
 constexpr int64_t kManyWorkgroups = 2048;  // that the work is dealt to, where there is as much
+
+// Sequences of many rows among some of few.
+struct Chunks {
+  uint32_t count, tiles, pieces;  // sequences, their tiles of keys, pieces of each tile's rows
+  uint32_t unused;
+  uint2 of[1];  // {sequence, tiles before it}
+};
 
 struct WeightArgs {
   PagedAttentionArgs batch;
@@ -33,6 +45,7 @@ struct WeightArgs {
   uint32_t tiles;     // of keys, of the longest sequence that the page table has room for
   uint32_t pieces;    // of each tile's rows
   uint32_t steps;     // few rows: of a wave
+  Chunks* chunks;     // of a mixed batch; else all sequences are one kernel's
   uint64_t row_count;
 };
 
@@ -56,8 +69,11 @@ __device__ __forceinline__ void add_weight(const WeightArgs& a, const int32_t* p
 constexpr int kSets = 4;  // of 16 keys, of a wave
 constexpr uint32_t kTile = 4 * 16 * kSets;  // keys of a workgroup
 
+// What a workgroup does to one tile of a sequence's keys: piece `piece` of `pieces` of its
+// rows, whose sums go to `parts` if there are several.
 template <class Tag, Store kStore, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(WeightArgs w) {
+__device__ __forceinline__ void weigh_tile(const WeightArgs& w, uint32_t g, uint32_t sequence, uint32_t tile, uint32_t piece,
+                                           uint32_t pieces, float* parts) {
   const PagedAttentionArgs& a = w.batch;
   constexpr bool kFp8 = kStore == kE4M3;
   constexpr bool kFp4 = kStore == kE2M1;
@@ -70,15 +86,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
   __shared__ float2 row_of[2][kStage];     // {log2 sum, keys that the row sees (as bits)}
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = tid / kWave, col = lane & 15u, quad = lane >> 4;
 
-  // Heads vary fastest, then pieces, then tiles: a causal chunk's first keys, which
-  // most rows see, come first.
-  uint32_t id = blockIdx.x;
-  const uint32_t g = id % a.cache.kv_heads;
-  id /= a.cache.kv_heads;
-  const uint32_t piece = id % w.pieces;
-  id /= w.pieces;
-  const uint32_t sequence = id % a.sequences;
-  const uint32_t tile = id / a.sequences;
   const uint32_t length = keys_of(a, sequence);
   const uint32_t tile0 = tile * 4u * kKeys;
   if (tile0 >= length) return;
@@ -87,7 +94,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
   const int64_t before = (int64_t)length - span.count;  // keys that token 0 sees, less its own
   const uint32_t first = a.causal ? (uint32_t)min((int64_t)span.count, max((int64_t)0, (int64_t)tile0 - before)) : 0u;
   const uint32_t rows_all = (span.count - first) * a.group;
-  const uint32_t each = ((rows_all + w.pieces - 1u) / w.pieces + kStage - 1u) / kStage * kStage;
+  const uint32_t each = ((rows_all + pieces - 1u) / pieces + kStage - 1u) / kStage * kStage;
   const uint32_t begin = min(piece * each, rows_all), end = min(begin + each, rows_all);
   const uint32_t key0 = tile0 + wave * kKeys;
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
@@ -275,8 +282,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
     if (col < 4u) {
       const float v = col == 0 ? sum[s][0] : col == 1 ? sum[s][1] : col == 2 ? sum[s][2] : sum[s][3];
       const uint32_t key = key0 + 16u * s + 4u * quad + col;
-      if (w.pieces > 1u) {
-        w.parts[(((uint64_t)sequence * a.cache.kv_heads + g) * w.pieces + piece) * (w.tiles * 4u * kKeys) + key] = v;
+      if (pieces > 1u) {
+        parts[key - tile0] = v;
       } else if (key < length && begin < end) {
         add_weight(w, pages, g, key, v);
       }
@@ -284,7 +291,88 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
   }
 }
 
-// Few rows: kStage of a sequence lie in LDS while its keys pass by, 32 a wave and step,
+// Heads vary fastest, then pieces, then tiles: a causal chunk's first keys, which most
+// rows see, come first.
+template <class Tag, Store kStore, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(WeightArgs w) {
+  const uint32_t heads = w.batch.cache.kv_heads;
+  uint32_t id = blockIdx.x;
+  const uint32_t g = id % heads;
+  id /= heads;
+  const uint32_t piece = id % w.pieces;
+  id /= w.pieces;
+  const uint32_t sequence = id % w.batch.sequences, tile = id / w.batch.sequences;
+  weigh_tile<Tag, kStore, D>(w, g, sequence, tile, piece, w.pieces,
+                             w.parts + ((((uint64_t)sequence * heads + g) * w.pieces + piece) * w.tiles + tile) * kTile);
+}
+
+// A listed sequence's tile.
+struct ChunkTile {
+  uint32_t sequence, tile;
+};
+__device__ __forceinline__ ChunkTile chunk_tile(const Chunks* chunks, uint32_t at) {
+  uint32_t low = 0, high = chunks->count;  // the last sequence with at most `at` tiles before it
+  while (high - low > 1u) {
+    const uint32_t middle = (low + high) / 2u;
+    if (chunks->of[middle].y <= at)
+      low = middle;
+    else
+      high = middle;
+  }
+  const uint2 of = chunks->of[low];
+  return {of.x, at - of.y};
+}
+
+// The same for the listed sequences of a mixed batch, dealt to the workgroups in turn.
+template <class Tag, Store kStore, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_chunks_kernel(WeightArgs w) {
+  const uint32_t heads = w.batch.cache.kv_heads;
+  const uint32_t pieces = w.chunks->pieces, all = w.chunks->tiles * heads * pieces;
+  for (uint32_t item = blockIdx.x; item < all; item += gridDim.x) {
+    uint32_t id = item;
+    const uint32_t g = id % heads;
+    id /= heads;
+    const uint32_t piece = id % pieces;
+    id /= pieces;
+    const ChunkTile t = chunk_tile(w.chunks, id);
+    weigh_tile<Tag, kStore, D>(w, g, t.sequence, t.tile, piece, pieces, w.parts + (((uint64_t)id * heads + g) * pieces + piece) * kTile);
+  }
+}
+
+// Lists the sequences of more than kStage rows, and cuts their tiles' rows into as many
+// pieces as leave every workgroup some.  One workgroup's work.
+__device__ __forceinline__ void list_chunks(const WeightArgs& w, uint32_t* scan) {
+  const PagedAttentionArgs& a = w.batch;
+  uint32_t count = 0, tiles = 0, most = 0;
+  for (uint32_t base = 0; base < a.sequences; base += 256u) {
+    const uint32_t sequence = base + threadIdx.x;
+    uint32_t own = 0, rows = 0;
+    if (sequence < a.sequences) {
+      rows = tokens_of(a, sequence).count * a.group;
+      if (rows > kStage) own = (keys_of(a, sequence) + kTile - 1u) / kTile;
+    }
+    uint32_t all, all_tiles;
+    const uint32_t rank = block_excl_scan<4>(own > 0u ? 1u : 0u, scan, all);
+    const uint32_t before = block_excl_scan<4>(own, scan + 4, all_tiles);
+    if (own > 0) w.chunks->of[count + rank] = make_uint2(sequence, tiles + before);
+    most = max(most, own > 0 ? rows : 0u);
+    count += all, tiles += all_tiles;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) scan[0] = 0;
+  __syncthreads();
+  if (most) atomicMax(scan, most);
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+  const uint32_t wide = tiles * a.cache.kv_heads;
+  uint32_t pieces = 1;
+  if (wide > 0) pieces = min(((uint32_t)kManyWorkgroups + wide - 1u) / wide, (scan[0] + 4u * kStage - 1u) / (4u * kStage));
+  w.chunks->count = count;
+  w.chunks->tiles = tiles;
+  w.chunks->pieces = pieces;
+}
+
+// Few rows: those of a sequence, up to kStage, lie in LDS while its keys pass by, 32 a wave and step,
 // loaded as 128 neighbouring bytes by eight lanes, through LDS of the wave's own.  A
 // workgroup takes w.steps steps of each of its four waves.  A wave has 16 KiB of keys on
 // their way, whatever their type (8 KiB: 227 us for 16 sequences of 32K bf16 keys), and
@@ -315,6 +403,13 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = tid / kWave, col = lane & 15u, quad = lane >> 4;
 
   uint32_t id = blockIdx.x;
+  if (w.chunks) {
+    if (id == 0) {
+      list_chunks(w, reinterpret_cast<uint32_t*>(rows_tile));
+      return;
+    }
+    --id;
+  }
   const uint32_t g = id % a.cache.kv_heads;
   id /= a.cache.kv_heads;
   const uint32_t sequence = id % a.sequences;
@@ -324,6 +419,7 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
   const Span span = tokens_of(a, sequence);
   const int64_t before = (int64_t)length - span.count;
   const uint32_t rows = span.count * a.group;
+  if (rows == 0 || rows > kStage) return;  // (more: listed)
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
   const uint32_t steps = min(w.steps, (length - tile0 + 4u * kStep - 1u) / (4u * kStep));
   const uint32_t load_row = lane / kLanes, load_chunk = lane % kLanes;
@@ -372,148 +468,167 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
     }
   };
 
-  for (uint32_t r0 = 0; r0 < rows; r0 += kStage) {
-    const uint32_t live = min(kStage, rows - r0);
-    Tile t[kAhead];
-    look(0);
-    place(0);
+  Tile t[kAhead];
+  look(0);
+  place(0);
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) load(t[i], min(i, steps - 1u));
-    if (r0 > 0) __syncthreads();
-    for (uint32_t at = tid; at < live * kRuns; at += 256u) {
-      const uint32_t r = r0 + at / kRuns;
-      const uint32_t i = w.by_group(r);
-      *reinterpret_cast<u32x4*>(rows_tile + at / kRuns * kRow + at % kRuns * 16u) =
-          *reinterpret_cast<const u32x4*>(a.queries + (int64_t)(span.first + i) * a.query_stride +
-                                          ((uint64_t)(g * a.group + r - i * a.group) * D + at % kRuns * 8u) * 2u);
+  for (uint32_t i = 0; i < kAhead; ++i) load(t[i], min(i, steps - 1u));
+  for (uint32_t at = tid; at < rows * kRuns; at += 256u) {
+    const uint32_t r = at / kRuns;
+    const uint32_t i = w.by_group(r);
+    *reinterpret_cast<u32x4*>(rows_tile + r * kRow + at % kRuns * 16u) =
+        *reinterpret_cast<const u32x4*>(a.queries + (int64_t)(span.first + i) * a.query_stride +
+                                        ((uint64_t)(g * a.group + r - i * a.group) * D + at % kRuns * 8u) * 2u);
+  }
+  if (tid < kStage) {
+    const uint32_t r = min(tid, rows - 1u);
+    const uint32_t i = w.by_group(r);
+    const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
+    const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r - i * a.group];
+    row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
+  }
+  __syncthreads();
+  auto compute = [&](uint32_t step, float scale, const uint32_t (&power)[kPowerWords]) {
+    const char* mine = key_tile[wave];
+    const uint32_t key0 = first_key(step);
+    uint4 k[2][kQ];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const char* key = mine + (16u * h + col) * kKeyRow;
+      if constexpr (kFp4) {
+        uint32_t of[kPowerWords];
+#pragma unroll
+        for (int i = 0; i < kPowerWords; ++i) of[i] = (uint32_t)__shfl((int)power[i], 16 * h + col, kWave);
+        // this lane's quarter of the key's blocks: half a block, one, or two
+        const uint32_t mine_of = D == 256 ? (quad < 2u ? of[0] : of[kPowerWords - 1]) : of[0];
+        const uint32_t at = D == 64 ? quad / 2u : D == 128 ? quad : 2u * (quad & 1u);
+#pragma unroll
+        for (int j = 0; j < kQ; ++j)
+          k[h][j] = fp4x8_to_bf16x8(*reinterpret_cast<const uint32_t*>(key + D / 8u * quad + 4u * j),
+                                    power_of(mine_of >> 8u * (at + j / 4) & 0xffu));
+      } else if constexpr (kFp8) {
+#pragma unroll
+        for (int j = 0; j < kQ / 2; ++j) {
+          const uint4 v = *reinterpret_cast<const uint4*>(key + 64u * j + 16u * quad);
+          k[h][2 * j] = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
+          k[h][2 * j + 1] = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kQ; ++j) k[h][j] = *reinterpret_cast<const uint4*>(key + 64u * j + 16u * quad);
+      }
     }
-    if (tid < kStage) {
-      const uint32_t r = min(r0 + tid, rows - 1u);
-      const uint32_t i = w.by_group(r);
-      const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
-      const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r - i * a.group];
-      row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(r0 + tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
+    float by[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) by[e] = kFp8 ? __shfl(scale, 16 * (e / 4) + 4 * quad + e % 4, kWave) * a.scale : a.scale;
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (uint32_t sub = 0; sub < rows; sub += 16u) {
+      const char* from = rows_tile + (sub + col) * kRow;
+      const float2 of = row_of[sub + col];
+      const uint32_t sees = __float_as_uint(of.y);
+      floatx4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int j = 0; j < kQ; ++j) {
+        const uint32_t d = kFp4   ? D / 4u * quad + 8u * j
+                           : kFp8 ? 64u * (j / 2) + 16u * quad + 8u * (j % 2)
+                                  : 32u * j + 8u * quad;
+        const uint4 q = *reinterpret_cast<const uint4*>(from + 2u * d);
+        x[0] = mfma_16x16x32(Tag{}, k[0][j], q, x[0]);
+        x[1] = mfma_16x16x32(Tag{}, k[1][j], q, x[1]);
+      }
+      const bool partly = __any(sees < key0 + kStep);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float p = exp2_fast(fmaf(x[e / 4][e % 4], by[e], -of.x));
+        if (partly) p = key0 + 16u * (e / 4) + 4u * quad + e % 4 < sees ? p : 0.f;
+        sum[e] += p;
+      }
     }
-    __syncthreads();
-    auto compute = [&](uint32_t step, float scale, const uint32_t (&power)[kPowerWords]) {
-      const char* mine = key_tile[wave];
-      const uint32_t key0 = first_key(step);
-      uint4 k[2][kQ];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const char* key = mine + (16u * h + col) * kKeyRow;
-        if constexpr (kFp4) {
-          uint32_t of[kPowerWords];
+    for (int e = 0; e < 8; ++e) sum[e] = row16_sum(sum[e]);
+    if (col < 8u) {
+      float v = sum[0];
 #pragma unroll
-          for (int i = 0; i < kPowerWords; ++i) of[i] = (uint32_t)__shfl((int)power[i], 16 * h + col, kWave);
-          // this lane's quarter of the key's blocks: half a block, one, or two
-          const uint32_t mine_of = D == 256 ? (quad < 2u ? of[0] : of[kPowerWords - 1]) : of[0];
-          const uint32_t at = D == 64 ? quad / 2u : D == 128 ? quad : 2u * (quad & 1u);
+      for (int e = 1; e < 8; ++e) v = col == (uint32_t)e ? sum[e] : v;
+      const uint32_t of = 16u * (col / 4u) + 4u * quad + col % 4u;  // the key that this lane adds to
+      if (key0 + of < length)
+        __hip_atomic_fetch_add(weights_of(w, g) + rows_at(step)[of], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    wave_order();
+  };
+  for (uint32_t step0 = 0; step0 < steps; step0 += kAhead) {
 #pragma unroll
-          for (int j = 0; j < kQ; ++j)
-            k[h][j] = fp4x8_to_bf16x8(*reinterpret_cast<const uint32_t*>(key + D / 8u * quad + 4u * j),
-                                      power_of(mine_of >> 8u * (at + j / 4) & 0xffu));
-        } else if constexpr (kFp8) {
-#pragma unroll
-          for (int j = 0; j < kQ / 2; ++j) {
-            const uint4 v = *reinterpret_cast<const uint4*>(key + 64u * j + 16u * quad);
-            k[h][2 * j] = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
-            k[h][2 * j + 1] = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kQ; ++j) k[h][j] = *reinterpret_cast<const uint4*>(key + 64u * j + 16u * quad);
-        }
+    for (uint32_t i = 0; i < kAhead; ++i) {
+      const uint32_t step = step0 + i;
+      const uint32_t group = step / kGroup + 1u;
+      if (group * kGroup < steps) {
+        if (step % kGroup == 0) look(group);
+        if (step % kGroup == 3) place(group);
       }
-      float by[8];
+      char* mine = key_tile[wave];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) by[e] = kFp8 ? __shfl(scale, 16 * (e / 4) + 4 * quad + e % 4, kWave) * a.scale : a.scale;
-      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (uint32_t sub = 0; sub < live; sub += 16u) {
-        const char* from = rows_tile + (sub + col) * kRow;
-        const float2 of = row_of[sub + col];
-        const uint32_t sees = __float_as_uint(of.y);
-        floatx4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-        for (int j = 0; j < kQ; ++j) {
-          const uint32_t d = kFp4   ? D / 4u * quad + 8u * j
-                             : kFp8 ? 64u * (j / 2) + 16u * quad + 8u * (j % 2)
-                                    : 32u * j + 8u * quad;
-          const uint4 q = *reinterpret_cast<const uint4*>(from + 2u * d);
-          x[0] = mfma_16x16x32(Tag{}, k[0][j], q, x[0]);
-          x[1] = mfma_16x16x32(Tag{}, k[1][j], q, x[1]);
-        }
-        const bool partly = __any(sees < key0 + kStep);
+        for (int j = 0; j < kLoads; ++j)
+          *reinterpret_cast<u32x4*>(mine + (kRows * p + load_row) * kKeyRow + (kLanes * j + load_chunk) * 16u) = t[i].k[p][j];
+      const float scale = t[i].scale;
+      uint32_t power[kPowerWords];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float p = exp2_fast(fmaf(x[e / 4][e % 4], by[e], -of.x));
-          if (partly) p = key0 + 16u * (e / 4) + 4u * quad + e % 4 < sees ? p : 0.f;
-          sum[e] += p;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = row16_sum(sum[e]);
-      if (col < 8u) {
-        float v = sum[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) v = col == (uint32_t)e ? sum[e] : v;
-        const uint32_t of = 16u * (col / 4u) + 4u * quad + col % 4u;  // the key that this lane adds to
-        if (key0 + of < length)
-          __hip_atomic_fetch_add(weights_of(w, g) + rows_at(step)[of], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+      for (int p = 0; p < kPowerWords; ++p) power[p] = t[i].power[p];
       wave_order();
-    };
-    for (uint32_t step0 = 0; step0 < steps; step0 += kAhead) {
-#pragma unroll
-      for (uint32_t i = 0; i < kAhead; ++i) {
-        const uint32_t step = step0 + i;
-        const uint32_t group = step / kGroup + 1u;
-        if (group * kGroup < steps) {
-          if (step % kGroup == 0) look(group);
-          if (step % kGroup == 3) place(group);
-        }
-        char* mine = key_tile[wave];
-#pragma unroll
-        for (int p = 0; p < kPasses; ++p)
-#pragma unroll
-          for (int j = 0; j < kLoads; ++j)
-            *reinterpret_cast<u32x4*>(mine + (kRows * p + load_row) * kKeyRow + (kLanes * j + load_chunk) * 16u) = t[i].k[p][j];
-        const float scale = t[i].scale;
-        uint32_t power[kPowerWords];
-#pragma unroll
-        for (int p = 0; p < kPowerWords; ++p) power[p] = t[i].power[p];
-        wave_order();
-        load(t[i], min(step + kAhead, steps - 1u));
-        __builtin_amdgcn_sched_barrier(0);
-        if (step < steps) compute(step, scale, power);
-      }
+      load(t[i], min(step + kAhead, steps - 1u));
+      __builtin_amdgcn_sched_barrier(0);
+      if (step < steps) compute(step, scale, power);
     }
   }
 }
 
-// Adds the pieces of each key, a key a thread.
-__global__ __launch_bounds__(256) void paged_weights_join_kernel(WeightArgs w, uint32_t keys) {
+// Adds the pieces of each key, a key a thread: of a batch's tiles, or of the listed
+// sequences'.
+__global__ __launch_bounds__(kTile) void paged_weights_join_kernel(WeightArgs w) {
   const PagedAttentionArgs& a = w.batch;
-  const uint32_t key = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t g = blockIdx.y, sequence = blockIdx.z;
+  const uint32_t heads = a.cache.kv_heads;
+  const uint32_t pieces = w.chunks ? w.chunks->pieces : w.pieces;
+  const uint32_t g = blockIdx.x % heads, at = blockIdx.x / heads;
+  uint32_t sequence, tile;
+  uint64_t part, apart;  // of piece 0, and from a piece to the next
+  if (w.chunks) {
+    if (pieces == 1u || at >= w.chunks->tiles) return;
+    const ChunkTile t = chunk_tile(w.chunks, at);
+    sequence = t.sequence, tile = t.tile;
+    part = ((uint64_t)at * heads + g) * pieces * kTile;
+    apart = kTile;
+  } else {
+    sequence = at / w.tiles, tile = at % w.tiles;
+    part = (((uint64_t)sequence * heads + g) * pieces * w.tiles + tile) * kTile;
+    apart = (uint64_t)w.tiles * kTile;
+  }
+  const uint32_t key = tile * kTile + threadIdx.x;
   if (key >= keys_of(a, sequence)) return;
-  const float* from = w.parts + ((uint64_t)sequence * a.cache.kv_heads + g) * w.pieces * keys + key;
+  const float* from = w.parts + part + threadIdx.x;
   float sum = 0.f;
 #pragma unroll 4
-  for (uint32_t p = 0; p < w.pieces; ++p) sum += from[(uint64_t)p * keys];
+  for (uint32_t p = 0; p < pieces; ++p) sum += from[p * apart];
   add_weight(w, a.page_table + (int64_t)sequence * a.table_stride, g, key, sum);
 }
 
 struct WeightPlan {
-  bool few;
-  int64_t tiles, steps, pieces, part_bytes;
+  bool few, mixed;
+  int64_t tiles, steps, pieces, list_bytes, part_bytes;  // mixed: pieces at most
+  int64_t chunk_workgroups;
+  int64_t bytes() const { return list_bytes + part_bytes; }
 };
 
 WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens, int64_t heads, int64_t capacity,
                        bool uniform) {
   const int64_t group = heads / cache->kv_heads;
   WeightPlan p = {};
-  p.few = tokens * group <= kStage * sequences;
+  // With `starts` each sequence has the kernel of its own rows.  (us, so / all in the
+  // kernel that the average rows say, 32 heads on 8 of 128 dims: 256 tokens over 4096 bf16
+  // keys each and a chunk of 2048 over as many 335 / 5670; 8 over 32K and a prompt of 4096
+  // 182 / 402; chunks of 300, 60, 200 and 40 tokens, a launch or two less, 22 / 16.)
+  p.mixed = !uniform && sequences > 1 && tokens * group > kStage;
+  p.few = p.mixed || tokens * group <= kStage * sequences;
   const int64_t keys = p.few ? 128 : kTile;  // of a tile, at least
   p.tiles = (capacity + keys - 1) / keys;
   const int64_t wide = p.tiles * cache->kv_heads * sequences;
@@ -523,12 +638,20 @@ WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t 
     p.steps = wide / kManyWorkgroups;
     p.steps = p.steps < 1 ? 1 : p.steps > 32 ? 32 : p.steps;
     p.tiles = (p.tiles + p.steps - 1) / p.steps;
+    if (p.mixed) {
+      // What can be listed: sequences of more than kStage rows, pieces of 4 kStage each.
+      const int64_t listed = std::min(sequences, tokens * group / (kStage + 1));
+      p.pieces = std::min(kManyWorkgroups, (tokens * group + 4 * kStage - 1) / (4 * kStage));
+      p.chunk_workgroups = std::min(kManyWorkgroups, listed * ((capacity + kTile - 1) / kTile) * cache->kv_heads * p.pieces);
+      p.list_bytes = (16 + sequences * 8 + 15) / 16 * 16;
+      if (p.pieces > 1) p.part_bytes = 2 * kManyWorkgroups * kTile * 4;  // several pieces are fewer than twice the workgroups
+    }
   } else {
     // As many pieces of every tile's rows, a causal tile's fewer rows in shorter ones:
     // the longest come first, and the short ones fill what they leave.  (Prompt of 4096
     // tokens over as many 4-bit keys, 32 heads on 8, us: 16 pieces a tile 92, 8 98;
     // pieces of one length, twice or four times what runs at a time, 120 and 108.)
-    const int64_t rows = (uniform ? tokens / sequences : tokens) * group;  // of a sequence, at most
+    const int64_t rows = tokens / sequences * group;  // of a sequence: all have as many, or there is one
     p.pieces = std::min((kManyWorkgroups + wide - 1) / wide, (rows + 4 * kStage - 1) / (4 * kStage));
     if (p.pieces > 1) p.part_bytes = sequences * cache->kv_heads * p.pieces * p.tiles * keys * 4;
   }
@@ -536,21 +659,24 @@ WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t 
 }
 
 template <class Tag, Store kStore, int D>
-void launch_dim(const WeightArgs& w, uint32_t grid, hipStream_t s) {
-  if (w.steps)
+void launch_dim(const WeightArgs& w, uint32_t grid, uint32_t chunk_grid, hipStream_t s) {
+  if (w.chunks) {
+    hipLaunchKernelGGL((paged_weights_few_kernel<Tag, kStore, D>), dim3(grid + 1u), dim3(256), 0, s, w);
+    hipLaunchKernelGGL((paged_weights_chunks_kernel<Tag, kStore, D>), dim3(chunk_grid), dim3(256), 0, s, w);
+  } else if (w.steps)
     hipLaunchKernelGGL((paged_weights_few_kernel<Tag, kStore, D>), dim3(grid), dim3(256), 0, s, w);
   else
     hipLaunchKernelGGL((paged_weights_kernel<Tag, kStore, D>), dim3(grid), dim3(256), 0, s, w);
 }
 
 template <class Tag, Store kStore>
-void launch_weights(const WeightArgs& w, int32_t dim, uint32_t grid, hipStream_t s) {
+void launch_weights(const WeightArgs& w, int32_t dim, uint32_t grid, uint32_t chunk_grid, hipStream_t s) {
   if (dim == 64)
-    launch_dim<Tag, kStore, 64>(w, grid, s);
+    launch_dim<Tag, kStore, 64>(w, grid, chunk_grid, s);
   else if (dim == 128)
-    launch_dim<Tag, kStore, 128>(w, grid, s);
+    launch_dim<Tag, kStore, 128>(w, grid, chunk_grid, s);
   else
-    launch_dim<Tag, kStore, 256>(w, grid, s);
+    launch_dim<Tag, kStore, 256>(w, grid, chunk_grid, s);
 }
 
 }  // namespace
@@ -563,7 +689,7 @@ extern "C" int64_t dsa_paged_weights_workspace_bytes(const dsa_paged_cache* cach
   if (!cache || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads || sequences <= 0 || tokens <= 0 ||
       columns <= 0 || cache->page_size <= 0)
     return 0;
-  return weight_plan(cache, sequences, tokens, heads, columns * cache->page_size, uniform != 0).part_bytes;
+  return weight_plan(cache, sequences, tokens, heads, columns * cache->page_size, uniform != 0).bytes();
 }
 
 extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queries, int64_t query_stride,
@@ -580,34 +706,34 @@ extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queri
   DSA_REQUIRE(tokens * w.batch.group < (1LL << 31), "too many rows for one call");
   const int64_t capacity = columns * cache->page_size;
   const WeightPlan p = weight_plan(cache, sequences, tokens, heads, capacity, !starts);
-  if (p.part_bytes && (!workspace || workspace_bytes < p.part_bytes || reinterpret_cast<uintptr_t>(workspace) % 16))
+  if (p.bytes() && (!workspace || workspace_bytes < p.bytes() || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(DSA_STATUS_WORKSPACE_TOO_SMALL, "paged weights need %lld bytes of 16-byte aligned workspace",
-                (long long)p.part_bytes);
+                (long long)p.bytes());
   w.by_group = quotient_by(w.batch.group);
   w.batch.causal = causal != 0;
   w.batch.lse = const_cast<float*>(lse);
   w.weights = weights;
-  w.parts = static_cast<float*>(workspace);
+  w.chunks = p.mixed ? static_cast<Chunks*>(workspace) : nullptr;
+  w.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.list_bytes);
   w.tiles = (uint32_t)p.tiles;
   w.pieces = (uint32_t)p.pieces;
   w.steps = (uint32_t)p.steps;
   w.row_count = (uint64_t)cache->pages * cache->page_size;
-  const int64_t grid = p.tiles * sequences * p.pieces * cache->kv_heads;
+  const int64_t grid = p.tiles * sequences * (p.mixed ? 1 : p.pieces) * cache->kv_heads;
   DSA_REQUIRE(grid < (1LL << 24), "too many keys for one call");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->dtype == kFP4E2M1)
-    launch_weights<Bf16Tag, kE2M1>(w, cache->head_dim, (uint32_t)grid, s);
+    launch_weights<Bf16Tag, kE2M1>(w, cache->head_dim, (uint32_t)grid, (uint32_t)p.chunk_workgroups, s);
   else if (cache->dtype == kFP8E4M3)
-    launch_weights<Bf16Tag, kE4M3>(w, cache->head_dim, (uint32_t)grid, s);
+    launch_weights<Bf16Tag, kE4M3>(w, cache->head_dim, (uint32_t)grid, (uint32_t)p.chunk_workgroups, s);
   else if (cache->dtype == kBF16)
-    launch_weights<Bf16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, s);
+    launch_weights<Bf16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, (uint32_t)p.chunk_workgroups, s);
   else
-    launch_weights<F16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, s);
+    launch_weights<F16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, (uint32_t)p.chunk_workgroups, s);
   if (int st = check_launch("paged_weights_kernel")) return st;
   if (p.pieces == 1) return 0;
-  const uint32_t keys = (uint32_t)(p.tiles * kTile);
-  // (Several pieces: fewer sequences than workgroups that the work is dealt to.)
-  const dim3 join((keys + 255) / 256, (unsigned)cache->kv_heads, (unsigned)sequences);
-  hipLaunchKernelGGL(paged_weights_join_kernel, join, dim3(256), 0, s, w, keys);
+  // A workgroup a tile and head; with several pieces there are fewer than kManyWorkgroups.
+  const int64_t join = p.mixed ? kManyWorkgroups : p.tiles * sequences * cache->kv_heads;
+  hipLaunchKernelGGL(paged_weights_join_kernel, dim3((unsigned)join), dim3(kTile), 0, s, w);
   return check_launch("paged_weights_join_kernel");
 }

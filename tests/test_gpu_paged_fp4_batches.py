@@ -70,7 +70,6 @@ def test_weights_of_a_chunk_among_single_tokens(device, dtype, dim, group, causa
     lengths = [700, 4500] + [33, 1, 300] * 6
     chunks = [150, 1] + [1, 1, 1] * 6
     kv_heads = 2
-    assert sum(chunks) * group <= 64 * len(lengths)  # few rows a sequence, on average
     c = _case(device, 97, lengths, chunks, group * kv_heads, kv_heads, dim, 16, dtype)
     q, args = c.q.to(device), c.device_args()
     _, lse = paged.attention(q, c.cache, *args, causal=causal, return_lse=True)
@@ -82,6 +81,36 @@ def test_weights_of_a_chunk_among_single_tokens(device, dtype, dim, group, causa
     again = eviction.new_weights(c.cache)
     eviction.accumulate_weights(again, q, c.cache, *args[:2], lse, args[2], causal=causal)
     assert torch.equal(again, weights)
+
+
+@pytest.mark.parametrize("lengths,chunks,group,kv_heads,dim,dtype", [
+    # more sequences than threads, chunks of some, one that has more tokens than keys, one that has no keys
+    ([20 + b % 7 for b in range(300)] + [700, 30, 0, 90] + [20] * 300 + [300], [1] * 300 + [80, 60, 70, 90] + [0, 1, 1] * 100 + [17],
+     4, 2, 64, BF16),
+    ([20 + b % 7 for b in range(300)] + [700, 30, 0, 90] + [20] * 300 + [300], [1] * 300 + [80, 60, 70, 90] + [0, 1, 1] * 100 + [17],
+     4, 2, 128, FP4),
+    ([1000, 10] * 8, [70, 1] * 8, 1, 64, 64, F16),          # tiles enough without pieces of rows
+    ([1000, 10] * 8, [70, 1] * 8, 1, 64, 64, FP8),
+    ([100, 90, 80], [64, 1, 2], 1, 2, 128, BF16),           # as many rows as stay in the kernel of few
+    ([100, 90, 80], [65, 1, 2], 1, 2, 128, BF16),           # and one more
+    ([900, 5000, 300, 1], [900, 1, 200, 1], 8, 2, 128, FP4),  # most rows a chunk's
+    ([9, 300, 700], [0, 0, 600], 3, 2, 64, BF16),
+])
+def test_weights_of_chunks_among_single_tokens(device, lengths, chunks, group, kv_heads, dim, dtype) -> None:
+    print(f"weights of chunks among tokens: {len(lengths)} x {group}/{kv_heads}x{dim} {dtype}", flush=True)
+    c = _case(device, 100, lengths, chunks, group * kv_heads, kv_heads, dim, 16, dtype)
+    q, args = c.q.to(device), c.device_args()
+    _, lse = paged.attention(q, c.cache, *args, return_lse=True)
+    weights = eviction.new_weights(c.cache)
+    want, off = oracle.added_weights(_f64(c.q), np.nan_to_num(c.keys64), c.table.numpy(), lengths, c.starts,
+                                     lse.double().cpu().numpy(), dim**-0.5)
+    first = None
+    for _ in range(3):
+        weights.zero_()
+        eviction.accumulate_weights(weights, q, c.cache, *args[:2], lse, args[2])
+        assert (np.abs(weights.double().cpu().numpy() - want) <= off).all()
+        first = weights.clone() if first is None else first
+        assert torch.equal(weights, first)
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP4])
