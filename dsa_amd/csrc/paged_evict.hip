@@ -12,7 +12,8 @@
 // over the weights' order-preserving 32-bit keys, 11, 11 and 10 bits, and from it its
 // holes and its sources, the i-th of either being one move; the last launch moves keys,
 // values, scales and weights.  Up to 16K positions a list is one workgroup's, beyond
-// that the passes are launches.
+// that the passes are launches.  Where the page table has room for more, the device
+// knows which lists are longer: they are listed, and the launches deal out their chunks.
 #include <algorithm>
 #include <type_traits>
 
@@ -25,6 +26,13 @@ namespace {
 constexpr uint32_t kThreads = 1024;
 
 struct Threshold;
+
+// Lists that are longer than a workgroup's LDS has room for.
+struct Listed {
+  uint32_t count, chunks;
+  uint32_t unused[2];
+  uint2 of[1];  // {list, chunks of those before it}
+};
 
 struct EvictArgs {
   PagedView cache;
@@ -39,15 +47,16 @@ struct EvictArgs {
   int32_t* out_lengths;
   int64_t* kept;          // [sequences][lists][keep]
   // Workspace, for each list: the three passes' bins, its moves
-  // {to, from} (keep apart) and how many there are, and for long lists each chunk's
-  // counts and the order of every weight.
+  // {to, from} (keep apart) and how many there are; and of the chunks of long lists, one
+  // behind the other, counts and the order of every weight.
   uint32_t* bins;
   uint2* moves;
   uint32_t* counts;
   uint4* chunks;
   Threshold* thresholds;  // after each pass
   uint32_t* order;
-  uint64_t order_stride;
+  Listed* listed;         // null where no list can be long
+  uint32_t most_chunks;   // that there is room for
 };
 
 __device__ __forceinline__ uint32_t cache_row(const EvictArgs& a, const int32_t* table, uint32_t key) {
@@ -227,6 +236,36 @@ __device__ __forceinline__ void fill_kept(const EvictArgs& a, const List& l, uin
   for (uint32_t i = (l.n > l.m ? l.m : 0u) + first; i < a.keep; i += step) kept[i] = i < l.m ? (int64_t)i : -1;
 }
 
+// A list in one workgroup's LDS up to this many positions: 64 KiB of orders.
+constexpr uint32_t kMostInLds = 16 * kThreads;
+// Longer lists: a chunk of one a workgroup, one launch a pass.  The passes' counts meet
+// in global memory.
+constexpr uint32_t kChunkEach = 8;
+constexpr uint32_t kChunk = kThreads * kChunkEach;
+
+// Lists what is too long for one workgroup and loses keys.  One workgroup's work.  (Keys
+// of one place in the cache each have room; past that nothing is listed.)
+__device__ __forceinline__ void list_long(const EvictArgs& a, uint32_t lists, uint32_t* scan, uint32_t* listed) {
+  uint32_t count = 0, chunks = 0;  // `chunks` stops past the room, before it could wrap
+  if (threadIdx.x == 0) *listed = 0;
+  for (uint32_t base = 0; base < lists; base += kThreads) {
+    const uint32_t list = base + threadIdx.x;
+    const uint32_t n = list < lists ? keys_of(a, list / a.lists) : 0u;
+    const uint32_t own = n > kMostInLds && n > a.keep ? (n + kChunk - 1u) / kChunk : 0u;
+    uint32_t all_chunks, all;
+    const uint32_t before = chunks + block_excl_scan<16>(own, scan, all_chunks);
+    const bool fits = own > 0 && before + own <= a.most_chunks;  // those that do are the first
+    const uint32_t rank = block_excl_scan<16>(fits ? 1u : 0u, scan + 16, all);
+    if (fits) a.listed->of[count + rank] = make_uint2(list, before);
+    if (fits && rank + 1u == all) *listed = before + own;
+    count += all, chunks = min(chunks + all_chunks, a.most_chunks + 1u);
+    __syncthreads();
+  }
+  if (threadIdx.x > 0) return;
+  a.listed->count = count;
+  a.listed->chunks = *listed;
+}
+
 // One workgroup a list, whose orders lie in LDS: kEach neighbouring positions a thread,
 // so that every rank is one scan.  Latency bound: 11 us for one list of 4160 positions,
 // 19 us for 128 of 16K.
@@ -237,14 +276,24 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
   __shared__ __attribute__((aligned(16))) uint32_t scan[2][16];
   __shared__ Locate found;
   const uint32_t tid = threadIdx.x;
-  const uint32_t list = blockIdx.x;
+  if (a.listed && blockIdx.x == 0) {
+    list_long(a, gridDim.x - 1u, scan[0], bins);
+    return;
+  }
+  const uint32_t list = blockIdx.x - (a.listed ? 1u : 0u);
   const List l = list_of(a, list);
+  const bool whole = l.n == l.m || l.n > kThreads * kEach;  // nothing to evict, or other launches do
   if (tid == 0) {
     if (l.g == 0) a.out_lengths[l.sequence] = (int32_t)l.m;
-    if (l.n == l.m) a.counts[list] = 0;
+    if (whole) a.counts[list] = 0;
   }
   fill_kept(a, l, list, tid, kThreads);
   if (l.n == l.m) return;
+  if (whole) {
+    if (!a.listed) return;  // more keys than the cache has rows
+    for (uint32_t i = tid; i < 3u * kBins; i += kThreads) a.bins[(uint64_t)list * 3u * kBins + i] = 0;
+    return;
+  }
   for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
   uint32_t key[kEach];
   // (eight at a time, which leaves the registers of 1024 threads room)
@@ -296,34 +345,24 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
   if (tid == 0) a.counts[list] = holes;
 }
 
-// Longer lists: a chunk of one a workgroup, one launch a pass.  The passes' counts meet
-// in global memory.
-constexpr uint32_t kChunkEach = 8;
-constexpr uint32_t kChunk = kThreads * kChunkEach;
-
-// What a call's other launches add to, and what stays as it is.
-__global__ __launch_bounds__(256) void paged_evict_begin_kernel(EvictArgs a) {
-  const uint32_t list = blockIdx.y;
-  const List l = list_of(a, list);
-  const uint32_t at = blockIdx.x * 256u + threadIdx.x, step = gridDim.x * 256u;
-  if (at == 0) {
-    if (l.g == 0) a.out_lengths[l.sequence] = (int32_t)l.m;
-    a.counts[list] = 0;
-  }
-  for (uint32_t i = at; i < 3u * kBins; i += step) a.bins[(uint64_t)list * 3u * kBins + i] = 0;
-  fill_kept(a, l, list, at, step);
+// A chunk of a listed list.
+struct ChunkAt {
+  uint32_t list, before, chunk;  // chunks of other lists before the list's, and which of its own
+};
+__device__ __forceinline__ ChunkAt chunk_at(const Listed* listed, uint32_t item) {
+  const uint2 of = listed->of[last_at_most(listed->of, listed->count, item)];
+  return {of.x, of.y, item - of.y};
 }
-
 // The threshold after kPass passes: what the launch before this one's left of it, and
 // the digit that its bins say.
 template <int kPass>
-__device__ __forceinline__ Threshold threshold_of(const EvictArgs& a, const List& l, uint32_t list, Locate& found) {
+__device__ __forceinline__ Threshold threshold_of(const EvictArgs& a, const List& l, uint32_t list, uint32_t chunk, Locate& found) {
   Threshold t = {0u, l.want, 0u};
   if (kPass == 0 || l.want == 0) return t;
   Threshold* kept = a.thresholds + (uint64_t)list * 3u;
   if (kPass > 1) t = kept[kPass > 1 ? kPass - 2 : 0];
   locate_digit(a.bins + ((uint64_t)list * 3u + kPass - 1) * kBins, kPass - 1, found, t);
-  if (blockIdx.x == 0 && threadIdx.x == 0) kept[kPass - 1] = t;
+  if (chunk == 0 && threadIdx.x == 0) kept[kPass - 1] = t;
   return t;
 }
 
@@ -332,43 +371,46 @@ __global__ __launch_bounds__(kThreads) void paged_evict_count_kernel(EvictArgs a
   __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
   __shared__ Locate found;
   const uint32_t tid = threadIdx.x;
-  const uint32_t list = blockIdx.y;
-  const List l = list_of(a, list);
-  const uint32_t first = blockIdx.x * kChunk;
-  if (l.n == l.m || first >= l.old || l.want == 0) return;
-  const Threshold t = threshold_of<kPass>(a, l, list, found);
-  for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
-  __syncthreads();
-  uint32_t* order = a.order + (uint64_t)list * a.order_stride;
-  uint32_t own[kChunkEach];
-  if (kPass == 0) orders_of<kChunkEach>(a, l, first, own);
+  for (uint32_t item = blockIdx.x; item < a.listed->chunks; item += gridDim.x) {
+    const ChunkAt c = chunk_at(a.listed, item);
+    const List l = list_of(a, c.list);
+    const uint32_t first = c.chunk * kChunk;
+    if (first >= l.old || l.want == 0) continue;
+    const Threshold t = threshold_of<kPass>(a, l, c.list, c.chunk, found);
+    for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
+    __syncthreads();
+    uint32_t* order = a.order + (uint64_t)item * kChunk;
+    uint32_t own[kChunkEach];
+    if (kPass == 0) orders_of<kChunkEach>(a, l, first, own);
 #pragma unroll
-  for (uint32_t e = 0; e < kChunkEach; ++e) {
-    const uint32_t i = first + tid + kThreads * e;  // (inside the chunk's room, past the list's end too)
-    if (kPass == 0)
-      order[i] = own[e];
-    else
-      own[e] = order[i];
-  }
+    for (uint32_t e = 0; e < kChunkEach; ++e) {
+      const uint32_t i = tid + kThreads * e;  // (inside the chunk's room, past the list's end too)
+      if (kPass == 0)
+        order[i] = own[e];
+      else
+        own[e] = order[i];
+    }
 #pragma unroll
-  for (uint32_t e = 0; e < kChunkEach; ++e) {
-    const uint32_t i = first + tid + kThreads * e;
-    const uint32_t key = own[e];
-    const bool counts = i < l.old && (kPass == 0 || key >> kShift[kPass ? kPass - 1 : 0] == t.prefix >> kShift[kPass ? kPass - 1 : 0]);
-    if (counts) atomicAdd(&bins[key >> kShift[kPass] & (kPass == 2 ? 1023u : 2047u)], 1u);
+    for (uint32_t e = 0; e < kChunkEach; ++e) {
+      const uint32_t i = first + tid + kThreads * e;
+      const uint32_t key = own[e];
+      const bool counts = i < l.old && (kPass == 0 || key >> kShift[kPass ? kPass - 1 : 0] == t.prefix >> kShift[kPass ? kPass - 1 : 0]);
+      if (counts) atomicAdd(&bins[key >> kShift[kPass] & (kPass == 2 ? 1023u : 2047u)], 1u);
+    }
+    __syncthreads();
+    uint32_t* to = a.bins + ((uint64_t)c.list * 3u + kPass) * kBins;
+    for (uint32_t i = tid; i < kBins; i += kThreads)
+      if (bins[i]) atomicAdd(&to[i], bins[i]);
+    __syncthreads();
   }
-  __syncthreads();
-  uint32_t* to = a.bins + ((uint64_t)list * 3u + kPass) * kBins;
-  for (uint32_t i = tid; i < kBins; i += kThreads)
-    if (bins[i]) atomicAdd(&to[i], bins[i]);
 }
 
 // A thread's orders in a chunk: kChunkEach neighbouring positions.
-__device__ __forceinline__ void load_orders(const EvictArgs& a, const List& l, uint32_t list, uint32_t at,
+__device__ __forceinline__ void load_orders(const EvictArgs& a, const List& l, uint32_t item, uint32_t at,
                                             uint32_t (&key)[kChunkEach]) {
-  const uint32_t* order = a.order + (uint64_t)list * a.order_stride;
-  if (at < l.old && l.want > 0) {  // the chunk's room ends on a multiple of kChunkEach, and holds 0 past the list
-    const uint4 lo = *reinterpret_cast<const uint4*>(order + at), hi = *reinterpret_cast<const uint4*>(order + at + 4u);
+  const uint32_t* order = a.order + (uint64_t)item * kChunk + threadIdx.x * kChunkEach;
+  if (at < l.old && l.want > 0) {  // the chunk's room holds 0 past the list
+    const uint4 lo = *reinterpret_cast<const uint4*>(order), hi = *reinterpret_cast<const uint4*>(order + 4);
     key[0] = lo.x, key[1] = lo.y, key[2] = lo.z, key[3] = lo.w;
     key[4] = hi.x, key[5] = hi.y, key[6] = hi.z, key[7] = hi.w;
   } else {
@@ -382,33 +424,35 @@ __device__ __forceinline__ void load_orders(const EvictArgs& a, const List& l, u
 __global__ __launch_bounds__(kThreads) void paged_evict_chunk_kernel(EvictArgs a) {
   __shared__ Locate found;
   __shared__ uint32_t sums[4];
-  const uint32_t list = blockIdx.y;
-  const List l = list_of(a, list);
-  const uint32_t first = blockIdx.x * kChunk;
-  if (l.n == l.m || first >= l.n) return;
-  const Threshold t = threshold_of<3>(a, l, list, found);
-  if (threadIdx.x < 4u) sums[threadIdx.x] = 0;
-  __syncthreads();
-  const uint32_t at = first + threadIdx.x * kChunkEach;
-  uint32_t key[kChunkEach];
-  load_orders(a, l, list, at, key);
-  uint32_t count[4] = {0u, 0u, 0u, 0u};
+  for (uint32_t item = blockIdx.x; item < a.listed->chunks; item += gridDim.x) {
+    const ChunkAt c = chunk_at(a.listed, item);
+    const List l = list_of(a, c.list);
+    const uint32_t first = c.chunk * kChunk;
+    const Threshold t = threshold_of<3>(a, l, c.list, c.chunk, found);
+    if (threadIdx.x < 4u) sums[threadIdx.x] = 0;
+    __syncthreads();
+    const uint32_t at = first + threadIdx.x * kChunkEach;
+    uint32_t key[kChunkEach];
+    load_orders(a, l, item, at, key);
+    uint32_t count[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-  for (uint32_t e = 0; e < kChunkEach; ++e) {
-    const uint32_t past = at + e >= l.m ? 2u : 0u;
-    const bool level = l.want > 0 && at + e < l.old && key[e] == t.prefix;
-    const bool sure = at + e < l.n && (at + e >= l.old || (l.want > 0 && key[e] > t.prefix));
+    for (uint32_t e = 0; e < kChunkEach; ++e) {
+      const uint32_t past = at + e >= l.m ? 2u : 0u;
+      const bool level = l.want > 0 && at + e < l.old && key[e] == t.prefix;
+      const bool sure = at + e < l.n && (at + e >= l.old || (l.want > 0 && key[e] > t.prefix));
 #pragma unroll
-    for (uint32_t c = 0; c < 4; ++c) count[c] += (c == past && level) || (c == past + 1u && sure);
+      for (uint32_t i = 0; i < 4; ++i) count[i] += (i == past && level) || (i == past + 1u && sure);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(count[i]), kWave - 1);
+      if (lane_id() == 0 && all) atomicAdd(&sums[i], all);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      a.chunks[item] = make_uint4(sums[0], sums[1], sums[2], sums[3]);
+    __syncthreads();
   }
-#pragma unroll
-  for (uint32_t c = 0; c < 4; ++c) {
-    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(count[c]), kWave - 1);
-    if (lane_id() == 0 && all) atomicAdd(&sums[c], all);
-  }
-  __syncthreads();
-  if (threadIdx.x == 0)
-    a.chunks[(uint64_t)list * gridDim.x + blockIdx.x] = make_uint4(sums[0], sums[1], sums[2], sums[3]);
 }
 
 // What is kept, a chunk a workgroup, from the counts of the chunks before it.
@@ -416,48 +460,50 @@ __global__ __launch_bounds__(kThreads) void paged_evict_settle_kernel(EvictArgs 
   __shared__ __attribute__((aligned(16))) uint32_t scan[2][16];
   __shared__ uint32_t moving[kChunk], masks[kThreads];
   __shared__ uint32_t start[3];  // ranks of the chunk's first: key at the threshold, hole, source
-  const uint32_t list = blockIdx.y;
-  const List l = list_of(a, list);
-  const uint32_t first = blockIdx.x * kChunk;
-  if (l.n == l.m || first >= l.n) return;
-  const Threshold t = l.want > 0 ? a.thresholds[(uint64_t)list * 3u + 2u] : Threshold{0u, 0u, 0u};
-  if (threadIdx.x < kWave) {
-    // Keys at the threshold are kept while their rank is below t.rest; that rank follows
-    // the chunks, so a chunk keeps as many as are left of them.
-    uint32_t level = 0, kept_below = 0, kept_past = 0;
-    for (uint32_t base = 0; base < blockIdx.x; base += kWave) {
-      const uint32_t c = base + lane_id();
-      const uint4 v = c < blockIdx.x ? a.chunks[(uint64_t)list * gridDim.x + c] : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t upto = level + wave_incl_scan(v.x + v.z);
-      const uint32_t from = upto - v.x - v.z;
-      const uint32_t limit = t.ties ? t.rest : 0xffffffffu;
-      const uint32_t below = min(v.x, limit - min(limit, from));
-      const uint32_t past = min(v.z, limit - min(limit, from + v.x));
-      kept_below += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(v.y + below), kWave - 1);
-      kept_past += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(v.w + past), kWave - 1);
-      level = (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
+  for (uint32_t item = blockIdx.x; item < a.listed->chunks; item += gridDim.x) {
+    const ChunkAt c = chunk_at(a.listed, item);
+    const List l = list_of(a, c.list);
+    const uint32_t first = c.chunk * kChunk;
+    const Threshold t = l.want > 0 ? a.thresholds[(uint64_t)c.list * 3u + 2u] : Threshold{0u, 0u, 0u};
+    if (threadIdx.x < kWave) {
+      // Keys at the threshold are kept while their rank is below t.rest; that rank follows
+      // the chunks, so a chunk keeps as many as are left of them.
+      uint32_t level = 0, kept_below = 0, kept_past = 0;
+      for (uint32_t base = 0; base < c.chunk; base += kWave) {
+        const uint32_t i = base + lane_id();
+        const uint4 v = i < c.chunk ? a.chunks[c.before + i] : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t upto = level + wave_incl_scan(v.x + v.z);
+        const uint32_t from = upto - v.x - v.z;
+        const uint32_t limit = t.ties ? t.rest : 0xffffffffu;
+        const uint32_t below = min(v.x, limit - min(limit, from));
+        const uint32_t past = min(v.z, limit - min(limit, from + v.x));
+        kept_below += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(v.y + below), kWave - 1);
+        kept_past += (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan(v.w + past), kWave - 1);
+        level = (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
+      }
+      if (threadIdx.x == 0) {
+        start[0] = level;
+        start[1] = min(first, l.m) - kept_below;
+        start[2] = kept_past;
+      }
     }
-    if (threadIdx.x == 0) {
-      start[0] = level;
-      start[1] = min(first, l.m) - kept_below;
-      start[2] = kept_past;
-    }
-  }
-  __syncthreads();
-  const uint32_t at = first + threadIdx.x * kChunkEach;
-  uint32_t key[kChunkEach];
-  load_orders(a, l, list, at, key);
-  uint32_t rank = start[0], all;
-  if (t.ties) {
-    uint32_t level = 0;
+    __syncthreads();
+    const uint32_t at = first + threadIdx.x * kChunkEach;
+    uint32_t key[kChunkEach];
+    load_orders(a, l, item, at, key);
+    uint32_t rank = start[0], all;
+    if (t.ties) {
+      uint32_t level = 0;
 #pragma unroll
-    for (uint32_t e = 0; e < kChunkEach; ++e) level += at + e < l.old && key[e] == t.prefix;
-    rank += block_excl_scan<16>(level, scan[0], all);
+      for (uint32_t e = 0; e < kChunkEach; ++e) level += at + e < l.old && key[e] == t.prefix;
+      rank += block_excl_scan<16>(level, scan[0], all);
+    }
+    const uint32_t keeps = kept_of<kChunkEach>(l, t, key, at, rank);
+    const uint32_t before = block_excl_scan<16>(count_moves<kChunkEach>(l, at, keeps), scan[1], all);
+    settle<kChunkEach>(a, l, c.list, first, keeps, before, all, start[1], start[2], moving, masks);
+    if (threadIdx.x == 0 && first < l.m && l.m <= first + kChunk) a.counts[c.list] = start[1] + (all & 0xffffu);
+    __syncthreads();
   }
-  const uint32_t keeps = kept_of<kChunkEach>(l, t, key, at, rank);
-  const uint32_t before = block_excl_scan<16>(count_moves<kChunkEach>(l, at, keeps), scan[1], all);
-  settle<kChunkEach>(a, l, list, first, keeps, before, all, start[1], start[2], moving, masks);
-  if (threadIdx.x == 0 && first < l.m && l.m <= first + kChunk) a.counts[list] = start[1] + (all & 0xffffu);
 }
 
 // Moves: 16 bytes of a head's key and of its value a thread, two at a time; a move's
@@ -476,7 +522,7 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a) {
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
   const uint2* moves = a.moves + (uint64_t)list * a.keep;
   const uint32_t count = a.counts[list];
-  if (a.chunks) {
+  if (a.listed) {  // (a long list's; the others' again)
     for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < count; i += gridDim.x * 256u)
       a.kept[(uint64_t)list * a.keep + moves[i].x] = moves[i].y;
   }
@@ -573,27 +619,33 @@ void launch_move(const EvictArgs& a, int32_t pieces, dim3 grid, hipStream_t s) {
   }
 }
 
-// A list in one workgroup's LDS up to this room in the page table: 64 KiB of orders.
-constexpr int64_t kMostInLds = 16 * kThreads;
+constexpr int64_t kChunkWorkgroups = 512;  // that long lists' chunks are dealt to: what runs at a time
 
 struct EvictPlan {
-  int64_t lists, chunks, order_stride;  // no chunks: one workgroup a list
-  int64_t bins, moves, counts, thresholds, chunk_counts, bytes;  // offsets
+  int64_t lists, most_chunks;  // no chunks: every list is one workgroup's
+  int64_t moves, counts, thresholds, listed, chunk_counts, order, bytes;  // offsets, after the bins
 };
 
 EvictPlan evict_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t columns, int64_t keep, bool per_head) {
   EvictPlan p = {};
-  const int64_t capacity = columns * cache->page_size;
-  p.lists = sequences * (per_head ? cache->kv_heads : 1);
-  if (capacity > kMostInLds) {
-    p.chunks = (capacity + kChunk - 1) / kChunk;
-    p.order_stride = p.chunks * kChunk;
+  const int64_t capacity = columns * cache->page_size, heads = per_head ? cache->kv_heads : 1;
+  p.lists = sequences * heads;
+  const int64_t rows = cache->pages * cache->page_size;
+  if (std::min(capacity, rows) > kMostInLds) {
+    // A cache row is one sequence's, and a list of more than two chunks has at most half
+    // as many again as its keys fill.  (Each list by its own length: 256 sequences of 4160
+    // keys, a list a head of 8, in tables with room for 128K: 140 us, and 1490 with every
+    // list in chunks; with room for 8K 101.)
+    static_assert(kMostInLds == 2 * kChunk, "");
+    p.most_chunks = std::min(heads * std::min(sequences * ((capacity + kChunk - 1) / kChunk), rows * 3 / kMostInLds), (int64_t)1 << 30);
   }
-  p.moves = p.chunks ? p.lists * 3 * kBins * 4 : 0;
+  p.moves = p.most_chunks ? p.lists * 3 * kBins * 4 : 0;
   p.counts = p.moves + p.lists * keep * 8;
   p.thresholds = p.counts + p.lists * 4;
-  p.chunk_counts = (p.thresholds + p.lists * 36 + 15) / 16 * 16;
-  p.bytes = p.chunk_counts + p.lists * p.chunks * 16 + p.lists * p.order_stride * 4;
+  p.listed = (p.thresholds + p.lists * 36 + 15) / 16 * 16;
+  p.chunk_counts = p.listed + (p.most_chunks ? (16 + p.lists * 8 + 15) / 16 * 16 : 0);
+  p.order = p.chunk_counts + p.most_chunks * 16;
+  p.bytes = p.order + p.most_chunks * kChunk * 4;
   return p;
 }
 
@@ -641,26 +693,26 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
   a.moves = reinterpret_cast<uint2*>(base + p.moves);
   a.counts = reinterpret_cast<uint32_t*>(base + p.counts);
   a.thresholds = reinterpret_cast<Threshold*>(base + p.thresholds);
-  a.chunks = p.chunks ? reinterpret_cast<uint4*>(base + p.chunk_counts) : nullptr;
-  a.order = reinterpret_cast<uint32_t*>(base + p.chunk_counts + p.lists * p.chunks * 16);
-  a.order_stride = (uint64_t)p.order_stride;
+  a.chunks = reinterpret_cast<uint4*>(base + p.chunk_counts);
+  a.order = reinterpret_cast<uint32_t*>(base + p.order);
+  a.listed = p.most_chunks ? reinterpret_cast<Listed*>(base + p.listed) : nullptr;
+  a.most_chunks = (uint32_t)p.most_chunks;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t capacity = columns * cache->page_size;
-  const dim3 lists((unsigned)p.lists);
-  if (p.chunks) {
-    const dim3 chunks((unsigned)p.chunks, (unsigned)p.lists);
-    hipLaunchKernelGGL(paged_evict_begin_kernel, dim3(4, (unsigned)p.lists), dim3(256), 0, s, a);
+  const dim3 lists((unsigned)p.lists + (p.most_chunks ? 1u : 0u));
+  if (capacity > 8 * kThreads)
+    hipLaunchKernelGGL(paged_evict_select_kernel<16>, lists, dim3(kThreads), 0, s, a);
+  else if (capacity > 2 * kThreads)
+    hipLaunchKernelGGL(paged_evict_select_kernel<8>, lists, dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(paged_evict_select_kernel<2>, lists, dim3(kThreads), 0, s, a);
+  if (p.most_chunks) {
+    const dim3 chunks((unsigned)std::min(p.most_chunks, kChunkWorkgroups));
     hipLaunchKernelGGL(paged_evict_count_kernel<0>, chunks, dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL(paged_evict_count_kernel<1>, chunks, dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL(paged_evict_count_kernel<2>, chunks, dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL(paged_evict_chunk_kernel, chunks, dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL(paged_evict_settle_kernel, chunks, dim3(kThreads), 0, s, a);
-  } else if (capacity > 8 * kThreads) {
-    hipLaunchKernelGGL(paged_evict_select_kernel<16>, lists, dim3(kThreads), 0, s, a);
-  } else if (capacity > 2 * kThreads) {
-    hipLaunchKernelGGL(paged_evict_select_kernel<8>, lists, dim3(kThreads), 0, s, a);
-  } else {
-    hipLaunchKernelGGL(paged_evict_select_kernel<2>, lists, dim3(kThreads), 0, s, a);
   }
   if (int st = check_launch("paged_evict_select_kernel")) return st;
   // A list moves at most keep keys, and no more than lie past it.

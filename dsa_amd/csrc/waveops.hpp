@@ -71,6 +71,19 @@ __device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* ws, ui
   return before + incl - v;
 }
 
+// The last of `count` ascending entries whose y is at most `at`; that of the first is 0.
+// For whole waves: 64 entries are looked at at a time.
+__device__ __forceinline__ uint32_t last_at_most(const uint2* of, uint32_t count, uint32_t at) {
+  uint32_t low = 0, high = count;
+  while (high - low > 1u) {
+    const uint32_t apart = (high - low + kWave - 1u) / kWave;
+    const uint32_t i = low + lane_id() * apart;
+    low += ((uint32_t)__popcll(__ballot(i < high && of[min(i, high - 1u)].y <= at)) - 1u) * apart;
+    high = min(low + apart, high);
+  }
+  return low;
+}
+
 __device__ __forceinline__ uint32_t lanes_below(uint64_t m) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
 }

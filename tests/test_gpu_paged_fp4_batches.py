@@ -11,7 +11,7 @@ import torch
 
 from dsa_amd import eviction, paged
 from oracle import eviction as oracle
-from test_gpu_eviction import _case
+from test_gpu_eviction import _case, _check_eviction
 from test_gpu_paged import BF16, F16, FP8, _f64
 from test_gpu_paged_fp4 import FP4, Case4
 from test_gpu_paged_padded import _check_padding, _padded, _soil_memory
@@ -111,6 +111,46 @@ def test_weights_of_chunks_among_single_tokens(device, lengths, chunks, group, k
         assert (np.abs(weights.double().cpu().numpy() - want) <= off).all()
         first = weights.clone() if first is None else first
         assert torch.equal(weights, first)
+
+
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("lengths,kv_heads,page,dtype,room,keep,recent", [
+    ([300, 64, 63, 65], 2, 16, BF16, 40000, 64, 10),             # short lists, room for long ones
+    ([5000, 4097, 4096], 2, 32, FP4, 1 << 20, 4000, 77),
+    ([16384, 16385, 0, 40000, 9000], 2, 64, BF16, 1 << 17, 5000, 9),
+    ([30000, 16390, 20], 1, 16, FP8, 30016, 30000, 0),           # long, and nothing to evict
+    ([3] * 150 + [17000] + [5, 2, 9] * 200 + [16500, 1, 25000], 2, 4, FP4, 30000, 4, 1),  # more lists than threads
+])
+def test_eviction_with_room_for_more(device, lengths, kv_heads, page, dtype, room, keep, recent, per_head) -> None:
+    """Each list by its own length, whatever the page table has room for; page ids past
+    the lengths are any."""
+
+    print(f"room for {room}: {len(lengths)} x {kv_heads} {dtype} keep {keep} {per_head}", flush=True)
+    c = _case(device, 101, lengths, [0] * len(lengths), kv_heads, kv_heads, 64, page, dtype)
+    more = -(-room // page) - c.table.shape[1]
+    gen = torch.Generator().manual_seed(7)
+    if more > 0:
+        c.table = torch.cat([c.table, torch.randint(-5, 1 << 30, (len(lengths), more), generator=gen, dtype=torch.int32)], 1)
+    weights = torch.randint(0, 1000, (kv_heads, c.cache.rows), generator=gen) * 0.125
+    _check_eviction(device, c, weights.to(device), keep, recent, per_head)
+
+
+def test_lengths_beyond_a_small_cache(device) -> None:
+    """More keys than the cache has rows: unspecified results, and the next call's are
+    what they should be."""
+
+    cache = paged.new_cache(20, 16, 2, 64, device=device)
+    cache.keys.zero_(), cache.values.zero_()
+    table = torch.zeros(2, 2000, dtype=torch.int32, device=device)
+    weights = eviction.new_weights(cache)
+    for n in (20000, 16384, 1 << 30, -5):
+        lengths = torch.tensor([n, 3], dtype=torch.int32, device=device)
+        out, _ = eviction.evict(cache, table, lengths, weights, 64, recent=3, per_head=True)
+        assert out.tolist() == [max(0, min(n, 64)), 3]
+    table[0, :20] = torch.arange(20)
+    weights[:] = torch.arange(320, device=device).flip(0)
+    out, kept = eviction.evict(cache, table[:1], torch.tensor([320], dtype=torch.int32, device=device), weights, 64)
+    assert out.tolist() == [64] and kept[0].tolist() == list(range(64))
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP4])
