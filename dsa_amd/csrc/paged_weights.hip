@@ -29,6 +29,12 @@ namespace {
 
 constexpr uint32_t kStage = 64;  // rows in LDS at a time
 constexpr int64_t kManyWorkgroups = 2048;  // that the work is dealt to, where there is as much
+// The same for few rows, two a CU, each then of up to 32 steps in turn: a start and an end
+// cost as much as some steps.  (us, dealt to 256 / 512 / 1024 / 2048: one sequence of 32K
+// bf16 keys, 8 heads of 128 dims, 16.6 / 16.8 / 19.9 / 25.0, 16 of 4096 4-bit ones 18.6 /
+// 15.4 / 16.4 / 18.8; 16 of 32K bf16 keys, which have more steps than that, 218 to 220.)
+constexpr int64_t kFewWorkgroups = 512;
+constexpr uint32_t kMostSteps = 32;
 
 // Sequences of many rows among some of few.
 struct Chunks {
@@ -41,10 +47,12 @@ struct WeightArgs {
   PagedAttentionArgs batch;
   Quotient by_group;  // of a row: its token
   float* weights;     // [kv_heads][cache rows]
-  float* parts;       // of several pieces: [sequences][kv_heads][pieces][tiles * keys of a tile]
-  uint32_t tiles;     // of keys, of the longest sequence that the page table has room for
-  uint32_t pieces;    // of each tile's rows
-  uint32_t steps;     // few rows: of a wave
+  float* parts;       // of several pieces: [sequences][kv_heads][share][keys of a tile]
+  // Workgroups of each sequence and kv head: what there is work for (its tiles of keys are
+  // cut into that many pieces of rows, or spread over as many workgroups), and how many
+  // there are, which a sequence of more takes in turn.
+  uint32_t share, slots;
+  uint32_t few_share, few_slots;
   Chunks* chunks;     // of a mixed batch; else all sequences are one kernel's
   uint64_t row_count;
 };
@@ -291,6 +299,17 @@ __device__ __forceinline__ void weigh_tile(const WeightArgs& w, uint32_t g, uint
   }
 }
 
+// How a sequence's work is cut where it has w.share workgroups: by its own keys, whatever
+// the page table has room for.
+struct Cut {
+  uint32_t tiles, pieces;  // of each tile's rows
+};
+__device__ __forceinline__ Cut cut_of(const WeightArgs& w, uint32_t sequence) {
+  const uint32_t tiles = (keys_of(w.batch, sequence) + kTile - 1u) / kTile;
+  const uint32_t rows = tokens_of(w.batch, sequence).count * w.batch.group;
+  return {tiles, max(1u, min(w.share / max(tiles, 1u), (rows + 4u * kStage - 1u) / (4u * kStage)))};
+}
+
 // Heads vary fastest, then pieces, then tiles: a causal chunk's first keys, which most
 // rows see, come first.
 template <class Tag, Store kStore, int D>
@@ -299,11 +318,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_weights_kernel(We
   uint32_t id = blockIdx.x;
   const uint32_t g = id % heads;
   id /= heads;
-  const uint32_t piece = id % w.pieces;
-  id /= w.pieces;
-  const uint32_t sequence = id % w.batch.sequences, tile = id / w.batch.sequences;
-  weigh_tile<Tag, kStore, D>(w, g, sequence, tile, piece, w.pieces,
-                             w.parts + ((((uint64_t)sequence * heads + g) * w.pieces + piece) * w.tiles + tile) * kTile);
+  const uint32_t sequence = id % w.batch.sequences;
+  const Cut cut = cut_of(w, sequence);
+  for (uint32_t item = id / w.batch.sequences; item < cut.tiles * cut.pieces; item += w.slots)
+    weigh_tile<Tag, kStore, D>(w, g, sequence, item / cut.pieces, item % cut.pieces, cut.pieces,
+                               w.parts + (((uint64_t)sequence * heads + g) * w.share + item) * kTile);
 }
 
 // A listed sequence's tile.
@@ -366,7 +385,7 @@ __device__ __forceinline__ void list_chunks(const WeightArgs& w, uint32_t* scan)
 
 // Few rows: those of a sequence, up to kStage, lie in LDS while its keys pass by, 32 a wave and step,
 // loaded as 128 neighbouring bytes by eight lanes, through LDS of the wave's own.  A
-// workgroup takes w.steps steps of each of its four waves.  A wave has 16 KiB of keys on
+// workgroup takes up to kMostSteps steps of each of its four waves, and more in turn.  A wave has 16 KiB of keys on
 // their way, whatever their type (8 KiB: 227 us for 16 sequences of 32K bf16 keys), and
 // nothing that the steps wait for is loaded after them: cache rows are looked up a group
 // of steps ahead, a row's powers of two come with it.
@@ -406,14 +425,16 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
   id /= a.cache.kv_heads;
   const uint32_t sequence = id % a.sequences;
   const uint32_t length = keys_of(a, sequence);
-  const uint32_t tile0 = id / a.sequences * (4u * kStep * w.steps);
+  // Neighbouring steps a workgroup, as many as its share of the sequence.
+  const uint32_t most = min(max((length + 4u * kStep * w.few_share - 1u) / (4u * kStep * w.few_share), 1u), kMostSteps);
+  uint32_t tile0 = id / a.sequences * (4u * kStep * most);
   if (tile0 >= length) return;
   const Span span = tokens_of(a, sequence);
   const int64_t before = (int64_t)length - span.count;
   const uint32_t rows = span.count * a.group;
   if (rows == 0 || rows > kStage) return;  // (more: listed)
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
-  const uint32_t steps = min(w.steps, (length - tile0 + 4u * kStep - 1u) / (4u * kStep));
+  uint32_t steps;
   const uint32_t load_row = lane / kLanes, load_chunk = lane % kLanes;
   const char* key_base = a.cache.keys + g * a.cache.key_head + 16u * load_chunk;
   auto first_key = [&](uint32_t step) { return tile0 + (4u * step + wave) * kStep; };
@@ -460,26 +481,6 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
     }
   };
 
-  Tile t[kAhead];
-  look(0);
-  place(0);
-#pragma unroll
-  for (uint32_t i = 0; i < kAhead; ++i) load(t[i], min(i, steps - 1u));
-  for (uint32_t at = tid; at < rows * kRuns; at += 256u) {
-    const uint32_t r = at / kRuns;
-    const uint32_t i = w.by_group(r);
-    *reinterpret_cast<u32x4*>(rows_tile + r * kRow + at % kRuns * 16u) =
-        *reinterpret_cast<const u32x4*>(a.queries + (int64_t)(span.first + i) * a.query_stride +
-                                        ((uint64_t)(g * a.group + r - i * a.group) * D + at % kRuns * 8u) * 2u);
-  }
-  if (tid < kStage) {
-    const uint32_t r = min(tid, rows - 1u);
-    const uint32_t i = w.by_group(r);
-    const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
-    const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r - i * a.group];
-    row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
-  }
-  __syncthreads();
   auto compute = [&](uint32_t step, float scale, const uint32_t (&power)[kPowerWords]) {
     const char* mine = key_tile[wave];
     const uint32_t key0 = first_key(step);
@@ -548,29 +549,54 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
     }
     wave_order();
   };
-  for (uint32_t step0 = 0; step0 < steps; step0 += kAhead) {
+  for (bool first = true; tile0 < length; first = false, tile0 += w.few_slots * (4u * kStep * most)) {
+    steps = min(most, (length - tile0 + 4u * kStep - 1u) / (4u * kStep));
+    Tile t[kAhead];
+    look(0);
+    place(0);
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) {
-      const uint32_t step = step0 + i;
-      const uint32_t group = step / kGroup + 1u;
-      if (group * kGroup < steps) {
-        if (step % kGroup == 0) look(group);
-        if (step % kGroup == 3) place(group);
+    for (uint32_t i = 0; i < kAhead; ++i) load(t[i], min(i, steps - 1u));
+    if (first) {
+      for (uint32_t at = tid; at < rows * kRuns; at += 256u) {
+        const uint32_t r = at / kRuns;
+        const uint32_t i = w.by_group(r);
+        *reinterpret_cast<u32x4*>(rows_tile + r * kRow + at % kRuns * 16u) =
+            *reinterpret_cast<const u32x4*>(a.queries + (int64_t)(span.first + i) * a.query_stride +
+                                            ((uint64_t)(g * a.group + r - i * a.group) * D + at % kRuns * 8u) * 2u);
       }
-      char* mine = key_tile[wave];
+      if (tid < kStage) {
+        const uint32_t r = min(tid, rows - 1u);
+        const uint32_t i = w.by_group(r);
+        const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
+        const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r - i * a.group];
+        row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
+      }
+      __syncthreads();
+    }
+    for (uint32_t step0 = 0; step0 < steps; step0 += kAhead) {
 #pragma unroll
-      for (int p = 0; p < kPasses; ++p)
+      for (uint32_t i = 0; i < kAhead; ++i) {
+        const uint32_t step = step0 + i;
+        const uint32_t group = step / kGroup + 1u;
+        if (group * kGroup < steps) {
+          if (step % kGroup == 0) look(group);
+          if (step % kGroup == 3) place(group);
+        }
+        char* mine = key_tile[wave];
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j)
-          *reinterpret_cast<u32x4*>(mine + (kRows * p + load_row) * kKeyRow + (kLanes * j + load_chunk) * 16u) = t[i].k[p][j];
-      const float scale = t[i].scale;
-      uint32_t power[kPowerWords];
+        for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-      for (int p = 0; p < kPowerWords; ++p) power[p] = t[i].power[p];
-      wave_order();
-      load(t[i], min(step + kAhead, steps - 1u));
-      __builtin_amdgcn_sched_barrier(0);
-      if (step < steps) compute(step, scale, power);
+          for (int j = 0; j < kLoads; ++j)
+            *reinterpret_cast<u32x4*>(mine + (kRows * p + load_row) * kKeyRow + (kLanes * j + load_chunk) * 16u) = t[i].k[p][j];
+        const float scale = t[i].scale;
+        uint32_t power[kPowerWords];
+#pragma unroll
+        for (int p = 0; p < kPowerWords; ++p) power[p] = t[i].power[p];
+        wave_order();
+        load(t[i], min(step + kAhead, steps - 1u));
+        __builtin_amdgcn_sched_barrier(0);
+        if (step < steps) compute(step, scale, power);
+      }
     }
   }
 }
@@ -580,40 +606,42 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
 __global__ __launch_bounds__(kTile) void paged_weights_join_kernel(WeightArgs w) {
   const PagedAttentionArgs& a = w.batch;
   const uint32_t heads = a.cache.kv_heads;
-  const uint32_t pieces = w.chunks ? w.chunks->pieces : w.pieces;
   const uint32_t g = blockIdx.x % heads, at = blockIdx.x / heads;
-  uint32_t sequence, tile;
-  uint64_t part, apart;  // of piece 0, and from a piece to the next
+  uint32_t sequence, tile, pieces;
+  uint64_t part;
   if (w.chunks) {
+    pieces = w.chunks->pieces;
     if (pieces == 1u || at >= w.chunks->tiles) return;
     const ChunkTile t = chunk_tile(w.chunks, at);
     sequence = t.sequence, tile = t.tile;
-    part = ((uint64_t)at * heads + g) * pieces * kTile;
-    apart = kTile;
+    part = ((uint64_t)at * heads + g) * pieces;
   } else {
-    sequence = at / w.tiles, tile = at % w.tiles;
-    part = (((uint64_t)sequence * heads + g) * pieces * w.tiles + tile) * kTile;
-    apart = (uint64_t)w.tiles * kTile;
+    sequence = at % a.sequences, tile = at / a.sequences;
+    const Cut cut = cut_of(w, sequence);
+    pieces = cut.pieces;
+    if (pieces == 1u || tile >= cut.tiles) return;
+    part = ((uint64_t)sequence * heads + g) * w.share + tile * pieces;
   }
   const uint32_t key = tile * kTile + threadIdx.x;
   if (key >= keys_of(a, sequence)) return;
-  const float* from = w.parts + part + threadIdx.x;
+  const float* from = w.parts + part * kTile + threadIdx.x;
   float sum = 0.f;
 #pragma unroll 4
-  for (uint32_t p = 0; p < pieces; ++p) sum += from[p * apart];
+  for (uint32_t p = 0; p < pieces; ++p) sum += from[(uint64_t)p * kTile];
   add_weight(w, a.page_table + (int64_t)sequence * a.table_stride, g, key, sum);
 }
 
 struct WeightPlan {
   bool few, mixed;
-  int64_t tiles, steps, pieces, list_bytes, part_bytes;  // mixed: pieces at most
-  int64_t chunk_workgroups;
+  int64_t share, slots, few_share, few_slots;
+  int64_t pieces;  // of a tile's rows, at most
+  int64_t chunk_workgroups, list_bytes, part_bytes;
   int64_t bytes() const { return list_bytes + part_bytes; }
 };
 
 WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens, int64_t heads, int64_t capacity,
                        bool uniform) {
-  const int64_t group = heads / cache->kv_heads;
+  const int64_t group = heads / cache->kv_heads, pairs = sequences * cache->kv_heads;
   WeightPlan p = {};
   // With `starts` each sequence has the kernel of its own rows.  (us, so / all in the
   // kernel that the average rows say, 32 heads on 8 of 128 dims: 256 tokens over 4096 bf16
@@ -621,33 +649,37 @@ WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t 
   // 182 / 402; chunks of 300, 60, 200 and 40 tokens, a launch or two less, 22 / 16.)
   p.mixed = !uniform && sequences > 1 && tokens * group > kStage;
   p.few = p.mixed || tokens * group <= kStage * sequences;
-  const int64_t keys = p.few ? 128 : kTile;  // of a tile, at least
-  p.tiles = (capacity + keys - 1) / keys;
-  const int64_t wide = p.tiles * cache->kv_heads * sequences;
-  p.pieces = 1;
+  // Workgroups by what keeps the GPU busy; for sequences of more keys than that has tiles
+  // for, as many as the page table's room asks for, while their starts cost little.  What
+  // each does follows from the keys that its sequence has.  (Prompt of 4096 tokens, bf16,
+  // in a table with room for 128K keys: 92 us, and 365 with the work cut by the room.)
+  const int64_t tiles = (capacity + kTile - 1) / kTile;
+  auto slots = [&](int64_t share, int64_t of_room) {
+    return std::max(share, std::min(of_room, 4 * kManyWorkgroups / pairs));
+  };
   if (p.few) {
-    // Steps that leave the GPU some rounds of workgroups, up to what hides a start.
-    p.steps = wide / kManyWorkgroups;
-    p.steps = p.steps < 1 ? 1 : p.steps > 32 ? 32 : p.steps;
-    p.tiles = (p.tiles + p.steps - 1) / p.steps;
-    if (p.mixed) {
-      // What can be listed: sequences of more than kStage rows, pieces of 4 kStage each.
-      const int64_t listed = std::min(sequences, tokens * group / (kStage + 1));
-      p.pieces = std::min(kManyWorkgroups, (tokens * group + 4 * kStage - 1) / (4 * kStage));
-      // (12 sequences of 240 rows over 116K keys of 64 dims, 5460 tiles, by 2048 workgroups
-      // 115 us, by 4096 109; nothing listed, no difference.)
-      p.chunk_workgroups = std::min(2 * kManyWorkgroups, listed * ((capacity + kTile - 1) / kTile) * cache->kv_heads * p.pieces);
-      p.list_bytes = (16 + sequences * 8 + 15) / 16 * 16;
-      if (p.pieces > 1) p.part_bytes = 2 * kManyWorkgroups * kTile * 4;  // several pieces are fewer than twice the workgroups
-    }
-  } else {
+    p.few_share = (kFewWorkgroups + pairs - 1) / pairs;
+    p.few_slots = std::min(slots(p.few_share, (2 * tiles + kMostSteps - 1) / kMostSteps), 2 * tiles);
+  }
+  if (p.mixed) {
+    // What can be listed: sequences of more than kStage rows, pieces of 4 kStage each.
+    const int64_t listed = std::min(sequences, tokens * group / (kStage + 1));
+    p.pieces = std::min(kManyWorkgroups, (tokens * group + 4 * kStage - 1) / (4 * kStage));
+    // (12 sequences of 240 rows over 116K keys of 64 dims, 5460 tiles, by 2048 workgroups
+    // 115 us, by 4096 109; nothing listed, no difference.)
+    p.chunk_workgroups = std::min(2 * kManyWorkgroups, listed * tiles * cache->kv_heads * p.pieces);
+    p.list_bytes = (16 + sequences * 8 + 15) / 16 * 16;
+    if (p.pieces > 1) p.part_bytes = 2 * kManyWorkgroups * kTile * 4;  // several pieces are fewer than twice the workgroups
+  } else if (!p.few) {
     // As many pieces of every tile's rows, a causal tile's fewer rows in shorter ones:
     // the longest come first, and the short ones fill what they leave.  (Prompt of 4096
     // tokens over as many 4-bit keys, 32 heads on 8, us: 16 pieces a tile 92, 8 98;
     // pieces of one length, twice or four times what runs at a time, 120 and 108.)
     const int64_t rows = tokens / sequences * group;  // of a sequence: all have as many, or there is one
-    p.pieces = std::min((kManyWorkgroups + wide - 1) / wide, (rows + 4 * kStage - 1) / (4 * kStage));
-    if (p.pieces > 1) p.part_bytes = sequences * cache->kv_heads * p.pieces * p.tiles * keys * 4;
+    p.share = (kManyWorkgroups + pairs - 1) / pairs;
+    p.slots = slots(p.share, tiles);
+    p.pieces = std::min(p.share, (rows + 4 * kStage - 1) / (4 * kStage));
+    if (p.pieces > 1) p.part_bytes = pairs * p.share * kTile * 4;
   }
   return p;
 }
@@ -657,7 +689,7 @@ void launch_dim(const WeightArgs& w, uint32_t grid, uint32_t chunk_grid, hipStre
   if (w.chunks) {
     hipLaunchKernelGGL((paged_weights_few_kernel<Tag, kStore, D>), dim3(grid + 1u), dim3(256), 0, s, w);
     hipLaunchKernelGGL((paged_weights_chunks_kernel<Tag, kStore, D>), dim3(chunk_grid), dim3(256), 0, s, w);
-  } else if (w.steps)
+  } else if (w.few_share)
     hipLaunchKernelGGL((paged_weights_few_kernel<Tag, kStore, D>), dim3(grid), dim3(256), 0, s, w);
   else
     hipLaunchKernelGGL((paged_weights_kernel<Tag, kStore, D>), dim3(grid), dim3(256), 0, s, w);
@@ -709,12 +741,15 @@ extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queri
   w.weights = weights;
   w.chunks = p.mixed ? static_cast<Chunks*>(workspace) : nullptr;
   w.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.list_bytes);
-  w.tiles = (uint32_t)p.tiles;
-  w.pieces = (uint32_t)p.pieces;
-  w.steps = (uint32_t)p.steps;
+  w.share = (uint32_t)p.share;
+  w.slots = (uint32_t)p.slots;
+  w.few_share = (uint32_t)p.few_share;
+  w.few_slots = (uint32_t)p.few_slots;
   w.row_count = (uint64_t)cache->pages * cache->page_size;
-  const int64_t grid = p.tiles * sequences * (p.mixed ? 1 : p.pieces) * cache->kv_heads;
-  DSA_REQUIRE(grid < (1LL << 24), "too many keys for one call");
+  const int64_t pairs = sequences * cache->kv_heads;
+  const int64_t grid = pairs * (p.few ? p.few_slots : p.slots);
+  DSA_REQUIRE(grid < (1LL << 24), "too many sequences for one call");
+  DSA_REQUIRE((capacity + kTile - 1) / kTile * pairs < (1LL << 30), "too many keys for one call");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->dtype == kFP4E2M1)
     launch_weights<Bf16Tag, kE2M1>(w, cache->head_dim, (uint32_t)grid, (uint32_t)p.chunk_workgroups, s);
@@ -725,9 +760,9 @@ extern "C" int dsa_paged_weights(const dsa_paged_cache* cache, const void* queri
   else
     launch_weights<F16Tag, k16Bit>(w, cache->head_dim, (uint32_t)grid, (uint32_t)p.chunk_workgroups, s);
   if (int st = check_launch("paged_weights_kernel")) return st;
-  if (p.pieces == 1) return 0;
-  // A workgroup a tile and head; with several pieces there are fewer than kManyWorkgroups.
-  const int64_t join = p.mixed ? kManyWorkgroups : p.tiles * sequences * cache->kv_heads;
+  if (p.pieces <= 1) return 0;
+  // A workgroup a tile and head that has several pieces.
+  const int64_t join = p.mixed ? kManyWorkgroups : pairs * (p.share / 2);
   hipLaunchKernelGGL(paged_weights_join_kernel, dim3((unsigned)join), dim3(kTile), 0, s, w);
   return check_launch("paged_weights_join_kernel");
 }

@@ -113,6 +113,38 @@ def test_weights_of_chunks_among_single_tokens(device, lengths, chunks, group, k
         assert torch.equal(weights, first)
 
 
+@pytest.mark.parametrize("lengths,chunk,group,kv_heads,dim,dtype,starts", [
+    ([4160], 1, 4, 2, 128, FP4, False),
+    ([700, 0, 5000, 33], 1, 4, 2, 64, BF16, False),
+    ([9000] + [3] * 1099, 1, 1, 8, 64, BF16, False),      # more keys than a sequence's workgroups take at once
+    ([9000] + [3] * 1099, 1, 1, 8, 128, FP4, True),
+    ([900], 300, 4, 2, 128, FP8, False),                  # pieces of rows
+    ([900, 90, 3000], 40, 4, 2, 64, FP4, False),
+    ([700] + [2] * 599, 2, 33, 8, 64, F16, False),        # more tiles than a sequence's workgroups
+    ([900, 90, 3000], 40, 4, 2, 256, BF16, True),
+])
+def test_weights_with_room_for_more(device, lengths, chunk, group, kv_heads, dim, dtype, starts) -> None:
+    """The same bits whatever the page table has room for; page ids past the lengths are
+    any."""
+
+    print(f"weights with room: {len(lengths)} x {chunk} x {group}/{kv_heads}x{dim} {dtype} {starts}", flush=True)
+    c = _case(device, 102, lengths, [chunk] * len(lengths), group * kv_heads, kv_heads, dim, 16, dtype)
+    q, (table, keys, first) = c.q.to(device), c.device_args()
+    first = first if starts else None
+    _, lse = paged.attention(q, c.cache, table, keys, first, return_lse=True)
+    want, off = oracle.added_weights(_f64(c.q), np.nan_to_num(c.keys64), c.table.numpy(), lengths, c.starts,
+                                     lse.double().cpu().numpy(), dim**-0.5)
+    weights = eviction.new_weights(c.cache)
+    eviction.accumulate_weights(weights, q, c.cache, table, keys, lse, first)
+    assert (np.abs(weights.double().cpu().numpy() - want) <= off).all()
+    for room in (20000, 1 << 17):
+        more = room // 16 - table.shape[1]
+        wide = torch.cat([table, torch.randint(-5, 1 << 30, (len(lengths), more), dtype=torch.int32, device=device)], 1)
+        again = eviction.new_weights(c.cache)
+        eviction.accumulate_weights(again, q, c.cache, wide, keys, lse, first)
+        assert torch.equal(again, weights)
+
+
 @pytest.mark.parametrize("per_head", [False, True])
 @pytest.mark.parametrize("lengths,kv_heads,page,dtype,room,keep,recent", [
     ([300, 64, 63, 65], 2, 16, BF16, 40000, 64, 10),             # short lists, room for long ones
