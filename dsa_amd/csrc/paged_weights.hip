@@ -59,6 +59,11 @@ struct WeightArgs {
 
 __device__ __forceinline__ float* weights_of(const WeightArgs& a, uint32_t g) { return a.weights + g * a.row_count; }
 
+// A row's log sum in powers of two.  One of -inf says that no key had any weight, also
+// where the row sees some whose scores are all -inf: less +inf those give 0, and NaN less
+// -inf.
+__device__ __forceinline__ float log2_sum(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2E; }
+
 // The sum over the 16 lanes of a row, in each of them.
 __device__ __forceinline__ float row16_sum(float v) {
   v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));  // row_ror:8
@@ -146,7 +151,7 @@ __device__ __forceinline__ void weigh_tile(const WeightArgs& w, uint32_t g, uint
         const uint32_t r = min(r0 + tid, rows_all - 1u), t = w.by_group(r);
         const int64_t sees = a.causal ? before + first + t + 1 : (int64_t)length;
         const float lse = base_lse[(uint64_t)t * a.heads + (r - t * a.group)];
-        staged_of = make_float2(lse * kLog2E, __uint_as_float(r0 + tid < end ? (uint32_t)max((int64_t)0, sees) : 0u));
+        staged_of = make_float2(log2_sum(lse), __uint_as_float(r0 + tid < end ? (uint32_t)max((int64_t)0, sees) : 0u));
       }
     };
     auto stage = [&](uint32_t slot) {
@@ -569,7 +574,7 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
         const uint32_t i = w.by_group(r);
         const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
         const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r - i * a.group];
-        row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
+        row_of[tid] = make_float2(log2_sum(lse), __uint_as_float(tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
       }
       __syncthreads();
     }

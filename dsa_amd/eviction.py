@@ -60,8 +60,8 @@ def accumulate_weights(
     heads of the key's kv head) that see it, the sum of exp(scale q.k - lse).
 
     The other arguments are those of :func:`dsa_amd.paged.attention`, and ``lse``
-    ``[T, heads]`` fp32 what it returned for them.  Some of a prompt's tokens, its
-    last ones say, may be given alone.  Sums are fp32; the same inputs give the same
+    ``[T, heads]`` fp32 what it returned for them; a row whose log sum is -inf adds
+    nothing.  Some of a prompt's tokens, its last ones say, may be given alone.  Sums are fp32; the same inputs give the same
     bits, unless sequences share pages, whose keys get the sums of all of them.
     """
 

@@ -939,7 +939,8 @@ int dsa_paged_selected_attention(const dsa_paged_cache* cache, const void* queri
  * added to weights [kv_heads][pages * page_size] (fp32, by cache row):
  *   weights[g][row(j)] += sum over tokens t and heads h of kv head g that see key j
  *                         of exp(scale q[t][h] . k[j][g] - lse[t][h])
- * Arguments as of dsa_paged_attention, lse [tokens][heads] as it returns them.  Sums
+ * Arguments as of dsa_paged_attention, lse [tokens][heads] as it returns them; a row
+ * whose lse is -inf adds nothing.  Sums
  * are fp32 in an order that the tokens and keys of each sequence set, so two calls on
  * the same inputs give the same bits unless two sequences share a page, whose sums are
  * both added.  What a row does not see does not reach a weight.  Workspace: the bytes of
