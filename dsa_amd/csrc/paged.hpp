@@ -92,7 +92,8 @@ __device__ __forceinline__ uint4 fp8x8_to_bf16x8_paired(uint2 v) {
   return make_uint4(two(v.x, Low{}), two(v.x, High{}), two(v.y, Low{}), two(v.y, High{}));
 }
 
-// 8 e2m1 codes times a power of two to 8 bf16, exactly (NaN for a power of NaN).
+// 8 e2m1 codes times a power of two to 8 bf16, exactly (NaN for a power of NaN; infinite
+// from 2^128 on, which powers from 2^126 on reach).
 __device__ __forceinline__ uint4 fp4x8_to_bf16x8(uint32_t w, float power) {
   typedef __bf16 pair __attribute__((ext_vector_type(2)));
   const pair p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, 0);
@@ -103,8 +104,15 @@ __device__ __forceinline__ uint4 fp4x8_to_bf16x8(uint32_t w, float power) {
                     __builtin_bit_cast(uint32_t, p3));
 }
 __device__ __forceinline__ float power_of(uint32_t byte) { return __uint_as_float(byte << 23); }
-// Bytes of `w` that are 255, as 0x80 in their place.
-__device__ __forceinline__ uint32_t nan_powers(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+// Codes of 8 whose values bf16 does not hold (4 and 6 under a power of 2^126, those from 2
+// on under 2^127, all of a block that is NaN) become 0; whether there were any.
+__device__ __forceinline__ bool drop_nonfinite_codes(uint32_t& codes, uint32_t power) {
+  if (power < 253u) return false;
+  uint32_t found = 0x11111111u;
+  if (power < 255u) found &= (codes >> 2) & (power == 254u ? 0xffffffffu : codes >> 1);
+  codes &= ~(found * 15u);
+  return found != 0;
+}
 
 // LDS that the lanes of one wave share: a wave's LDS accesses are served in
 // order, so only the compiler has to keep them so.

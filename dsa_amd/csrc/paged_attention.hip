@@ -315,11 +315,6 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
 #pragma unroll
       for (int i = 0; i < Powers<D>::kWords; ++i) {
         if (kListed && at[lane & 31u] < 0) powers.w[i] = 0;  // of padding: what NaN is there has no weight
-        if (hides && lane >= 32u && key0 + lane - 32u >= all_see) {
-          const uint32_t found = nan_powers(powers.w[i]);
-          powers.w[i] &= ~((found >> 7) * 0xffu);
-          dropped |= found != 0;
-        }
       }
       reinterpret_cast<Powers<D>*>(scales[wave])[lane] = powers;
       wave_order();
@@ -339,10 +334,19 @@ __global__ __launch_bounds__(256 * kHeadsOf<kWork>, (kPerSimd<D, kWork>)) void p
           if (hides && key0 + r >= all_see) dropped |= drop_nonfinite<Tag, kStore>(v);
         }
         if constexpr (kFp4) {
-          const float power = power_of(reinterpret_cast<const uint8_t*>(scales[wave])[(32u + r) * kPowers + c]);
+          uint32_t power = reinterpret_cast<const uint8_t*>(scales[wave])[(32u + r) * kPowers + c];
+          if (hides && key0 + r >= all_see) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t codes = v[w];
+              dropped |= drop_nonfinite_codes(codes, power);
+              v[w] = codes;
+            }
+            if (power == 255u) power = 0;
+          }
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            *reinterpret_cast<uint4*>(mine + widened_place<D>(r, 4u * c + w)) = fp4x8_to_bf16x8(v[w], power);
+            *reinterpret_cast<uint4*>(mine + widened_place<D>(r, 4u * c + w)) = fp4x8_to_bf16x8(v[w], power_of(power));
         } else if constexpr (kFp8) {
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c)) = fp8x8_to_bf16x8_paired(make_uint2(v.x, v.y));
           *reinterpret_cast<uint4*>(mine + tile_place<2 * D>(r, 2u * c + 1u)) = fp8x8_to_bf16x8_paired(make_uint2(v.z, v.w));

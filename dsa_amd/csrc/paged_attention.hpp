@@ -242,10 +242,10 @@ __device__ __forceinline__ float2 load_shared(const float2* p) {
 // 3 % of ragged chunks, whose tiles are many of them a sequence's last (109, 112 us).
 
 // Whether any of a 16-byte run of a value row is not finite; those become 0.
-// (Codes of an e2m1 cache are all finite; its powers of two are looked at apart.)
+// (Of an e2m1 cache: drop_nonfinite_codes.)
 template <class Tag, Store kStore>
 __device__ __forceinline__ bool drop_nonfinite(u32x4& v) {
-  static_assert(kStore != kE2M1, "no code is infinite");
+  static_assert(kStore != kE2M1, "codes are finite by their power of two");
   constexpr bool kFp8 = kStore == kE4M3;
   constexpr uint32_t kExponent = kFp8 ? 0x7f7f7f7fu : std::is_same<Tag, Bf16Tag>::value ? 0x7f807f80u : 0x7c007c00u;
   constexpr uint32_t kUnit = kFp8 ? 0x01010101u : std::is_same<Tag, Bf16Tag>::value ? 0x00800080u : 0x04000400u;
@@ -266,13 +266,14 @@ __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) 
 template <class Tag, Store kStore, int D>
 __device__ __forceinline__ void add_nonfinite(const PagedAttentionArgs& a, uint32_t row, uint32_t g, uint32_t dim,
                                               float* o) {
-  if constexpr (kStore == kE2M1) {
-    if (a.cache.value_powers[a.cache.power_offset<D>(row, g) + dim / kPowerDims] == 255u) o[0] = o[1] = o[2] = o[3] = NAN;
-    return;
-  }
   const char* at = a.cache.values + g * a.cache.value_head + a.cache.value_offset(row);
   float v[4];
-  if constexpr (kStore == kE4M3) {
+  if constexpr (kStore == kE2M1) {
+    const uint32_t power = a.cache.value_powers[a.cache.power_offset<D>(row, g) + dim / kPowerDims];
+    const uint4 w = fp4x8_to_bf16x8(*reinterpret_cast<const uint16_t*>(at + dim / 2u), power_of(power));
+    const float2 lo = unpack2(Tag{}, w.x), hi = unpack2(Tag{}, w.y);
+    v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
+  } else if constexpr (kStore == kE4M3) {
     const int w = *reinterpret_cast<const int*>(at + dim);
     const float scale = a.cache.value_scales[(uint64_t)row * a.cache.kv_heads + g];
     v[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0) * scale;

@@ -155,10 +155,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_prefill_kernel(
       for (int i = 0; i < kLoads; ++i) {
         if (key0 + load_row + kPass * i < all_rows_see) continue;
         if constexpr (kFp4) {
-          if (vp[i] == 255u) {
-            vp[i] = 0;
-            dropped = 1;
+#pragma unroll
+          for (uint32_t w = 0; w < kWords; ++w) {
+            uint32_t codes = vr[i][w];
+            if (drop_nonfinite_codes(codes, vp[i])) dropped = 1;
+            vr[i][w] = codes;
           }
+          if (vp[i] == 255u) vp[i] = 0;
         } else {
           if (drop_nonfinite<Tag, kStore>(vr[i])) dropped = 1;
         }

@@ -245,9 +245,10 @@ def append(
     With ``queries`` ``[T, heads, head_dim]`` the rotated queries are returned.
     Tokens whose row is outside the cache (-1: padding) are not written; no two
     tokens may have the same row.  An fp8 cache scales each head by its largest
-    magnitude, an fp4 one each 32 dims by the least power of two under which theirs is
-    7 or less: no value is then off by more than half a step of the codes, and what
-    is not finite makes its 32 dims NaN.  The angles are exact to fp32 at any position; taken as an fp32
+    magnitude, an fp4 one each 32 dims by the least power of two, 2^125 at most, under
+    which theirs is 7 or less: no value up to 7 * 2^125 (2.98e38; larger ones become 6 *
+    2^125) is then off by more than half a step of the codes, and what is not finite
+    makes its 32 dims NaN.  The angles are exact to fp32 at any position; taken as an fp32
     product, as the sidecar's encoders and many models take theirs, they are 0.0006
     rad off at position 65535, so keys and queries are best rotated by one of the two.
     """
@@ -292,8 +293,8 @@ def append(
 def read(cache: PagedCache, rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and the values ``[n, kv_heads, head_dim]`` that cache rows ``rows``
     ``[n]`` stand for, in the type that rows are appended in: the rows themselves
-    of a 16-bit cache, bf16 for fp8 (rounded) and fp4 (exact).  Rows outside the cache
-    (-1: padding) give zeros."""
+    of a 16-bit cache, bf16 for fp8 (rounded) and fp4 (exact, infinite from 2^128
+    on).  Rows outside the cache (-1: padding) give zeros."""
 
     if rows.ndim != 1:
         raise ValueError("rows must be [n]")

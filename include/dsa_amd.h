@@ -854,7 +854,8 @@ int dsa_encode_queries_gemm(const void* hidden, int64_t hidden_stride, int64_t t
  * [pages][page_size][kv_heads].  An fp4 cache holds two codes a byte, the first in
  * the low half, its strides count those bytes, and it stands for code * 2^(power -
  * 127), with one power byte (e8m0; 255: NaN) per 32 dims in contiguous, 16-byte
- * aligned [pages][kv_heads][page_size][head_dim / 32].
+ * aligned [pages][kv_heads][page_size][head_dim / 32]; values from 2^128 on, which
+ * only powers past those of dsa_paged_append give, are infinite.
  * page_size a power of two, head_dim 64, 128 or 256, pages * page_size below
  * 2^31; pointers and strides 16-byte aligned, page and slot strides below 4 GiB.
  * Offsets are 64-bit.  The descriptor is host memory, read during the call.
