@@ -677,6 +677,9 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
     return fail(DSA_STATUS_WORKSPACE_TOO_SMALL, "paged eviction needs %lld bytes of 16-byte aligned workspace",
                 (long long)p.bytes);
   DSA_REQUIRE(p.lists < 65536, "too many sequences for one call");
+  // The first launch writes the new lengths, and every one reads the old ones.
+  DSA_REQUIRE(out_lengths + sequences <= lengths || lengths + sequences <= out_lengths,
+              "out_lengths must not overlap lengths");
   a.page_table = page_table;
   a.table_stride = table_stride;
   a.columns = (uint32_t)columns;

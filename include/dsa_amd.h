@@ -960,9 +960,9 @@ int dsa_paged_weights(const dsa_paged_cache* cache, const void* queries, int64_t
  * from m on go, in order, to the positions below m that are freed.  per_head: each kv
  * head keeps keys of its own, by its own weights; else all keep the same, by their
  * weights' sum (held in fp64, rounded to fp32).  Weights move with their keys, those of
- * positions m .. n become 0.  out_lengths[s] = m; kept [sequences][kv_heads if
- * per_head else 1][keep] is the former position of the key now at each position, -1
- * from m on.  No other byte of the cache is written.  A page may be of one
+ * positions m .. n become 0.  out_lengths[s] = m (they may not overlap lengths); kept
+ * [sequences][kv_heads if per_head else 1][keep] is the former position of the key now
+ * at each position, -1 from m on.  No other byte of the cache is written.  A page may be of one
  * sequence alone.  Workspace (16-byte aligned): the bytes of the query. */
 int64_t dsa_paged_evict_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t columns, int64_t keep,
                                         int32_t per_head);
