@@ -29,8 +29,9 @@ _TORCH_DTYPES = {
     torch.float16: DTYPE_F16,
     torch.bfloat16: DTYPE_BF16,
     torch.float8_e4m3fn: DTYPE_FP8_E4M3,
-    torch.float4_e2m1fn_x2: DTYPE_FP4_E2M1,
 }
+if hasattr(torch, "float4_e2m1fn_x2"):  # a torch without it has everything else
+    _TORCH_DTYPES[torch.float4_e2m1fn_x2] = DTYPE_FP4_E2M1
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32

@@ -121,13 +121,15 @@ def attend(args: argparse.Namespace) -> None:
         raise ValueError("the budget must be at least 2 keys")
     if args.steps < 1 or args.length < 1 or args.batch < 1 or args.k < 1:
         raise ValueError("length, steps, batch and k must be at least 1")
+    if args.cache_dtype == "fp4" and paged.FP4 is None:
+        raise ValueError("this torch has no 4-bit type (float4_e2m1fn_x2)")
     device = torch.device("cuda", 0)
     gen = torch.Generator(device).manual_seed(args.seed)
     batch, heads, kv_heads, dim = args.batch, args.heads, args.kv_heads, args.head_dim
     longest = args.length + args.steps
     columns = -(-longest // args.page_size)
     dtype = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp8": torch.float8_e4m3fn,
-             "fp4": torch.float4_e2m1fn_x2}[args.cache_dtype]
+             "fp4": paged.FP4}[args.cache_dtype]
     cache = paged.new_cache(batch * columns, args.page_size, kv_heads, dim, dtype=dtype, device=device)
     table = torch.randperm(batch * columns, generator=gen, device=device).to(torch.int32).view(batch, columns)
     # A token's keys of every head share a part, which is the indexer's key and which

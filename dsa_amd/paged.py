@@ -37,8 +37,8 @@ from . import _lib
 
 HEAD_DIMS = (64, 128, 256)
 POWER_DIMS = 32  # dims of an fp4 head that share a power of two
-FP4 = torch.float4_e2m1fn_x2
-_CACHE_DTYPES = (torch.bfloat16, torch.float16, torch.float8_e4m3fn, FP4)
+FP4 = getattr(torch, "float4_e2m1fn_x2", None)  # None: a torch without it, which has the other caches
+_CACHE_DTYPES = tuple(t for t in (torch.bfloat16, torch.float16, torch.float8_e4m3fn, FP4) if t is not None)
 
 
 class PagedCache:
@@ -126,7 +126,7 @@ def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, dtype
     was not appended.  In an fp4 one a page's rows of one head lie together: a row
     of its own is 64 bytes at head_dim 128, half of what memory serves well."""
 
-    if dtype == FP4:
+    if FP4 is not None and dtype == FP4:
         if head_dim not in HEAD_DIMS:
             raise ValueError("head_dim must be 64, 128 or 256")
         parts = [torch.empty((pages, kv_heads, page_size, n), dtype=torch.uint8, device=device)
