@@ -47,7 +47,7 @@ struct EvictArgs {
   int32_t* out_lengths;
   int64_t* kept;          // [sequences][lists][keep]
   // Workspace, for each list: the three passes' bins, its moves
-  // {to, from} (keep apart) and how many there are; and of the chunks of long lists, one
+  // {to, from} (most_moves apart) and how many there are; and of the chunks of long lists, one
   // behind the other, counts and the order of every weight.
   uint32_t* bins;
   uint2* moves;
@@ -57,6 +57,7 @@ struct EvictArgs {
   uint32_t* order;
   Listed* listed;         // null where no list can be long
   uint32_t most_chunks;   // that there is room for
+  uint32_t most_moves;    // of a list: no more than it keeps, nor than lie past those
 };
 
 __device__ __forceinline__ uint32_t cache_row(const EvictArgs& a, const int32_t* table, uint32_t key) {
@@ -202,7 +203,7 @@ __device__ __forceinline__ void settle(const EvictArgs& a, const List& l, uint32
   }
   __syncthreads();
   int64_t* kept = a.kept + (uint64_t)list * a.keep;
-  uint2* moves = a.moves + (uint64_t)list * a.keep;
+  uint2* moves = a.moves + (uint64_t)list * a.most_moves;
   for (uint32_t i = tid; i < holes; i += kThreads) moves[hole + i].x = moving[i];
   for (uint32_t i = tid; i < sources; i += kThreads) moves[source + i].y = moving[holes + i];
   uint32_t row[kEach];
@@ -520,7 +521,7 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictArgs a) {
   const uint32_t list = blockIdx.y;
   const uint32_t sequence = list / a.lists;
   const int32_t* pages = a.page_table + (int64_t)sequence * a.table_stride;
-  const uint2* moves = a.moves + (uint64_t)list * a.keep;
+  const uint2* moves = a.moves + (uint64_t)list * a.most_moves;
   const uint32_t count = a.counts[list];
   if (a.listed) {  // (a long list's; the others' again)
     for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < count; i += gridDim.x * 256u)
@@ -623,6 +624,7 @@ constexpr int64_t kChunkWorkgroups = 512;  // that long lists' chunks are dealt 
 
 struct EvictPlan {
   int64_t lists, most_chunks;  // no chunks: every list is one workgroup's
+  int64_t most_moves;          // of a list
   int64_t moves, counts, thresholds, listed, chunk_counts, order, bytes;  // offsets, after the bins
 };
 
@@ -640,7 +642,8 @@ EvictPlan evict_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t co
     p.most_chunks = std::min(heads * std::min(sequences * ((capacity + kChunk - 1) / kChunk), rows * 3 / kMostInLds), (int64_t)1 << 30);
   }
   p.moves = p.most_chunks ? p.lists * 3 * kBins * 4 : 0;
-  p.counts = p.moves + p.lists * keep * 8;
+  p.most_moves = std::max(std::min(keep, capacity - keep), (int64_t)0);
+  p.counts = p.moves + p.lists * p.most_moves * 8;
   p.thresholds = p.counts + p.lists * 4;
   p.listed = (p.thresholds + p.lists * 36 + 15) / 16 * 16;
   p.chunk_counts = p.listed + (p.most_chunks ? (16 + p.lists * 8 + 15) / 16 * 16 : 0);
@@ -700,6 +703,7 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
   a.order = reinterpret_cast<uint32_t*>(base + p.order);
   a.listed = p.most_chunks ? reinterpret_cast<Listed*>(base + p.listed) : nullptr;
   a.most_chunks = (uint32_t)p.most_chunks;
+  a.most_moves = (uint32_t)p.most_moves;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t capacity = columns * cache->page_size;
   const dim3 lists((unsigned)p.lists + (p.most_chunks ? 1u : 0u));
@@ -718,16 +722,14 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
     hipLaunchKernelGGL(paged_evict_settle_kernel, chunks, dim3(kThreads), 0, s, a);
   }
   if (int st = check_launch("paged_evict_select_kernel")) return st;
-  // A list moves at most keep keys, and no more than lie past it.
-  const int64_t most = std::min(keep, capacity - keep);
-  if (most <= 0) return 0;
+  if (p.most_moves == 0) return 0;
   const int32_t bytes = cache->dtype == kFP4E2M1   ? cache->head_dim / 2
                         : cache->dtype == kFP8E4M3 ? cache->head_dim
                                                    : 2 * cache->head_dim;
   const int32_t pieces = bytes / 16;
   const int64_t heads = per_head ? 1 : cache->kv_heads;
   const int64_t fill = (4096 + p.lists - 1) / p.lists;
-  const int64_t blocks = std::min((most * heads * pieces + 511) / 512, fill);
+  const int64_t blocks = std::min((p.most_moves * heads * pieces + 511) / 512, fill);
   const dim3 grid((unsigned)blocks, (unsigned)p.lists);
   if (cache->dtype == kFP4E2M1)
     launch_move<kE2M1>(a, pieces, grid, s);
