@@ -46,9 +46,9 @@ struct EvictArgs {
   uint32_t lists;         // of a sequence: kv_heads or 1
   int32_t* out_lengths;
   int64_t* kept;          // [sequences][lists][keep]
-  // Workspace, for each list: the three passes' bins, its moves
-  // {to, from} (most_moves apart) and how many there are; and of the chunks of long lists, one
-  // behind the other, counts and the order of every weight.
+  // Workspace, for each list: its moves {to, from} (most_moves apart) and how many there
+  // are; for each long one, in their order: the three passes' bins and thresholds; and of
+  // their chunks, one behind the other, counts and the order of every weight.
   uint32_t* bins;
   uint2* moves;
   uint32_t* counts;
@@ -56,7 +56,7 @@ struct EvictArgs {
   Threshold* thresholds;  // after each pass
   uint32_t* order;
   Listed* listed;         // null where no list can be long
-  uint32_t most_chunks;   // that there is room for
+  uint32_t most_chunks, most_long;  // that there is room for
   uint32_t most_moves;    // of a list: no more than it keeps, nor than lie past those
 };
 
@@ -244,6 +244,9 @@ constexpr uint32_t kMostInLds = 16 * kThreads;
 constexpr uint32_t kChunkEach = 8;
 constexpr uint32_t kChunk = kThreads * kChunkEach;
 
+// Whether a list of n keys is too long for one workgroup, and loses some.
+__device__ __forceinline__ bool is_long(uint32_t n, uint32_t keep) { return n > kMostInLds && n > keep; }
+
 // Lists what is too long for one workgroup and loses keys.  One workgroup's work.  (Keys
 // of one place in the cache each have room; past that nothing is listed.)
 __device__ __forceinline__ void list_long(const EvictArgs& a, uint32_t lists, uint32_t* scan, uint32_t* listed) {
@@ -252,7 +255,7 @@ __device__ __forceinline__ void list_long(const EvictArgs& a, uint32_t lists, ui
   for (uint32_t base = 0; base < lists; base += kThreads) {
     const uint32_t list = base + threadIdx.x;
     const uint32_t n = list < lists ? keys_of(a, list / a.lists) : 0u;
-    const uint32_t own = n > kMostInLds && n > a.keep ? (n + kChunk - 1u) / kChunk : 0u;
+    const uint32_t own = is_long(n, a.keep) ? (n + kChunk - 1u) / kChunk : 0u;
     uint32_t all_chunks, all;
     const uint32_t before = chunks + block_excl_scan<16>(own, scan, all_chunks);
     const bool fits = own > 0 && before + own <= a.most_chunks;  // those that do are the first
@@ -265,6 +268,14 @@ __device__ __forceinline__ void list_long(const EvictArgs& a, uint32_t lists, ui
   if (threadIdx.x > 0) return;
   a.listed->count = count;
   a.listed->chunks = *listed;
+}
+
+// How many of the lists before a sequence's are long.  For a whole workgroup.
+__device__ __forceinline__ uint32_t long_before(const EvictArgs& a, uint32_t sequence, uint32_t* scan) {
+  uint32_t own = 0, all;
+  for (uint32_t s = threadIdx.x; s < sequence; s += kThreads) own += is_long(keys_of(a, s), a.keep);
+  block_excl_scan<16>(own, scan, all);
+  return all * a.lists;
 }
 
 // One workgroup a list, whose orders lie in LDS: kEach neighbouring positions a thread,
@@ -292,7 +303,9 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
   if (l.n == l.m) return;
   if (whole) {
     if (!a.listed) return;  // more keys than the cache has rows
-    for (uint32_t i = tid; i < 3u * kBins; i += kThreads) a.bins[(uint64_t)list * 3u * kBins + i] = 0;
+    const uint32_t rank = long_before(a, l.sequence, scan[0]) + l.g;
+    if (rank >= a.most_long) return;  // (the same, of several sequences)
+    for (uint32_t i = tid; i < 3u * kBins; i += kThreads) a.bins[(uint64_t)rank * 3u * kBins + i] = 0;
     return;
   }
   for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
@@ -348,22 +361,23 @@ __global__ __launch_bounds__(kThreads) void paged_evict_select_kernel(EvictArgs 
 
 // A chunk of a listed list.
 struct ChunkAt {
-  uint32_t list, before, chunk;  // chunks of other lists before the list's, and which of its own
+  uint32_t rank, list, before, chunk;  // the list's place among the listed, chunks of others before its, which of its own
 };
 __device__ __forceinline__ ChunkAt chunk_at(const Listed* listed, uint32_t item) {
-  const uint2 of = listed->of[last_at_most(listed->of, listed->count, item)];
-  return {of.x, of.y, item - of.y};
+  const uint32_t rank = last_at_most(listed->of, listed->count, item);
+  const uint2 of = listed->of[rank];
+  return {rank, of.x, of.y, item - of.y};
 }
 // The threshold after kPass passes: what the launch before this one's left of it, and
 // the digit that its bins say.
 template <int kPass>
-__device__ __forceinline__ Threshold threshold_of(const EvictArgs& a, const List& l, uint32_t list, uint32_t chunk, Locate& found) {
+__device__ __forceinline__ Threshold threshold_of(const EvictArgs& a, const List& l, const ChunkAt& c, Locate& found) {
   Threshold t = {0u, l.want, 0u};
   if (kPass == 0 || l.want == 0) return t;
-  Threshold* kept = a.thresholds + (uint64_t)list * 3u;
+  Threshold* kept = a.thresholds + (uint64_t)c.rank * 3u;
   if (kPass > 1) t = kept[kPass > 1 ? kPass - 2 : 0];
-  locate_digit(a.bins + ((uint64_t)list * 3u + kPass - 1) * kBins, kPass - 1, found, t);
-  if (chunk == 0 && threadIdx.x == 0) kept[kPass - 1] = t;
+  locate_digit(a.bins + ((uint64_t)c.rank * 3u + kPass - 1) * kBins, kPass - 1, found, t);
+  if (c.chunk == 0 && threadIdx.x == 0) kept[kPass - 1] = t;
   return t;
 }
 
@@ -377,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_count_kernel(EvictArgs a
     const List l = list_of(a, c.list);
     const uint32_t first = c.chunk * kChunk;
     if (first >= l.old || l.want == 0) continue;
-    const Threshold t = threshold_of<kPass>(a, l, c.list, c.chunk, found);
+    const Threshold t = threshold_of<kPass>(a, l, c, found);
     for (uint32_t i = tid; i < kBins; i += kThreads) bins[i] = 0;
     __syncthreads();
     uint32_t* order = a.order + (uint64_t)item * kChunk;
@@ -399,7 +413,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_count_kernel(EvictArgs a
       if (counts) atomicAdd(&bins[key >> kShift[kPass] & (kPass == 2 ? 1023u : 2047u)], 1u);
     }
     __syncthreads();
-    uint32_t* to = a.bins + ((uint64_t)c.list * 3u + kPass) * kBins;
+    uint32_t* to = a.bins + ((uint64_t)c.rank * 3u + kPass) * kBins;
     for (uint32_t i = tid; i < kBins; i += kThreads)
       if (bins[i]) atomicAdd(&to[i], bins[i]);
     __syncthreads();
@@ -429,7 +443,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_chunk_kernel(EvictArgs a
     const ChunkAt c = chunk_at(a.listed, item);
     const List l = list_of(a, c.list);
     const uint32_t first = c.chunk * kChunk;
-    const Threshold t = threshold_of<3>(a, l, c.list, c.chunk, found);
+    const Threshold t = threshold_of<3>(a, l, c, found);
     if (threadIdx.x < 4u) sums[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t at = first + threadIdx.x * kChunkEach;
@@ -465,7 +479,7 @@ __global__ __launch_bounds__(kThreads) void paged_evict_settle_kernel(EvictArgs 
     const ChunkAt c = chunk_at(a.listed, item);
     const List l = list_of(a, c.list);
     const uint32_t first = c.chunk * kChunk;
-    const Threshold t = l.want > 0 ? a.thresholds[(uint64_t)c.list * 3u + 2u] : Threshold{0u, 0u, 0u};
+    const Threshold t = l.want > 0 ? a.thresholds[(uint64_t)c.rank * 3u + 2u] : Threshold{0u, 0u, 0u};
     if (threadIdx.x < kWave) {
       // Keys at the threshold are kept while their rank is below t.rest; that rank follows
       // the chunks, so a chunk keeps as many as are left of them.
@@ -624,7 +638,7 @@ constexpr int64_t kChunkWorkgroups = 512;  // that long lists' chunks are dealt 
 
 struct EvictPlan {
   int64_t lists, most_chunks;  // no chunks: every list is one workgroup's
-  int64_t most_moves;          // of a list
+  int64_t most_long, most_moves;  // long lists, moves of a list
   int64_t moves, counts, thresholds, listed, chunk_counts, order, bytes;  // offsets, after the bins
 };
 
@@ -641,11 +655,12 @@ EvictPlan evict_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t co
     static_assert(kMostInLds == 2 * kChunk, "");
     p.most_chunks = std::min(heads * std::min(sequences * ((capacity + kChunk - 1) / kChunk), rows * 3 / kMostInLds), (int64_t)1 << 30);
   }
-  p.moves = p.most_chunks ? p.lists * 3 * kBins * 4 : 0;
+  p.most_long = std::min(p.lists, p.most_chunks / 3);  // what is listed has three chunks at least, within their room
+  p.moves = p.most_long * 3 * kBins * 4;
   p.most_moves = std::max(std::min(keep, capacity - keep), (int64_t)0);
   p.counts = p.moves + p.lists * p.most_moves * 8;
   p.thresholds = p.counts + p.lists * 4;
-  p.listed = (p.thresholds + p.lists * 36 + 15) / 16 * 16;
+  p.listed = (p.thresholds + p.most_long * 36 + 15) / 16 * 16;
   p.chunk_counts = p.listed + (p.most_chunks ? (16 + p.lists * 8 + 15) / 16 * 16 : 0);
   p.order = p.chunk_counts + p.most_chunks * 16;
   p.bytes = p.order + p.most_chunks * kChunk * 4;
@@ -703,6 +718,7 @@ extern "C" int dsa_paged_evict(const dsa_paged_cache* cache, const int32_t* page
   a.order = reinterpret_cast<uint32_t*>(base + p.order);
   a.listed = p.most_chunks ? reinterpret_cast<Listed*>(base + p.listed) : nullptr;
   a.most_chunks = (uint32_t)p.most_chunks;
+  a.most_long = (uint32_t)p.most_long;
   a.most_moves = (uint32_t)p.most_moves;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t capacity = columns * cache->page_size;
