@@ -61,8 +61,10 @@ def accumulate_weights(
 
     The other arguments are those of :func:`dsa_amd.paged.attention`, and ``lse``
     ``[T, heads]`` fp32 what it returned for them; a row whose log sum is -inf adds
-    nothing.  Some of a prompt's tokens, its last ones say, may be given alone.  Sums are fp32; the same inputs give the same
-    bits, unless sequences share pages, whose keys get the sums of all of them.
+    nothing.  Some of a prompt's tokens, its last ones say, may be given alone.  Sums
+    are fp32; the same call gives the same bits, unless sequences share pages, whose keys
+    get the sums of all of them.  A sequence batched with others may get other last bits:
+    the order of its sums follows the whole call.
     """
 
     weights = _weights(weights, cache)

@@ -941,10 +941,11 @@ int dsa_paged_selected_attention(const dsa_paged_cache* cache, const void* queri
  *   weights[g][row(j)] += sum over tokens t and heads h of kv head g that see key j
  *                         of exp(scale q[t][h] . k[j][g] - lse[t][h])
  * Arguments as of dsa_paged_attention, lse [tokens][heads] as it returns them; a row
- * whose lse is -inf adds nothing.  Sums
- * are fp32 in an order that the tokens and keys of each sequence set, so two calls on
- * the same inputs give the same bits unless two sequences share a page, whose sums are
- * both added.  What a row does not see does not reach a weight.  Workspace: the bytes of
+ * whose lse is -inf adds nothing.  Sums are fp32, in an order that the whole call sets:
+ * how many sequences, tokens and heads it has, whether starts is given, and every
+ * sequence's tokens and keys, but not the page table's room.  Two calls alike give the
+ * same bits unless two sequences share a page, whose sums are both added; a sequence
+ * that is batched with others may get other last bits.  What a row does not see does not reach a weight.  Workspace: the bytes of
  * the query. */
 int64_t dsa_paged_weights_workspace_bytes(const dsa_paged_cache* cache, int64_t sequences, int64_t tokens,
                                           int32_t heads, int64_t columns, int32_t uniform);
