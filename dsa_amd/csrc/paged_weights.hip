@@ -59,11 +59,6 @@ struct WeightArgs {
 
 __device__ __forceinline__ float* weights_of(const WeightArgs& a, uint32_t g) { return a.weights + g * a.row_count; }
 
-// A row's log sum in powers of two.  One of -inf says that no key had any weight, also
-// where the row sees some whose scores are all -inf: less +inf those give 0, and NaN less
-// -inf.
-__device__ __forceinline__ float log2_sum(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2E; }
-
 // The sum over the 16 lanes of a row, in each of them.
 __device__ __forceinline__ float row16_sum(float v) {
   v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));  // row_ror:8
@@ -96,7 +91,9 @@ __device__ __forceinline__ void weigh_tile(const WeightArgs& w, uint32_t g, uint
   constexpr uint32_t kRuns = D / 8;        // 16-byte runs of a row
   constexpr uint32_t kLoads = kStage * kRuns / 256;
   __shared__ __attribute__((aligned(16))) char rows_tile[2][kStage * kRow];
-  __shared__ float2 row_of[2][kStage];     // {log2 sum, keys that the row sees (as bits)}
+  // {log2 sum, keys that the row sees (as bits)}.  A row whose log sum is -inf has no weight
+  // to give, also to keys that it sees (their scores are all -inf then): it sees none here.
+  __shared__ float2 row_of[2][kStage];
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = tid / kWave, col = lane & 15u, quad = lane >> 4;
 
   const uint32_t length = keys_of(a, sequence);
@@ -151,7 +148,7 @@ __device__ __forceinline__ void weigh_tile(const WeightArgs& w, uint32_t g, uint
         const uint32_t r = min(r0 + tid, rows_all - 1u), t = w.by_group(r);
         const int64_t sees = a.causal ? before + first + t + 1 : (int64_t)length;
         const float lse = base_lse[(uint64_t)t * a.heads + (r - t * a.group)];
-        staged_of = make_float2(log2_sum(lse), __uint_as_float(r0 + tid < end ? (uint32_t)max((int64_t)0, sees) : 0u));
+        staged_of = make_float2(lse * kLog2E, __uint_as_float(r0 + tid < end && lse != -INFINITY ? (uint32_t)max((int64_t)0, sees) : 0u));
       }
     };
     auto stage = [&](uint32_t slot) {
@@ -229,9 +226,8 @@ __device__ __forceinline__ void weigh_tile(const WeightArgs& w, uint32_t g, uint
     for (uint32_t r0 = begin; r0 < end; r0 += kStage, slot ^= 1u) {
       const bool more = r0 + kStage < end;
       if (more) load(r0 + kStage);
-      // Rows ascend by token, so the first sees least.
-      const uint32_t least = (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(row_of[slot][0].y));
-      if (r0 + kStage <= end && least >= (uint32_t)__builtin_amdgcn_readfirstlane((int)key0) + kKeys) {
+      static_assert(kStage == kWave, "a lane a row");
+      if (__all(__float_as_uint(row_of[slot][lane].y) >= key0 + kKeys)) {
         // Every row sees every key: the products of 16 rows under the exponentials of
         // the 16 before, operands read from LDS a turn ahead.
         constexpr uint32_t kTurns = kStage / 16u;
@@ -574,7 +570,7 @@ __global__ __launch_bounds__(256, D == 256 && kStore == k16Bit ? 1 : 2) void pag
         const uint32_t i = w.by_group(r);
         const int64_t sees = a.causal ? before + i + 1 : (int64_t)length;
         const float lse = a.lse[(uint64_t)(span.first + i) * a.heads + g * a.group + r - i * a.group];
-        row_of[tid] = make_float2(log2_sum(lse), __uint_as_float(tid < rows ? (uint32_t)max((int64_t)0, sees) : 0u));
+        row_of[tid] = make_float2(lse * kLog2E, __uint_as_float(tid < rows && lse != -INFINITY ? (uint32_t)max((int64_t)0, sees) : 0u));
       }
       __syncthreads();
     }

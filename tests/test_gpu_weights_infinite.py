@@ -68,3 +68,30 @@ def test_rows_of_fp8_keys(device, chunk) -> None:
     eviction.accumulate_weights(got, q, c.cache, *args[:2], lse, args[2])
     eviction.accumulate_weights(want, q[1:], c.cache, *args[:2], lse[1:], args[2] - torch.tensor([0, 1], device=device, dtype=torch.int32))
     assert torch.isfinite(got).all() and torch.allclose(got, want, rtol=2.0**-18, atol=0)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,chunks,heads,kv_heads,dim,dtype", [
+    ([70], [1], 8, 2, 128, BF16), ([300], [300], 8, 2, 128, BF16), ([2000], [700], 4, 1, 64, F16),
+    ([400, 50, 9], [150, 1, 1], 4, 1, 256, BF16), ([900], [300], 8, 2, 128, FP8), ([90, 33], [3, 2], 8, 2, 64, FP8),
+])
+def test_rows_without_a_log_sum_add_nothing_whatever_they_hold(device, lengths, chunks, heads, kv_heads, dim, dtype, causal) -> None:
+    """A log sum of -inf leaves a row out: its query may be NaN."""
+
+    print(f"left out: {lengths} {chunks} {heads}/{kv_heads}x{dim} {dtype} {causal}", flush=True)
+    c = _case(device, 23, lengths, chunks, heads, kv_heads, dim, 16, dtype)
+    args = c.device_args()
+    _, lse = paged.attention(c.q.to(device), c.cache, *args, causal=causal, return_lse=True)
+    out = torch.rand(c.q.shape[:2], generator=torch.Generator().manual_seed(4)) < 0.02
+    out[0, 0] = out[-1, -1] = True
+    q = c.q.clone()
+    q[out] = math.nan
+    lse = lse.masked_fill(out.to(device), -math.inf)
+    got = eviction.new_weights(c.cache)
+    eviction.accumulate_weights(got, q.to(device), c.cache, *args[:2], lse, args[2], causal=causal)
+    sums, kept = lse.double().cpu().numpy(), _f64(c.q)
+    sums[out.numpy()], kept[out.numpy()] = 1e4, 0
+    want, off = oracle.added_weights(kept, np.nan_to_num(c.keys64), c.table.numpy(), lengths, c.starts, sums, dim**-0.5,
+                                     causal=causal)
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all() and (np.abs(got - want) <= off).all()
