@@ -11,9 +11,9 @@
 // the 16 lanes of a key add theirs once, at the end.
 //
 // That is the kernel of many rows, bound by the exponentials and the products (prompt of
-// 4096 tokens over as many 4-bit keys, 32 heads on 8, 91 us).  Where
-// the keys are too few workgroups for them, the rows are cut into pieces, whose sums a
-// second kernel adds in order.  Few rows (a decoded token) are bound by reading the
+// 4096 tokens over as many 4-bit keys, 32 heads on 8, 78 us, 84 where its inputs are in
+// no cache).  Where the keys are too few workgroups for them, the rows are cut into
+// pieces, whose sums a second kernel adds in order (5 us).  Few rows (a decoded token) are bound by reading the
 // keys: there the rows stay, in LDS, and the keys pass by, loaded a step ahead.
 //
 // Which of the two takes a sequence is known to the device alone where `starts` says how
@@ -387,7 +387,7 @@ __device__ __forceinline__ void list_chunks(const WeightArgs& w, uint32_t* scan)
 // Few rows: those of a sequence, up to kStage, lie in LDS while its keys pass by, 32 a wave and step,
 // loaded as 128 neighbouring bytes by eight lanes, through LDS of the wave's own.  A
 // workgroup takes up to kMostSteps steps of each of its four waves, and more in turn.  A wave has 16 KiB of keys on
-// their way, whatever their type (8 KiB: 227 us for 16 sequences of 32K bf16 keys), and
+// their way, whatever their type (16 sequences of 32K bf16 keys: 217 us; 227 with 8 KiB, 220 with 16 in one run), and
 // nothing that the steps wait for is loaded after them: cache rows are looked up a group
 // of steps ahead, a row's powers of two come with it.
 template <class Tag, Store kStore, int D>
@@ -644,16 +644,17 @@ WeightPlan weight_plan(const dsa_paged_cache* cache, int64_t sequences, int64_t 
                        bool uniform) {
   const int64_t group = heads / cache->kv_heads, pairs = sequences * cache->kv_heads;
   WeightPlan p = {};
-  // With `starts` each sequence has the kernel of its own rows.  (us, so / all in the
-  // kernel that the average rows say, 32 heads on 8 of 128 dims: 256 tokens over 4096 bf16
-  // keys each and a chunk of 2048 over as many 335 / 5670; 8 over 32K and a prompt of 4096
-  // 182 / 402; chunks of 300, 60, 200 and 40 tokens, a launch or two less, 22 / 16.)
+  // With `starts` each sequence has the kernel of its own rows.  (us, so / as a call for the
+  // single tokens and one for the others, 32 heads on 8 of 128 dims, bf16: 256 tokens over
+  // 4096 keys each and a chunk of 2048 over as many 509 / 433 + 75; 8 over 32K and a prompt
+  // of 4096 203 / 110 + 95.  A batch that has no single tokens pays for the list: 4 x 150
+  // tokens over 4096 keys each 49, without `starts` 46; 4 prompts of 150 19 and 15.)
   p.mixed = !uniform && sequences > 1 && tokens * group > kStage;
   p.few = p.mixed || tokens * group <= kStage * sequences;
   // Workgroups by what keeps the GPU busy; for sequences of more keys than that has tiles
   // for, as many as the page table's room asks for, while their starts cost little.  What
   // each does follows from the keys that its sequence has.  (Prompt of 4096 tokens, bf16,
-  // in a table with room for 128K keys: 92 us, and 365 with the work cut by the room.)
+  // in a table with room for 128K keys: 95 us as in one without, and 365 cut by the room.)
   const int64_t tiles = (capacity + kTile - 1) / kTile;
   auto slots = [&](int64_t share, int64_t of_room) {
     return std::max(share, std::min(of_room, 4 * kManyWorkgroups / pairs));
